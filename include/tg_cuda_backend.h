@@ -476,6 +476,108 @@ TG_API int tg_attention_noalloc(void* cuda_stream, const float* q, const void* k
                                 int n_head, int n_kv_head, int head_dim,
                                 const int32_t* past_len, float* out, int* device_status);
 
+/* ------------------------------------------------- paged KV caches */
+
+/* No counterpart in the reference (one contiguous cache per layer,
+ * tmac_gguf.cpp:200-201).  A cache of pages that sequences hold through a
+ * block table, for serving: sequences grow page by page, share the pages of
+ * a common prefix, and may attend to selected pages only.
+ *
+ * K and V are each laid out [n_layers][n_pages][n_kv_head][page_size]
+ * [head_dim] of `dtype`; page_size is a power of two from 8 to 256.  bounds
+ * (with_bounds), [n_layers][n_pages][n_kv_head][2][head_dim] of `dtype`,
+ * holds the minimum and maximum of every key dimension over a page's rows,
+ * which tg_paged_select needs.  k and v (both or neither) and bounds may
+ * name device memory of the caller, 16-byte aligned, used in place and not
+ * freed; where they are NULL the library allocates and zeroes them.
+ * Positions 0..max_pos-1 can be rotated.
+ *
+ * Block tables are [n_seqs][max_blocks] int32: entry j of row s is the page
+ * of positions j*page_size.. of sequence s.  Entries that a call needs must
+ * lie in [0, n_pages): host arrays are checked, device arrays by the
+ * kernels, which leave such an entry's rows out (tg_paged_select ranks it
+ * last) and report device error 0x106; 0x103 reports a position outside the
+ * table or the rotation table, whose query counts as empty.  Several tokens
+ * of one sequence in a call are several rows with the same entries.  A page
+ * that tg_paged_append writes belongs to one sequence only.
+ * Pointer and stream rules are those of the batched calls above; calls on
+ * device pointers can be captured into graphs, once the same call ran
+ * before. */
+typedef struct tg_paged_kv tg_paged_kv;
+typedef struct tg_paged_desc {
+  int n_layers, n_pages, page_size, n_head, n_kv_head, head_dim, dtype;
+  int max_pos;
+  int with_bounds;
+  float rope_base;
+  void* k;
+  void* v;
+  void* bounds;
+} tg_paged_desc;
+
+TG_API int tg_paged_create(tg_context* ctx, const tg_paged_desc* desc, tg_paged_kv** out);
+/* Destroy before tg_shutdown of its context; tg_shutdown frees caches that
+ * are still alive, after which their handles must not be used. */
+TG_API int tg_paged_destroy(tg_paged_kv* pk);
+/* Device pointers of one layer; bounds NULL when the cache keeps none. */
+TG_API int tg_paged_layer_ptrs(tg_paged_kv* pk, int layer, void** k, void** v, void** bounds);
+
+/* Appends n_tokens rows: the tokens of sequence s are rows
+ * cu_tokens[s] .. cu_tokens[s+1]-1 of k and v ([n_tokens][n_kv*head_dim],
+ * un-rotated), at the positions pos0[s], pos0[s]+1, ...  cu_tokens
+ * [n_seqs+1] may be NULL: token s is sequence s's (a decode step; n_tokens
+ * must equal n_seqs).  k is rotated as by tg_rope_op (bit for bit), k and v
+ * go to the page of their position (round to nearest even for bf16), and
+ * with bounds every page written gets its bounds anew, over its rows up to
+ * the last one written.  q ([n_tokens][n_head*head_dim], may be NULL) is
+ * rotated into q_out (which may be q).  Tokens behind cu_tokens[n_seqs] are
+ * padding: nothing of them is written. */
+TG_API int tg_paged_append(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, int n_tokens,
+                           const int32_t* cu_tokens, const int32_t* pos0,
+                           const int32_t* block_table, int max_blocks, const float* k,
+                           const float* v, const float* q, float* q_out);
+
+/* Decode attention through the block table: query s attends positions
+ * 0..past_len[s] (tmac_gguf.cpp:1093-1128 per sequence); past_len[s] = -1
+ * attends nothing and gives zeros (a padding row of a batch).  q (rotated)
+ * and out are [n_seqs][n_head*head_dim]. */
+TG_API int tg_paged_attention(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs,
+                              const float* q, const int32_t* past_len,
+                              const int32_t* block_table, int max_blocks, float* out);
+
+/* tg_paged_attention for a batch whose sequences share their first
+ * shared_len positions: the first shared_len / page_size entries (rounded
+ * down) of every table row are the same pages, named by row 0, and are read
+ * once for all queries.  past_len[s] may lie inside the shared part. */
+TG_API int tg_paged_attention_shared(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs,
+                                     const float* q, const int32_t* past_len,
+                                     const int32_t* block_table, int max_blocks, int shared_len,
+                                     float* out);
+
+/* For every query and KV head the n_sel table entries j (of those that hold
+ * positions 0..past_len[s]) with the highest scores, ascending, -1 behind
+ * the last: pages [n_seqs][n_kv_head][n_sel].  The score is the largest,
+ * over the query heads h of the KV head's group, of
+ * sum_d max(q_hd * lo_d, q_hd * hi_d) with the page's bounds lo and hi --
+ * no key of the page has a larger product with q.  The first keep_first and
+ * the last keep_last entries rank above all others; ties go to the lower
+ * index, NaN ranks last.  Needs a cache with bounds. */
+TG_API int tg_paged_select(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs,
+                           const float* q, const int32_t* past_len, const int32_t* block_table,
+                           int max_blocks, int keep_first, int keep_last, int n_sel,
+                           int32_t* pages);
+
+/* Decode attention over listed pages only: query s, KV head g attends the
+ * rows at positions 0..past_len[s] of the table entries
+ * pages[s][g][0..n_sel-1] (as tg_paged_select writes them).  Entries that
+ * are -1 or hold no such position count as nothing, an entry listed twice
+ * counts twice, and with P = past_len[s] / page_size + 1 pages in use only
+ * the first min(n_sel, P) entries are read.  A query without a row gives
+ * zeros. */
+TG_API int tg_paged_attention_sparse(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs,
+                                     const float* q, const int32_t* past_len,
+                                     const int32_t* block_table, int max_blocks, int n_sel,
+                                     const int32_t* pages, float* out);
+
 /* ------------------------------------------------- introspection */
 
 /* Kernel launches this context has issued since creation (all kinds). */

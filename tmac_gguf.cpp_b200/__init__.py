@@ -74,6 +74,14 @@ class tg_kv_desc(C.Structure):
                 ("global_ctx", C.c_int), ("rope_base", C.c_float)]
 
 
+class tg_paged_desc(C.Structure):
+    _fields_ = [("n_layers", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int),
+                ("n_head", C.c_int), ("n_kv_head", C.c_int), ("head_dim", C.c_int),
+                ("dtype", C.c_int), ("max_pos", C.c_int), ("with_bounds", C.c_int),
+                ("rope_base", C.c_float), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("bounds", C.c_void_p)]
+
+
 class tg_qkv_weights(C.Structure):
     _fields_ = [("q_type", C.c_int), ("k_type", C.c_int), ("v_type", C.c_int),
                 ("cols", C.c_int), ("w_q", C.c_void_p), ("w_k", C.c_void_p),
@@ -176,6 +184,19 @@ _SIGS = {
     "tg_attention_block_splitkv": (C.c_int, [_vp, _vp, C.c_int, C.c_int,
                                              C.POINTER(tg_qkv_weights), C.c_int, _vp, _vp,
                                              _vp, _vp]),
+    "tg_paged_create": (C.c_int, [_vp, C.POINTER(tg_paged_desc), C.POINTER(_vp)]),
+    "tg_paged_destroy": (C.c_int, [_vp]),
+    "tg_paged_layer_ptrs": (C.c_int, [_vp, C.c_int, C.POINTER(_vp), C.POINTER(_vp),
+                                      C.POINTER(_vp)]),
+    "tg_paged_append": (C.c_int, [_vp, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, C.c_int,
+                                  _vp, _vp, _vp, _vp]),
+    "tg_paged_attention": (C.c_int, [_vp, _vp, C.c_int, C.c_int, _vp, _vp, _vp, C.c_int, _vp]),
+    "tg_paged_attention_shared": (C.c_int, [_vp, _vp, C.c_int, C.c_int, _vp, _vp, _vp, C.c_int,
+                                            C.c_int, _vp]),
+    "tg_paged_select": (C.c_int, [_vp, _vp, C.c_int, C.c_int, _vp, _vp, _vp, C.c_int, C.c_int,
+                                  C.c_int, C.c_int, _vp]),
+    "tg_paged_attention_sparse": (C.c_int, [_vp, _vp, C.c_int, C.c_int, _vp, _vp, _vp, C.c_int,
+                                            C.c_int, _vp, _vp]),
 }
 
 _lib: Optional[C.CDLL] = None
@@ -628,6 +649,164 @@ class KVCache:
         _check(lib().tg_decode_layer_splitkv(self.backend.handle, self._h,
                                              layer, n, _ptr(q), _ptr(k_new),
                                              _ptr(v_new), _ptr(pos), _ptr(out)))
+
+
+class PagedKVCache:
+    """A paged K/V cache (tg_paged_*): pages [n_layers][n_pages][n_kv_head]
+    [page_size][head_dim] that sequences hold through block tables ([n_seqs]
+    [max_blocks] int32).  k, v (both or neither) and bounds may be contiguous
+    device tensors of that shape (bounds [n_layers][n_pages][n_kv_head][2]
+    [head_dim]), used in place and kept referenced; otherwise the library
+    allocates them.  q, k, v and outputs are fp32; tables, positions and page
+    lists int32; numpy arrays (staged) or device tensors."""
+
+    def __init__(self, backend: CudaBackend, n_layers: int, n_pages: int, page_size: int,
+                 n_head: int = N_HEAD, n_kv_head: int = N_KV_HEAD, head_dim: int = HEAD_DIM,
+                 dtype: int = DTYPE_BF16, max_pos: int = 131072, rope_base: float = ROPE_BASE,
+                 with_bounds: bool = True, k=None, v=None, bounds=None):
+        n = n_layers * n_pages * n_kv_head * page_size * head_dim
+        for name, x, size in (("k", k, n), ("v", v, n),
+                              ("bounds", bounds, 2 * n // max(page_size, 1))):
+            if hasattr(x, "numel"):
+                if x.numel() != size:
+                    raise ValueError(f"{name} has {x.numel()} elements, not {size}")
+                if x.element_size() != (4 if dtype == DTYPE_F32 else 2):
+                    raise ValueError(f"{name} is not of the cache's type")
+                if x.device.type != "cuda" or x.device.index != backend.device:
+                    raise ValueError(f"{name} is not on device {backend.device}")
+        self.backend = backend
+        self._keep = (k, v, bounds)
+        self.desc = tg_paged_desc(n_layers, n_pages, page_size, n_head, n_kv_head, head_dim,
+                                  dtype, max_pos, 1 if with_bounds or bounds is not None else 0,
+                                  rope_base, _ptr(k), _ptr(v), _ptr(bounds))
+        h = C.c_void_p()
+        _check(lib().tg_paged_create(backend.handle, C.byref(self.desc), C.byref(h)))
+        self._h = h
+        self.n_layers, self.n_pages, self.page_size = n_layers, n_pages, page_size
+        self.n_head, self.n_kv_head, self.head_dim = n_head, n_kv_head, head_dim
+        self.dtype = dtype
+        self.qdim, self.row = n_head * head_dim, n_kv_head * head_dim
+
+    @property
+    def handle(self) -> C.c_void_p:
+        return self._h
+
+    def destroy(self) -> None:
+        # After the backend's shutdown the C side has freed the cache already.
+        if self._h and self.backend.handle:
+            _check(lib().tg_paged_destroy(self._h))
+        self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            if getattr(self, "_h", None) and self.backend.handle:
+                lib().tg_paged_destroy(self._h)
+        except Exception:
+            pass
+
+    def layer_ptrs(self, layer: int):
+        """Device addresses of a layer's K, V and bounds (None without)."""
+        k, v, b = C.c_void_p(), C.c_void_p(), C.c_void_p()
+        _check(lib().tg_paged_layer_ptrs(self._h, layer, C.byref(k), C.byref(v), C.byref(b)))
+        return k.value, v.value, b.value
+
+    def append(self, layer: int, k, v, pos0, block_table, q=None, q_out=None,
+               cu_tokens=None) -> None:
+        """Rotate and append tokens (tg_paged_append): k, v [n_tokens][row];
+        sequence s's tokens are cu_tokens[s]..cu_tokens[s+1]-1, or token s
+        without cu_tokens, at positions pos0[s]..  q is rotated into q_out
+        (q itself when q_out is None)."""
+        n, blocks = _table_shape(block_table)
+        toks = _rows(k, self.row, "k")
+        if _rows(v, self.row, "v") != toks:
+            raise ValueError("k and v differ in tokens")
+        if q is not None:
+            q_out = q if q_out is None else q_out
+            if _rows(q, self.qdim, "q") != toks or _rows(q_out, self.qdim, "q_out") != toks:
+                raise ValueError("q, q_out and k differ in tokens")
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        _check(lib().tg_paged_append(
+            self.backend.handle, self._h, layer, n, toks, _ints(cu_tokens, n + 1, "cu_tokens"),
+            _ints(pos0, n, "pos0"), _ints(block_table, n * blocks, "block_table"), blocks,
+            _ptr(k), _ptr(v), _ptr(q), _ptr(q_out)))
+
+    def _query_args(self, q, past_len, block_table, out=None):
+        n, blocks = _table_shape(block_table)
+        if _rows(q, self.qdim, "q") != n:
+            raise ValueError(f"q has not {n} rows, as block_table has")
+        if out is not None and _rows(out, self.qdim, "out") != n:
+            raise ValueError(f"out has not {n} rows, as block_table has")
+        return (n, _ptr(q), _ints(past_len, n, "past_len"),
+                _ints(block_table, n * blocks, "block_table"), blocks)
+
+    def attention(self, layer: int, q, past_len, block_table, out) -> None:
+        """Decode attention through the block table (tg_paged_attention);
+        past_len -1 gives zeros."""
+        _check(lib().tg_paged_attention(self.backend.handle, self._h, layer,
+                                        *self._query_args(q, past_len, block_table, out),
+                                        _ptr(out)))
+
+    def attention_shared(self, layer: int, q, past_len, block_table, shared_len: int,
+                         out) -> None:
+        """The same for a batch whose first shared_len positions lie in the
+        same pages (tg_paged_attention_shared)."""
+        _check(lib().tg_paged_attention_shared(
+            self.backend.handle, self._h, layer,
+            *self._query_args(q, past_len, block_table, out), int(shared_len), _ptr(out)))
+
+    def select_pages(self, layer: int, q, past_len, block_table, pages, keep_first: int = 1,
+                     keep_last: int = 1) -> None:
+        """The pages.shape[-1] best table entries of every query and KV head
+        into pages [n][n_kv_head][n_sel] (tg_paged_select)."""
+        args = self._query_args(q, past_len, block_table)
+        n_sel = self._n_sel(pages, args[0])
+        _check(lib().tg_paged_select(self.backend.handle, self._h, layer, *args, keep_first,
+                                     keep_last, n_sel,
+                                     _ints(pages, args[0] * self.n_kv_head * n_sel, "pages")))
+
+    def attention_sparse(self, layer: int, q, past_len, block_table, pages, out) -> None:
+        """Attention over the listed table entries only
+        (tg_paged_attention_sparse)."""
+        args = self._query_args(q, past_len, block_table, out)
+        n_sel = self._n_sel(pages, args[0])
+        _check(lib().tg_paged_attention_sparse(
+            self.backend.handle, self._h, layer, *args, n_sel,
+            _ints(pages, args[0] * self.n_kv_head * n_sel, "pages"), _ptr(out)))
+
+    def _n_sel(self, pages, n: int) -> int:
+        shape = tuple(pages.shape)
+        if len(shape) != 3 or shape[:2] != (n, self.n_kv_head):
+            raise ValueError(f"pages is {shape}, not [{n}][{self.n_kv_head}][n_sel]")
+        return shape[2]
+
+
+def _table_shape(t):
+    shape = tuple(t.shape)
+    if len(shape) != 2:
+        raise ValueError(f"block_table is {shape}, not [n_seqs][max_blocks]")
+    return shape
+
+
+def _rows(x, width: int, what: str) -> int:
+    """Rows of a float32 array of `width` columns."""
+    if not str(x.dtype).endswith("float32"):
+        raise ValueError(f"{what} is {x.dtype}, not float32")
+    n = x.numel() if hasattr(x, "numel") else x.size
+    if n % width:
+        raise ValueError(f"{what} has {n} values, not rows of {width}")
+    return n // width
+
+
+def _ints(x, n: int, what: str):
+    """Address of an int32 array of n values (None for None)."""
+    if x is None:
+        return None
+    if not str(x.dtype).endswith("int32") or str(x.dtype).endswith("uint32"):
+        raise ValueError(f"{what} is {x.dtype}, not int32")
+    if (x.numel() if hasattr(x, "numel") else x.size) != n:
+        raise ValueError(f"{what} has not {n} values")
+    return _ptr(x)
 
 
 def _as_i32(x):

@@ -25,6 +25,7 @@
 
 #include "../../include/tg_cuda_backend.h"
 #include "tg_kernels.h"
+#include "tg_paged.h"
 #include "tg_shared.h"
 
 #define TG_VERSION "tmac_gguf.cpp_b200 0.1.0"
@@ -223,6 +224,15 @@ struct tg_context {
 
   std::vector<tg_kv_cache*> caches;  // freed by tg_shutdown if still alive
 
+  // Paged caches.  A captured graph keeps the addresses of these scratch
+  // buffers (and of the RoPE tables), so outgrown ones stay allocated in
+  // `kept` until shutdown; sizes grow geometrically.
+  std::vector<tg_paged_kv*> paged;
+  float* ppart = nullptr;                 size_t ppart_cap = 0;   // floats
+  unsigned* pcount = nullptr;             size_t pcount_cap = 0;  // zero between launches
+  unsigned long long* pkeys = nullptr;    size_t pkeys_cap = 0;
+  std::vector<void*> kept;
+
   // Optional CUDA-event timing of each decode-attention kernel launch.
   int prof_on = 0;  // TG_PROFILE_* mask
   std::vector<cudaEvent_t> prof_ev;  // start/stop pairs
@@ -265,6 +275,18 @@ struct tg_kv_cache {
   alignas(64) CUtensorMap tmk128;
   alignas(64) CUtensorMap tmv128;
   int global_ctx = 0;
+};
+
+struct tg_paged_kv {
+  tg_context* ctx = nullptr;
+  tg_paged_desc d{};
+  int log2p = 0;
+  size_t esize = 0;
+  size_t layer_elems = 0, bounds_elems = 0;  // per layer
+  char* k = nullptr;
+  char* v = nullptr;
+  char* bounds = nullptr;
+  bool own_kv = false, own_bounds = false;
 };
 
 namespace {
@@ -339,6 +361,7 @@ int check_device_error(tg_context* ctx, bool queued = false) {
                        : h == tg::kDevErrWaitFull     ? "bounded wait for a K/V tile expired"
                        : h == tg::kDevErrWaitEmpty    ? "bounded wait for a free stage expired"
                        : h == tg::kDevErrPeerTimeout  ? "another GPU's softmax record did not arrive"
+                       : h == tg::kDevErrBadPage      ? "block table entry outside the paged cache"
                            : "device error";
     return fail(TG_ERR_DEVICE, "kernel reported 0x%x: %s", h, what);
   }
@@ -917,7 +940,7 @@ int get_table(tg_context* ctx, float base, int head_dim, int need_len, RopeTable
     t->base_bits = bits;
     t->head_dim = head_dim;
   } else {
-    ctx->graveyard.push_back(t->d);
+    ctx->kept.push_back(t->d);  // captured graphs may read it
   }
   t->len = len;
   t->d = d;
@@ -1524,12 +1547,130 @@ int check_kv_call(tg_context* ctx, tg_kv_cache* kv, int layer, int n_seqs) {
   return set_device(ctx);
 }
 
+void paged_free(tg_paged_kv* pk) {
+  if (pk->own_kv) {
+    cudaFree(pk->k);
+    cudaFree(pk->v);
+  }
+  if (pk->own_bounds) cudaFree(pk->bounds);
+  delete pk;
+}
+
 // Host position arrays are validated here; device ones by the kernels.
 int check_host_pos(const int32_t* pos, int n, int limit, const char* what) {
   if (!pos || is_device_ptr(pos)) return TG_OK;
   for (int i = 0; i < n; ++i)
     if (pos[i] < 0 || pos[i] >= limit)
       return fail(TG_ERR_INVALID_ARG, "%s[%d] = %d outside [0, %d)", what, i, pos[i], limit);
+  return TG_OK;
+}
+
+// ------------------------------------------------ paged KV caches
+
+// As ensure_buf, for buffers that captured graphs may name: the old one is
+// kept until shutdown.  zero: the new one is zeroed on the stream.
+template <typename T>
+int ensure_kept(tg_context* ctx, T** buf, size_t* cap, size_t need, bool zero = false) {
+  if (need <= *cap) return TG_OK;
+  if (ctx->capturing)
+    return fail(TG_ERR_STATE,
+                "scratch must be sized before graph capture: run the same call once first");
+  size_t n = need < 1024 ? 1024 : need;
+  n = n + n / 2;
+  T* nb = nullptr;
+  TG_CUDA(cudaMalloc(&nb, n * sizeof(T)));
+  if (zero) {
+    cudaError_t e = cudaMemsetAsync(nb, 0, n * sizeof(T), ctx->stream);
+    if (e != cudaSuccess) {
+      cudaFree(nb);
+      return fail(TG_ERR_CUDA, "cudaMemsetAsync: %s", cudaGetErrorString(e));
+    }
+  }
+  if (*buf) ctx->kept.push_back(*buf);
+  *buf = nb;
+  *cap = n;
+  return TG_OK;
+}
+
+int check_paged_call(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, int max_blocks) {
+  if (!ctx || !pk) return fail(TG_ERR_INVALID_ARG, "null context or cache");
+  if (pk->ctx != ctx) return fail(TG_ERR_INVALID_ARG, "cache belongs to another context");
+  if (layer < 0 || layer >= pk->d.n_layers)
+    return fail(TG_ERR_INVALID_ARG, "layer %d outside [0, %d)", layer, pk->d.n_layers);
+  if (n_seqs < 0) return fail(TG_ERR_INVALID_ARG, "n_seqs %d < 0", n_seqs);
+  if (max_blocks < 1 || ((long long)max_blocks << pk->log2p) >= (1LL << 31))
+    return fail(TG_ERR_INVALID_ARG, "max_blocks %d of %d positions", max_blocks, pk->d.page_size);
+  return set_device(ctx);
+}
+
+// Host arrays: last positions in [-1, max_blocks*page_size) and, when the
+// table is on the host too, the entries they use in [0, n_pages).
+int check_host_pages(const tg_paged_kv* pk, const int32_t* past, const int32_t* table, int n,
+                     int max_blocks) {
+  if (is_device_ptr(past)) return TG_OK;
+  const bool host_table = !is_device_ptr(table);
+  const long long limit = (long long)max_blocks << pk->log2p;
+  for (int s = 0; s < n; ++s) {
+    if (past[s] < -1 || past[s] >= limit)
+      return fail(TG_ERR_INVALID_ARG, "past_len[%d] = %d outside [-1, %lld)", s, past[s], limit);
+    if (!host_table || past[s] < 0) continue;
+    for (int j = 0; j <= past[s] >> pk->log2p; ++j) {
+      const int page = table[(size_t)s * max_blocks + j];
+      if (page < 0 || page >= pk->d.n_pages)
+        return fail(TG_ERR_INVALID_ARG, "block_table[%d][%d] = %d outside [0, %d)", s, j, page,
+                    pk->d.n_pages);
+    }
+  }
+  return TG_OK;
+}
+
+// Attention launches on device pointers, kPagedMaxQueries queries at a time.
+int run_paged(tg_context* ctx, const tg_paged_kv* pk, int layer, int n, const float* q,
+              const int* past, const int* table, int max_blocks, const int* sel, int n_sel,
+              float* out) {
+  TG_TRY(commit_inputs(ctx));
+  TG_TRY(check_align8(q, "q"));
+  TG_TRY(check_align8(out, "out"));
+  const tg_paged_desc& d = pk->d;
+  const int qdim = d.n_head * d.head_dim;
+  tg::PagedAttnParams p{};
+  p.kp = pk->k + (size_t)layer * pk->layer_elems * pk->esize;
+  p.vp = pk->v + (size_t)layer * pk->layer_elems * pk->esize;
+  p.page0 = (long long)layer * d.n_pages;
+  p.err = ctx->d_err;
+  p.n_head = d.n_head;
+  p.n_kv = d.n_kv_head;
+  p.group = d.n_head / d.n_kv_head;
+  p.hblocks = (p.group + tg::kPagedHeads - 1) / tg::kPagedHeads;
+  p.hd = d.head_dim;
+  p.max_blocks = max_blocks;
+  p.n_pages = d.n_pages;
+  p.log2p = pk->log2p;
+  p.n_sel = n_sel;
+  p.scale_log2 = kLog2e / sqrtf((float)d.head_dim);
+  const int streams = p.n_kv * p.hblocks;
+  for (int s0 = 0; s0 < n; s0 += tg::kPagedMaxQueries) {
+    p.n = std::min(n - s0, tg::kPagedMaxQueries);
+    p.q = q + (size_t)s0 * qdim;
+    p.out = out + (size_t)s0 * qdim;
+    p.past = past + s0;
+    p.table = table + (size_t)s0 * max_blocks;
+    p.sel = sel ? sel + (size_t)s0 * p.n_kv * n_sel : nullptr;
+    const size_t smem = tg::paged_core_smem(p.n, p.hd);
+    const int grid = ctx->num_sms * (2 * (smem + 1024) <= 227 * 1024 ? 2 : 1);
+    TG_TRY(ensure_kept(ctx, &ctx->ppart, &ctx->ppart_cap,
+                       (size_t)2 * grid * tg::kPagedHeads * (p.hd + 2)));
+    TG_TRY(ensure_kept(ctx, &ctx->pcount, &ctx->pcount_cap, (size_t)p.n * streams, true));
+    p.part = ctx->ppart;
+    p.count = ctx->pcount;
+    cudaEvent_t ev = nullptr;
+    TG_TRY(prof_begin(ctx, TG_PROFILE_ATTENTION, &ev));
+    cudaError_t e = tg::launch_paged_core(p, d.dtype, grid, ctx->stream);
+    if (e != cudaSuccess)
+      return fail(TG_ERR_CUDA, "paged attention launch: %s", cudaGetErrorString(e));
+    ctx->launches++;
+    TG_TRY(prof_end(ctx, ev));
+  }
   return TG_OK;
 }
 
@@ -1612,6 +1753,12 @@ int tg_shutdown(tg_context* ctx) {
     delete kv;
   }
   ctx->caches.clear();
+  for (tg_paged_kv* pk : ctx->paged) paged_free(pk);
+  ctx->paged.clear();
+  cudaFree(ctx->ppart);
+  cudaFree(ctx->pcount);
+  cudaFree(ctx->pkeys);
+  for (void* b : ctx->kept) cudaFree(b);
   for (auto& kv : ctx->regions) cudaFree(kv.second.dev);
   for (RopeTable& t : ctx->tables) cudaFree(t.d);
   for (cudaEvent_t ev : ctx->prof_ev) cudaEventDestroy(ev);
@@ -2754,6 +2901,305 @@ int tg_prefill_layer(tg_context* ctx, tg_kv_cache* kv, int layer, int n_seqs, in
   ctx->launches++;
   TG_TRY(prof_end(ctx, ev_stop));
   return finish_call(ctx);
+}
+
+// ------------------------------------------------ paged KV caches
+
+int tg_paged_create(tg_context* ctx, const tg_paged_desc* desc, tg_paged_kv** out) {
+  TG_TRY(set_device(ctx));
+  if (!desc || !out) return fail(TG_ERR_INVALID_ARG, "null argument");
+  *out = nullptr;
+  const tg_paged_desc& d = *desc;
+  TG_TRY(check_shape(d.n_head, d.n_kv_head, d.head_dim));
+  if (d.n_layers <= 0 || d.n_pages <= 0 || d.max_pos <= 0)
+    return fail(TG_ERR_INVALID_ARG, "paged_create: bad sizes");
+  if (d.page_size < tg::kPagedMinPage || d.page_size > tg::kPagedMaxPage ||
+      (d.page_size & (d.page_size - 1)))
+    return fail(TG_ERR_INVALID_ARG, "paged_create: page_size %d (a power of two, %d to %d)",
+                d.page_size, tg::kPagedMinPage, tg::kPagedMaxPage);
+  if (d.dtype != TG_DTYPE_F32 && d.dtype != TG_DTYPE_BF16)
+    return fail(TG_ERR_INVALID_ARG, "paged_create: dtype %d", d.dtype);
+  if (!(d.rope_base > 0.f)) return fail(TG_ERR_INVALID_ARG, "paged_create: rope_base must be > 0");
+  const long long rows = (long long)d.n_pages * d.page_size;
+  if (rows >= (1LL << 31) || rows * d.n_kv_head >= (1LL << 31) ||
+      rows * d.n_kv_head * d.n_layers >= (1LL << 31))
+    return fail(TG_ERR_INVALID_ARG, "paged_create: %d layers of %lld rows are too many",
+                d.n_layers, rows * d.n_kv_head);
+  if (!d.k != !d.v) return fail(TG_ERR_INVALID_ARG, "paged_create: k and v, both or neither");
+  if (d.bounds && !d.with_bounds)
+    return fail(TG_ERR_INVALID_ARG, "paged_create: bounds without with_bounds");
+  for (const void* m : {d.k, d.v, d.bounds}) {
+    if (!m) continue;
+    if (!is_device_ptr(m)) return fail(TG_ERR_INVALID_ARG, "paged_create: pools are device memory");
+    if (reinterpret_cast<uintptr_t>(m) & 15)
+      return fail(TG_ERR_INVALID_ARG, "paged_create: pools must be 16-byte aligned");
+  }
+  if (ctx->capturing) return fail(TG_ERR_STATE, "paged_create inside a graph capture");
+  RopeTable* t = nullptr;
+  TG_TRY(get_table(ctx, d.rope_base, d.head_dim, d.max_pos, &t));
+  tg_paged_kv* pk = new tg_paged_kv();
+  pk->ctx = ctx;
+  pk->d = d;
+  while ((1 << pk->log2p) < d.page_size) ++pk->log2p;
+  pk->esize = d.dtype == TG_DTYPE_F32 ? 4 : 2;
+  pk->layer_elems = (size_t)rows * d.n_kv_head * d.head_dim;
+  pk->bounds_elems = (size_t)d.n_pages * d.n_kv_head * 2 * d.head_dim;
+  pk->k = static_cast<char*>(d.k);
+  pk->v = static_cast<char*>(d.v);
+  pk->bounds = static_cast<char*>(d.bounds);
+  const size_t bytes = pk->layer_elems * d.n_layers * pk->esize;
+  const size_t bbytes = pk->bounds_elems * d.n_layers * pk->esize;
+  bool ok = true;
+  if (!pk->k) {
+    pk->own_kv = true;
+    ok = cudaMalloc(&pk->k, bytes) == cudaSuccess && cudaMalloc(&pk->v, bytes) == cudaSuccess &&
+         cudaMemsetAsync(pk->k, 0, bytes, ctx->stream) == cudaSuccess &&
+         cudaMemsetAsync(pk->v, 0, bytes, ctx->stream) == cudaSuccess;
+  }
+  if (ok && d.with_bounds && !pk->bounds) {
+    pk->own_bounds = true;
+    ok = cudaMalloc(&pk->bounds, bbytes) == cudaSuccess &&
+         cudaMemsetAsync(pk->bounds, 0, bbytes, ctx->stream) == cudaSuccess;
+  }
+  if (!ok) {
+    cudaGetLastError();
+    paged_free(pk);
+    return fail(TG_ERR_OUT_OF_MEMORY, "paged_create: %zu bytes per cache", bytes);
+  }
+  if (pk->own_kv || pk->own_bounds) {
+    cudaError_t e = cudaStreamSynchronize(ctx->stream);
+    if (e != cudaSuccess) {
+      paged_free(pk);
+      return fail(TG_ERR_CUDA, "paged_create: %s", cudaGetErrorString(e));
+    }
+  }
+  ctx->paged.push_back(pk);
+  *out = pk;
+  return TG_OK;
+}
+
+int tg_paged_destroy(tg_paged_kv* pk) {
+  if (!pk) return TG_OK;
+  cudaSetDevice(pk->ctx->device);
+  if (cudaStreamSynchronize(pk->ctx->stream) == cudaSuccess) stream_idle(pk->ctx);
+  auto& ps = pk->ctx->paged;
+  for (size_t i = 0; i < ps.size(); ++i)
+    if (ps[i] == pk) {
+      ps.erase(ps.begin() + i);
+      break;
+    }
+  paged_free(pk);
+  return TG_OK;
+}
+
+int tg_paged_layer_ptrs(tg_paged_kv* pk, int layer, void** k, void** v, void** bounds) {
+  if (!pk || layer < 0 || layer >= pk->d.n_layers)
+    return fail(TG_ERR_INVALID_ARG, "bad cache or layer");
+  const size_t off = (size_t)layer * pk->layer_elems * pk->esize;
+  if (k) *k = pk->k + off;
+  if (v) *v = pk->v + off;
+  if (bounds)
+    *bounds = pk->bounds ? pk->bounds + (size_t)layer * pk->bounds_elems * pk->esize : nullptr;
+  return TG_OK;
+}
+
+int tg_paged_append(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, int n_tokens,
+                    const int32_t* cu_tokens, const int32_t* pos0, const int32_t* block_table,
+                    int max_blocks, const float* k, const float* v, const float* q, float* q_out) {
+  TG_TRY(check_paged_call(ctx, pk, layer, n_seqs, max_blocks));
+  if (n_tokens < 0) return fail(TG_ERR_INVALID_ARG, "n_tokens %d < 0", n_tokens);
+  if (!cu_tokens && n_tokens != n_seqs)
+    return fail(TG_ERR_INVALID_ARG, "%d tokens of %d sequences need cu_tokens", n_tokens, n_seqs);
+  if (n_tokens == 0 || n_seqs == 0) return TG_OK;
+  if (!pos0 || !block_table || !k || !v || !q != !q_out)
+    return fail(TG_ERR_INVALID_ARG, "null argument");
+  const tg_paged_desc& d = pk->d;
+  const int row = d.n_kv_head * d.head_dim, qrow = d.n_head * d.head_dim;
+  // Host arrays are checked here, device ones by the kernel.
+  const bool host_cu = cu_tokens && !is_device_ptr(cu_tokens);
+  if (host_cu) {
+    if (cu_tokens[0] < 0 || cu_tokens[n_seqs] > n_tokens)
+      return fail(TG_ERR_INVALID_ARG, "cu_tokens outside [0, %d]", n_tokens);
+    for (int s = 0; s < n_seqs; ++s)
+      if (cu_tokens[s + 1] < cu_tokens[s])
+        return fail(TG_ERR_INVALID_ARG, "cu_tokens[%d] decreases", s + 1);
+  }
+  if (!is_device_ptr(pos0) && (host_cu || !cu_tokens)) {
+    const bool host_table = !is_device_ptr(block_table);
+    const long long limit = std::min((long long)max_blocks << pk->log2p, (long long)d.max_pos);
+    for (int s = 0; s < n_seqs; ++s) {
+      const int n = cu_tokens ? cu_tokens[s + 1] - cu_tokens[s] : 1;
+      if (n == 0) continue;
+      if (pos0[s] < 0 || (long long)pos0[s] + n > limit)
+        return fail(TG_ERR_INVALID_ARG, "pos0[%d] = %d and %d tokens: outside [0, %lld)", s,
+                    pos0[s], n, limit);
+      if (!host_table) continue;
+      for (int j = pos0[s] >> pk->log2p; j <= (pos0[s] + n - 1) >> pk->log2p; ++j) {
+        const int page = block_table[(size_t)s * max_blocks + j];
+        if (page < 0 || page >= d.n_pages)
+          return fail(TG_ERR_INVALID_ARG, "block_table[%d][%d] = %d outside [0, %d)", s, j, page,
+                      d.n_pages);
+      }
+    }
+  }
+  const void *dk = nullptr, *dv = nullptr, *dq = nullptr, *dcu = nullptr, *dp = nullptr, *dt = nullptr;
+  void* dqo = nullptr;
+  TG_TRY(stage_in(ctx, k, (size_t)n_tokens * row * 4, &dk));
+  TG_TRY(stage_in(ctx, v, (size_t)n_tokens * row * 4, &dv));
+  TG_TRY(stage_in(ctx, cu_tokens, cu_tokens ? (size_t)(n_seqs + 1) * 4 : 0, &dcu));
+  TG_TRY(stage_in(ctx, pos0, (size_t)n_seqs * 4, &dp));
+  TG_TRY(stage_in(ctx, block_table, (size_t)n_seqs * max_blocks * 4, &dt));
+  if (q) {
+    TG_TRY(stage_in(ctx, q, (size_t)n_tokens * qrow * 4, &dq));
+    // Host rows of padding tokens come back as they went in.
+    TG_TRY(stage_out(ctx, q_out, (size_t)n_tokens * qrow * 4, true, &dqo));
+  }
+  TG_TRY(commit_inputs(ctx));
+  const void* io[4] = {dk, dv, dq, dqo};
+  const char* what[4] = {"k", "v", "q", "q_out"};
+  bool vec4 = d.head_dim % 4 == 0;
+  for (int i = 0; i < 4; ++i) {
+    TG_TRY(check_align8(io[i], what[i]));
+    vec4 = vec4 && reinterpret_cast<uintptr_t>(io[i]) % 16 == 0;
+  }
+  RopeTable* t = nullptr;
+  TG_TRY(get_table(ctx, d.rope_base, d.head_dim, d.max_pos, &t));
+  tg::PagedAppendParams p{};
+  p.k = static_cast<const float*>(dk);
+  p.v = static_cast<const float*>(dv);
+  p.q = static_cast<const float*>(dq);
+  p.q_out = static_cast<float*>(dqo);
+  p.cu = static_cast<const int*>(dcu);
+  p.pos0 = static_cast<const int*>(dp);
+  p.table = static_cast<const int*>(dt);
+  p.cs = t->d;
+  p.table_len = d.max_pos;
+  p.kp = pk->k + (size_t)layer * pk->layer_elems * pk->esize;
+  p.vp = pk->v + (size_t)layer * pk->layer_elems * pk->esize;
+  p.bounds = pk->bounds ? pk->bounds + (size_t)layer * pk->bounds_elems * pk->esize : nullptr;
+  p.err = ctx->d_err;
+  p.n_seqs = n_seqs;
+  p.n_tokens = n_tokens;
+  p.max_blocks = max_blocks;
+  p.n_pages = d.n_pages;
+  p.log2p = pk->log2p;
+  p.n_head = d.n_head;
+  p.n_kv = d.n_kv_head;
+  p.hd = d.head_dim;
+  p.dtype = d.dtype;
+  p.vec4 = vec4 ? 1 : 0;
+  cudaError_t e = tg::launch_paged_append(p, ctx->stream);
+  if (e != cudaSuccess) return fail(TG_ERR_CUDA, "paged append launch: %s", cudaGetErrorString(e));
+  ctx->launches++;
+  return finish_call(ctx);
+}
+
+namespace {
+int paged_attention(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, const float* q,
+                    const int32_t* past_len, const int32_t* block_table, int max_blocks,
+                    int shared_len, int n_sel, const int32_t* pages, float* out) {
+  TG_TRY(check_paged_call(ctx, pk, layer, n_seqs, max_blocks));
+  if (n_seqs == 0) return TG_OK;
+  if (!q || !past_len || !block_table || !out) return fail(TG_ERR_INVALID_ARG, "null argument");
+  TG_TRY(check_host_pages(pk, past_len, block_table, n_seqs, max_blocks));
+  const tg_paged_desc& d = pk->d;
+  const size_t qb = (size_t)n_seqs * d.n_head * d.head_dim * 4;
+  const void *dq = nullptr, *dp = nullptr, *dt = nullptr, *dsel = nullptr;
+  void* dout = nullptr;
+  TG_TRY(stage_in(ctx, q, qb, &dq));
+  TG_TRY(stage_in(ctx, past_len, (size_t)n_seqs * 4, &dp));
+  TG_TRY(stage_in(ctx, block_table, (size_t)n_seqs * max_blocks * 4, &dt));
+  if (pages) TG_TRY(stage_in(ctx, pages, (size_t)n_seqs * d.n_kv_head * n_sel * 4, &dsel));
+  TG_TRY(stage_out(ctx, out, qb, false, &dout));
+  (void)shared_len;
+  TG_TRY(run_paged(ctx, pk, layer, n_seqs, static_cast<const float*>(dq),
+                   static_cast<const int*>(dp), static_cast<const int*>(dt), max_blocks,
+                   static_cast<const int*>(dsel), n_sel, static_cast<float*>(dout)));
+  return finish_call(ctx);
+}
+}  // namespace
+
+int tg_paged_attention(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, const float* q,
+                       const int32_t* past_len, const int32_t* block_table, int max_blocks,
+                       float* out) {
+  return paged_attention(ctx, pk, layer, n_seqs, q, past_len, block_table, max_blocks, 0, 0,
+                         nullptr, out);
+}
+
+int tg_paged_attention_shared(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs,
+                              const float* q, const int32_t* past_len,
+                              const int32_t* block_table, int max_blocks, int shared_len,
+                              float* out) {
+  TG_TRY(check_paged_call(ctx, pk, layer, n_seqs, max_blocks));
+  if (shared_len < 0 || shared_len > (long long)max_blocks << pk->log2p)
+    return fail(TG_ERR_INVALID_ARG, "shared_len %d outside [0, %lld]", shared_len,
+                (long long)max_blocks << pk->log2p);
+  return paged_attention(ctx, pk, layer, n_seqs, q, past_len, block_table, max_blocks, shared_len,
+                         0, nullptr, out);
+}
+
+int tg_paged_select(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, const float* q,
+                    const int32_t* past_len, const int32_t* block_table, int max_blocks,
+                    int keep_first, int keep_last, int n_sel, int32_t* pages) {
+  TG_TRY(check_paged_call(ctx, pk, layer, n_seqs, max_blocks));
+  if (!pk->bounds) return fail(TG_ERR_UNSUPPORTED, "the cache keeps no bounds (with_bounds)");
+  if (n_sel < 1 || keep_first < 0 || keep_last < 0)
+    return fail(TG_ERR_INVALID_ARG, "n_sel %d, keep_first %d, keep_last %d", n_sel, keep_first,
+                keep_last);
+  if (n_seqs == 0) return TG_OK;
+  if (!q || !past_len || !block_table || !pages) return fail(TG_ERR_INVALID_ARG, "null argument");
+  TG_TRY(check_host_pages(pk, past_len, block_table, n_seqs, max_blocks));
+  const tg_paged_desc& d = pk->d;
+  const int qrow = d.n_head * d.head_dim;
+  const void *dq = nullptr, *dp = nullptr, *dt = nullptr;
+  void* dpg = nullptr;
+  TG_TRY(stage_in(ctx, q, (size_t)n_seqs * qrow * 4, &dq));
+  TG_TRY(stage_in(ctx, past_len, (size_t)n_seqs * 4, &dp));
+  TG_TRY(stage_in(ctx, block_table, (size_t)n_seqs * max_blocks * 4, &dt));
+  TG_TRY(stage_out(ctx, pages, (size_t)n_seqs * d.n_kv_head * n_sel * 4, false, &dpg));
+  TG_TRY(commit_inputs(ctx));
+  // Queries per launch: at most 32M scores (256 MB) of scratch.
+  const long long per_query = (long long)d.n_kv_head * max_blocks;
+  const int step = (int)std::max(1LL, std::min((long long)tg::kPagedMaxQueries, (1LL << 25) / per_query));
+  TG_TRY(ensure_kept(ctx, &ctx->pkeys, &ctx->pkeys_cap,
+                     (size_t)std::min(step, n_seqs) * per_query));
+  tg::PagedSelectParams p{};
+  p.bounds = pk->bounds + (size_t)layer * pk->bounds_elems * pk->esize;
+  p.keys = ctx->pkeys;
+  p.err = ctx->d_err;
+  p.n_head = d.n_head;
+  p.n_kv = d.n_kv_head;
+  p.group = d.n_head / d.n_kv_head;
+  p.hd = d.head_dim;
+  p.dtype = d.dtype;
+  p.max_blocks = max_blocks;
+  p.n_pages = d.n_pages;
+  p.log2p = pk->log2p;
+  p.n_sel = n_sel;
+  p.keep_first = keep_first;
+  p.keep_last = keep_last;
+  for (int s0 = 0; s0 < n_seqs; s0 += step) {
+    p.n = std::min(step, n_seqs - s0);
+    p.q = static_cast<const float*>(dq) + (size_t)s0 * qrow;
+    p.past = static_cast<const int*>(dp) + s0;
+    p.table = static_cast<const int*>(dt) + (size_t)s0 * max_blocks;
+    p.pages = static_cast<int*>(dpg) + (size_t)s0 * d.n_kv_head * n_sel;
+    cudaError_t e = tg::launch_paged_select(p, ctx->stream);
+    if (e != cudaSuccess)
+      return fail(TG_ERR_CUDA, "paged select launch: %s", cudaGetErrorString(e));
+    ctx->launches += 2;
+  }
+  return finish_call(ctx);
+}
+
+int tg_paged_attention_sparse(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs,
+                              const float* q, const int32_t* past_len,
+                              const int32_t* block_table, int max_blocks, int n_sel,
+                              const int32_t* pages, float* out) {
+  TG_TRY(check_paged_call(ctx, pk, layer, n_seqs, max_blocks));
+  if (n_sel < 1 || !pages) return fail(TG_ERR_INVALID_ARG, "n_sel %d or null pages", n_sel);
+  return paged_attention(ctx, pk, layer, n_seqs, q, past_len, block_table, max_blocks, 0, n_sel,
+                         pages, out);
 }
 
 // ------------------------------------------------ introspection

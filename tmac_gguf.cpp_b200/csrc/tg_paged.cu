@@ -1,0 +1,815 @@
+// tg_paged.cu -- kernels over a paged KV cache: keys and values appended with
+// the position rotation applied on the way, decode attention through a block
+// table (dense, or over listed pages), and the selection of pages by a bound
+// on their scores.
+//
+// The reference keeps one contiguous [pos][n_kv*head_dim] cache per layer
+// (g_k_cache / g_v_cache, tmac_gguf.cpp:200-201) and has no counterpart of
+// any of these; the rotation is its apply_rope (tmac_gguf.cpp:990-1016) and
+// the attention its GQA block (tmac_gguf.cpp:1093-1128).
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <mutex>
+#include <utility>
+
+#include "tg_device.cuh"
+#include "tg_paged.h"
+#include "tg_shared.h"
+
+namespace tg {
+
+namespace {
+
+template <typename... KArgs, typename... Args>
+cudaError_t launch_chained(void (*fn)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                           cudaStream_t st, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fn, std::forward<Args>(args)...);
+}
+
+// Raises a kernel's dynamic shared-memory limit to the most a CTA can have,
+// once per device.
+template <typename F>
+cudaError_t allow_max_smem(F* fn, bool* done) {
+  static std::mutex mu;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  std::lock_guard<std::mutex> lock(mu);
+  if (done[dev]) return cudaSuccess;
+  cudaError_t e =
+      cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  if (e == cudaSuccess) done[dev] = true;
+  return e;
+}
+
+}  // namespace
+
+// ------------------------------------------------------------ append
+
+// U consecutive elements of a row (2 or 4: one or two rotation pairs).
+template <int U>
+struct Unit {
+  float x[U];
+};
+
+template <int U>
+__device__ __forceinline__ Unit<U> load_unit(const float* p) {
+  Unit<U> r;
+  if constexpr (U == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    r.x[0] = a.x; r.x[1] = a.y; r.x[2] = a.z; r.x[3] = a.w;
+  } else {
+    const float2 a = *reinterpret_cast<const float2*>(p);
+    r.x[0] = a.x; r.x[1] = a.y;
+  }
+  return r;
+}
+
+template <int U>
+__device__ __forceinline__ Unit<U> load_unit(const __nv_bfloat16* p) {
+  Unit<U> r;
+#pragma unroll
+  for (int i = 0; i < U; i += 2) {
+    const __nv_bfloat162 b = *reinterpret_cast<const __nv_bfloat162*>(p + i);
+    r.x[i] = __low2float(b);
+    r.x[i + 1] = __high2float(b);
+  }
+  return r;
+}
+
+template <int U>
+__device__ __forceinline__ void store_unit(float* p, const Unit<U>& r) {
+  if constexpr (U == 4)
+    *reinterpret_cast<float4*>(p) = make_float4(r.x[0], r.x[1], r.x[2], r.x[3]);
+  else
+    *reinterpret_cast<float2*>(p) = make_float2(r.x[0], r.x[1]);
+}
+
+template <int U>
+__device__ __forceinline__ void store_unit(__nv_bfloat16* p, const Unit<U>& r) {
+  if constexpr (U == 4) {
+    *reinterpret_cast<uint2*>(p) =
+        make_uint2(pack_bf16x2(r.x[0], r.x[1]), pack_bf16x2(r.x[2], r.x[3]));
+  } else {
+    *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(r.x[0], r.x[1]);
+  }
+}
+
+// x0*c - x1*s, x0*s + x1*c with one rounding per product and sum
+// (tmac_gguf.cpp:999-1000 without contraction).
+template <int U>
+__device__ __forceinline__ Unit<U> rotate_unit(const Unit<U>& v, const Unit<U>& cs) {
+  Unit<U> r;
+#pragma unroll
+  for (int i = 0; i < U; i += 2) {
+    r.x[i] = __fsub_rn(__fmul_rn(v.x[i], cs.x[i]), __fmul_rn(v.x[i + 1], cs.x[i + 1]));
+    r.x[i + 1] = __fadd_rn(__fmul_rn(v.x[i], cs.x[i + 1]), __fmul_rn(v.x[i + 1], cs.x[i]));
+  }
+  return r;
+}
+
+// The value as the pool holds it (fp32, or rounded to nearest even bf16).
+template <typename T>
+__device__ __forceinline__ float as_stored(float v) {
+  if constexpr (sizeof(T) == 2) return __bfloat162float(__float2bfloat16_rn(v));
+  return v;
+}
+
+constexpr int kAppendWarps = 8;
+constexpr int kAppendBatch = 8;  // loads a lane has in flight
+
+// One warp per token: its q row rotated, its k row rotated and written with
+// its v row to the page of its position.  The warp of the first new token of
+// a page also writes the page's bounds: min and max over the page's rows up
+// to the last one of this call, the earlier rows from the pool and the new
+// ones rotated again from k (the few extra reads come from L2), so that no
+// warp waits for another and the bounds are the same however the rows were
+// cut into calls.
+template <typename T, int U>
+__global__ void __launch_bounds__(32 * kAppendWarps) paged_append_kernel(const PagedAppendParams p) {
+  __shared__ int seq_of[kAppendWarps];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t0 = blockIdx.x * kAppendWarps, t = t0 + warp;
+  int s = -1;
+  if (p.cu) {
+    // The sequences of this CTA's tokens: every thread looks at some of the
+    // sequences (one round of loads; a search would be a chain of them).
+    if (threadIdx.x < kAppendWarps) seq_of[threadIdx.x] = -1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.n_seqs; i += 32 * kAppendWarps) {
+      const int lo = max(p.cu[i], t0), hi = min(p.cu[i + 1], t0 + kAppendWarps);
+      for (int x = lo; x < hi; ++x) seq_of[x - t0] = i;
+    }
+    __syncthreads();
+    s = seq_of[warp];
+  } else if (t < p.n_seqs) {
+    s = t;
+  }
+  if (t >= p.n_tokens || s < 0) return;  // padding tokens stay as they are
+  const int first = p.cu ? p.cu[s] : t, last = p.cu ? min(p.cu[s + 1], p.n_tokens) : t + 1;
+  const int P = 1 << p.log2p, hd = p.hd;
+  const long long pos_ll = (long long)p.pos0[s] + (t - first);
+  if (p.pos0[s] < 0 || pos_ll >= p.table_len || (pos_ll >> p.log2p) >= p.max_blocks) {
+    if (lane == 0) record_error(p.err, kDevErrBadPos);
+    return;
+  }
+  const int pos = (int)pos_ll, slot = pos & (P - 1);
+  const int page = p.table[(size_t)s * p.max_blocks + (pos >> p.log2p)];
+  if (page < 0 || page >= p.n_pages) {
+    if (lane == 0) record_error(p.err, kDevErrBadPage);
+    return;
+  }
+  const float* cs = p.cs + (size_t)pos * hd;
+  if (p.q) {
+    const int nq = p.n_head * hd;
+    const float* q = p.q + (size_t)t * nq;
+    float* qo = p.q_out + (size_t)t * nq;
+    for (int i0 = lane * U; i0 < nq; i0 += kAppendBatch * 32 * U) {
+      Unit<U> x[kAppendBatch];
+#pragma unroll
+      for (int u = 0; u < kAppendBatch; ++u) {
+        const int i = i0 + u * 32 * U;
+        if (i < nq) x[u] = load_unit<U>(q + i);
+      }
+#pragma unroll
+      for (int u = 0; u < kAppendBatch; ++u) {
+        const int i = i0 + u * 32 * U;
+        if (i < nq) store_unit<U>(qo + i, rotate_unit<U>(x[u], load_unit<U>(cs + i % hd)));
+      }
+    }
+  }
+  const int row = p.n_kv * hd;
+  const float* k = p.k + (size_t)t * row;
+  const float* v = p.v + (size_t)t * row;
+  T* kp = static_cast<T*>(p.kp);
+  T* vp = static_cast<T*>(p.vp);
+  const size_t base = (size_t)page * p.n_kv;
+  for (int i = lane * U; i < row; i += 32 * U) {
+    const int g = i / hd, d = i - g * hd;
+    const Unit<U> xk = load_unit<U>(k + i), xv = load_unit<U>(v + i), c = load_unit<U>(cs + d);
+    const size_t at = (((base + g) << p.log2p) + slot) * hd + d;
+    store_unit<U>(kp + at, rotate_unit<U>(xk, c));
+    store_unit<U>(vp + at, xv);
+  }
+  if (!p.bounds || (t != first && slot != 0)) return;
+  // Rows [0, slot) of the page from the pool, [slot, end) from k.
+  const int end = min(min(P, slot + (last - t)), slot + (p.table_len - pos));
+  T* bounds = static_cast<T*>(p.bounds);
+  for (int i = lane * U; i < row; i += 32 * U) {
+    const int g = i / hd, d = i - g * hd;
+    Unit<U> lo, hi;
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      lo.x[e] = INFINITY;
+      hi.x[e] = -INFINITY;
+    }
+    const T* old = kp + ((base + g) << p.log2p) * hd + d;
+#pragma unroll 8
+    for (int r = 0; r < slot; ++r) {
+      const Unit<U> x = load_unit<U>(old + (size_t)r * hd);
+#pragma unroll
+      for (int e = 0; e < U; ++e) {
+        lo.x[e] = fminf(lo.x[e], x.x[e]);
+        hi.x[e] = fmaxf(hi.x[e], x.x[e]);
+      }
+    }
+#pragma unroll 4
+    for (int r = slot; r < end; ++r) {
+      const Unit<U> x = rotate_unit<U>(load_unit<U>(k + (size_t)(r - slot) * row + i),
+                                       load_unit<U>(cs + (size_t)(r - slot) * hd + d));
+#pragma unroll
+      for (int e = 0; e < U; ++e) {
+        const float y = as_stored<T>(x.x[e]);
+        lo.x[e] = fminf(lo.x[e], y);
+        hi.x[e] = fmaxf(hi.x[e], y);
+      }
+    }
+    store_unit<U>(bounds + (base + g) * 2 * hd + d, lo);
+    store_unit<U>(bounds + ((base + g) * 2 + 1) * hd + d, hi);
+  }
+}
+
+cudaError_t launch_paged_append(const PagedAppendParams& p, cudaStream_t st) {
+  const dim3 grid((unsigned)((p.n_tokens + kAppendWarps - 1) / kAppendWarps)), block(32 * kAppendWarps);
+  if (p.dtype == 1)
+    return p.vec4 ? launch_chained(paged_append_kernel<__nv_bfloat16, 4>, grid, block, 0, st, p)
+                  : launch_chained(paged_append_kernel<__nv_bfloat16, 2>, grid, block, 0, st, p);
+  return p.vec4 ? launch_chained(paged_append_kernel<float, 4>, grid, block, 0, st, p)
+                : launch_chained(paged_append_kernel<float, 2>, grid, block, 0, st, p);
+}
+
+// ------------------------------------------------------------ the schedule
+
+// Pages that query i attends (before listing); a position outside the table
+// counts as none and is reported.
+__device__ __forceinline__ int query_blocks(const PagedAttnParams& p, int past, bool report) {
+  if (past < 0) {
+    if (past < -1 && report) record_error(p.err, kDevErrBadPos);
+    return 0;
+  }
+  const int nb = (past >> p.log2p) + 1;
+  if (nb > p.max_blocks) {
+    if (report) record_error(p.err, kDevErrBadPos);
+    return 0;
+  }
+  return nb;
+}
+
+__device__ __forceinline__ int query_chunks(const PagedAttnParams& p, int nb) {
+  const int list = p.sel ? min(p.n_sel, nb) : max(0, nb - p.skip);
+  return (int)((((long long)list << p.log2p) + kPagedChunk - 1) / kPagedChunk);
+}
+
+// Chunk prefix over the queries (per stream of a query) and their last
+// positions in shared memory; every thread of the CTA takes part.
+__device__ void paged_schedule(const PagedAttnParams& p, int* prefix, int* past_s, int* warp_tot) {
+  const int NT = blockDim.x, t = threadIdx.x, lane = t & 31, w = t >> 5;
+  const int per = (p.n + NT - 1) / NT;
+  const int b0 = min(t * per, p.n), b1 = min(b0 + per, p.n);
+  int sum = 0;
+  for (int s = b0; s < b1; ++s) {
+    const int past = p.past[s];
+    const int nb = query_blocks(p, past, blockIdx.x == 0);
+    past_s[s] = nb > 0 ? past : -1;
+    const int c = query_chunks(p, nb);
+    prefix[s + 1] = c;
+    sum += c;
+  }
+  int incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) warp_tot[w] = incl;
+  __syncthreads();
+  int off = 0;
+  for (int i = 0; i < w; ++i) off += warp_tot[i];
+  int run = off + incl - sum;
+  if (t == 0) prefix[0] = 0;
+  for (int s = b0; s < b1; ++s) {
+    run += prefix[s + 1];
+    prefix[s + 1] = run;
+  }
+  __syncthreads();
+}
+
+// Query that owns flat chunk t when every query has `streams` streams: the
+// last s with prefix[s] * streams <= t and a non-empty share.
+__device__ __forceinline__ int query_of(const int* prefix, int n, int streams, long long t) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((long long)prefix[mid] * streams <= t) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// CTAs that take part: enough that each has a chunk for each of its warps.
+__device__ __forceinline__ int paged_active(int grid, long long T, int warps) {
+  const long long g = (T + warps - 1) / warps;
+  return (int)min((long long)grid, g);
+}
+
+// ------------------------------------------------------------ segment results
+
+// One stream segment's result as the CTA's threads produce it: dst is the
+// output row, the record, or a partial record slot.
+struct SegmentOut {
+  float* o;        // element (h, d) at o[h*stride + d]
+  float* m;        // or null (normalised output)
+  float* l;
+  size_t stride, ml_stride;
+};
+
+__device__ __forceinline__ SegmentOut segment_out(const PagedAttnParams& p, int s, int g, int hb) {
+  const int h0 = g * p.group + hb * kPagedHeads;
+  SegmentOut r;
+  if (p.mode == 0) {
+    r.o = p.out + ((size_t)s * p.n_head + h0) * p.hd;
+    r.stride = p.hd;
+    r.m = r.l = nullptr;
+    r.ml_stride = 0;
+  } else {
+    r.o = p.records + ((size_t)s * p.n_head + h0) * (p.hd + 2);
+    r.stride = r.ml_stride = p.hd + 2;
+    r.m = r.o + p.hd;
+    r.l = r.m + 1;
+  }
+  return r;
+}
+
+__device__ __forceinline__ SegmentOut part_out(const PagedAttnParams& p, int slot) {
+  SegmentOut r;
+  r.o = p.part + (size_t)slot * kPagedHeads * (p.hd + 2);
+  r.stride = p.hd;
+  r.m = r.o + kPagedHeads * p.hd;
+  r.l = r.m + kPagedHeads;
+  r.ml_stride = 1;
+  return r;
+}
+
+// Streams without a row: zeros, or neutral records.
+__device__ void write_empty(const PagedAttnParams& p, const int* prefix) {
+  const int per = p.n_head * p.hd;
+  for (int s = blockIdx.x; s < p.n; s += gridDim.x) {
+    if (prefix[s + 1] != prefix[s]) continue;
+    if (p.mode == 0) {
+      for (int e = threadIdx.x; e < per; e += blockDim.x) p.out[(size_t)s * per + e] = 0.f;
+    } else {
+      for (int e = threadIdx.x; e < p.n_head * (p.hd + 2); e += blockDim.x)
+        p.records[(size_t)s * p.n_head * (p.hd + 2) + e] = (e % (p.hd + 2)) == p.hd ? kNegBig : 0.f;
+    }
+  }
+}
+
+// The last CTA to leave its part of a split stream merges all parts.  Parts
+// lie in slot order c1 (its last segment, or its first if the stream starts
+// there), then the first segments of c1 + 1 .. c2.
+__device__ void merge_parts(const PagedAttnParams& p, const SegmentOut& dst, int heads,
+                            int first_slot, int c1, int n_parts, int tid, int nthreads) {
+  constexpr int B = 8;
+  const int hd = p.hd;
+  for (int e = tid; e < heads * hd; e += nthreads) {
+    const int h = e / hd, d = e - h * hd;
+    float M = kNegBig, L = 0.f, O = 0.f;
+    for (int k0 = 0; k0 < n_parts; k0 += B) {
+      float m[B], l[B], o[B];
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        const int k = k0 + u;
+        m[u] = kNegBig;
+        l[u] = o[u] = 0.f;
+        if (k < n_parts) {
+          const SegmentOut a = part_out(p, k == 0 ? first_slot : 2 * (c1 + k));
+          m[u] = __ldcg(a.m + h);
+          l[u] = __ldcg(a.l + h);
+          o[u] = __ldcg(a.o + e);
+        }
+      }
+      float mb = M;
+#pragma unroll
+      for (int u = 0; u < B; ++u) mb = fmaxf(mb, m[u]);
+      const float w0 = ex2(M - mb);
+      M = mb;
+      L *= w0;
+      O *= w0;
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        const float w = ex2(m[u] - M);
+        L = fmaf(l[u], w, L);
+        O = fmaf(o[u], w, O);
+      }
+    }
+    if (dst.m) {
+      dst.o[h * dst.stride + d] = O;
+      if (d == 0) {
+        dst.m[h * dst.ml_stride] = M;
+        dst.l[h * dst.ml_stride] = L;
+      }
+    } else {
+      dst.o[h * dst.stride + d] = L > 0.f ? O / L : (L == 0.f ? 0.f : L);
+    }
+  }
+}
+
+// ------------------------------------------------------------ CUDA-core attention
+
+constexpr int kCoreWarps = 8;
+constexpr int kCoreThreads = 32 * kCoreWarps;
+
+size_t paged_core_smem(int n, int hd) {
+  const size_t floats = (size_t)kPagedHeads * hd                          // q
+                        + (size_t)kCoreWarps * kPagedHeads * kPagedChunk    // probabilities
+                        + (size_t)kCoreWarps * kPagedHeads * (hd + 2);      // warp results
+  return floats * 4 + (size_t)(2 * n + 1 + kCoreWarps + 4) * 4;
+}
+
+template <typename T>
+__device__ __forceinline__ float2 load_pair(const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    return *reinterpret_cast<const float2*>(p);
+  } else {
+    const __nv_bfloat162 b = *reinterpret_cast<const __nv_bfloat162*>(p);
+    return make_float2(__low2float(b), __high2float(b));
+  }
+}
+
+// Any head_dim (even, at most 128), type and group: one warp per chunk of 32
+// rows, lane r forming the scores of row r, then lane i the dimension pairs
+// i, i + 32 of P.V.  All sums in binary32.
+template <typename T>
+__global__ void __launch_bounds__(kCoreThreads) paged_core_kernel(const PagedAttnParams p) {
+  extern __shared__ float sm[];
+  const int hd = p.hd, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  float* q_s = sm;
+  float* p_s = q_s + kPagedHeads * hd + warp * kPagedHeads * kPagedChunk;
+  float* res = sm + kPagedHeads * hd + kCoreWarps * kPagedHeads * kPagedChunk;
+  int* prefix = reinterpret_cast<int*>(res + kCoreWarps * kPagedHeads * (hd + 2));
+  int* past_s = prefix + p.n + 1;
+  int* warp_tot = past_s + p.n;
+  int* flag = warp_tot + kCoreWarps;
+  float* my_res = res + warp * kPagedHeads * (hd + 2);
+
+  griddep_launch_dependents();
+  griddep_wait();
+  paged_schedule(p, prefix, past_s, warp_tot);
+  const int streams = p.n_kv * p.hblocks;
+  const long long T_all = (long long)prefix[p.n] * streams;
+  write_empty(p, prefix);
+  const int G = paged_active(gridDim.x, T_all, kCoreWarps), cta = blockIdx.x;
+  if (cta >= G) return;
+  const long long t_lo = cta_tile_lo(cta, G, T_all), t_hi = cta_tile_lo(cta + 1, G, T_all);
+  const T* kp = static_cast<const T*>(p.kp);
+  const T* vp = static_cast<const T*>(p.vp);
+  const int P = 1 << p.log2p;
+
+  int s = query_of(prefix, p.n, streams, t_lo);
+  for (long long t = t_lo; t < t_hi;) {
+    while ((long long)prefix[s + 1] * streams <= t) ++s;
+    const int C = prefix[s + 1] - prefix[s];
+    const long long q_base = (long long)prefix[s] * streams;
+    const int u = (int)((t - q_base) / C);
+    const long long s_lo = q_base + (long long)u * C, s_hi = s_lo + C;
+    const long long e_hi = min(t_hi, s_hi);
+    const int g = u / p.hblocks, hb = u - g * p.hblocks;
+    const int heads = min(kPagedHeads, p.group - hb * kPagedHeads);
+    const int past = past_s[s];
+    const int nb = (past >> p.log2p) + 1;
+    const int list = p.sel ? min(p.n_sel, nb) : nb - p.skip;
+    const int* sel = p.sel ? p.sel + ((size_t)s * p.n_kv + g) * p.n_sel : nullptr;
+    const int* table = p.table + (size_t)s * p.max_blocks;
+
+    __syncthreads();
+    const float* q = p.q + ((size_t)s * p.n_head + g * p.group + hb * kPagedHeads) * hd;
+    for (int e = tid; e < kPagedHeads * hd; e += kCoreThreads)
+      q_s[e] = e < heads * hd ? q[e] * p.scale_log2 : 0.f;
+    __syncthreads();
+
+    float m[kPagedHeads], l[kPagedHeads];
+    float2 o[kPagedHeads][2];
+#pragma unroll
+    for (int h = 0; h < kPagedHeads; ++h) {
+      m[h] = kNegBig;
+      l[h] = 0.f;
+      o[h][0] = o[h][1] = make_float2(0.f, 0.f);
+    }
+    for (long long c = t + warp; c < e_hi; c += kCoreWarps) {
+      const int r = (int)(c - s_lo) * kPagedChunk + lane;
+      const int i = r >> p.log2p, slot = r & (P - 1);
+      bool ok = i < list;
+      size_t row = 0;
+      if (ok) {
+        const int j = sel ? sel[i] : p.skip + i;
+        ok = j >= 0 && j < nb && (long long)j * P + slot <= past;
+        if (ok) {
+          const int page = table[j];
+          if (page < 0 || page >= p.n_pages) {
+            record_error(p.err, kDevErrBadPage);
+            ok = false;
+          } else {
+            row = ((((size_t)page * p.n_kv + g) << p.log2p) + slot) * hd;
+          }
+        }
+      }
+      float sc[kPagedHeads];
+#pragma unroll
+      for (int h = 0; h < kPagedHeads; ++h) sc[h] = 0.f;
+      if (ok) {
+#pragma unroll 4
+        for (int d = 0; d < hd; d += 2) {
+          const float2 x = load_pair(kp + row + d);
+#pragma unroll
+          for (int h = 0; h < kPagedHeads; ++h) {
+            const float2 y = *reinterpret_cast<const float2*>(q_s + h * hd + d);
+            sc[h] = fmaf(y.x, x.x, fmaf(y.y, x.y, sc[h]));
+          }
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int h = 0; h < kPagedHeads; ++h) {
+        const float x = ok ? sc[h] : -INFINITY;
+        const float mn = fmaxf(m[h], warp_max(x));
+        const float a = ex2(m[h] - mn), e = ex2(x - mn);
+        m[h] = mn;
+        l[h] = l[h] * a + e;
+        o[h][0].x *= a; o[h][0].y *= a; o[h][1].x *= a; o[h][1].y *= a;
+        p_s[h * kPagedChunk + lane] = e;
+      }
+      __syncwarp();
+      const unsigned live = __ballot_sync(0xffffffffu, ok);
+#pragma unroll 4
+      for (int rr = 0; rr < kPagedChunk; ++rr) {
+        const size_t at = __shfl_sync(0xffffffffu, (unsigned long long)row, rr);
+        if (!((live >> rr) & 1)) continue;
+#pragma unroll
+        for (int c2 = 0; c2 < 2; ++c2) {
+          const int d = 2 * lane + 64 * c2;
+          if (d >= hd) continue;
+          const float2 x = load_pair(vp + at + d);
+#pragma unroll
+          for (int h = 0; h < kPagedHeads; ++h) {
+            const float w = p_s[h * kPagedChunk + rr];
+            o[h][c2].x = fmaf(w, x.x, o[h][c2].x);
+            o[h][c2].y = fmaf(w, x.y, o[h][c2].y);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < kPagedHeads; ++h) {
+      const float lt = warp_sum(l[h]);
+#pragma unroll
+      for (int c2 = 0; c2 < 2; ++c2) {
+        const int d = 2 * lane + 64 * c2;
+        if (d < hd) *reinterpret_cast<float2*>(my_res + h * hd + d) = o[h][c2];
+      }
+      if (lane == 0) {
+        my_res[kPagedHeads * hd + h] = m[h];
+        my_res[kPagedHeads * (hd + 1) + h] = lt;
+      }
+    }
+    __syncthreads();
+    // Segment result over the warps.
+    const bool complete = t == s_lo && e_hi == s_hi;
+    const bool at_start = t == t_lo;
+    const SegmentOut fin = segment_out(p, s, g, hb);
+    const SegmentOut dst = complete ? fin : part_out(p, 2 * cta + (at_start ? 0 : 1));
+    for (int e = tid; e < heads * hd; e += kCoreThreads) {
+      const int h = e / hd, d = e - h * hd;
+      float M = kNegBig;
+#pragma unroll
+      for (int w = 0; w < kCoreWarps; ++w)
+        M = fmaxf(M, res[w * kPagedHeads * (hd + 2) + kPagedHeads * hd + h]);
+      float L = 0.f, O = 0.f;
+#pragma unroll
+      for (int w = 0; w < kCoreWarps; ++w) {
+        const float* rw = res + w * kPagedHeads * (hd + 2);
+        const float f = ex2(rw[kPagedHeads * hd + h] - M);
+        L = fmaf(rw[kPagedHeads * (hd + 1) + h], f, L);
+        O = fmaf(rw[e], f, O);
+      }
+      if (dst.m) {
+        dst.o[h * dst.stride + d] = O;
+        if (d == 0) {
+          dst.m[h * dst.ml_stride] = M;
+          dst.l[h * dst.ml_stride] = L;
+        }
+      } else {
+        dst.o[h * dst.stride + d] = L > 0.f ? O / L : (L == 0.f ? 0.f : L);
+      }
+    }
+    if (!complete) {
+      const int c1 = cta_of_tile(s_lo, G, T_all), c2 = cta_of_tile(s_hi - 1, G, T_all);
+      unsigned* count = p.count + (size_t)s * streams + u;
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) *flag = atomicAdd(count, 1u) == (unsigned)(c2 - c1);
+      __syncthreads();
+      if (*flag) {
+        __threadfence();
+        merge_parts(p, fin, heads, 2 * c1 + (cta_tile_lo(c1, G, T_all) == s_lo ? 0 : 1), c1,
+                    c2 - c1 + 1, tid, kCoreThreads);
+        if (tid == 0) *count = 0;
+      }
+    }
+    t = e_hi;
+  }
+}
+
+cudaError_t launch_paged_core(const PagedAttnParams& p, int dtype, int grid, cudaStream_t st) {
+  static bool done_f32[64] = {}, done_bf16[64] = {};
+  const size_t smem = paged_core_smem(p.n, p.hd);
+  if (dtype == 1) {
+    cudaError_t e = allow_max_smem(paged_core_kernel<__nv_bfloat16>, done_bf16);
+    if (e != cudaSuccess) return e;
+    return launch_chained(paged_core_kernel<__nv_bfloat16>, dim3(grid), dim3(kCoreThreads), smem, st, p);
+  }
+  cudaError_t e = allow_max_smem(paged_core_kernel<float>, done_f32);
+  if (e != cudaSuccess) return e;
+  return launch_chained(paged_core_kernel<float>, dim3(grid), dim3(kCoreThreads), smem, st, p);
+}
+
+// ------------------------------------------------------------ page selection
+
+constexpr unsigned long long kKeyForced = ~0ull;  // pages that are always taken
+
+// Unsigned integers in the order of the doubles; NaN below everything.
+__device__ __forceinline__ unsigned long long ordered_key(double v) {
+  v += 0.0;  // -0 and +0 are equal
+  const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+  if (v != v) return 0ull;
+  return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
+}
+
+constexpr int kScoreThreads = 128;
+constexpr int kScoreLanes = 4;  // lanes per page
+constexpr int kScorePages = kScoreThreads / kScoreLanes;
+
+// Score of a page for one KV head: the largest, over the head's query group,
+// of sum_d max(q_d lo_d, q_d hi_d), an upper bound of q . k for every key of
+// the page.  Sums in binary64: which of two pages is taken must not hang on
+// the order of a sum's roundings (products of a 24-bit q and a bf16 or fp32
+// bound are exact there).  Four lanes per page, each a quarter of the
+// dimension pairs.
+template <typename T>
+__global__ void __launch_bounds__(kScoreThreads) paged_score_kernel(const PagedSelectParams p) {
+  extern __shared__ double q_d[];  // [group][hd]
+  griddep_launch_dependents();
+  griddep_wait();
+  const int s = blockIdx.x / p.n_kv, g = blockIdx.x - s * p.n_kv;
+  const int past = p.past[s];
+  const int nb = past < 0 ? 0 : (past >> p.log2p) + 1;
+  if (past < -1 || nb > p.max_blocks) {
+    if (blockIdx.y == 0 && threadIdx.x == 0) record_error(p.err, kDevErrBadPos);
+    return;
+  }
+  if ((int)blockIdx.y * kScorePages >= nb) return;
+  const int hd = p.hd;
+  const float* q = p.q + ((size_t)s * p.n_head + g * p.group) * hd;
+  for (int e = threadIdx.x; e < p.group * hd; e += kScoreThreads) q_d[e] = (double)q[e];
+  __syncthreads();
+  const int j = blockIdx.y * kScorePages + threadIdx.x / kScoreLanes;
+  const int part = threadIdx.x % kScoreLanes;
+  const bool live = j < nb;
+  int page = live ? p.table[(size_t)s * p.max_blocks + j] : 0;
+  const bool bad = page < 0 || page >= p.n_pages;
+  if (bad) {
+    if (part == 0) record_error(p.err, kDevErrBadPage);
+    page = 0;
+  }
+  const T* lo = static_cast<const T*>(p.bounds) + ((size_t)page * p.n_kv + g) * 2 * hd;
+  const T* hi = lo + hd;
+  double best = -INFINITY;
+  bool nan = false;
+  for (int h = 0; h < p.group; ++h) {
+    double sum = 0.0;
+    for (int d = 2 * part; d < hd; d += 2 * kScoreLanes) {
+      const float2 a = load_pair(lo + d), b = load_pair(hi + d);
+      const double q0 = q_d[h * hd + d], q1 = q_d[h * hd + d + 1];
+      sum = fma(q0, (double)(q0 >= 0.0 ? b.x : a.x), sum);
+      sum = fma(q1, (double)(q1 >= 0.0 ? b.y : a.y), sum);
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    nan |= sum != sum;
+    best = fmax(best, sum);
+  }
+  if (live && part == 0) {
+    unsigned long long key = (nan || bad) ? 0ull : ordered_key(best);
+    if (j < p.keep_first || j >= nb - p.keep_last) key = kKeyForced;
+    p.keys[((size_t)s * p.n_kv + g) * p.max_blocks + j] = key;
+  }
+}
+
+constexpr int kPickThreads = 512;
+
+// The n_sel largest keys of one (query, KV head), ties to the lowest index:
+// a radix search for the smallest key taken, 8 bits per pass, then the taken
+// indices in ascending order.
+__global__ void __launch_bounds__(kPickThreads) paged_pick_kernel(const PagedSelectParams p) {
+  __shared__ unsigned hist[256];
+  __shared__ unsigned wsum[kPickThreads / 32][2];
+  __shared__ unsigned long long sh_prefix;
+  __shared__ unsigned sh_need, sh_done;
+  griddep_launch_dependents();
+  griddep_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int row = blockIdx.x, s = row / p.n_kv;
+  const int past = p.past[s];
+  int nb = past < 0 ? 0 : (past >> p.log2p) + 1;
+  if (nb > p.max_blocks) nb = 0;
+  const unsigned long long* keys = p.keys + (size_t)row * p.max_blocks;
+  int* out = p.pages + (size_t)row * p.n_sel;
+  if (nb <= p.n_sel) {
+    for (int i = tid; i < p.n_sel; i += kPickThreads) out[i] = i < nb ? i : -1;
+    return;
+  }
+  unsigned long long prefix = 0, mask = 0;
+  unsigned need = (unsigned)p.n_sel;  // still to take among keys that match the prefix
+  bool exact = false;                 // every matching key is taken
+  for (int shift = 56; shift >= 0 && !exact; shift -= 8) {
+    for (int i = tid; i < 256; i += kPickThreads) hist[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < nb; i += kPickThreads) {
+      const unsigned long long k = keys[i];
+      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
+    }
+    __syncthreads();
+    if (tid == 0) {
+      unsigned left = need;
+      int b = 255;
+      while (b > 0 && hist[b] < left) left -= hist[b--];
+      sh_prefix = prefix | ((unsigned long long)b << shift);
+      sh_need = left;
+      sh_done = hist[b] == left;
+    }
+    __syncthreads();
+    prefix = sh_prefix;
+    need = sh_need;
+    exact = sh_done != 0;
+    mask |= 255ull << shift;
+    __syncthreads();
+  }
+  // Keys above the prefix are taken, of those that match it the first `need`.
+  unsigned taken = 0, ties = 0;
+  for (int i0 = 0; i0 < nb; i0 += kPickThreads) {
+    const int i = i0 + tid;
+    const unsigned long long k = i < nb ? keys[i] & mask : 0ull;
+    const bool tie = i < nb && k == prefix, above = i < nb && k > prefix;
+    const unsigned bt = __ballot_sync(0xffffffffu, tie), ba = __ballot_sync(0xffffffffu, above);
+    if (lane == 0) {
+      wsum[warp][0] = __popc(bt);
+      wsum[warp][1] = __popc(ba);
+    }
+    __syncthreads();
+    unsigned tie_at = ties, above_at = 0, tie_all = 0, above_all = 0;
+    for (int w = 0; w < kPickThreads / 32; ++w) {
+      if (w < warp) {
+        tie_at += wsum[w][0];
+        above_at += wsum[w][1];
+      }
+      tie_all += wsum[w][0];
+      above_all += wsum[w][1];
+    }
+    const unsigned below = (1u << lane) - 1u;
+    tie_at += __popc(bt & below);
+    above_at += __popc(ba & below);
+    // Slot: everything taken before this index.
+    const unsigned ties_before = min(tie_at, need) - min(ties, need);
+    const unsigned at = taken + above_at + ties_before;
+    if ((above || (tie && tie_at < need)) && at < (unsigned)p.n_sel) out[at] = i;
+    taken += above_all + min(ties + tie_all, need) - min(ties, need);
+    ties += tie_all;
+    __syncthreads();
+  }
+}
+
+cudaError_t launch_paged_select(const PagedSelectParams& p, cudaStream_t st) {
+  const dim3 grid((unsigned)(p.n * p.n_kv),
+                  (unsigned)((p.max_blocks + kScorePages - 1) / kScorePages));
+  const size_t smem = (size_t)p.group * p.hd * sizeof(double);
+  cudaError_t e =
+      p.dtype == 1
+          ? launch_chained(paged_score_kernel<__nv_bfloat16>, grid, dim3(kScoreThreads), smem, st, p)
+          : launch_chained(paged_score_kernel<float>, grid, dim3(kScoreThreads), smem, st, p);
+  if (e != cudaSuccess) return e;
+  return launch_chained(paged_pick_kernel, dim3((unsigned)(p.n * p.n_kv)), dim3(kPickThreads), 0, st, p);
+}
+
+}  // namespace tg

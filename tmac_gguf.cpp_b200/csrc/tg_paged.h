@@ -1,0 +1,83 @@
+// tg_paged.h -- parameters and launchers of the paged-cache kernels
+// (tg_paged.cu): append with rotation, decode attention through a block
+// table, and page selection.
+//
+// Pool layout of one layer: K and V [page][kv head][row in page][head_dim],
+// so that one head's rows of a page are one contiguous run (2 KB for 16 bf16
+// rows of 64); bounds [page][kv head][min, max][head_dim].  Page sizes are
+// powers of two.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "tg_shared.h"
+
+namespace tg {
+
+constexpr int kPagedMinPage = 8, kPagedMaxPage = 256;
+// Queries per launch: the schedule of a launch lives in shared memory.
+constexpr int kPagedMaxQueries = 4096;
+constexpr int kPagedHeads = 8;    // query heads of one stream (a KV head's group in blocks of 8)
+constexpr int kPagedChunk = 32;   // cache rows per warp step
+
+struct PagedAppendParams {
+  const float* k;        // [n_tokens][n_kv*hd] un-rotated
+  const float* v;        // [n_tokens][n_kv*hd]
+  const float* q;        // [n_tokens][n_head*hd] un-rotated, or null
+  float* q_out;          // rotated q (may be q itself)
+  const int* cu;         // [n_seqs+1] first token of each sequence, or null: token s is sequence s's
+  const int* pos0;       // [n_seqs] position of each sequence's first new token
+  const int* table;      // [n_seqs][max_blocks] pages
+  const float* cs;       // RoPE table [table_len][hd/2][cos, sin]
+  void* kp;              // layer base of the pools
+  void* vp;
+  void* bounds;          // or null
+  int* err;
+  int table_len, n_seqs, n_tokens, max_blocks, n_pages, log2p;
+  int n_head, n_kv, hd, dtype;
+  int vec4;              // rows and pointers are 16-byte aligned, hd a multiple of 4
+};
+
+// Decode attention.  A stream is one query's block of up to kPagedHeads query
+// heads over one KV head; its rows are the rows of a list of pages: entries
+// skip, skip + 1, ... of the query's table row (dense), or the listed ones
+// (sel).  The rows form chunks of kPagedChunk; the chunks of all streams lie
+// end to end and every CTA takes an equal contiguous range of them.
+struct PagedAttnParams {
+  const float* q;        // [n][n_head*hd], rotated
+  float* out;            // [n][n_head*hd] (mode 0)
+  float* records;        // [n][n_head][hd+2] o (un-normalised), m, l (mode 1)
+  const int* past;       // [n] last attended position, -1: none
+  const int* table;      // [n][max_blocks]
+  const int* sel;        // [n][n_kv][n_sel] listed table entries, or null: dense
+  const void* kp;        // layer base of the pools
+  const void* vp;
+  float* part;           // [2*grid][kPagedHeads*(hd+2)] records of split streams
+  unsigned* count;       // [n*n_kv*hblocks] arrivals at split streams, all 0 between launches
+  int* err;
+  long long page0;       // pages before this layer's (TMA rows)
+  int n, n_head, n_kv, group, hblocks, hd;
+  int max_blocks, n_pages, log2p, n_sel, skip;
+  float scale_log2;      // log2(e) / sqrt(hd)
+  int mode;              // 0 output, 1 records
+};
+
+struct PagedSelectParams {
+  const float* q;                // [n][n_head*hd], rotated
+  const int* past;               // [n]
+  const int* table;              // [n][max_blocks]
+  const void* bounds;            // layer base
+  unsigned long long* keys;      // [n][n_kv][max_blocks] ordered scores
+  int* pages;                    // [n][n_kv][n_sel]
+  int* err;
+  int n, n_head, n_kv, group, hd, dtype;
+  int max_blocks, n_pages, log2p, n_sel, keep_first, keep_last;
+};
+
+cudaError_t launch_paged_append(const PagedAppendParams& p, cudaStream_t st);
+cudaError_t launch_paged_core(const PagedAttnParams& p, int dtype, int grid, cudaStream_t st);
+size_t paged_core_smem(int n, int hd);
+cudaError_t launch_paged_select(const PagedSelectParams& p, cudaStream_t st);
+
+}  // namespace tg

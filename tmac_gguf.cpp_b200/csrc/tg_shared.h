@@ -32,6 +32,7 @@ enum DeviceError : int {
   kDevErrBadPos = 0x103,     // position outside the RoPE table / cache
   kDevErrTooManySeqs = 0x104,
   kDevErrPeerTimeout = 0x105,  // a peer GPU's softmax record did not arrive in time
+  kDevErrBadPage = 0x106,      // a block table entry outside the paged cache
 };
 
 // Per-CTA %globaltimer stamps (ns) of a profiled decode step: decode CTAs
