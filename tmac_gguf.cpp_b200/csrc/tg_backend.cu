@@ -287,6 +287,9 @@ struct tg_paged_kv {
   char* v = nullptr;
   char* bounds = nullptr;
   bool own_kv = false, own_bounds = false;
+  bool tmap_ok = false;  // the tensor-core kernels serve this shape
+  alignas(64) CUtensorMap tmk;
+  alignas(64) CUtensorMap tmv;
 };
 
 namespace {
@@ -1647,6 +1650,7 @@ int run_paged(tg_context* ctx, const tg_paged_kv* pk, int layer, int n, const fl
   p.n_pages = d.n_pages;
   p.log2p = pk->log2p;
   p.n_sel = n_sel;
+  p.lchunk = pk->tmap_ok ? tg::paged_mma_lchunk(d.dtype, d.head_dim) : 5;
   p.scale_log2 = kLog2e / sqrtf((float)d.head_dim);
   const int streams = p.n_kv * p.hblocks;
   for (int s0 = 0; s0 < n; s0 += tg::kPagedMaxQueries) {
@@ -1656,8 +1660,8 @@ int run_paged(tg_context* ctx, const tg_paged_kv* pk, int layer, int n, const fl
     p.past = past + s0;
     p.table = table + (size_t)s0 * max_blocks;
     p.sel = sel ? sel + (size_t)s0 * p.n_kv * n_sel : nullptr;
-    const size_t smem = tg::paged_core_smem(p.n, p.hd);
-    const int grid = ctx->num_sms * (2 * (smem + 1024) <= 227 * 1024 ? 2 : 1);
+    int grid = ctx->num_sms;
+    if (!pk->tmap_ok && 2 * (tg::paged_core_smem(p.n, p.hd) + 1024) <= 227 * 1024) grid *= 2;
     TG_TRY(ensure_kept(ctx, &ctx->ppart, &ctx->ppart_cap,
                        (size_t)2 * grid * tg::kPagedHeads * (p.hd + 2)));
     TG_TRY(ensure_kept(ctx, &ctx->pcount, &ctx->pcount_cap, (size_t)p.n * streams, true));
@@ -1665,7 +1669,9 @@ int run_paged(tg_context* ctx, const tg_paged_kv* pk, int layer, int n, const fl
     p.count = ctx->pcount;
     cudaEvent_t ev = nullptr;
     TG_TRY(prof_begin(ctx, TG_PROFILE_ATTENTION, &ev));
-    cudaError_t e = tg::launch_paged_core(p, d.dtype, grid, ctx->stream);
+    cudaError_t e = pk->tmap_ok
+                        ? tg::launch_paged_mma(pk->tmk, pk->tmv, p, d.dtype, grid, ctx->stream)
+                        : tg::launch_paged_core(p, d.dtype, grid, ctx->stream);
     if (e != cudaSuccess)
       return fail(TG_ERR_CUDA, "paged attention launch: %s", cudaGetErrorString(e));
     ctx->launches++;
@@ -2965,6 +2971,25 @@ int tg_paged_create(tg_context* ctx, const tg_paged_desc* desc, tg_paged_kv** ou
     cudaGetLastError();
     paged_free(pk);
     return fail(TG_ERR_OUT_OF_MEMORY, "paged_create: %zu bytes per cache", bytes);
+  }
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (enc && (d.head_dim == 64 || d.head_dim == 128)) {
+    const CUtensorMapDataType ty = d.dtype == TG_DTYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    cuuint64_t gdim[2] = {(cuuint64_t)d.head_dim,
+                          (cuuint64_t)(rows * d.n_kv_head * d.n_layers)};
+    cuuint64_t gstride[1] = {(cuuint64_t)(d.head_dim * pk->esize)};
+    cuuint32_t box[2] = {(cuuint32_t)(128 / pk->esize),
+                         (cuuint32_t)std::min(d.page_size,
+                                              1 << tg::paged_mma_lchunk(d.dtype, d.head_dim))};
+    cuuint32_t estr[2] = {1, 1};
+    pk->tmap_ok = true;
+    for (int i = 0; i < 2; ++i)
+      if (enc(i ? &pk->tmv : &pk->tmk, ty, 2, i ? pk->v : pk->k, gdim, gstride, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        pk->tmap_ok = false;
   }
   if (pk->own_kv || pk->own_bounds) {
     cudaError_t e = cudaStreamSynchronize(ctx->stream);

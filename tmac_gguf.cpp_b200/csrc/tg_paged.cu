@@ -7,6 +7,7 @@
 // (g_k_cache / g_v_cache, tmac_gguf.cpp:200-201) and has no counterpart of
 // any of these; the rotation is its apply_rope (tmac_gguf.cpp:990-1016) and
 // the attention its GQA block (tmac_gguf.cpp:1093-1128).
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -271,7 +272,7 @@ __device__ __forceinline__ int query_blocks(const PagedAttnParams& p, int past, 
 
 __device__ __forceinline__ int query_chunks(const PagedAttnParams& p, int nb) {
   const int list = p.sel ? min(p.n_sel, nb) : max(0, nb - p.skip);
-  return (int)((((long long)list << p.log2p) + kPagedChunk - 1) / kPagedChunk);
+  return (int)((((long long)list << p.log2p) + (1 << p.lchunk) - 1) >> p.lchunk);
 }
 
 // Chunk prefix over the queries (per stream of a query) and their last
@@ -361,6 +362,22 @@ __device__ __forceinline__ SegmentOut part_out(const PagedAttnParams& p, int slo
   r.l = r.m + kPagedHeads;
   r.ml_stride = 1;
   return r;
+}
+
+// Four elements of a result: as they are with (m, l), or normalised.
+__device__ __forceinline__ void store_segment4(const SegmentOut& dst, int h, int d, float4 O,
+                                               float M, float L) {
+  if (!dst.m) {
+    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+    O.x *= inv; O.y *= inv; O.z *= inv; O.w *= inv;
+  } else if (d == 0) {
+    dst.m[h * dst.ml_stride] = M;
+    dst.l[h * dst.ml_stride] = L;
+  }
+  // Output rows are 8-byte aligned, records of hd + 2 floats too.
+  float2* o = reinterpret_cast<float2*>(dst.o + h * dst.stride + d);
+  o[0] = make_float2(O.x, O.y);
+  o[1] = make_float2(O.z, O.w);
 }
 
 // Streams without a row: zeros, or neutral records.
@@ -643,6 +660,555 @@ cudaError_t launch_paged_core(const PagedAttnParams& p, int dtype, int grid, cud
   cudaError_t e = allow_max_smem(paged_core_kernel<float>, done_f32);
   if (e != cudaSuccess) return e;
   return launch_chained(paged_core_kernel<float>, dim3(grid), dim3(kCoreThreads), smem, st, p);
+}
+
+// ------------------------------------------------------------ tensor-core attention
+
+// D = A(16x8 tf32, row) * B(8x8 tf32, col) + D, fp32 accumulate.
+__device__ __forceinline__ void mma_tf32_1688(float* d, const uint32_t* a, uint32_t b0,
+                                              uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 "
+      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// x = hi + lo with hi the 11 leading significant bits (a tf32 value) and lo
+// exact; as an operand lo keeps its own 11 leading bits: 2^-21 of x is lost.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = __float_as_uint(x) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
+
+// Shapes of the kernel for a pool of T and head_dim HD.
+template <typename T, int HD>
+struct MmaPaged {
+  static constexpr bool kHalf = sizeof(T) == 2;
+  static constexpr int LCH = (kHalf && HD == 64) ? 5 : 4;   // log2 of a chunk's rows
+  static constexpr int CH = 1 << LCH;
+  // Consumers; one more warp produces.  12 warps leave a thread 168
+  // registers, which head_dim 64 keeps to without spilling, 8 warps 255.
+  static constexpr int WARPS = HD == 64 ? 11 : kHalf ? 7 : 5;
+  static constexpr int CTHREADS = 32 * WARPS;
+  static constexpr int THREADS = CTHREADS + 32;
+  static constexpr int NX = HD * (int)sizeof(T) / 128;    // 128-byte column blocks of a row
+  static constexpr int HALF = CH * HD * (int)sizeof(T);   // K (or V) bytes of a chunk
+  static constexpr int STAGE = 2 * HALF;
+  static constexpr int DEPTH = (HD == 128 && kHalf) ? 3 : 2;  // stages of a warp
+  static constexpr int STAGES = DEPTH * WARPS;
+  static constexpr int OSTRIDE = HD + 8;                  // floats per head in the merge area
+  static constexpr int MRG = kPagedHeads * OSTRIDE + 2 * kPagedHeads;
+  static constexpr int OFF_BAR = STAGES * STAGE;
+  static constexpr int OFF_META = OFF_BAR + 2 * STAGES * 8;
+  static constexpr int OFF_MRG = (OFF_META + STAGES * 4 + 15) & ~15;
+  static constexpr int OFF_MISC = OFF_MRG + WARPS * MRG * 4;
+  static constexpr int OFF_SCHED = OFF_MISC + 16 * 4;
+  static constexpr size_t smem_bytes(int n) { return 1024 + (size_t)OFF_SCHED + (size_t)(2 * n + 1) * 4; }
+};
+
+__device__ __forceinline__ void consumers_sync(int n) {
+  asm volatile("bar.sync 1, %0;" ::"r"(n) : "memory");
+}
+
+// Parts k0, k0 + step, ... of 16-byte item `it` (head h), merged.
+struct Merged4 {
+  float M, L;
+  float4 O;
+};
+
+__device__ __forceinline__ Merged4 merge_item(const PagedAttnParams& p, int it, int h, int k0,
+                                              int step, int n_parts, int first_slot, int c1) {
+  constexpr int B = 4;
+  Merged4 a{kNegBig, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+  for (; k0 < n_parts; k0 += step * B) {
+    float m[B], l[B];
+    float4 o[B];
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const int k = k0 + u * step;
+      m[u] = kNegBig;
+      l[u] = 0.f;
+      o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k < n_parts) {
+        const SegmentOut x = part_out(p, k == 0 ? first_slot : 2 * (c1 + k));
+        m[u] = __ldcg(x.m + h);
+        l[u] = __ldcg(x.l + h);
+        o[u] = __ldcg(reinterpret_cast<const float4*>(x.o) + it);
+      }
+    }
+    float mb = a.M;
+#pragma unroll
+    for (int u = 0; u < B; ++u) mb = fmaxf(mb, m[u]);
+    const float w0 = ex2(a.M - mb);
+    a.M = mb;
+    a.L *= w0;
+    a.O.x *= w0; a.O.y *= w0; a.O.z *= w0; a.O.w *= w0;
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const float w = ex2(m[u] - mb);
+      a.L = fmaf(l[u], w, a.L);
+      a.O.x = fmaf(o[u].x, w, a.O.x);
+      a.O.y = fmaf(o[u].y, w, a.O.y);
+      a.O.z = fmaf(o[u].z, w, a.O.z);
+      a.O.w = fmaf(o[u].w, w, a.O.w);
+    }
+  }
+  return a;
+}
+
+// merge_parts for the tensor-core kernel: 16-byte items, the parts dealt out
+// to as many groups of threads as there are, joined in shared memory (`sh`,
+// 6 floats per thread).  All NT threads take part.
+template <int HD, int NT>
+__device__ void merge_parts_vec(const PagedAttnParams& p, const SegmentOut& dst, int heads,
+                                int first_slot, int c1, int n_parts, int tid, float* sh) {
+  const int items = heads * HD / 4, groups = min(4, NT / items);
+  if (groups < 2) {
+    for (int it = tid; it < items; it += NT) {
+      const int h = it * 4 / HD;
+      const Merged4 a = merge_item(p, it, h, 0, 1, n_parts, first_slot, c1);
+      store_segment4(dst, h, it * 4 - h * HD, a.O, a.M, a.L);
+    }
+    return;
+  }
+  const int grp = tid / items, it = tid - grp * items, h = it * 4 / HD;
+  Merged4 a{};
+  if (grp < groups) a = merge_item(p, it, h, grp, groups, n_parts, first_slot, c1);
+  if (grp > 0 && grp < groups) {
+    float* x = sh + ((grp - 1) * items + it) * 6;
+    x[0] = a.O.x; x[1] = a.O.y; x[2] = a.O.z; x[3] = a.O.w; x[4] = a.M; x[5] = a.L;
+  }
+  consumers_sync(NT);
+  if (grp != 0) return;
+  for (int k = 1; k < groups; ++k) {
+    const float* x = sh + ((k - 1) * items + it) * 6;
+    const float mb = fmaxf(a.M, x[4]), w0 = ex2(a.M - mb), w1 = ex2(x[4] - mb);
+    a.O.x = a.O.x * w0 + x[0] * w1;
+    a.O.y = a.O.y * w0 + x[1] * w1;
+    a.O.z = a.O.z * w0 + x[2] * w1;
+    a.O.w = a.O.w * w0 + x[3] * w1;
+    a.L = a.L * w0 + x[5] * w1;
+    a.M = mb;
+  }
+  store_segment4(dst, h, it * 4 - h * HD, a.O, a.M, a.L);
+}
+
+// bf16 or fp32 pool, head_dim 64 or 128.  Chunk k of the CTA's range is
+// consumer warp k % WARPS's, and each warp has DEPTH stages of its own (a
+// stage that changed hands could be two phases ahead of a waiting warp, which
+// a parity cannot tell), so the warps share nothing until a stream's segment
+// ends.  One producer warp streams the chunks in order into the stages by TMA
+// (boxes of min(page, CH) rows, 128-byte swizzle; a lane per box, their pages
+// looked up 32 boxes at a time, one batch ahead).
+//
+// Products are mma.sync: a step has at most 8 query rows, far below the 64 of
+// a tcgen05 tile.  The 8 spare rows of the 16-row operand carry the low part
+// of q (and of the probabilities): x = hi + lo, two bf16 (17 bits together)
+// against the exact bf16 rows, or two tf32 against the rows split the same
+// way, so results are those of binary32 products to 2^-17 and 2^-21.
+template <typename T, int HD>
+__global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
+    paged_mma_kernel(const __grid_constant__ CUtensorMap tmk,
+                     const __grid_constant__ CUtensorMap tmv, const PagedAttnParams p) {
+  using Cfg = MmaPaged<T, HD>;
+  constexpr int STAGES = Cfg::STAGES, NX = Cfg::NX, CH = Cfg::CH, NT = CH / 8;
+  constexpr int WARPS = Cfg::WARPS, DEPTH = Cfg::DEPTH;
+  constexpr bool kHalf = Cfg::kHalf;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
+  uint64_t* empty = full + STAGES;
+  uint32_t* meta = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_META);
+  float* mrg = reinterpret_cast<float*>(smem + Cfg::OFF_MRG);
+  int* warp_tot = reinterpret_cast<int*>(smem + Cfg::OFF_MISC);
+  int* flag = warp_tot + 14;
+  int* prefix = reinterpret_cast<int*>(smem + Cfg::OFF_SCHED);
+  int* past_s = prefix + p.n + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  griddep_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    fence_mbar_init();
+    tma_prefetch_desc(&tmk);
+    tma_prefetch_desc(&tmv);
+  }
+  griddep_wait();
+  paged_schedule(p, prefix, past_s, warp_tot);
+  const int streams = p.n_kv * p.hblocks;
+  const long long T_all = (long long)prefix[p.n] * streams;
+  write_empty(p, prefix);
+  const int G = paged_active(gridDim.x, T_all, Cfg::WARPS), cta = blockIdx.x;
+  if (cta >= G) return;
+  const long long t_lo = cta_tile_lo(cta, G, T_all), t_hi = cta_tile_lo(cta + 1, G, T_all);
+  const int s_first = query_of(prefix, p.n, streams, t_lo);
+  const int P = 1 << p.log2p;
+  const int box = min(P, CH), lbox = min(p.log2p, Cfg::LCH);   // rows of a TMA box
+  const int nbx = CH >> lbox;                                  // boxes of a chunk, 1, 2 or 4
+  const uint32_t cnt_full = (uint32_t)box * (nbx == 1 ? 1u : nbx == 2 ? 0x101u : 0x1010101u);
+
+  if (warp == Cfg::WARPS) {
+    // ------------------------------------------------------------ producer
+    // Lane l: box l of the batch that starts at chunk tb (its TMA row y and
+    // its attended rows cnt); te: the chunk behind the batch.
+    int y = 0, cnt = 0, y_n = 0, cnt_n = 0, s = s_first;
+    auto fetch = [&](long long tb, int& fy, int& fc) -> long long {
+      while ((long long)prefix[s + 1] * streams <= tb) ++s;
+      const int C = prefix[s + 1] - prefix[s];
+      const long long rel = tb - (long long)prefix[s] * streams;
+      const int u = (int)(rel / C), c0 = (int)(rel - (long long)u * C);
+      const int g = u / p.hblocks, past = past_s[s];
+      const int nb = (past >> p.log2p) + 1;
+      const int list = p.sel ? min(p.n_sel, nb) : nb - p.skip;
+      const long long r = ((long long)c0 * nbx + lane) << lbox;  // row of the stream
+      const int i = (int)(r >> p.log2p), off = (int)(r & (P - 1));
+      fy = fc = 0;
+      if (i < list) {
+        const int j = p.sel ? p.sel[((size_t)s * p.n_kv + g) * p.n_sel + i] : p.skip + i;
+        if (j >= 0 && j < nb) {
+          const int page = p.table[(size_t)s * p.max_blocks + j];
+          if (page < 0 || page >= p.n_pages) {
+            record_error(p.err, kDevErrBadPage);
+          } else {
+            fc = max(0, min(box, past + 1 - ((j << p.log2p) + off)));
+            fy = (int)(((p.page0 + page) * p.n_kv + g) << p.log2p) + off;
+          }
+        }
+      }
+      return min(t_hi, tb + min(C - c0, 32 / nbx));
+    };
+    int w = 0, slot = 0, issued = 0;   // next chunk: warp w, its stage `slot`
+    uint32_t ph = 0;
+    bool ok = true;
+    long long tb = t_lo, te = fetch(tb, y, cnt);
+    while (tb < t_hi && ok) {
+      long long tn = te;
+      if (te < t_hi) tn = fetch(te, y_n, cnt_n);
+      for (int c = 0; c < (int)(te - tb); ++c) {
+        uint32_t m = 0;
+        int loads = 0;
+        for (int b = 0; b < nbx; ++b) {
+          const int x = __shfl_sync(0xffffffffu, cnt, c * nbx + b);
+          m |= (uint32_t)x << (8 * b);
+          loads += x > 0;
+        }
+        const int st = w * DEPTH + slot;
+        if (!mbar_wait(&empty[st], ph ^ 1u, p.err, kDevErrWaitEmpty)) ok = false;
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          meta[st] = m;
+          if (loads)
+            mbar_arrive_expect_tx(&full[st], (uint32_t)(loads * box * 2 * NX * 128));
+          else
+            mbar_arrive(&full[st]);
+        }
+        __syncwarp();
+        const int b = lane / (2 * NX), kv = (lane / NX) & 1, x = lane % NX;
+        const int src = min(c * nbx + b, 31);
+        const int yb = __shfl_sync(0xffffffffu, y, src), cb = __shfl_sync(0xffffffffu, cnt, src);
+        if (b < nbx && cb > 0)
+          tma_load_2d(smem + st * Cfg::STAGE + kv * Cfg::HALF + x * (CH * 128) + b * box * 128,
+                      kv ? &tmv : &tmk, &full[st], x * (128 / (int)sizeof(T)), yb);
+        ++issued;
+        if (++w == WARPS) {
+          w = 0;
+          if (++slot == DEPTH) {
+            slot = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      tb = te;
+      te = tn;
+      y = y_n;
+      cnt = cnt_n;
+    }
+    // Every issued load lands before the CTA exits.
+    for (int k = max(0, issued - STAGES); k < issued; ++k)
+      mbar_wait(&full[(k % WARPS) * DEPTH + (k / WARPS) % DEPTH],
+                (uint32_t)((k / STAGES) & 1), p.err, kDevErrWaitFull);
+    return;
+  }
+
+  // -------------------------------------------------------------- consumers
+  constexpr int NCT = Cfg::CTHREADS;
+  const int r = lane >> 2, qd = lane & 3;
+  float* my_mrg = mrg + warp * Cfg::MRG;
+  const float sl2 = p.scale_log2;
+  bool failed = false;
+  int s = s_first;
+  int ki = warp;                               // this warp's next chunk, counted from t_lo
+  int slot = 0;
+  uint32_t ph = 0;
+  uint32_t qa[kHalf ? HD / 16 : HD / 8][4];
+  float o[HD / 8][4];
+  for (long long t = t_lo; t < t_hi;) {
+    while ((long long)prefix[s + 1] * streams <= t) ++s;
+    const int C = prefix[s + 1] - prefix[s];
+    const long long q_base = (long long)prefix[s] * streams;
+    const int u = (int)((t - q_base) / C);
+    const long long s_lo = q_base + (long long)u * C, s_hi = s_lo + C, e_hi = min(t_hi, s_hi);
+    const int g = u / p.hblocks, hb = u - g * p.hblocks;
+    const int heads = min(kPagedHeads, p.group - hb * kPagedHeads);
+    {
+      const float* qh = p.q + ((size_t)s * p.n_head + g * p.group + hb * kPagedHeads + r) * HD;
+      const bool row_ok = r < heads;
+      if constexpr (kHalf) {
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float2 v = make_float2(0.f, 0.f);
+            if (row_ok) v = *reinterpret_cast<const float2*>(qh + 16 * kk + 8 * half + 2 * qd);
+            float h0, l0, h1, l1;
+            split_bf16(v.x, h0, l0);
+            split_bf16(v.y, h1, l1);
+            qa[kk][2 * half] = pack_bf16x2(h0, h1);
+            qa[kk][2 * half + 1] = pack_bf16x2(l0, l1);
+          }
+      } else {
+#pragma unroll
+        for (int kk = 0; kk < HD / 8; ++kk)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            split_tf32(row_ok ? qh[8 * kk + 4 * half + qd] : 0.f, qa[kk][2 * half],
+                       qa[kk][2 * half + 1]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < HD / 8; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
+    float m_run = kNegBig, l_run = 0.f;
+
+    const int k_end = (int)(e_hi - t_lo);
+    for (; ki < k_end; ki += WARPS) {
+      const int st = warp * DEPTH + slot;
+      if (!failed && !mbar_wait(&full[st], ph, p.err, kDevErrWaitFull)) failed = true;
+      const uint32_t cm = meta[st];
+      if (!__any_sync(0xffffffffu, failed) && cm != 0) {
+        uint8_t* kbox = smem + st * Cfg::STAGE;
+        uint8_t* vbox = kbox + Cfg::HALF;
+        const bool whole = cm == cnt_full;
+        if (!whole) {
+          // Rows that are not attended may hold anything: their V becomes
+          // zero, so that weight 0 adds exactly zero.
+          const int row = lane;
+          if (row < CH && (row & (box - 1)) >= (int)((cm >> (8 * (row >> lbox))) & 255u)) {
+#pragma unroll
+            for (int x = 0; x < NX; ++x)
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                reinterpret_cast<uint4*>(vbox + x * (CH * 128) + row * 128)[(e + row) & 7] =
+                    make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        const uint32_t kb = smem_u32(kbox), vb = smem_u32(vbox);
+        // S = q . K^T in blocks of 8 rows.
+        float sc[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+          if constexpr (kHalf) {
+            const int row = 8 * nt + (lane & 7);
+#pragma unroll
+            for (int kq = 0; kq < HD / 32; ++kq) {
+              const int chunk = 4 * (kq & 1) + (lane >> 3);
+              uint32_t b0, b1, b2, b3;
+              ldmatrix_x4(kb + (kq >> 1) * (CH * 128) + row * 128 + ((chunk ^ (row & 7)) << 4), b0,
+                          b1, b2, b3);
+              mma_bf16_16816(acc[kq & 1], qa[2 * kq], b0, b1);
+              mma_bf16_16816(acc[kq & 1], qa[2 * kq + 1], b2, b3);
+            }
+          } else {
+            const int row = 8 * nt + r;
+#pragma unroll
+            for (int kk = 0; kk < HD / 8; ++kk) {
+              const uint8_t* a = kbox + (kk >> 2) * (CH * 128) + row * 128 + qd * 4;
+              const int chunk = 2 * (kk & 3);
+              uint32_t h0, l0, h1, l1;
+              split_tf32(*reinterpret_cast<const float*>(a + ((chunk ^ (row & 7)) << 4)), h0, l0);
+              split_tf32(*reinterpret_cast<const float*>(a + (((chunk + 1) ^ (row & 7)) << 4)), h1,
+                         l1);
+              mma_tf32_1688(acc[0], qa[kk], h0, h1);
+              mma_tf32_1688(acc[1], qa[kk], l0, l1);
+            }
+          }
+          sc[nt][0] = ((acc[0][0] + acc[0][2]) + (acc[1][0] + acc[1][2])) * sl2;
+          sc[nt][1] = ((acc[0][1] + acc[0][3]) + (acc[1][1] + acc[1][3])) * sl2;
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int c = 8 * nt + 2 * qd + e;
+              if ((c & (box - 1)) >= (int)((cm >> (8 * (c >> lbox))) & 255u)) sc[nt][e] = -INFINITY;
+            }
+          }
+        }
+        // Online softmax over the chunk's rows (a query head is a quad of lanes).
+        float mx = fmaxf(sc[0][0], sc[0][1]);
+#pragma unroll
+        for (int nt = 1; nt < NT; ++nt) mx = fmaxf(mx, fmaxf(sc[nt][0], sc[nt][1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float m_new = fmaxf(m_run, mx);
+        const float alpha = ex2(m_run - m_new);
+        m_run = m_new;
+        float lsum = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          sc[nt][0] = ex2(sc[nt][0] - m_new);
+          sc[nt][1] = ex2(sc[nt][1] - m_new);
+          lsum += sc[nt][0] + sc[nt][1];
+        }
+        l_run = l_run * alpha + lsum;
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) {
+          o[c][0] *= alpha; o[c][1] *= alpha; o[c][2] *= alpha; o[c][3] *= alpha;
+        }
+        // O += P . V.
+        if constexpr (kHalf) {
+#pragma unroll
+          for (int kp = 0; kp < CH / 16; ++kp) {
+            uint32_t pa[4];
+            float h0, l0, h1, l1;
+            split_bf16(sc[2 * kp][0], h0, l0);
+            split_bf16(sc[2 * kp][1], h1, l1);
+            pa[0] = pack_bf16x2(h0, h1);
+            pa[1] = pack_bf16x2(l0, l1);
+            split_bf16(sc[2 * kp + 1][0], h0, l0);
+            split_bf16(sc[2 * kp + 1][1], h1, l1);
+            pa[2] = pack_bf16x2(h0, h1);
+            pa[3] = pack_bf16x2(l0, l1);
+            const int row = 16 * kp + ((lane >> 3) & 1) * 8 + (lane & 7);
+#pragma unroll
+            for (int cp = 0; cp < HD / 16; ++cp) {
+              const int chunk = 2 * (cp & 3) + (lane >> 4);
+              uint32_t b0, b1, b2, b3;
+              ldmatrix_x4_trans(vb + (cp >> 2) * (CH * 128) + row * 128 + ((chunk ^ (row & 7)) << 4),
+                                b0, b1, b2, b3);
+              mma_bf16_16816(o[2 * cp], pa, b0, b1);
+              mma_bf16_16816(o[2 * cp + 1], pa, b2, b3);
+            }
+          }
+        } else {
+          // Rows 2 qd and 2 qd + 1 of a block are the operand's k = qd and
+          // k = qd + 4, so the scores are its layout already (the order of
+          // the rows in a sum is free), and no two lanes share a bank.
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            uint32_t pa[4];
+            split_tf32(sc[nt][0], pa[0], pa[1]);
+            split_tf32(sc[nt][1], pa[2], pa[3]);
+            const int row = 8 * nt + 2 * qd;
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+              const uint8_t* a = vbox + (c >> 2) * (CH * 128) + row * 128 + (r & 3) * 4;
+              const int chunk = 2 * (c & 3) + (r >> 2);
+              uint32_t h0, l0, h1, l1;
+              split_tf32(*reinterpret_cast<const float*>(a + ((chunk ^ (row & 7)) << 4)), h0, l0);
+              split_tf32(*reinterpret_cast<const float*>(a + 128 + ((chunk ^ ((row + 1) & 7)) << 4)),
+                         h1, l1);
+              mma_tf32_1688(o[c], pa, h0, h1);
+              mma_tf32_1688(o[c], pa, l0, l1);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+      if (++slot == DEPTH) {
+        slot = 0;
+        ph ^= 1u;
+      }
+    }
+    // ---------------------------------------------------------- segment end
+    l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
+    l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
+#pragma unroll
+    for (int c = 0; c < HD / 8; ++c)
+      *reinterpret_cast<float2*>(my_mrg + r * Cfg::OSTRIDE + 8 * c + 2 * qd) =
+          make_float2(o[c][0] + o[c][2], o[c][1] + o[c][3]);
+    if (qd == 0) {
+      my_mrg[kPagedHeads * Cfg::OSTRIDE + r] = m_run;
+      my_mrg[kPagedHeads * (Cfg::OSTRIDE + 1) + r] = l_run;
+    }
+    consumers_sync(NCT);
+    const bool complete = t == s_lo && e_hi == s_hi;
+    const SegmentOut fin = segment_out(p, s, g, hb);
+    const SegmentOut dst = complete ? fin : part_out(p, 2 * cta + (t == t_lo ? 0 : 1));
+    for (int e = threadIdx.x; e < heads * HD / 4; e += NCT) {
+      const int h = e * 4 / HD, d = e * 4 - h * HD;
+      float M = kNegBig;
+#pragma unroll
+      for (int w = 0; w < Cfg::WARPS; ++w)
+        M = fmaxf(M, mrg[w * Cfg::MRG + kPagedHeads * Cfg::OSTRIDE + h]);
+      float L = 0.f;
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < Cfg::WARPS; ++w) {
+        const float* mw = mrg + w * Cfg::MRG;
+        const float f = ex2(mw[kPagedHeads * Cfg::OSTRIDE + h] - M);
+        const float4 x = *reinterpret_cast<const float4*>(mw + h * Cfg::OSTRIDE + d);
+        L = fmaf(mw[kPagedHeads * (Cfg::OSTRIDE + 1) + h], f, L);
+        O.x = fmaf(x.x, f, O.x);
+        O.y = fmaf(x.y, f, O.y);
+        O.z = fmaf(x.z, f, O.z);
+        O.w = fmaf(x.w, f, O.w);
+      }
+      store_segment4(dst, h, d, O, M, L);
+    }
+    if (!complete) {
+      const int c1 = cta_of_tile(s_lo, G, T_all), c2 = cta_of_tile(s_hi - 1, G, T_all);
+      unsigned* count = p.count + (size_t)s * streams + u;
+      __threadfence();
+      consumers_sync(NCT);
+      if (threadIdx.x == 0) *flag = atomicAdd(count, 1u) == (unsigned)(c2 - c1);
+      consumers_sync(NCT);
+      if (*flag) {
+        __threadfence();
+        merge_parts_vec<HD, NCT>(p, fin, heads, 2 * c1 + (cta_tile_lo(c1, G, T_all) == s_lo ? 0 : 1),
+                                 c1, c2 - c1 + 1, threadIdx.x, mrg);
+        if (threadIdx.x == 0) *count = 0;
+      }
+    }
+    consumers_sync(NCT);
+    t = e_hi;
+  }
+}
+
+template <typename T, int HD>
+static cudaError_t launch_mma_cfg(const CUtensorMap& tk, const CUtensorMap& tv,
+                                  const PagedAttnParams& p, int grid, cudaStream_t st) {
+  static bool done[64] = {};
+  cudaError_t e = allow_max_smem(paged_mma_kernel<T, HD>, done);
+  if (e != cudaSuccess) return e;
+  return launch_chained(paged_mma_kernel<T, HD>, dim3(grid), dim3(MmaPaged<T, HD>::THREADS),
+                        MmaPaged<T, HD>::smem_bytes(p.n), st, tk, tv, p);
+}
+
+int paged_mma_lchunk(int dtype, int hd) {
+  return dtype == 1 && hd == 64 ? MmaPaged<__nv_bfloat16, 64>::LCH : MmaPaged<float, 64>::LCH;
+}
+
+cudaError_t launch_paged_mma(const CUtensorMap& tk, const CUtensorMap& tv, const PagedAttnParams& p,
+                             int dtype, int grid, cudaStream_t st) {
+  static_assert(MmaPaged<float, 128>::smem_bytes(kPagedMaxQueries) <= 227 * 1024, "shared memory");
+  static_assert(MmaPaged<__nv_bfloat16, 128>::smem_bytes(kPagedMaxQueries) <= 227 * 1024, "shared memory");
+  static_assert(MmaPaged<float, 64>::smem_bytes(kPagedMaxQueries) <= 227 * 1024, "shared memory");
+  static_assert(MmaPaged<__nv_bfloat16, 64>::smem_bytes(kPagedMaxQueries) <= 227 * 1024, "shared memory");
+  if (p.hd == 64)
+    return dtype == 1 ? launch_mma_cfg<__nv_bfloat16, 64>(tk, tv, p, grid, st)
+                      : launch_mma_cfg<float, 64>(tk, tv, p, grid, st);
+  return dtype == 1 ? launch_mma_cfg<__nv_bfloat16, 128>(tk, tv, p, grid, st)
+                    : launch_mma_cfg<float, 128>(tk, tv, p, grid, st);
 }
 
 // ------------------------------------------------------------ page selection

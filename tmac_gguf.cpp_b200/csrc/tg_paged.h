@@ -8,6 +8,7 @@
 // powers of two.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -17,9 +18,9 @@ namespace tg {
 
 constexpr int kPagedMinPage = 8, kPagedMaxPage = 256;
 // Queries per launch: the schedule of a launch lives in shared memory.
-constexpr int kPagedMaxQueries = 4096;
+constexpr int kPagedMaxQueries = 2048;
 constexpr int kPagedHeads = 8;    // query heads of one stream (a KV head's group in blocks of 8)
-constexpr int kPagedChunk = 32;   // cache rows per warp step
+constexpr int kPagedChunk = 32;   // cache rows per warp step of the CUDA-core kernel
 
 struct PagedAppendParams {
   const float* k;        // [n_tokens][n_kv*hd] un-rotated
@@ -42,7 +43,7 @@ struct PagedAppendParams {
 // Decode attention.  A stream is one query's block of up to kPagedHeads query
 // heads over one KV head; its rows are the rows of a list of pages: entries
 // skip, skip + 1, ... of the query's table row (dense), or the listed ones
-// (sel).  The rows form chunks of kPagedChunk; the chunks of all streams lie
+// (sel).  The rows form chunks of 16 or 32; the chunks of all streams lie
 // end to end and every CTA takes an equal contiguous range of them.
 struct PagedAttnParams {
   const float* q;        // [n][n_head*hd], rotated
@@ -59,6 +60,7 @@ struct PagedAttnParams {
   long long page0;       // pages before this layer's (TMA rows)
   int n, n_head, n_kv, group, hblocks, hd;
   int max_blocks, n_pages, log2p, n_sel, skip;
+  int lchunk;            // log2 of the rows of a chunk
   float scale_log2;      // log2(e) / sqrt(hd)
   int mode;              // 0 output, 1 records
 };
@@ -78,6 +80,11 @@ struct PagedSelectParams {
 cudaError_t launch_paged_append(const PagedAppendParams& p, cudaStream_t st);
 cudaError_t launch_paged_core(const PagedAttnParams& p, int dtype, int grid, cudaStream_t st);
 size_t paged_core_smem(int n, int hd);
+// head_dim 64 or 128; tk / tv are 2-D maps of the pools ({head_dim, rows}, box
+// {128 bytes, min(page, 1 << paged_mma_lchunk) rows}, 128-byte swizzle).
+int paged_mma_lchunk(int dtype, int hd);
+cudaError_t launch_paged_mma(const CUtensorMap& tk, const CUtensorMap& tv, const PagedAttnParams& p,
+                             int dtype, int grid, cudaStream_t st);
 cudaError_t launch_paged_select(const PagedSelectParams& p, cudaStream_t st);
 
 }  // namespace tg
