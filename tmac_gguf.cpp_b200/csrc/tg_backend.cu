@@ -1653,8 +1653,14 @@ int run_paged(tg_context* ctx, const tg_paged_kv* pk, int layer, int n, const fl
   p.lchunk = pk->tmap_ok ? tg::paged_mma_lchunk(d.dtype, d.head_dim) : 5;
   p.scale_log2 = kLog2e / sqrtf((float)d.head_dim);
   const int streams = p.n_kv * p.hblocks;
-  for (int s0 = 0; s0 < n; s0 += tg::kPagedMaxQueries) {
-    p.n = std::min(n - s0, tg::kPagedMaxQueries);
+  // A launch's chunks are counted in 32 bits.
+  const long long per_query = (((long long)max_blocks << pk->log2p) >> p.lchunk) + 1;
+  if (per_query * streams >= (1LL << 31))
+    return fail(TG_ERR_INVALID_ARG, "max_blocks %d: too many rows for one query", max_blocks);
+  const int step = (int)std::min((long long)tg::kPagedMaxQueries,
+                                 ((1LL << 31) - 1) / (per_query * streams));
+  for (int s0 = 0; s0 < n; s0 += step) {
+    p.n = std::min(n - s0, step);
     p.q = q + (size_t)s0 * qdim;
     p.out = out + (size_t)s0 * qdim;
     p.past = past + s0;

@@ -311,19 +311,18 @@ __device__ void paged_schedule(const PagedAttnParams& p, int* prefix, int* past_
 
 // Query that owns flat chunk t when every query has `streams` streams: the
 // last s with prefix[s] * streams <= t and a non-empty share.
-__device__ __forceinline__ int query_of(const int* prefix, int n, int streams, long long t) {
+__device__ __forceinline__ int query_of(const int* prefix, int n, int streams, int t) {
   int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if ((long long)prefix[mid] * streams <= t) lo = mid; else hi = mid - 1;
+    if (prefix[mid] * streams <= t) lo = mid; else hi = mid - 1;
   }
   return lo;
 }
 
 // CTAs that take part: enough that each has a chunk for each of its warps.
-__device__ __forceinline__ int paged_active(int grid, long long T, int warps) {
-  const long long g = (T + warps - 1) / warps;
-  return (int)min((long long)grid, g);
+__device__ __forceinline__ int paged_active(int grid, int T, int warps) {
+  return min(grid, (T + warps - 1) / warps);
 }
 
 // ------------------------------------------------------------ segment results
@@ -486,23 +485,21 @@ __global__ void __launch_bounds__(kCoreThreads) paged_core_kernel(const PagedAtt
   griddep_wait();
   paged_schedule(p, prefix, past_s, warp_tot);
   const int streams = p.n_kv * p.hblocks;
-  const long long T_all = (long long)prefix[p.n] * streams;
+  const int T_all = prefix[p.n] * streams;
   write_empty(p, prefix);
   const int G = paged_active(gridDim.x, T_all, kCoreWarps), cta = blockIdx.x;
   if (cta >= G) return;
-  const long long t_lo = cta_tile_lo(cta, G, T_all), t_hi = cta_tile_lo(cta + 1, G, T_all);
+  const int t_lo = (int)cta_tile_lo(cta, G, T_all), t_hi = (int)cta_tile_lo(cta + 1, G, T_all);
   const T* kp = static_cast<const T*>(p.kp);
   const T* vp = static_cast<const T*>(p.vp);
   const int P = 1 << p.log2p;
 
   int s = query_of(prefix, p.n, streams, t_lo);
-  for (long long t = t_lo; t < t_hi;) {
-    while ((long long)prefix[s + 1] * streams <= t) ++s;
+  for (int t = t_lo; t < t_hi;) {
+    while (prefix[s + 1] * streams <= t) ++s;
     const int C = prefix[s + 1] - prefix[s];
-    const long long q_base = (long long)prefix[s] * streams;
-    const int u = (int)((t - q_base) / C);
-    const long long s_lo = q_base + (long long)u * C, s_hi = s_lo + C;
-    const long long e_hi = min(t_hi, s_hi);
+    const int q_base = prefix[s] * streams, u = (t - q_base) / C;
+    const int s_lo = q_base + u * C, s_hi = s_lo + C, e_hi = min(t_hi, s_hi);
     const int g = u / p.hblocks, hb = u - g * p.hblocks;
     const int heads = min(kPagedHeads, p.group - hb * kPagedHeads);
     const int past = past_s[s];
@@ -525,8 +522,8 @@ __global__ void __launch_bounds__(kCoreThreads) paged_core_kernel(const PagedAtt
       l[h] = 0.f;
       o[h][0] = o[h][1] = make_float2(0.f, 0.f);
     }
-    for (long long c = t + warp; c < e_hi; c += kCoreWarps) {
-      const int r = (int)(c - s_lo) * kPagedChunk + lane;
+    for (int c = t + warp; c < e_hi; c += kCoreWarps) {
+      const int r = (c - s_lo) * kPagedChunk + lane;
       const int i = r >> p.log2p, slot = r & (P - 1);
       bool ok = i < list;
       size_t row = 0;
@@ -640,7 +637,7 @@ __global__ void __launch_bounds__(kCoreThreads) paged_core_kernel(const PagedAtt
       __syncthreads();
       if (*flag) {
         __threadfence();
-        merge_parts(p, fin, heads, 2 * c1 + (cta_tile_lo(c1, G, T_all) == s_lo ? 0 : 1), c1,
+        merge_parts(p, fin, heads, 2 * c1 + ((int)cta_tile_lo(c1, G, T_all) == s_lo ? 0 : 1), c1,
                     c2 - c1 + 1, tid, kCoreThreads);
         if (tid == 0) *count = 0;
       }
@@ -687,11 +684,10 @@ struct MmaPaged {
   static constexpr bool kHalf = sizeof(T) == 2;
   static constexpr int LCH = (kHalf && HD == 64) ? 5 : 4;   // log2 of a chunk's rows
   static constexpr int CH = 1 << LCH;
-  // Consumers; one more warp produces.  12 warps leave a thread 168
-  // registers, which head_dim 64 keeps to without spilling, 8 warps 255.
+  // 12 warps leave a thread 168 registers, which head_dim 64 keeps to without
+  // spilling, 8 warps 255.
   static constexpr int WARPS = HD == 64 ? 11 : kHalf ? 7 : 5;
-  static constexpr int CTHREADS = 32 * WARPS;
-  static constexpr int THREADS = CTHREADS + 32;
+  static constexpr int THREADS = 32 * WARPS;
   static constexpr int NX = HD * (int)sizeof(T) / 128;    // 128-byte column blocks of a row
   static constexpr int HALF = CH * HD * (int)sizeof(T);   // K (or V) bytes of a chunk
   static constexpr int STAGE = 2 * HALF;
@@ -700,7 +696,7 @@ struct MmaPaged {
   static constexpr int OSTRIDE = HD + 8;                  // floats per head in the merge area
   static constexpr int MRG = kPagedHeads * OSTRIDE + 2 * kPagedHeads;
   static constexpr int OFF_BAR = STAGES * STAGE;
-  static constexpr int OFF_META = OFF_BAR + 2 * STAGES * 8;
+  static constexpr int OFF_META = OFF_BAR + STAGES * 8;
   static constexpr int OFF_MRG = (OFF_META + STAGES * 4 + 15) & ~15;
   static constexpr int OFF_MISC = OFF_MRG + WARPS * MRG * 4;
   static constexpr int OFF_SCHED = OFF_MISC + 16 * 4;
@@ -794,13 +790,14 @@ __device__ void merge_parts_vec(const PagedAttnParams& p, const SegmentOut& dst,
   store_segment4(dst, h, it * 4 - h * HD, a.O, a.M, a.L);
 }
 
-// bf16 or fp32 pool, head_dim 64 or 128.  Chunk k of the CTA's range is
-// consumer warp k % WARPS's, and each warp has DEPTH stages of its own (a
-// stage that changed hands could be two phases ahead of a waiting warp, which
-// a parity cannot tell), so the warps share nothing until a stream's segment
-// ends.  One producer warp streams the chunks in order into the stages by TMA
-// (boxes of min(page, CH) rows, 128-byte swizzle; a lane per box, their pages
-// looked up 32 boxes at a time, one batch ahead).
+// bf16 or fp32 pool, head_dim 64 or 128.  Chunk k of the CTA's range is warp
+// k % WARPS's, and each warp has DEPTH stages of its own that it fills by TMA
+// itself (boxes of min(page, CH) rows, 128-byte swizzle): a stage just read
+// is refilled with the warp's chunk DEPTH further on, whose page was looked
+// up one step earlier.  The warps share nothing until a stream's segment
+// ends, and no warp's loads wait for another's (with one producer warp for
+// all, its walk of page look-ups, waits and small boxes took 740 to 950
+// cycles per 8 KB chunk where the memory delivers one in 350).
 //
 // Products are mma.sync: a step has at most 8 query rows, far below the 64 of
 // a tcgen05 tile.  The 8 spare rows of the 16-row operand carry the low part
@@ -813,13 +810,12 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
                      const __grid_constant__ CUtensorMap tmv, const PagedAttnParams p) {
   using Cfg = MmaPaged<T, HD>;
   constexpr int STAGES = Cfg::STAGES, NX = Cfg::NX, CH = Cfg::CH, NT = CH / 8;
-  constexpr int WARPS = Cfg::WARPS, DEPTH = Cfg::DEPTH;
+  constexpr int WARPS = Cfg::WARPS, DEPTH = Cfg::DEPTH, NCT = Cfg::THREADS;
   constexpr bool kHalf = Cfg::kHalf;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
-  uint64_t* empty = full + STAGES;
   uint32_t* meta = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_META);
   float* mrg = reinterpret_cast<float*>(smem + Cfg::OFF_MRG);
   int* warp_tot = reinterpret_cast<int*>(smem + Cfg::OFF_MISC);
@@ -830,10 +826,7 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
 
   griddep_launch_dependents();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
+    for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1);
     fence_mbar_init();
     tma_prefetch_desc(&tmk);
     tma_prefetch_desc(&tmv);
@@ -841,121 +834,107 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
   griddep_wait();
   paged_schedule(p, prefix, past_s, warp_tot);
   const int streams = p.n_kv * p.hblocks;
-  const long long T_all = (long long)prefix[p.n] * streams;
+  const int T_all = prefix[p.n] * streams;
   write_empty(p, prefix);
-  const int G = paged_active(gridDim.x, T_all, Cfg::WARPS), cta = blockIdx.x;
+  const int G = paged_active(gridDim.x, T_all, WARPS), cta = blockIdx.x;
   if (cta >= G) return;
-  const long long t_lo = cta_tile_lo(cta, G, T_all), t_hi = cta_tile_lo(cta + 1, G, T_all);
-  const int s_first = query_of(prefix, p.n, streams, t_lo);
+  const int t_lo = (int)cta_tile_lo(cta, G, T_all), t_hi = (int)cta_tile_lo(cta + 1, G, T_all);
   const int P = 1 << p.log2p;
   const int box = min(P, CH), lbox = min(p.log2p, Cfg::LCH);   // rows of a TMA box
   const int nbx = CH >> lbox;                                  // boxes of a chunk, 1, 2 or 4
   const uint32_t cnt_full = (uint32_t)box * (nbx == 1 ? 1u : nbx == 2 ? 0x101u : 0x1010101u);
 
-  if (warp == Cfg::WARPS) {
-    // ------------------------------------------------------------ producer
-    // Lane l: box l of the batch that starts at chunk tb (its TMA row y and
-    // its attended rows cnt); te: the chunk behind the batch.
-    int y = 0, cnt = 0, y_n = 0, cnt_n = 0, s = s_first;
-    auto fetch = [&](long long tb, int& fy, int& fc) -> long long {
-      while ((long long)prefix[s + 1] * streams <= tb) ++s;
-      const int C = prefix[s + 1] - prefix[s];
-      const long long rel = tb - (long long)prefix[s] * streams;
-      const int u = (int)(rel / C), c0 = (int)(rel - (long long)u * C);
-      const int g = u / p.hblocks, past = past_s[s];
-      const int nb = (past >> p.log2p) + 1;
-      const int list = p.sel ? min(p.n_sel, nb) : nb - p.skip;
-      const long long r = ((long long)c0 * nbx + lane) << lbox;  // row of the stream
-      const int i = (int)(r >> p.log2p), off = (int)(r & (P - 1));
-      fy = fc = 0;
-      if (i < list) {
-        const int j = p.sel ? p.sel[((size_t)s * p.n_kv + g) * p.n_sel + i] : p.skip + i;
-        if (j >= 0 && j < nb) {
-          const int page = p.table[(size_t)s * p.max_blocks + j];
-          if (page < 0 || page >= p.n_pages) {
-            record_error(p.err, kDevErrBadPage);
-          } else {
-            fc = max(0, min(box, past + 1 - ((j << p.log2p) + off)));
-            fy = (int)(((p.page0 + page) * p.n_kv + g) << p.log2p) + off;
-          }
-        }
+  // The stream that the look-up stands in: query ls, stream lu of it, its
+  // flat chunks [l_lo, l_hi).
+  int ls = query_of(prefix, p.n, streams, t_lo);
+  int l_c = prefix[ls + 1] - prefix[ls], lu = (t_lo - prefix[ls] * streams) / l_c;
+  int l_lo = prefix[ls] * streams + lu * l_c, l_hi = l_lo + l_c;
+  int s = ls;
+  // Lane b: TMA row y and attended rows cnt of box b of chunk t.
+  auto look_up = [&](int t, int& y, int& cnt) {
+    while (t >= l_hi) {
+      if (++lu == streams) {
+        lu = 0;
+        do ++ls; while (prefix[ls + 1] == prefix[ls]);
+        l_c = prefix[ls + 1] - prefix[ls];
       }
-      return min(t_hi, tb + min(C - c0, 32 / nbx));
-    };
-    int w = 0, slot = 0, issued = 0;   // next chunk: warp w, its stage `slot`
-    uint32_t ph = 0;
-    bool ok = true;
-    long long tb = t_lo, te = fetch(tb, y, cnt);
-    while (tb < t_hi && ok) {
-      long long tn = te;
-      if (te < t_hi) tn = fetch(te, y_n, cnt_n);
-      for (int c = 0; c < (int)(te - tb); ++c) {
-        uint32_t m = 0;
-        int loads = 0;
-        for (int b = 0; b < nbx; ++b) {
-          const int x = __shfl_sync(0xffffffffu, cnt, c * nbx + b);
-          m |= (uint32_t)x << (8 * b);
-          loads += x > 0;
-        }
-        const int st = w * DEPTH + slot;
-        if (!mbar_wait(&empty[st], ph ^ 1u, p.err, kDevErrWaitEmpty)) ok = false;
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) {
-          meta[st] = m;
-          if (loads)
-            mbar_arrive_expect_tx(&full[st], (uint32_t)(loads * box * 2 * NX * 128));
-          else
-            mbar_arrive(&full[st]);
-        }
-        __syncwarp();
-        const int b = lane / (2 * NX), kv = (lane / NX) & 1, x = lane % NX;
-        const int src = min(c * nbx + b, 31);
-        const int yb = __shfl_sync(0xffffffffu, y, src), cb = __shfl_sync(0xffffffffu, cnt, src);
-        if (b < nbx && cb > 0)
-          tma_load_2d(smem + st * Cfg::STAGE + kv * Cfg::HALF + x * (CH * 128) + b * box * 128,
-                      kv ? &tmv : &tmk, &full[st], x * (128 / (int)sizeof(T)), yb);
-        ++issued;
-        if (++w == WARPS) {
-          w = 0;
-          if (++slot == DEPTH) {
-            slot = 0;
-            ph ^= 1u;
-          }
-        }
-      }
-      tb = te;
-      te = tn;
-      y = y_n;
-      cnt = cnt_n;
+      l_lo = l_hi;
+      l_hi += l_c;
     }
-    // Every issued load lands before the CTA exits.
-    for (int k = max(0, issued - STAGES); k < issued; ++k)
-      mbar_wait(&full[(k % WARPS) * DEPTH + (k / WARPS) % DEPTH],
-                (uint32_t)((k / STAGES) & 1), p.err, kDevErrWaitFull);
-    return;
-  }
+    y = cnt = 0;
+    if (lane >= nbx) return;
+    const int g = lu / p.hblocks, past = past_s[ls];
+    const int nb = (past >> p.log2p) + 1;
+    const int list = p.sel ? min(p.n_sel, nb) : nb - p.skip;
+    const long long r = ((long long)(t - l_lo) * nbx + lane) << lbox;  // row of the stream
+    const int i = (int)(r >> p.log2p), off = (int)(r & (P - 1));
+    if (i >= list) return;
+    const int j = p.sel ? p.sel[((size_t)ls * p.n_kv + g) * p.n_sel + i] : p.skip + i;
+    if (j < 0 || j >= nb) return;
+    const int page = p.table[(size_t)ls * p.max_blocks + j];
+    if (page < 0 || page >= p.n_pages) {
+      record_error(p.err, kDevErrBadPage);
+      return;
+    }
+    cnt = max(0, min(box, past + 1 - ((j << p.log2p) + off)));
+    y = (int)(((p.page0 + page) * p.n_kv + g) << p.log2p) + off;
+  };
+  // Fills stage st with the chunk whose boxes lanes 0..nbx-1 looked up.
+  auto load = [&](int st, int y, int cnt) {
+    uint32_t m = 0;
+    int loads = 0;
+    for (int b = 0; b < nbx; ++b) {
+      const int x = __shfl_sync(0xffffffffu, cnt, b);
+      m |= (uint32_t)x << (8 * b);
+      loads += x > 0;
+    }
+    if (lane == 0) {
+      meta[st] = m;
+      if (loads)
+        mbar_arrive_expect_tx(&full[st], (uint32_t)(loads * box * 2 * NX * 128));
+      else
+        mbar_arrive(&full[st]);
+    }
+    for (int b = 0; b < nbx; ++b) {
+      const int yb = __shfl_sync(0xffffffffu, y, b);
+      if (lane == 0 && ((m >> (8 * b)) & 255u)) {
+        uint8_t* to = smem + st * Cfg::STAGE + b * box * 128;
+#pragma unroll
+        for (int x = 0; x < NX; ++x) {
+          tma_load_2d(to + x * (CH * 128), &tmk, &full[st], x * (128 / (int)sizeof(T)), yb);
+          tma_load_2d(to + Cfg::HALF + x * (CH * 128), &tmv, &full[st],
+                      x * (128 / (int)sizeof(T)), yb);
+        }
+      }
+    }
+    __syncwarp();
+  };
 
-  // -------------------------------------------------------------- consumers
-  constexpr int NCT = Cfg::CTHREADS;
   const int r = lane >> 2, qd = lane & 3;
   float* my_mrg = mrg + warp * Cfg::MRG;
   const float sl2 = p.scale_log2;
+  int ti = t_lo + warp;   // this warp's next chunk to compute
+  int tl = ti;            // ... to load
+  int tn_y = 0, tn_cnt = 0;
+  if (tl < t_hi) look_up(tl, tn_y, tn_cnt);
+#pragma unroll 1
+  for (int i = 0; i < DEPTH; ++i) {
+    if (tl >= t_hi) break;
+    load(warp * DEPTH + i, tn_y, tn_cnt);
+    tl += WARPS;
+    if (tl < t_hi) look_up(tl, tn_y, tn_cnt);
+  }
   bool failed = false;
-  int s = s_first;
-  int ki = warp;                               // this warp's next chunk, counted from t_lo
   int slot = 0;
   uint32_t ph = 0;
   uint32_t qa[kHalf ? HD / 16 : HD / 8][4];
   float o[HD / 8][4];
-  for (long long t = t_lo; t < t_hi;) {
-    while ((long long)prefix[s + 1] * streams <= t) ++s;
+  for (int t = t_lo; t < t_hi;) {
+    while (prefix[s + 1] * streams <= t) ++s;
     const int C = prefix[s + 1] - prefix[s];
-    const long long q_base = (long long)prefix[s] * streams;
-    const int u = (int)((t - q_base) / C);
-    const long long s_lo = q_base + (long long)u * C, s_hi = s_lo + C, e_hi = min(t_hi, s_hi);
+    const int q_base = prefix[s] * streams;
+    const int u = (t - q_base) / C;
+    const int s_lo = q_base + u * C, s_hi = s_lo + C, e_hi = min(t_hi, s_hi);
     const int g = u / p.hblocks, hb = u - g * p.hblocks;
     const int heads = min(kPagedHeads, p.group - hb * kPagedHeads);
     {
@@ -987,12 +966,12 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     for (int c = 0; c < HD / 8; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
     float m_run = kNegBig, l_run = 0.f;
 
-    const int k_end = (int)(e_hi - t_lo);
-    for (; ki < k_end; ki += WARPS) {
+    for (; ti < e_hi; ti += WARPS) {
       const int st = warp * DEPTH + slot;
       if (!failed && !mbar_wait(&full[st], ph, p.err, kDevErrWaitFull)) failed = true;
+      failed = __any_sync(0xffffffffu, failed);
       const uint32_t cm = meta[st];
-      if (!__any_sync(0xffffffffu, failed) && cm != 0) {
+      if (!failed && cm != 0) {
         uint8_t* kbox = smem + st * Cfg::STAGE;
         uint8_t* vbox = kbox + Cfg::HALF;
         const bool whole = cm == cnt_full;
@@ -1123,7 +1102,11 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[st]);
+      if (tl < t_hi && !failed) {
+        load(st, tn_y, tn_cnt);
+        tl += WARPS;
+        if (tl < t_hi) look_up(tl, tn_y, tn_cnt);
+      }
       if (++slot == DEPTH) {
         slot = 0;
         ph ^= 1u;
@@ -1174,13 +1157,20 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
       consumers_sync(NCT);
       if (*flag) {
         __threadfence();
-        merge_parts_vec<HD, NCT>(p, fin, heads, 2 * c1 + (cta_tile_lo(c1, G, T_all) == s_lo ? 0 : 1),
+        merge_parts_vec<HD, NCT>(p, fin, heads, 2 * c1 + ((int)cta_tile_lo(c1, G, T_all) == s_lo ? 0 : 1),
                                  c1, c2 - c1 + 1, threadIdx.x, mrg);
         if (threadIdx.x == 0) *count = 0;
       }
     }
     consumers_sync(NCT);
     t = e_hi;
+  }
+  if (failed) {
+    // Loads still in flight land (bounded) before the CTA exits.
+    for (int i = 0; i < DEPTH; ++i) {
+      mbar_wait(&full[warp * DEPTH + i], 0, p.err, kDevErrWaitFull);
+      mbar_wait(&full[warp * DEPTH + i], 1, p.err, kDevErrWaitFull);
+    }
   }
 }
 
