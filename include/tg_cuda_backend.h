@@ -495,9 +495,10 @@ TG_API int tg_attention_noalloc(void* cuda_stream, const float* q, const void* k
  * Block tables are [n_seqs][max_blocks] int32: entry j of row s is the page
  * of positions j*page_size.. of sequence s.  Entries that a call needs must
  * lie in [0, n_pages): host arrays are checked, device arrays by the
- * kernels, which leave such an entry's rows out (tg_paged_select ranks it
- * last) and report device error 0x106; 0x103 reports a position outside the
- * table or the rotation table, whose query counts as empty.  Several tokens
+ * kernels, which access nothing outside the pool and report device error
+ * 0x106 (the queries concerned have no result); 0x103 reports a position
+ * outside the table or the rotation table, whose query counts as empty.
+ * Several tokens
  * of one sequence in a call are several rows with the same entries.  A page
  * that tg_paged_append writes belongs to one sequence only.
  * Pointer and stream rules are those of the batched calls above; calls on

@@ -231,6 +231,7 @@ struct tg_context {
   float* ppart = nullptr;                 size_t ppart_cap = 0;   // floats
   unsigned* pcount = nullptr;             size_t pcount_cap = 0;  // zero between launches
   unsigned long long* pkeys = nullptr;    size_t pkeys_cap = 0;
+  float* prec = nullptr;                  size_t prec_cap = 0;    // floats
   std::vector<void*> kept;
 
   // Optional CUDA-event timing of each decode-attention kernel launch.
@@ -1627,14 +1628,25 @@ int check_host_pages(const tg_paged_kv* pk, const int32_t* past, const int32_t* 
   return TG_OK;
 }
 
+// Whether the tensor-core kernel takes a shared prefix (see run_paged).
+bool use_prefix(int n, int group, int shared_len) {
+  return n >= 2 && shared_len >= 256;
+}
+
 // Attention launches on device pointers, kPagedMaxQueries queries at a time.
 int run_paged(tg_context* ctx, const tg_paged_kv* pk, int layer, int n, const float* q,
               const int* past, const int* table, int max_blocks, const int* sel, int n_sel,
-              float* out) {
+              int shared_len, float* out) {
   TG_TRY(commit_inputs(ctx));
   TG_TRY(check_align8(q, "q"));
   TG_TRY(check_align8(out, "out"));
   const tg_paged_desc& d = pk->d;
+  // The part of a shared prefix that the tensor-core kernel takes, in its
+  // steps: whole steps of whole pages.
+  const int unit = std::max(d.page_size, tg::kPrefixKeys);
+  const bool prefix = pk->tmap_ok && d.dtype == TG_DTYPE_BF16 && d.head_dim == 64 &&
+                      use_prefix(n, d.n_head / d.n_kv_head, shared_len);
+  const int shared = prefix ? shared_len / unit * unit : 0;
   const int qdim = d.n_head * d.head_dim;
   tg::PagedAttnParams p{};
   p.kp = pk->k + (size_t)layer * pk->layer_elems * pk->esize;
@@ -1674,13 +1686,50 @@ int run_paged(tg_context* ctx, const tg_paged_kv* pk, int layer, int n, const fl
     p.part = ctx->ppart;
     p.count = ctx->pcount;
     cudaEvent_t ev = nullptr;
+    tg::PagedPrefixParams x{};
+    if (shared > 0) {
+      x.q = p.q;
+      x.past = p.past;
+      x.table = table;
+      x.out = p.out;
+      x.err = ctx->d_err;
+      x.page0 = p.page0;
+      x.n = p.n;
+      x.n_head = p.n_head;
+      x.n_kv = p.n_kv;
+      x.group = p.group;
+      x.n_pages = p.n_pages;
+      x.log2p = p.log2p;
+      x.steps = shared / tg::kPrefixKeys;
+      x.scale_log2 = p.scale_log2;
+      tg::plan_paged_prefix(&x, ctx->num_sms);
+      const size_t rec = (size_t)p.n * p.n_head * (p.hd + 2);
+      TG_TRY(ensure_kept(ctx, &ctx->prec, &ctx->prec_cap, (size_t)(x.parts + 1) * rec));
+      x.own = ctx->prec;
+      x.records = ctx->prec + rec;
+      p.mode = 1;
+      p.records = ctx->prec;
+      p.skip = shared >> p.log2p;
+    }
     TG_TRY(prof_begin(ctx, TG_PROFILE_ATTENTION, &ev));
+    if (shared > 0) {
+      cudaError_t e = tg::launch_paged_prefix(pk->tmk, pk->tmv, x, ctx->stream);
+      if (e != cudaSuccess)
+        return fail(TG_ERR_CUDA, "paged prefix launch: %s", cudaGetErrorString(e));
+      ctx->launches++;
+    }
     cudaError_t e = pk->tmap_ok
                         ? tg::launch_paged_mma(pk->tmk, pk->tmv, p, d.dtype, grid, ctx->stream)
                         : tg::launch_paged_core(p, d.dtype, grid, ctx->stream);
     if (e != cudaSuccess)
       return fail(TG_ERR_CUDA, "paged attention launch: %s", cudaGetErrorString(e));
     ctx->launches++;
+    if (shared > 0) {
+      e = tg::launch_paged_prefix_merge(x, ctx->stream);
+      if (e != cudaSuccess)
+        return fail(TG_ERR_CUDA, "paged merge launch: %s", cudaGetErrorString(e));
+      ctx->launches++;
+    }
     TG_TRY(prof_end(ctx, ev));
   }
   return TG_OK;
@@ -1770,6 +1819,7 @@ int tg_shutdown(tg_context* ctx) {
   cudaFree(ctx->ppart);
   cudaFree(ctx->pcount);
   cudaFree(ctx->pkeys);
+  cudaFree(ctx->prec);
   for (void* b : ctx->kept) cudaFree(b);
   for (auto& kv : ctx->regions) cudaFree(kv.second.dev);
   for (RopeTable& t : ctx->tables) cudaFree(t.d);
@@ -3142,10 +3192,9 @@ int paged_attention(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, con
   TG_TRY(stage_in(ctx, block_table, (size_t)n_seqs * max_blocks * 4, &dt));
   if (pages) TG_TRY(stage_in(ctx, pages, (size_t)n_seqs * d.n_kv_head * n_sel * 4, &dsel));
   TG_TRY(stage_out(ctx, out, qb, false, &dout));
-  (void)shared_len;
   TG_TRY(run_paged(ctx, pk, layer, n_seqs, static_cast<const float*>(dq),
                    static_cast<const int*>(dp), static_cast<const int*>(dt), max_blocks,
-                   static_cast<const int*>(dsel), n_sel, static_cast<float*>(dout)));
+                   static_cast<const int*>(dsel), n_sel, shared_len, static_cast<float*>(dout)));
   return finish_call(ctx);
 }
 }  // namespace

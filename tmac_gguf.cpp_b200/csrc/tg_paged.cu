@@ -270,8 +270,14 @@ __device__ __forceinline__ int query_blocks(const PagedAttnParams& p, int past, 
   return nb;
 }
 
-__device__ __forceinline__ int query_chunks(const PagedAttnParams& p, int nb) {
-  const int list = p.sel ? min(p.n_sel, nb) : max(0, nb - p.skip);
+// First table entry of a query's list: those before it are attended elsewhere
+// by the queries that attend all of them.
+__device__ __forceinline__ int query_skip(const PagedAttnParams& p, int past) {
+  return ((long long)past + 1) >= ((long long)p.skip << p.log2p) ? p.skip : 0;
+}
+
+__device__ __forceinline__ int query_chunks(const PagedAttnParams& p, int past, int nb) {
+  const int list = p.sel ? min(p.n_sel, nb) : nb - min(nb, query_skip(p, past));
   return (int)((((long long)list << p.log2p) + (1 << p.lchunk) - 1) >> p.lchunk);
 }
 
@@ -286,7 +292,7 @@ __device__ void paged_schedule(const PagedAttnParams& p, int* prefix, int* past_
     const int past = p.past[s];
     const int nb = query_blocks(p, past, blockIdx.x == 0);
     past_s[s] = nb > 0 ? past : -1;
-    const int c = query_chunks(p, nb);
+    const int c = query_chunks(p, past, nb);
     prefix[s + 1] = c;
     sum += c;
   }
@@ -504,7 +510,8 @@ __global__ void __launch_bounds__(kCoreThreads) paged_core_kernel(const PagedAtt
     const int heads = min(kPagedHeads, p.group - hb * kPagedHeads);
     const int past = past_s[s];
     const int nb = (past >> p.log2p) + 1;
-    const int list = p.sel ? min(p.n_sel, nb) : nb - p.skip;
+    const int skip = query_skip(p, past);
+    const int list = p.sel ? min(p.n_sel, nb) : nb - skip;
     const int* sel = p.sel ? p.sel + ((size_t)s * p.n_kv + g) * p.n_sel : nullptr;
     const int* table = p.table + (size_t)s * p.max_blocks;
 
@@ -528,7 +535,7 @@ __global__ void __launch_bounds__(kCoreThreads) paged_core_kernel(const PagedAtt
       bool ok = i < list;
       size_t row = 0;
       if (ok) {
-        const int j = sel ? sel[i] : p.skip + i;
+        const int j = sel ? sel[i] : skip + i;
         ok = j >= 0 && j < nb && (long long)j * P + slot <= past;
         if (ok) {
           const int page = table[j];
@@ -865,11 +872,12 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     if (lane >= nbx) return;
     const int g = lu / p.hblocks, past = past_s[ls];
     const int nb = (past >> p.log2p) + 1;
-    const int list = p.sel ? min(p.n_sel, nb) : nb - p.skip;
+    const int skip = query_skip(p, past);
+    const int list = p.sel ? min(p.n_sel, nb) : nb - skip;
     const long long r = ((long long)(t - l_lo) * nbx + lane) << lbox;  // row of the stream
     const int i = (int)(r >> p.log2p), off = (int)(r & (P - 1));
     if (i >= list) return;
-    const int j = p.sel ? p.sel[((size_t)ls * p.n_kv + g) * p.n_sel + i] : p.skip + i;
+    const int j = p.sel ? p.sel[((size_t)ls * p.n_kv + g) * p.n_sel + i] : skip + i;
     if (j < 0 || j >= nb) return;
     const int page = p.table[(size_t)ls * p.max_blocks + j];
     if (page < 0 || page >= p.n_pages) {

@@ -42,8 +42,8 @@ struct PagedAppendParams {
 
 // Decode attention.  A stream is one query's block of up to kPagedHeads query
 // heads over one KV head; its rows are the rows of a list of pages: entries
-// skip, skip + 1, ... of the query's table row (dense), or the listed ones
-// (sel).  The rows form chunks of 16 or 32; the chunks of all streams lie
+// skip, skip + 1, ... of the query's table row (dense; skip 0 for a query that
+// ends before entry skip), or the listed ones (sel).  The rows form chunks of 16 or 32; the chunks of all streams lie
 // end to end and every CTA takes an equal contiguous range of them.
 struct PagedAttnParams {
   const float* q;        // [n][n_head*hd], rotated
@@ -59,7 +59,8 @@ struct PagedAttnParams {
   int* err;
   long long page0;       // pages before this layer's (TMA rows)
   int n, n_head, n_kv, group, hblocks, hd;
-  int max_blocks, n_pages, log2p, n_sel, skip;
+  int max_blocks, n_pages, log2p, n_sel;
+  int skip;              // leading entries left out for queries that attend all of them
   int lchunk;            // log2 of the rows of a chunk
   float scale_log2;      // log2(e) / sqrt(hd)
   int mode;              // 0 output, 1 records
@@ -76,6 +77,29 @@ struct PagedSelectParams {
   int n, n_head, n_kv, group, hd, dtype;
   int max_blocks, n_pages, log2p, n_sel, keep_first, keep_last;
 };
+
+// The shared prefix of a batch on the tensor cores (tg_paged_prefix.cu): bf16
+// pool, head_dim 64.  steps * kPrefixKeys positions, named by table row 0.
+constexpr int kPrefixKeys = 64;
+struct PagedPrefixParams {
+  const float* q;        // [n][n_head*64], rotated
+  const int* past;       // [n]
+  const int* table;      // pages of the prefix
+  float* records;        // [parts][n][n_head][66] o (un-normalised), m, l
+  const float* own;      // [n][n_head][66] records of the queries' own rows
+  float* out;            // [n][n_head*64]
+  int* err;
+  long long page0;
+  int n, n_head, n_kv, group, n_pages, log2p, steps;
+  int single, pairs, splits, parts;   // plan_paged_prefix
+  float scale_log2;
+};
+
+// Chooses single / pairs / splits / parts from n, group, n_kv and steps.
+void plan_paged_prefix(PagedPrefixParams* p, int num_sms);
+cudaError_t launch_paged_prefix(const CUtensorMap& tk, const CUtensorMap& tv,
+                                const PagedPrefixParams& p, cudaStream_t st);
+cudaError_t launch_paged_prefix_merge(const PagedPrefixParams& p, cudaStream_t st);
 
 cudaError_t launch_paged_append(const PagedAppendParams& p, cudaStream_t st);
 cudaError_t launch_paged_core(const PagedAttnParams& p, int dtype, int grid, cudaStream_t st);

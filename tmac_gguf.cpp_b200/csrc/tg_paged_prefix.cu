@@ -1,0 +1,461 @@
+// tg_paged_prefix.cu -- decode attention over the shared prefix of a batch on
+// the 5th-generation tensor cores (tcgen05 + TMEM), and the merge of its
+// softmax records with those of the queries' own rows (tg_paged.cu).  No
+// counterpart in the reference, which decodes one sequence at a time.
+//
+// The queries of one KV head over the same keys are a matrix: row
+// s * group + h of n * group rows.  For 128 rows x 64 keys the products
+// S = Q K^T and O += P V run on tcgen05, and a key is read once for 256 rows
+// instead of once for 8.
+//
+// Results have to be those of binary32 products, as everywhere else in the
+// paged cache: q and the probabilities are each split into two bf16, hi + lo
+// (17 significant bits), against the exact bf16 keys and values, which
+// doubles the tensor work.  What a 128 x 128 block costs an SM then: 1024
+// cycles of tensor core (4 x 128 x 128 x 64 multiply-adds at 4096 per cycle),
+// 1024 cycles of ex2 (16 per cycle), about 900 of instruction issue for the
+// splits: all three have to overlap.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "tg_device.cuh"
+#include "tg_paged.h"
+#include "tg_shared.h"
+#include "tg_tc.cuh"
+
+namespace tg {
+
+constexpr int PX_ROWS = 128;        // query rows of a slot (TMEM lanes)
+constexpr int PX_KEYS = 64;         // keys of a step
+constexpr int PX_STAGES = 12;       // K/V ring
+constexpr int PX_THREADS = 384;     // TMA warp, MMA warp, 2 idle, 2 x 4 softmax warps
+constexpr int PX_TILE = PX_KEYS * 128;           // bytes of a K (or V) tile
+constexpr int PX_OFF_BAR = PX_STAGES * 2 * PX_TILE;
+// kv_full[S], kv_empty[S], q_full, s_full[slot][buf], p_full[slot][buf], pv_done[slot]
+constexpr int PX_NBAR = 2 * PX_STAGES + 1 + 4 + 4 + 2;
+constexpr int PX_OFF_MISC = PX_OFF_BAR + PX_NBAR * 8;
+constexpr size_t PX_SMEM = 1024 + PX_OFF_MISC + 16;
+constexpr uint32_t PX_COLS = 512;
+// TMEM columns of slot x from 256 x: two buffers of 64 (S as binary32, then P
+// in its place: 32 columns hi, 32 lo, two bf16 each), O 64, Q 64 (hi, lo).
+__device__ __forceinline__ uint32_t px_s(int x, int buf) { return 256u * x + 64u * buf; }
+__device__ __forceinline__ uint32_t px_o(int x) { return 256u * x + 128u; }
+__device__ __forceinline__ uint32_t px_q(int x) { return 256u * x + 192u; }
+
+__device__ __forceinline__ bool px_wait(uint64_t* bar, uint32_t parity, int* err,
+                                        volatile int* abort_flag) {
+  if (*abort_flag) return false;
+  if (mbar_wait(bar, parity, err, kDevErrWaitFull)) return true;
+  *abort_flag = 1;
+  return false;
+}
+
+__device__ __forceinline__ bool px_wait_warp(uint64_t* bar, uint32_t parity, int* err,
+                                             volatile int* abort_flag) {
+  const bool got = px_wait(bar, parity, err, abort_flag);
+  return __all_sync(0xffffffffu, got) != 0;
+}
+
+// Two floats as the upper halves (truncated bf16) of one register, lo first,
+// and what is left of them as a second one (rounded): off by at most 2^-16.
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+  hi = __byte_perm(ua, ub, 0x7632);
+  lo = pack_bf16x2(a - __uint_as_float(ua & 0xffff0000u), b - __uint_as_float(ub & 0xffff0000u));
+}
+
+// One CTA: 256 query rows of a KV head (two slots of 128) x a range of the
+// prefix's keys, both slots over the same keys.  With at most 128 rows
+// (p.single) both slots hold the same rows and each takes half of the keys.
+//   warp 0      TMA: K and V tiles of 64 keys (boxes of min(page, 32) rows,
+//               128-byte swizzle) into a ring; the pages of the next tile are
+//               looked up while this one is issued.
+//   warp 1      owns TMEM; one thread issues the products.  S of step j + 2
+//               goes into the buffer that P of step j has just been read
+//               from (products of one thread run in their order), so S is
+//               ready when a softmax warp comes for it.
+//   warps 4-11  softmax, a thread per query row: S to registers, running
+//               maximum (the exponent's base moves only when the maximum
+//               grew by more than 2^8; then O is rescaled in TMEM), P = 2^(S
+//               - m) split into hi and lo in place of S.
+// Every wait is bounded; a failed one raises the abort flag, every role
+// leaves its loop, issued loads and products are drained and TMEM is freed.
+__global__ void __launch_bounds__(PX_THREADS, 1)
+    paged_prefix_kernel(const __grid_constant__ CUtensorMap tmk,
+                        const __grid_constant__ CUtensorMap tmv, const PagedPrefixParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PX_OFF_BAR);
+  uint64_t* kv_full = bars;
+  uint64_t* kv_empty = kv_full + PX_STAGES;
+  uint64_t* q_full = kv_empty + PX_STAGES;
+  uint64_t* s_full = q_full + 1;   // [slot * 2 + buf]
+  uint64_t* p_full = s_full + 4;   // [slot * 2 + buf]
+  uint64_t* pv_done = p_full + 4;  // [slot]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + PX_OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + PX_OFF_MISC + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  griddep_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < PX_STAGES; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    mbar_init(q_full, 8);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+    }
+    mbar_init(&pv_done[0], 1);
+    mbar_init(&pv_done[1], 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmk);
+    tma_prefetch_desc(&tmv);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(PX_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_wait();
+
+  // Item: KV head, pair of row tiles, range of key steps.
+  const int split = blockIdx.x % p.splits, gp = blockIdx.x / p.splits;
+  const int g = gp / p.pairs, pair = gp - g * p.pairs;
+  const int k0 = (int)((long long)split * p.steps / p.splits);
+  const int k1 = (int)((long long)(split + 1) * p.steps / p.splits);
+  const int rows = p.n * p.group;
+  const bool both = p.single || (2 * pair + 1) * PX_ROWS < rows;   // slot 1 has rows
+  // Steps of the slots, and the tile (from k0) of ring entry i.
+  const int n0 = p.single ? (k1 - k0 + 1) / 2 : k1 - k0;
+  const int n1 = p.single ? (k1 - k0) / 2 : (both ? k1 - k0 : 0);
+  const int entries = k1 - k0;
+  auto tile_of = [&](int i) { return p.single ? ((i & 1) ? n0 + (i >> 1) : i >> 1) : i; };
+
+  if (warp == 0) {
+    // ---------------------------------------------------------- TMA
+    const int box = min(1 << p.log2p, 32), lbox = min(p.log2p, 5), nbx = PX_KEYS >> lbox;
+    auto look_up = [&](int i) -> int {   // lane b: TMA row of box b of entry i
+      if (lane >= nbx) return 0;
+      const int r = (k0 + tile_of(i)) * PX_KEYS + (lane << lbox);
+      int page = p.table[r >> p.log2p];
+      if (page < 0 || page >= p.n_pages) {
+        record_error(p.err, kDevErrBadPage);
+        page = 0;
+      }
+      return (int)(((p.page0 + page) * p.n_kv + g) << p.log2p) + (r & ((1 << p.log2p) - 1));
+    };
+    int y = entries > 0 ? look_up(0) : 0, issued = 0;
+    for (int i = 0; i < entries; ++i) {
+      const int y_n = i + 1 < entries ? look_up(i + 1) : 0;
+      const int st = i % PX_STAGES;
+      if (!px_wait_warp(&kv_empty[st], (uint32_t)(((i / PX_STAGES) & 1) ^ 1), p.err, abort_flag))
+        break;
+      if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], 2 * PX_TILE);
+      uint8_t* to = smem + st * 2 * PX_TILE;
+      for (int b = 0; b < nbx; ++b) {
+        const int yb = __shfl_sync(0xffffffffu, y, b);
+        if (lane == 0) {
+          tma_load_2d(to + b * box * 128, &tmk, &kv_full[st], 0, yb);
+          tma_load_2d(to + PX_TILE + b * box * 128, &tmv, &kv_full[st], 0, yb);
+        }
+      }
+      y = y_n;
+      ++issued;
+    }
+    for (int i = max(0, issued - PX_STAGES); i < issued; ++i)
+      mbar_wait(&kv_full[i % PX_STAGES], (uint32_t)((i / PX_STAGES) & 1), p.err, kDevErrWaitFull);
+  } else if (warp == 1) {
+    // ---------------------------------------------------------- products
+    if (lane == 0) {
+      constexpr uint32_t IDESC_QK = idesc_bf16(PX_ROWS, PX_KEYS, false);
+      constexpr uint32_t IDESC_PV = idesc_bf16(PX_ROWS, 64, true);
+      const uint64_t dk0 = smem_desc_sw128(smem_u32(smem), 16, 1024);
+      const uint64_t dv0 = smem_desc_sw128(smem_u32(smem) + PX_TILE, PX_TILE, 1024);
+      const int n_x[2] = {n0, n1};
+      bool ok = px_wait(q_full, 0, p.err, abort_flag);
+      int last = -1;   // slot of the last product issued
+      auto entry = [&](int x, int j) { return p.single ? 2 * j + x : j; };
+      auto issue_qk = [&](int x, int j) -> bool {
+        const int i = entry(x, j), st = i % PX_STAGES;
+        if (!px_wait(&kv_full[st], (uint32_t)((i / PX_STAGES) & 1), p.err, abort_flag)) return false;
+        tc_fence_after();
+        const uint64_t b = dk0 + (uint64_t)(st * (2 * PX_TILE >> 4));
+        const uint32_t d = tmem + px_s(x, j & 1), a = tmem + px_q(x);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)   // 4 steps of 16 dimensions, hi then lo
+          umma_f16_ts(d, a + 8 * kk, b + 2 * (kk & 3), IDESC_QK, kk > 0 ? 1u : 0u);
+        umma_commit(&s_full[2 * x + (j & 1)]);
+        last = x;
+        return true;
+      };
+      auto issue_pv = [&](int x, int j) -> bool {
+        const int i = entry(x, j), st = i % PX_STAGES;
+        if (!px_wait(&p_full[2 * x + (j & 1)], (uint32_t)((j >> 1) & 1), p.err, abort_flag))
+          return false;
+        tc_fence_after();
+        const uint64_t b = dv0 + (uint64_t)(st * (2 * PX_TILE >> 4));
+        const uint32_t d = tmem + px_o(x), a = tmem + px_s(x, j & 1);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)   // 4 steps of 16 keys, hi then lo
+          umma_f16_ts(d, a + 8 * kk, b + 128 * (kk & 3), IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&pv_done[x]);
+        if (p.single || x == 1 || n1 == 0) umma_commit(&kv_empty[st]);
+        last = x;
+        return true;
+      };
+      for (int j = 0; j < 2; ++j)
+        for (int x = 0; x < 2; ++x)
+          if (ok && j < n_x[x]) ok = issue_qk(x, j);
+      for (int j = 0; j < n0 && ok; ++j)
+        for (int x = 0; x < 2 && ok; ++x)
+          if (j < n_x[x]) {
+            ok = issue_pv(x, j);
+            if (ok && j + 2 < n_x[x]) ok = issue_qk(x, j + 2);
+          }
+      // Everything issued has completed before TMEM is freed (q_full is
+      // done with: its second phase counts this commit and 7 arrivals).
+      if (last >= 0) {
+        for (int i = 0; i < 7; ++i) mbar_arrive(q_full);
+        umma_commit(q_full);
+        mbar_wait(q_full, 1, p.err, kDevErrWaitFull);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ---------------------------------------------------------- softmax
+    const int x = (warp - 4) >> 2, quarter = warp & 3;
+    const int row = (p.single ? 0 : (2 * pair + x) * PX_ROWS) + quarter * 32 + lane;
+    const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16);
+    const int steps = x ? n1 : n0;
+    const int s = row / p.group, h = g * p.group + row - s * p.group;
+    {
+      // This row of Q, scaled to log2 units, as hi and lo.
+      uint32_t w[64];
+      const float* q = p.q + ((size_t)(row < rows ? s : 0) * p.n_head + (row < rows ? h : 0)) * 64;
+#pragma unroll
+      for (int c = 0; c < 32; ++c) {
+        const float2 v = row < rows ? *reinterpret_cast<const float2*>(q + 2 * c) : make_float2(0.f, 0.f);
+        float h0, l0, h1, l1;
+        split_bf16(v.x * p.scale_log2, h0, l0);
+        split_bf16(v.y * p.scale_log2, h1, l1);
+        w[c] = pack_bf16x2(h0, h1);
+        w[32 + c] = pack_bf16x2(l0, l1);
+      }
+      TG_TMEM_ST64(base + px_q(x), w);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+    constexpr float kLazy = 8.f;
+    float m = kNegBig, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < steps; ++j) {
+      const int b = j & 1;
+      if (!px_wait_warp(&s_full[2 * x + b], (uint32_t)((j >> 1) & 1), p.err, abort_flag)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t sv[64];
+      TG_TMEM_LD64(base + px_s(x, b), sv);
+      float mx8[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) mx8[c] = __uint_as_float(sv[c]);
+#pragma unroll
+      for (int c = 8; c < 64; ++c) mx8[c & 7] = fmaxf(mx8[c & 7], __uint_as_float(sv[c]));
+      const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
+                             fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+      float alpha = 1.f;
+      if (j == 0) {
+        m = fmaxf(mx, kNegBig);
+      } else if (mx - m > kLazy) {
+        alpha = ex2(m - mx);
+        m = mx;
+      }
+      if (__any_sync(0xffffffffu, alpha != 1.f)) {
+        // O of the steps before this one is complete, and the next product
+        // on it waits for this step's P.
+        if (!px_wait_warp(&pv_done[x], (uint32_t)((j - 1) & 1), p.err, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll 1
+        for (int c0 = 0; c0 < 64; c0 += 32) {
+          uint32_t ov[32];
+          TG_TMEM_LD32(base + px_o(x) + c0, ov);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
+          TG_TMEM_ST32(base + px_o(x) + c0, ov);
+        }
+      }
+      float ls[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t w[64];
+#pragma unroll
+      for (int c = 0; c < 32; ++c) {
+        const float p0 = ex2(__uint_as_float(sv[2 * c]) - m);
+        const float p1 = ex2(__uint_as_float(sv[2 * c + 1]) - m);
+        ls[c & 3] += p0 + p1;
+        split_pair(p0, p1, w[c], w[32 + c]);
+      }
+      TG_TMEM_ST64(base + px_s(x, b), w);
+      l = l * alpha + ((ls[0] + ls[1]) + (ls[2] + ls[3]));
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[2 * x + b]);
+    }
+    uint32_t ov[64];
+    // The last two products in turn: a parity tells a phase only from its
+    // neighbours (s_full of the last step covers those before).
+    for (int j = max(0, steps - 2); j < steps && ok; ++j)
+      ok = px_wait_warp(&pv_done[x], (uint32_t)(j & 1), p.err, abort_flag);
+    if (ok && steps > 0) {
+      tc_fence_after();
+      TG_TMEM_LD64(base + px_o(x), ov);
+      tc_fence_before();
+    } else {
+#pragma unroll
+      for (int c = 0; c < 64; ++c) ov[c] = 0u;
+      m = kNegBig;
+      l = 0.f;
+    }
+    if (row < rows) {
+      const int part = p.single ? 2 * split + x : split;
+      float* rec = p.records + (((size_t)part * p.n + s) * p.n_head + h) * 66;
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        *reinterpret_cast<float2*>(rec + 2 * c) =
+            make_float2(__uint_as_float(ov[2 * c]), __uint_as_float(ov[2 * c + 1]));
+      *reinterpret_cast<float2*>(rec + 64) = make_float2(m, l);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(PX_COLS)
+                 : "memory");
+  }
+}
+
+// out of every (query, head): the records of the prefix (for queries that
+// attend all of it) and the record of the query's own rows.  A warp each,
+// two dimensions per lane.
+constexpr int kPrefixMergeWarps = 4;
+
+__global__ void __launch_bounds__(32 * kPrefixMergeWarps)
+    paged_prefix_merge_kernel(const PagedPrefixParams p) {
+  constexpr int B = 8;
+  griddep_launch_dependents();
+  griddep_wait();
+  const int lane = threadIdx.x & 31;
+  const int i = blockIdx.x * kPrefixMergeWarps + (threadIdx.x >> 5);  // (query, head)
+  if (i >= p.n * p.n_head) return;
+  const int s = i / p.n_head;
+  const float* own = p.own + (size_t)i * 66;
+  float M = own[64], L = own[65];
+  float2 O = *reinterpret_cast<const float2*>(own + 2 * lane);
+  const int parts = p.past[s] + 1 >= p.steps * PX_KEYS ? p.parts : 0;
+  for (int k0 = 0; k0 < parts; k0 += B) {
+    float2 o[B], ml[B];
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      ml[u] = make_float2(kNegBig, 0.f);
+      o[u] = make_float2(0.f, 0.f);
+      if (k0 + u < parts) {
+        const float* r = p.records + ((size_t)(k0 + u) * p.n * p.n_head + i) * 66;
+        o[u] = *reinterpret_cast<const float2*>(r + 2 * lane);
+        ml[u] = *reinterpret_cast<const float2*>(r + 64);
+      }
+    }
+    float mb = M;
+#pragma unroll
+    for (int u = 0; u < B; ++u) mb = fmaxf(mb, ml[u].x);
+    const float w0 = ex2(M - mb);
+    M = mb;
+    L *= w0;
+    O.x *= w0;
+    O.y *= w0;
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const float w = ex2(ml[u].x - M);
+      L = fmaf(ml[u].y, w, L);
+      O.x = fmaf(o[u].x, w, O.x);
+      O.y = fmaf(o[u].y, w, O.y);
+    }
+  }
+  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+  *reinterpret_cast<float2*>(p.out + (size_t)i * 64 + 2 * lane) = make_float2(O.x * inv, O.y * inv);
+}
+
+// ------------------------------------------------------------ launches
+
+static cudaError_t launch_prefix_pdl(const void* fn, dim3 grid, dim3 block, size_t smem,
+                                     cudaStream_t st, void** args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelExC(&cfg, fn, args);
+}
+
+cudaError_t launch_paged_prefix(const CUtensorMap& tk, const CUtensorMap& tv,
+                                const PagedPrefixParams& p, cudaStream_t st) {
+  static bool done[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!done[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(paged_prefix_kernel,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PX_SMEM);
+    if (e != cudaSuccess) return e;
+    done[dev] = true;
+  }
+  void* args[] = {const_cast<CUtensorMap*>(&tk), const_cast<CUtensorMap*>(&tv),
+                  const_cast<PagedPrefixParams*>(&p)};
+  return launch_prefix_pdl(reinterpret_cast<const void*>(paged_prefix_kernel),
+                           dim3((unsigned)(p.n_kv * p.pairs * p.splits)), dim3(PX_THREADS), PX_SMEM,
+                           st, args);
+}
+
+cudaError_t launch_paged_prefix_merge(const PagedPrefixParams& p, cudaStream_t st) {
+  void* args[] = {const_cast<PagedPrefixParams*>(&p)};
+  const int items = p.n * p.n_head;
+  return launch_prefix_pdl(reinterpret_cast<const void*>(paged_prefix_merge_kernel),
+                           dim3((unsigned)((items + kPrefixMergeWarps - 1) / kPrefixMergeWarps)),
+                           dim3(32 * kPrefixMergeWarps), 0, st, args);
+}
+
+void plan_paged_prefix(PagedPrefixParams* p, int num_sms) {
+  const int tiles = (p->n * p->group + PX_ROWS - 1) / PX_ROWS;
+  p->single = tiles == 1 ? 1 : 0;
+  p->pairs = (tiles + 1) / 2;
+  // One CTA per SM where the rows leave room for it, each with at least 2
+  // steps per slot.
+  const int most = p->steps / (p->single ? 4 : 2);
+  p->splits = num_sms / (p->n_kv * p->pairs);
+  if (p->splits > most) p->splits = most;
+  if (p->splits < 1) p->splits = 1;
+  p->parts = p->single ? 2 * p->splits : p->splits;
+}
+
+}  // namespace tg
