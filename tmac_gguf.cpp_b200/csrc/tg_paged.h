@@ -85,7 +85,7 @@ struct PagedPrefixParams {
   const float* q;        // [n][n_head*64], rotated
   const int* past;       // [n]
   const int* table;      // pages of the prefix
-  float* records;        // [parts][n][n_head][66] o (un-normalised), m, l
+  float* records;        // [parts][n_kv][66][n*group] o (un-normalised), m, l
   const float* own;      // [n][n_head][66] records of the queries' own rows
   float* out;            // [n][n_head*64]
   int* err;

@@ -52,8 +52,11 @@ __device__ __forceinline__ bool px_wait(uint64_t* bar, uint32_t parity, int* err
   return false;
 }
 
+// Every lane polls (and so acquires the phase itself), then the warp agrees.
+// The usual case, a phase that is already complete, reads nothing else.
 __device__ __forceinline__ bool px_wait_warp(uint64_t* bar, uint32_t parity, int* err,
                                              volatile int* abort_flag) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   const bool got = px_wait(bar, parity, err, abort_flag);
   return __all_sync(0xffffffffu, got) != 0;
 }
@@ -178,61 +181,87 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
       mbar_wait(&kv_full[i % PX_STAGES], (uint32_t)((i / PX_STAGES) & 1), p.err, kDevErrWaitFull);
   } else if (warp == 1) {
     // ---------------------------------------------------------- products
-    if (lane == 0) {
+    // The whole warp walks the loop, one lane issues (see umma_f16_ts_elect).
+    {
       constexpr uint32_t IDESC_QK = idesc_bf16(PX_ROWS, PX_KEYS, false);
       constexpr uint32_t IDESC_PV = idesc_bf16(PX_ROWS, 64, true);
       const uint64_t dk0 = smem_desc_sw128(smem_u32(smem), 16, 1024);
       const uint64_t dv0 = smem_desc_sw128(smem_u32(smem) + PX_TILE, PX_TILE, 1024);
       const int n_x[2] = {n0, n1};
-      bool ok = px_wait(q_full, 0, p.err, abort_flag);
+      const uint32_t utmem = __shfl_sync(0xffffffffu, tmem, 0);
+      bool ok = px_wait_warp(q_full, 0, p.err, abort_flag);
       int last = -1;   // slot of the last product issued
-      auto entry = [&](int x, int j) { return p.single ? 2 * j + x : j; };
+      // A ring position: stage and phase, stepped by 1 or 2.
+      struct Ring {
+        int st = 0;
+        uint32_t ph = 0;
+        __device__ __forceinline__ void step(int by) {
+          st += by;
+          if (st >= PX_STAGES) {
+            st -= PX_STAGES;
+            ph ^= 1u;
+          }
+        }
+      };
+      // Slot x's entries are x, x + 2, ... (single) or 0, 1, ... (both slots).
+      const int by = p.single ? 2 : 1;
+      Ring qk[2], pv[2];
+      if (p.single) {
+        qk[1].step(1);
+        pv[1].step(1);
+      }
       auto issue_qk = [&](int x, int j) -> bool {
-        const int i = entry(x, j), st = i % PX_STAGES;
-        if (!px_wait(&kv_full[st], (uint32_t)((i / PX_STAGES) & 1), p.err, abort_flag)) return false;
+        const int st = qk[x].st;
+        // Both slots over the same entry: slot 0 has waited for it.
+        if ((x == 0 || p.single) && !px_wait_warp(&kv_full[st], qk[x].ph, p.err, abort_flag))
+          return false;
         tc_fence_after();
         const uint64_t b = dk0 + (uint64_t)(st * (2 * PX_TILE >> 4));
-        const uint32_t d = tmem + px_s(x, j & 1), a = tmem + px_q(x);
+        const uint32_t d = utmem + px_s(x, j & 1), a = utmem + px_q(x);
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)   // 4 steps of 16 dimensions, hi then lo
-          umma_f16_ts(d, a + 8 * kk, b + 2 * (kk & 3), IDESC_QK, kk > 0 ? 1u : 0u);
-        umma_commit(&s_full[2 * x + (j & 1)]);
+          umma_f16_ts_elect(d, a + 8 * kk, b + 2 * (kk & 3), IDESC_QK, kk > 0 ? 1u : 0u);
+        umma_commit_elect(&s_full[2 * x + (j & 1)]);
+        qk[x].step(by);
         last = x;
         return true;
       };
       auto issue_pv = [&](int x, int j) -> bool {
-        const int i = entry(x, j), st = i % PX_STAGES;
-        if (!px_wait(&p_full[2 * x + (j & 1)], (uint32_t)((j >> 1) & 1), p.err, abort_flag))
+        const int st = pv[x].st;
+        if (!px_wait_warp(&p_full[2 * x + (j & 1)], (uint32_t)((j >> 1) & 1), p.err, abort_flag))
           return false;
         tc_fence_after();
         const uint64_t b = dv0 + (uint64_t)(st * (2 * PX_TILE >> 4));
-        const uint32_t d = tmem + px_o(x), a = tmem + px_s(x, j & 1);
+        const uint32_t d = utmem + px_o(x), a = utmem + px_s(x, j & 1);
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)   // 4 steps of 16 keys, hi then lo
-          umma_f16_ts(d, a + 8 * kk, b + 128 * (kk & 3), IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(&pv_done[x]);
-        if (p.single || x == 1 || n1 == 0) umma_commit(&kv_empty[st]);
+          umma_f16_ts_elect(d, a + 8 * kk, b + 128 * (kk & 3), IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
+        umma_commit_elect(&pv_done[x]);
+        if (p.single || x == 1 || n1 == 0) umma_commit_elect(&kv_empty[st]);
+        pv[x].step(by);
         last = x;
         return true;
       };
+#pragma unroll
       for (int j = 0; j < 2; ++j)
+#pragma unroll
         for (int x = 0; x < 2; ++x)
           if (ok && j < n_x[x]) ok = issue_qk(x, j);
       for (int j = 0; j < n0 && ok; ++j)
-        for (int x = 0; x < 2 && ok; ++x)
-          if (j < n_x[x]) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (ok && j < n_x[x]) {
             ok = issue_pv(x, j);
             if (ok && j + 2 < n_x[x]) ok = issue_qk(x, j + 2);
           }
       // Everything issued has completed before TMEM is freed (q_full is
       // done with: its second phase counts this commit and 7 arrivals).
       if (last >= 0) {
-        for (int i = 0; i < 7; ++i) mbar_arrive(q_full);
-        umma_commit(q_full);
+        if (lane < 7) mbar_arrive(q_full);
+        umma_commit_elect(q_full);
         mbar_wait(q_full, 1, p.err, kDevErrWaitFull);
       }
     }
-    __syncwarp();
   } else if (warp >= 4) {
     // ---------------------------------------------------------- softmax
     const int x = (warp - 4) >> 2, quarter = warp & 3;
@@ -333,12 +362,12 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
     }
     if (row < rows) {
       const int part = p.single ? 2 * split + x : split;
-      float* rec = p.records + (((size_t)part * p.n + s) * p.n_head + h) * 66;
+      // Column by column: a warp's 32 rows are neighbours there.
+      float* rec = p.records + ((size_t)part * p.n_kv + g) * 66 * rows + row;
 #pragma unroll
-      for (int c = 0; c < 32; ++c)
-        *reinterpret_cast<float2*>(rec + 2 * c) =
-            make_float2(__uint_as_float(ov[2 * c]), __uint_as_float(ov[2 * c + 1]));
-      *reinterpret_cast<float2*>(rec + 64) = make_float2(m, l);
+      for (int c = 0; c < 64; ++c) rec[(size_t)c * rows] = __uint_as_float(ov[c]);
+      rec[(size_t)64 * rows] = m;
+      rec[(size_t)65 * rows] = l;
     }
   }
 
@@ -352,53 +381,98 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
 }
 
 // out of every (query, head): the records of the prefix (for queries that
-// attend all of it) and the record of the query's own rows.  A warp each,
-// two dimensions per lane.
-constexpr int kPrefixMergeWarps = 4;
+// attend all of it) and the record of the query's own rows.  A CTA takes 32
+// rows of one KV head and 16 of the 64 dimensions: first lane = row (the
+// records' columns are contiguous), 8 warps = 2 halves of the dimensions x 4
+// groups of parts, joined in shared memory; then 8 threads per row, so that
+// the output is written in runs.
+constexpr int kPrefixMergeWarps = 8, kMergeDims = 16;
 
 __global__ void __launch_bounds__(32 * kPrefixMergeWarps)
     paged_prefix_merge_kernel(const PagedPrefixParams p) {
-  constexpr int B = 8;
+  constexpr int B = 4, GRP = 4, DW = kMergeDims / (kPrefixMergeWarps / GRP);
+  __shared__ float o_s[GRP][32][kMergeDims + 1];
+  __shared__ float ml_s[GRP][2][32];
   griddep_launch_dependents();
   griddep_wait();
-  const int lane = threadIdx.x & 31;
-  const int i = blockIdx.x * kPrefixMergeWarps + (threadIdx.x >> 5);  // (query, head)
-  if (i >= p.n * p.n_head) return;
-  const int s = i / p.n_head;
-  const float* own = p.own + (size_t)i * 66;
-  float M = own[64], L = own[65];
-  float2 O = *reinterpret_cast<const float2*>(own + 2 * lane);
-  const int parts = p.past[s] + 1 >= p.steps * PX_KEYS ? p.parts : 0;
-  for (int k0 = 0; k0 < parts; k0 += B) {
-    float2 o[B], ml[B];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows = p.n * p.group, blocks = (rows + 31) / 32;
+  const int g = blockIdx.x / blocks, row0 = (blockIdx.x - g * blocks) * 32;
+  const int d0 = blockIdx.y * kMergeDims;
+  {
+    const int grp = warp % GRP, dw = (warp / GRP) * DW;
+    const int row = row0 + lane;
+    const bool live = row < rows && p.past[row / p.group] + 1 >= p.steps * PX_KEYS;
+    const float* rec = p.records + (size_t)g * 66 * rows + (live ? row : 0);
+    const size_t part_stride = (size_t)p.n_kv * 66 * rows;
+    float M = kNegBig, L = 0.f, O[DW];
 #pragma unroll
-    for (int u = 0; u < B; ++u) {
-      ml[u] = make_float2(kNegBig, 0.f);
-      o[u] = make_float2(0.f, 0.f);
-      if (k0 + u < parts) {
-        const float* r = p.records + ((size_t)(k0 + u) * p.n * p.n_head + i) * 66;
-        o[u] = *reinterpret_cast<const float2*>(r + 2 * lane);
-        ml[u] = *reinterpret_cast<const float2*>(r + 64);
+    for (int c = 0; c < DW; ++c) O[c] = 0.f;
+    const int parts = live ? p.parts : 0;
+    for (int k0 = grp; k0 < parts; k0 += GRP * B) {
+      float m[B], l[B], o[B][DW];
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        const int k = k0 + u * GRP;
+        m[u] = kNegBig;
+        l[u] = 0.f;
+#pragma unroll
+        for (int c = 0; c < DW; ++c) o[u][c] = 0.f;
+        if (k < parts) {
+          const float* r = rec + (size_t)k * part_stride;
+          m[u] = r[(size_t)64 * rows];
+          l[u] = r[(size_t)65 * rows];
+#pragma unroll
+          for (int c = 0; c < DW; ++c) o[u][c] = r[(size_t)(d0 + dw + c) * rows];
+        }
+      }
+      float mb = M;
+#pragma unroll
+      for (int u = 0; u < B; ++u) mb = fmaxf(mb, m[u]);
+      const float w0 = ex2(M - mb);
+      M = mb;
+      L *= w0;
+#pragma unroll
+      for (int c = 0; c < DW; ++c) O[c] *= w0;
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        const float w = ex2(m[u] - M);
+        L = fmaf(l[u], w, L);
+#pragma unroll
+        for (int c = 0; c < DW; ++c) O[c] = fmaf(o[u][c], w, O[c]);
       }
     }
-    float mb = M;
 #pragma unroll
-    for (int u = 0; u < B; ++u) mb = fmaxf(mb, ml[u].x);
-    const float w0 = ex2(M - mb);
-    M = mb;
-    L *= w0;
-    O.x *= w0;
-    O.y *= w0;
-#pragma unroll
-    for (int u = 0; u < B; ++u) {
-      const float w = ex2(ml[u].x - M);
-      L = fmaf(ml[u].y, w, L);
-      O.x = fmaf(o[u].x, w, O.x);
-      O.y = fmaf(o[u].y, w, O.y);
+    for (int c = 0; c < DW; ++c) o_s[grp][lane][dw + c] = O[c];
+    if (dw == 0) {
+      ml_s[grp][0][lane] = M;
+      ml_s[grp][1][lane] = L;
     }
   }
+  __syncthreads();
+  const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 2;   // 8 threads per row
+  if (row0 + r >= rows) return;
+  const int row = row0 + r, s = row / p.group, h = g * p.group + row - s * p.group;
+  const float* own = p.own + ((size_t)s * p.n_head + h) * 66;
+  float2 O = *reinterpret_cast<const float2*>(own + d0 + c);
+  const float2 ml = *reinterpret_cast<const float2*>(own + 64);
+  float M = ml.x;
+#pragma unroll
+  for (int k = 0; k < GRP; ++k) M = fmaxf(M, ml_s[k][0][r]);
+  const float w = ex2(ml.x - M);
+  float L = ml.y * w;
+  O.x *= w;
+  O.y *= w;
+#pragma unroll
+  for (int k = 0; k < GRP; ++k) {
+    const float f = ex2(ml_s[k][0][r] - M);
+    L = fmaf(ml_s[k][1][r], f, L);
+    O.x = fmaf(o_s[k][r][c], f, O.x);
+    O.y = fmaf(o_s[k][r][c + 1], f, O.y);
+  }
   const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-  *reinterpret_cast<float2*>(p.out + (size_t)i * 64 + 2 * lane) = make_float2(O.x * inv, O.y * inv);
+  *reinterpret_cast<float2*>(p.out + ((size_t)s * p.n_head + h) * 64 + d0 + c) =
+      make_float2(O.x * inv, O.y * inv);
 }
 
 // ------------------------------------------------------------ launches
@@ -439,9 +513,8 @@ cudaError_t launch_paged_prefix(const CUtensorMap& tk, const CUtensorMap& tv,
 
 cudaError_t launch_paged_prefix_merge(const PagedPrefixParams& p, cudaStream_t st) {
   void* args[] = {const_cast<PagedPrefixParams*>(&p)};
-  const int items = p.n * p.n_head;
   return launch_prefix_pdl(reinterpret_cast<const void*>(paged_prefix_merge_kernel),
-                           dim3((unsigned)((items + kPrefixMergeWarps - 1) / kPrefixMergeWarps)),
+                           dim3((unsigned)(p.n_kv * ((p.n * p.group + 31) / 32)), 64 / kMergeDims),
                            dim3(32 * kPrefixMergeWarps), 0, st, args);
 }
 
