@@ -326,9 +326,35 @@ __device__ __forceinline__ int query_of(const int* prefix, int n, int streams, i
   return lo;
 }
 
-// CTAs that take part: enough that each has a chunk for each of its warps.
-__device__ __forceinline__ int paged_active(int grid, int T, int warps) {
-  return min(grid, (T + warps - 1) / warps);
+// CTAs that share the T chunks out: enough that each has a chunk for each of
+// its warps, and in any case some for every stream.
+__device__ __forceinline__ int paged_active(int grid, int T, int warps, int n_streams) {
+  return min(min(grid, T), max((T + warps - 1) / warps, 3 * n_streams));
+}
+
+// First chunk of CTA c's range: an equal share, moved to the nearer end of
+// the stream that it would cut if that stream is short (kWholeRounds steps of
+// all warps or less).  A cut costs its two CTAs a record, an arrival and a
+// merge, about 5000 cycles, as much as the chunks that a moved range has too
+// many.  A range may be empty.
+constexpr int kWholeRounds = 4;
+
+__device__ __forceinline__ int range_lo(const int* prefix, int n, int streams, int c, int G, int T,
+                                        int warps) {
+  const int t = (int)cta_tile_lo(c, G, T);
+  if (t <= 0 || t >= T) return t;
+  const int s = query_of(prefix, n, streams, t);
+  const int C = prefix[s + 1] - prefix[s], off = (t - prefix[s] * streams) % C;
+  if (C > kWholeRounds * warps) return t;
+  return 2 * off < C ? t - off : t + (C - off);
+}
+
+// One arrival at a split stream's count: the records written before it (by
+// all threads, ordered by the barrier) are seen by whoever arrives later.
+__device__ __forceinline__ unsigned arrive_acq_rel(unsigned* count) {
+  unsigned old;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(count) : "memory");
+  return old;
 }
 
 // ------------------------------------------------------------ segment results
@@ -399,11 +425,14 @@ __device__ void write_empty(const PagedAttnParams& p, const int* prefix) {
   }
 }
 
-// The last CTA to leave its part of a split stream merges all parts.  Parts
-// lie in slot order c1 (its last segment, or its first if the stream starts
-// there), then the first segments of c1 + 1 .. c2.
+// The last CTA to leave its part of a split stream merges all parts.  A CTA
+// has two slots: 2c for a stream it continues (its first segment), 2c + 1 for
+// one that it begins and does not end (its last), so the parts of a stream
+// are slot 2 c1 + 1 and the slots 2 (c1 + 1), ..., 2 c2.
+__device__ __forceinline__ int part_slot(int c1, int k) { return 2 * (c1 + k) + (k == 0 ? 1 : 0); }
+
 __device__ void merge_parts(const PagedAttnParams& p, const SegmentOut& dst, int heads,
-                            int first_slot, int c1, int n_parts, int tid, int nthreads) {
+                            int c1, int n_parts, int tid, int nthreads) {
   constexpr int B = 8;
   const int hd = p.hd;
   for (int e = tid; e < heads * hd; e += nthreads) {
@@ -417,7 +446,7 @@ __device__ void merge_parts(const PagedAttnParams& p, const SegmentOut& dst, int
         m[u] = kNegBig;
         l[u] = o[u] = 0.f;
         if (k < n_parts) {
-          const SegmentOut a = part_out(p, k == 0 ? first_slot : 2 * (c1 + k));
+          const SegmentOut a = part_out(p, part_slot(c1, k));
           m[u] = __ldcg(a.m + h);
           l[u] = __ldcg(a.l + h);
           o[u] = __ldcg(a.o + e);
@@ -493,9 +522,11 @@ __global__ void __launch_bounds__(kCoreThreads) paged_core_kernel(const PagedAtt
   const int streams = p.n_kv * p.hblocks;
   const int T_all = prefix[p.n] * streams;
   write_empty(p, prefix);
-  const int G = paged_active(gridDim.x, T_all, kCoreWarps), cta = blockIdx.x;
+  const int G = paged_active(gridDim.x, T_all, kCoreWarps, p.n * streams), cta = blockIdx.x;
   if (cta >= G) return;
-  const int t_lo = (int)cta_tile_lo(cta, G, T_all), t_hi = (int)cta_tile_lo(cta + 1, G, T_all);
+  const int t_lo = range_lo(prefix, p.n, streams, cta, G, T_all, kCoreWarps);
+  const int t_hi = range_lo(prefix, p.n, streams, cta + 1, G, T_all, kCoreWarps);
+  if (t_lo >= t_hi) return;
   const T* kp = static_cast<const T*>(p.kp);
   const T* vp = static_cast<const T*>(p.vp);
   const int P = 1 << p.log2p;
@@ -608,9 +639,8 @@ __global__ void __launch_bounds__(kCoreThreads) paged_core_kernel(const PagedAtt
     __syncthreads();
     // Segment result over the warps.
     const bool complete = t == s_lo && e_hi == s_hi;
-    const bool at_start = t == t_lo;
     const SegmentOut fin = segment_out(p, s, g, hb);
-    const SegmentOut dst = complete ? fin : part_out(p, 2 * cta + (at_start ? 0 : 1));
+    const SegmentOut dst = complete ? fin : part_out(p, 2 * cta + (t == s_lo ? 1 : 0));
     for (int e = tid; e < heads * hd; e += kCoreThreads) {
       const int h = e / hd, d = e - h * hd;
       float M = kNegBig;
@@ -638,14 +668,11 @@ __global__ void __launch_bounds__(kCoreThreads) paged_core_kernel(const PagedAtt
     if (!complete) {
       const int c1 = cta_of_tile(s_lo, G, T_all), c2 = cta_of_tile(s_hi - 1, G, T_all);
       unsigned* count = p.count + (size_t)s * streams + u;
-      __threadfence();
       __syncthreads();
-      if (tid == 0) *flag = atomicAdd(count, 1u) == (unsigned)(c2 - c1);
+      if (tid == 0) *flag = arrive_acq_rel(count) == (unsigned)(c2 - c1);
       __syncthreads();
       if (*flag) {
-        __threadfence();
-        merge_parts(p, fin, heads, 2 * c1 + ((int)cta_tile_lo(c1, G, T_all) == s_lo ? 0 : 1), c1,
-                    c2 - c1 + 1, tid, kCoreThreads);
+        merge_parts(p, fin, heads, c1, c2 - c1 + 1, tid, kCoreThreads);
         if (tid == 0) *count = 0;
       }
     }
@@ -721,7 +748,7 @@ struct Merged4 {
 };
 
 __device__ __forceinline__ Merged4 merge_item(const PagedAttnParams& p, int it, int h, int k0,
-                                              int step, int n_parts, int first_slot, int c1) {
+                                              int step, int n_parts, int c1) {
   constexpr int B = 4;
   Merged4 a{kNegBig, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
   for (; k0 < n_parts; k0 += step * B) {
@@ -734,7 +761,7 @@ __device__ __forceinline__ Merged4 merge_item(const PagedAttnParams& p, int it, 
       l[u] = 0.f;
       o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (k < n_parts) {
-        const SegmentOut x = part_out(p, k == 0 ? first_slot : 2 * (c1 + k));
+        const SegmentOut x = part_out(p, part_slot(c1, k));
         m[u] = __ldcg(x.m + h);
         l[u] = __ldcg(x.l + h);
         o[u] = __ldcg(reinterpret_cast<const float4*>(x.o) + it);
@@ -765,19 +792,19 @@ __device__ __forceinline__ Merged4 merge_item(const PagedAttnParams& p, int it, 
 // 6 floats per thread).  All NT threads take part.
 template <int HD, int NT>
 __device__ void merge_parts_vec(const PagedAttnParams& p, const SegmentOut& dst, int heads,
-                                int first_slot, int c1, int n_parts, int tid, float* sh) {
+                                int c1, int n_parts, int tid, float* sh) {
   const int items = heads * HD / 4, groups = min(4, NT / items);
   if (groups < 2) {
     for (int it = tid; it < items; it += NT) {
       const int h = it * 4 / HD;
-      const Merged4 a = merge_item(p, it, h, 0, 1, n_parts, first_slot, c1);
+      const Merged4 a = merge_item(p, it, h, 0, 1, n_parts, c1);
       store_segment4(dst, h, it * 4 - h * HD, a.O, a.M, a.L);
     }
     return;
   }
   const int grp = tid / items, it = tid - grp * items, h = it * 4 / HD;
   Merged4 a{};
-  if (grp < groups) a = merge_item(p, it, h, grp, groups, n_parts, first_slot, c1);
+  if (grp < groups) a = merge_item(p, it, h, grp, groups, n_parts, c1);
   if (grp > 0 && grp < groups) {
     float* x = sh + ((grp - 1) * items + it) * 6;
     x[0] = a.O.x; x[1] = a.O.y; x[2] = a.O.z; x[3] = a.O.w; x[4] = a.M; x[5] = a.L;
@@ -843,9 +870,11 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
   const int streams = p.n_kv * p.hblocks;
   const int T_all = prefix[p.n] * streams;
   write_empty(p, prefix);
-  const int G = paged_active(gridDim.x, T_all, WARPS), cta = blockIdx.x;
+  const int G = paged_active(gridDim.x, T_all, WARPS, p.n * streams), cta = blockIdx.x;
   if (cta >= G) return;
-  const int t_lo = (int)cta_tile_lo(cta, G, T_all), t_hi = (int)cta_tile_lo(cta + 1, G, T_all);
+  const int t_lo = range_lo(prefix, p.n, streams, cta, G, T_all, WARPS);
+  const int t_hi = range_lo(prefix, p.n, streams, cta + 1, G, T_all, WARPS);
+  if (t_lo >= t_hi) return;
   const int P = 1 << p.log2p;
   const int box = min(P, CH), lbox = min(p.log2p, Cfg::LCH);   // rows of a TMA box
   const int nbx = CH >> lbox;                                  // boxes of a chunk, 1, 2 or 4
@@ -1134,7 +1163,7 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     consumers_sync(NCT);
     const bool complete = t == s_lo && e_hi == s_hi;
     const SegmentOut fin = segment_out(p, s, g, hb);
-    const SegmentOut dst = complete ? fin : part_out(p, 2 * cta + (t == t_lo ? 0 : 1));
+    const SegmentOut dst = complete ? fin : part_out(p, 2 * cta + (t == s_lo ? 1 : 0));
     for (int e = threadIdx.x; e < heads * HD / 4; e += NCT) {
       const int h = e * 4 / HD, d = e * 4 - h * HD;
       float M = kNegBig;
@@ -1159,14 +1188,11 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     if (!complete) {
       const int c1 = cta_of_tile(s_lo, G, T_all), c2 = cta_of_tile(s_hi - 1, G, T_all);
       unsigned* count = p.count + (size_t)s * streams + u;
-      __threadfence();
       consumers_sync(NCT);
-      if (threadIdx.x == 0) *flag = atomicAdd(count, 1u) == (unsigned)(c2 - c1);
+      if (threadIdx.x == 0) *flag = arrive_acq_rel(count) == (unsigned)(c2 - c1);
       consumers_sync(NCT);
       if (*flag) {
-        __threadfence();
-        merge_parts_vec<HD, NCT>(p, fin, heads, 2 * c1 + ((int)cta_tile_lo(c1, G, T_all) == s_lo ? 0 : 1),
-                                 c1, c2 - c1 + 1, threadIdx.x, mrg);
+        merge_parts_vec<HD, NCT>(p, fin, heads, c1, c2 - c1 + 1, threadIdx.x, mrg);
         if (threadIdx.x == 0) *count = 0;
       }
     }
