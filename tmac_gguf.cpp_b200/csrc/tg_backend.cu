@@ -3243,7 +3243,10 @@ int tg_paged_select(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, con
   const int step = (int)std::max(1LL, std::min((long long)tg::kPagedMaxQueries, (1LL << 25) / per_query));
   TG_TRY(ensure_kept(ctx, &ctx->pkeys, &ctx->pkeys_cap,
                      (size_t)std::min(step, n_seqs) * per_query));
+  TG_TRY(ensure_kept(ctx, &ctx->pcount, &ctx->pcount_cap,
+                     (size_t)std::min(step, n_seqs) * d.n_kv_head, true));
   tg::PagedSelectParams p{};
+  p.count = ctx->pcount;
   p.bounds = pk->bounds + (size_t)layer * pk->bounds_elems * pk->esize;
   p.keys = ctx->pkeys;
   p.err = ctx->d_err;
@@ -3264,10 +3267,10 @@ int tg_paged_select(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, con
     p.past = static_cast<const int*>(dp) + s0;
     p.table = static_cast<const int*>(dt) + (size_t)s0 * max_blocks;
     p.pages = static_cast<int*>(dpg) + (size_t)s0 * d.n_kv_head * n_sel;
-    cudaError_t e = tg::launch_paged_select(p, ctx->stream);
+    cudaError_t e = tg::launch_paged_select(p, ctx->num_sms, ctx->stream);
     if (e != cudaSuccess)
       return fail(TG_ERR_CUDA, "paged select launch: %s", cudaGetErrorString(e));
-    ctx->launches += 2;
+    ctx->launches++;
   }
   return finish_call(ctx);
 }

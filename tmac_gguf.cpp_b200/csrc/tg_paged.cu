@@ -1247,159 +1247,348 @@ __device__ __forceinline__ unsigned long long ordered_key(double v) {
   return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
 }
 
-constexpr int kScoreThreads = 128;
-constexpr int kScoreLanes = 4;  // lanes per page
-constexpr int kScorePages = kScoreThreads / kScoreLanes;
-
 // Score of a page for one KV head: the largest, over the head's query group,
 // of sum_d max(q_d lo_d, q_d hi_d), an upper bound of q . k for every key of
 // the page.  Sums in binary64: which of two pages is taken must not hang on
 // the order of a sum's roundings (products of a 24-bit q and a bf16 or fp32
-// bound are exact there).  Four lanes per page, each a quarter of the
-// dimension pairs.
-template <typename T>
-__global__ void __launch_bounds__(kScoreThreads) paged_score_kernel(const PagedSelectParams p) {
-  extern __shared__ double q_d[];  // [group][hd]
-  griddep_launch_dependents();
-  griddep_wait();
-  const int s = blockIdx.x / p.n_kv, g = blockIdx.x - s * p.n_kv;
-  const int past = p.past[s];
-  const int nb = past < 0 ? 0 : (past >> p.log2p) + 1;
-  if (past < -1 || nb > p.max_blocks) {
-    if (blockIdx.y == 0 && threadIdx.x == 0) record_error(p.err, kDevErrBadPos);
-    return;
+// bound are exact there).  q >= 0 takes hi, else lo, so that an infinite
+// bound never meets the zero half of a split q.
+constexpr int kSelThreads = 512;
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kSelBits = 11, kSelBins = 1 << kSelBits;
+constexpr int kSelCached = 8192;   // keys that the picking CTA holds in shared memory
+
+// LPP lanes per page of 16 dimensions each: the bounds go to registers as
+// doubles once, then every head's q comes from shared memory (q_d, rows of 16
+// doubles padded to 18: the LPP rows of a read lie in different banks).
+template <typename T, int LPP>
+__device__ __forceinline__ unsigned long long page_key(const T* lo_p, const double* q_d, int group,
+                                                       int part) {
+  constexpr int HD = 16 * LPP, V = 16 / (int)sizeof(T);  // dimensions of a 16-byte piece
+  double lo[16], hi[16];
+#pragma unroll
+  for (int c = 0; c < 16 / V; ++c) {
+    const uint4 a = *reinterpret_cast<const uint4*>(lo_p + (c * LPP + part) * V);
+    const uint4 b = *reinterpret_cast<const uint4*>(lo_p + HD + (c * LPP + part) * V);
+    const T* ta = reinterpret_cast<const T*>(&a);
+    const T* tb = reinterpret_cast<const T*>(&b);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      lo[c * V + e] = (double)to_f32(ta[e]);
+      hi[c * V + e] = (double)to_f32(tb[e]);
+    }
   }
-  if ((int)blockIdx.y * kScorePages >= nb) return;
-  const int hd = p.hd;
-  const float* q = p.q + ((size_t)s * p.n_head + g * p.group) * hd;
-  for (int e = threadIdx.x; e < p.group * hd; e += kScoreThreads) q_d[e] = (double)q[e];
-  __syncthreads();
-  const int j = blockIdx.y * kScorePages + threadIdx.x / kScoreLanes;
-  const int part = threadIdx.x % kScoreLanes;
-  const bool live = j < nb;
-  int page = live ? p.table[(size_t)s * p.max_blocks + j] : 0;
-  const bool bad = page < 0 || page >= p.n_pages;
-  if (bad) {
-    if (part == 0) record_error(p.err, kDevErrBadPage);
-    page = 0;
-  }
-  const T* lo = static_cast<const T*>(p.bounds) + ((size_t)page * p.n_kv + g) * 2 * hd;
-  const T* hi = lo + hd;
   double best = -INFINITY;
   bool nan = false;
-  for (int h = 0; h < p.group; ++h) {
+  for (int h = 0; h < group; ++h) {
+    const double* q = q_d + (h * LPP + part) * 18;
+    double s0 = 0.0, s1 = 0.0;
+#pragma unroll
+    for (int d = 0; d < 16; d += 2) {
+      const double2 x = *reinterpret_cast<const double2*>(q + d);
+      s0 = fma(x.x, x.x >= 0.0 ? hi[d] : lo[d], s0);
+      s1 = fma(x.y, x.y >= 0.0 ? hi[d + 1] : lo[d + 1], s1);
+    }
+    double sum = s0 + s1;
+#pragma unroll
+    for (int o = 1; o < LPP; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    nan |= sum != sum;
+    best = fmax(best, sum);
+  }
+  return nan ? 0ull : ordered_key(best);
+}
+
+// Any even head_dim: one page per thread.
+template <typename T>
+__device__ unsigned long long page_key_any(const T* lo_p, const double* q_d, int group, int hd) {
+  double best = -INFINITY;
+  bool nan = false;
+  for (int h = 0; h < group; ++h) {
     double sum = 0.0;
-    for (int d = 2 * part; d < hd; d += 2 * kScoreLanes) {
-      const float2 a = load_pair(lo + d), b = load_pair(hi + d);
+    for (int d = 0; d < hd; d += 2) {
+      const float2 a = load_pair(lo_p + d), b = load_pair(lo_p + hd + d);
       const double q0 = q_d[h * hd + d], q1 = q_d[h * hd + d + 1];
       sum = fma(q0, (double)(q0 >= 0.0 ? b.x : a.x), sum);
       sum = fma(q1, (double)(q1 >= 0.0 ? b.y : a.y), sum);
     }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     nan |= sum != sum;
     best = fmax(best, sum);
   }
-  if (live && part == 0) {
-    unsigned long long key = (nan || bad) ? 0ull : ordered_key(best);
-    if (j < p.keep_first || j >= nb - p.keep_last) key = kKeyForced;
-    p.keys[((size_t)s * p.n_kv + g) * p.max_blocks + j] = key;
+  return nan ? 0ull : ordered_key(best);
+}
+
+// Inclusive sum over the block's threads; *total the sum of all.
+__device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* wsum, unsigned* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  if (lane == 31) wsum[warp] = v;
+  __syncthreads();
+  unsigned off = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) {
+    const unsigned x = wsum[w];
+    off += w < warp ? x : 0;
+    all += x;
+  }
+  __syncthreads();
+  *total = all;
+  return v + off;
+}
+
+// The n_sel largest of nb > n_sel keys, ties to the lowest index, ascending.
+// A radix search for the smallest key taken, 11 bits at a time from the
+// highest bit in which the keys differ at all (scores of one query share
+// sign and exponent bits); it ends when a digit's count is just what is
+// still needed.  Then every warp lists the taken ones of its share.
+__device__ void pick_pages(const unsigned long long* keys, int nb, int n_sel, int* out,
+                           unsigned* hist, unsigned* wsum, unsigned long long* sh) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // Bits in which the keys that are not forced differ.
+  unsigned long long any = 0, all = ~0ull;
+  unsigned forced = 0;
+  for (int i = tid; i < nb; i += kSelThreads) {
+    const unsigned long long k = keys[i];
+    if (k == kKeyForced) {
+      ++forced;
+    } else {
+      any |= k;
+      all &= k;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    any |= __shfl_xor_sync(0xffffffffu, any, o);
+    all &= __shfl_xor_sync(0xffffffffu, all, o);
+  }
+  if (lane == 0) {
+    sh[2 * warp] = any;
+    sh[2 * warp + 1] = all;
+  }
+  unsigned n_forced;
+  block_scan(forced, wsum, &n_forced);   // its barriers publish sh
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) {
+    any |= sh[2 * w];
+    all &= sh[2 * w + 1];
+  }
+  __syncthreads();
+  // Taken: forced keys (they are the largest), then keys above `prefix` in
+  // the bits of `mask`, then the first `need` that match it.
+  unsigned long long prefix = 0, mask = 0;
+  unsigned need = (unsigned)n_sel;
+  if (n_forced >= need) {
+    prefix = mask = ~0ull;
+  } else {
+    need -= n_forced;
+    const unsigned long long diff = any & ~all;
+    int top = diff ? 64 - __clzll(diff) : 0;   // bits [0, top) differ
+    mask = top < 64 ? ~0ull << top : 0ull;
+    prefix = all & mask;                       // unforced keys agree there
+    bool whole = false;
+    while (top > 0 && !whole) {
+      const int shift = max(0, top - kSelBits);
+      const unsigned bins = 1u << (top - shift);
+      for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
+      __syncthreads();
+      for (int i = tid; i < nb; i += kSelThreads) {
+        const unsigned long long k = keys[i];
+        if (k != kKeyForced && (k & mask) == prefix)
+          atomicAdd(&hist[(unsigned)(k >> shift) & (bins - 1)], 1u);
+      }
+      __syncthreads();
+      // Thread t sums the bins that are t-th from the top, 4 each.
+      unsigned h[kSelBins / kSelThreads], sum = 0;
+#pragma unroll
+      for (int u = 0; u < kSelBins / kSelThreads; ++u) {
+        h[u] = hist[kSelBins - 1 - (tid * (kSelBins / kSelThreads) + u)];
+        sum += h[u];
+      }
+      unsigned total;
+      const unsigned incl = block_scan(sum, wsum, &total);
+      unsigned before = incl - sum;
+      if (before < need && incl >= need) {   // exactly one thread
+#pragma unroll
+        for (int u = 0; u < kSelBins / kSelThreads; ++u) {
+          if (before < need && before + h[u] >= need) {
+            sh[0] = (unsigned long long)(kSelBins - 1 - (tid * (kSelBins / kSelThreads) + u));
+            sh[1] = need - before;
+            sh[2] = before + h[u] == need;
+            before = need;
+          } else if (before < need) {
+            before += h[u];
+          }
+        }
+      }
+      __syncthreads();
+      mask |= (unsigned long long)(bins - 1) << shift;
+      prefix |= sh[0] << shift;
+      need = (unsigned)sh[1];
+      whole = sh[2] != 0;
+      top = shift;
+      __syncthreads();
+    }
+  }
+  // Warp w lists keys [w, w + 1) * share.
+  const int share = ((nb + kSelWarps - 1) / kSelWarps + 31) & ~31;
+  const int i0 = min(nb, warp * share), i1 = min(nb, i0 + share);
+  const bool only_forced = mask == ~0ull && prefix == ~0ull;
+  unsigned ties = 0, above = 0;
+  for (int i = i0 + lane; i < i1; i += 32) {
+    const unsigned long long k = keys[i];
+    const bool f = k == kKeyForced;
+    const bool tie = only_forced ? f : (!f && (k & mask) == prefix);
+    const bool up = only_forced ? false : (f || (k & mask) > prefix);
+    ties += tie;
+    above += up;
+  }
+  ties = __reduce_add_sync(0xffffffffu, ties);
+  above = __reduce_add_sync(0xffffffffu, above);
+  if (lane == 0) {
+    wsum[warp] = ties;
+    hist[warp] = above;
+  }
+  __syncthreads();
+  unsigned tie_at = 0, up_at = 0;
+  for (int w = 0; w < warp; ++w) {
+    tie_at += wsum[w];
+    up_at += hist[w];
+  }
+  for (int b = i0; b < i1; b += 32) {
+    const int i = b + lane;
+    const unsigned long long k = i < i1 ? keys[i] : 0ull;
+    const bool f = i < i1 && k == kKeyForced;
+    const bool tie = i < i1 && (only_forced ? f : (!f && (k & mask) == prefix));
+    const bool up = i < i1 && !only_forced && (f || (k & mask) > prefix);
+    const unsigned bt = __ballot_sync(0xffffffffu, tie), bu = __ballot_sync(0xffffffffu, up);
+    const unsigned below = (1u << lane) - 1u;
+    const unsigned t = tie_at + __popc(bt & below);
+    const unsigned at = up_at + __popc(bu & below) + min(t, need);
+    if ((up || (tie && t < need)) && at < (unsigned)n_sel) out[at] = i;
+    tie_at += __popc(bt);
+    up_at += __popc(bu);
   }
 }
 
-constexpr int kPickThreads = 512;
-
-// The n_sel largest keys of one (query, KV head), ties to the lowest index:
-// a radix search for the smallest key taken, 8 bits per pass, then the taken
-// indices in ascending order.
-__global__ void __launch_bounds__(kPickThreads) paged_pick_kernel(const PagedSelectParams p) {
-  __shared__ unsigned hist[256];
-  __shared__ unsigned wsum[kPickThreads / 32][2];
-  __shared__ unsigned long long sh_prefix;
-  __shared__ unsigned sh_need, sh_done;
+// gridDim.y CTAs per (query, KV head) share its pages out; each writes its
+// keys, and the last to arrive picks (one CTA: from its own shared memory).
+// LPP 0: any head_dim.
+template <typename T, int LPP>
+__global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedSelectParams p) {
+  extern __shared__ unsigned long long sel_sm[];
+  unsigned long long* cache = sel_sm;                                   // [kSelCached]
+  unsigned long long* sh = cache + kSelCached;                          // [2 * kSelWarps]
+  unsigned* hist = reinterpret_cast<unsigned*>(sh + 2 * kSelWarps);     // [kSelBins]
+  unsigned* wsum = hist + kSelBins;                                     // [kSelWarps]
+  int* flag = reinterpret_cast<int*>(wsum + kSelWarps);
+  double* q_d = reinterpret_cast<double*>(wsum + kSelWarps + 4);        // [group][hd] (padded)
   griddep_launch_dependents();
   griddep_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.x, s = row / p.n_kv;
+  const int tid = threadIdx.x;
+  const int row = blockIdx.x, s = row / p.n_kv, g = row - s * p.n_kv;
   const int past = p.past[s];
   int nb = past < 0 ? 0 : (past >> p.log2p) + 1;
-  if (nb > p.max_blocks) nb = 0;
-  const unsigned long long* keys = p.keys + (size_t)row * p.max_blocks;
+  if (past < -1 || nb > p.max_blocks) {
+    if (blockIdx.y == 0 && tid == 0) record_error(p.err, kDevErrBadPos);
+    nb = 0;
+  }
   int* out = p.pages + (size_t)row * p.n_sel;
   if (nb <= p.n_sel) {
-    for (int i = tid; i < p.n_sel; i += kPickThreads) out[i] = i < nb ? i : -1;
+    if (blockIdx.y == 0)
+      for (int i = tid; i < p.n_sel; i += kSelThreads) out[i] = i < nb ? i : -1;
     return;
   }
-  unsigned long long prefix = 0, mask = 0;
-  unsigned need = (unsigned)p.n_sel;  // still to take among keys that match the prefix
-  bool exact = false;                 // every matching key is taken
-  for (int shift = 56; shift >= 0 && !exact; shift -= 8) {
-    for (int i = tid; i < 256; i += kPickThreads) hist[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < nb; i += kPickThreads) {
-      const unsigned long long k = keys[i];
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
+  // CTAs with pages: all have the same number of passes, or one more.
+  constexpr int PAGES = LPP ? kSelThreads / LPP : kSelThreads;   // per pass
+  const int ctas = min((int)gridDim.y, (nb + PAGES - 1) / PAGES);
+  if ((int)blockIdx.y >= ctas) return;
+  const int hd = LPP ? 16 * LPP : p.hd;
+  const float* q = p.q + ((size_t)s * p.n_head + g * p.group) * hd;
+  for (int e = tid; e < p.group * hd; e += kSelThreads) {
+    int at = e;
+    if constexpr (LPP > 0) {
+      // Piece c of V dimensions belongs to lane c % LPP.
+      constexpr int V = 16 / (int)sizeof(T);
+      const int h = e / hd, d = e - h * hd, c = d / V;
+      at = (h * LPP + c % LPP) * 18 + (c / LPP) * V + d % V;
     }
-    __syncthreads();
-    if (tid == 0) {
-      unsigned left = need;
-      int b = 255;
-      while (b > 0 && hist[b] < left) left -= hist[b--];
-      sh_prefix = prefix | ((unsigned long long)b << shift);
-      sh_need = left;
-      sh_done = hist[b] == left;
-    }
-    __syncthreads();
-    prefix = sh_prefix;
-    need = sh_need;
-    exact = sh_done != 0;
-    mask |= 255ull << shift;
-    __syncthreads();
+    q_d[at] = (double)q[e];
   }
-  // Keys above the prefix are taken, of those that match it the first `need`.
-  unsigned taken = 0, ties = 0;
-  for (int i0 = 0; i0 < nb; i0 += kPickThreads) {
-    const int i = i0 + tid;
-    const unsigned long long k = i < nb ? keys[i] & mask : 0ull;
-    const bool tie = i < nb && k == prefix, above = i < nb && k > prefix;
-    const unsigned bt = __ballot_sync(0xffffffffu, tie), ba = __ballot_sync(0xffffffffu, above);
-    if (lane == 0) {
-      wsum[warp][0] = __popc(bt);
-      wsum[warp][1] = __popc(ba);
+  __syncthreads();
+  const bool alone = ctas == 1 && nb <= kSelCached;
+  unsigned long long* keys = alone ? cache : p.keys + (size_t)row * p.max_blocks;
+  const int* table = p.table + (size_t)s * p.max_blocks;
+  const int stride = ctas * PAGES;
+  int j = blockIdx.y * PAGES + (LPP ? tid / (LPP ? LPP : 1) : tid);
+  const int part = LPP ? tid % (LPP ? LPP : 1) : 0;
+  int page = j < nb ? table[j] : 0;
+  for (int j0 = blockIdx.y * PAGES; j0 < nb; j0 += stride, j += stride) {
+    const int page_n = j + stride < nb ? table[j + stride] : 0;   // one pass ahead
+    const bool bad = page < 0 || page >= p.n_pages;
+    if (bad && part == 0) record_error(p.err, kDevErrBadPage);
+    const T* lo = static_cast<const T*>(p.bounds) + ((size_t)(bad ? 0 : page) * p.n_kv + g) * 2 * hd;
+    unsigned long long key;
+    if constexpr (LPP > 0)
+      key = page_key<T, LPP>(lo, q_d, p.group, part);
+    else
+      key = page_key_any<T>(lo, q_d, p.group, hd);
+    if (bad) key = 0ull;
+    if (j < p.keep_first || j >= nb - p.keep_last) key = kKeyForced;
+    if (j < nb && part == 0) keys[j] = key;
+    page = page_n;
+  }
+  __syncthreads();
+  if (!alone) {
+    if (ctas > 1) {
+      if (tid == 0) *flag = arrive_acq_rel(p.count + row) == (unsigned)(ctas - 1);
+      __syncthreads();
+      if (!*flag) return;
+      if (tid == 0) p.count[row] = 0;
     }
-    __syncthreads();
-    unsigned tie_at = ties, above_at = 0, tie_all = 0, above_all = 0;
-    for (int w = 0; w < kPickThreads / 32; ++w) {
-      if (w < warp) {
-        tie_at += wsum[w][0];
-        above_at += wsum[w][1];
-      }
-      tie_all += wsum[w][0];
-      above_all += wsum[w][1];
+    if (nb <= kSelCached) {
+      for (int i = tid; i < nb; i += kSelThreads) cache[i] = __ldcg(keys + i);
+      __syncthreads();
+      keys = cache;
     }
-    const unsigned below = (1u << lane) - 1u;
-    tie_at += __popc(bt & below);
-    above_at += __popc(ba & below);
-    // Slot: everything taken before this index.
-    const unsigned ties_before = min(tie_at, need) - min(ties, need);
-    const unsigned at = taken + above_at + ties_before;
-    if ((above || (tie && tie_at < need)) && at < (unsigned)p.n_sel) out[at] = i;
-    taken += above_all + min(ties + tie_all, need) - min(ties, need);
-    ties += tie_all;
-    __syncthreads();
+  }
+  pick_pages(keys, nb, p.n_sel, out, hist, wsum, sh);
+}
+
+template <typename T, int LPP>
+static cudaError_t launch_select_cfg(const PagedSelectParams& p, int ctas, cudaStream_t st) {
+  static bool done[64] = {};
+  cudaError_t e = allow_max_smem(paged_select_kernel<T, LPP>, done);
+  if (e != cudaSuccess) return e;
+  const size_t smem = (size_t)(kSelCached + 2 * kSelWarps) * 8 + (size_t)(kSelBins + kSelWarps + 4) * 4 +
+                      (size_t)p.group * (LPP ? LPP * 18 : p.hd) * 8;
+  return launch_chained(paged_select_kernel<T, LPP>, dim3((unsigned)(p.n * p.n_kv), (unsigned)ctas),
+                        dim3(kSelThreads), smem, st, p);
+}
+
+template <typename T>
+static cudaError_t launch_select_type(const PagedSelectParams& p, int num_sms, cudaStream_t st) {
+  // Two CTAs fit an SM (keys in shared memory); more than one per row only
+  // while there are SMs without one and pages for another pass.
+  const int lpp = p.hd == 64 ? 4 : p.hd == 128 ? 8 : p.hd == 32 ? 2 : 0;
+  const int pages = lpp ? kSelThreads / lpp : kSelThreads;
+  const int most = (p.max_blocks + pages - 1) / pages;
+  int ctas = 2 * num_sms / (p.n * p.n_kv);
+  if (ctas > most) ctas = most;
+  if (ctas < 1) ctas = 1;
+  switch (lpp) {
+    case 2: return launch_select_cfg<T, 2>(p, ctas, st);
+    case 4: return launch_select_cfg<T, 4>(p, ctas, st);
+    case 8: return launch_select_cfg<T, 8>(p, ctas, st);
+    default: return launch_select_cfg<T, 0>(p, ctas, st);
   }
 }
 
-cudaError_t launch_paged_select(const PagedSelectParams& p, cudaStream_t st) {
-  const dim3 grid((unsigned)(p.n * p.n_kv),
-                  (unsigned)((p.max_blocks + kScorePages - 1) / kScorePages));
-  const size_t smem = (size_t)p.group * p.hd * sizeof(double);
-  cudaError_t e =
-      p.dtype == 1
-          ? launch_chained(paged_score_kernel<__nv_bfloat16>, grid, dim3(kScoreThreads), smem, st, p)
-          : launch_chained(paged_score_kernel<float>, grid, dim3(kScoreThreads), smem, st, p);
-  if (e != cudaSuccess) return e;
-  return launch_chained(paged_pick_kernel, dim3((unsigned)(p.n * p.n_kv)), dim3(kPickThreads), 0, st, p);
+cudaError_t launch_paged_select(const PagedSelectParams& p, int num_sms, cudaStream_t st) {
+  return p.dtype == 1 ? launch_select_type<__nv_bfloat16>(p, num_sms, st)
+                      : launch_select_type<float>(p, num_sms, st);
 }
 
 }  // namespace tg

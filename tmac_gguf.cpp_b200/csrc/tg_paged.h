@@ -72,6 +72,7 @@ struct PagedSelectParams {
   const int* table;              // [n][max_blocks]
   const void* bounds;            // layer base
   unsigned long long* keys;      // [n][n_kv][max_blocks] ordered scores
+  unsigned* count;               // [n][n_kv] arrivals, all 0 between launches
   int* pages;                    // [n][n_kv][n_sel]
   int* err;
   int n, n_head, n_kv, group, hd, dtype;
@@ -109,6 +110,6 @@ size_t paged_core_smem(int n, int hd);
 int paged_mma_lchunk(int dtype, int hd);
 cudaError_t launch_paged_mma(const CUtensorMap& tk, const CUtensorMap& tv, const PagedAttnParams& p,
                              int dtype, int grid, cudaStream_t st);
-cudaError_t launch_paged_select(const PagedSelectParams& p, cudaStream_t st);
+cudaError_t launch_paged_select(const PagedSelectParams& p, int num_sms, cudaStream_t st);
 
 }  // namespace tg
