@@ -3238,13 +3238,13 @@ int tg_paged_select(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, con
   TG_TRY(stage_in(ctx, block_table, (size_t)n_seqs * max_blocks * 4, &dt));
   TG_TRY(stage_out(ctx, pages, (size_t)n_seqs * d.n_kv_head * n_sel * 4, false, &dpg));
   TG_TRY(commit_inputs(ctx));
-  // Queries per launch: at most 32M scores (256 MB) of scratch.
-  const long long per_query = (long long)d.n_kv_head * max_blocks;
+  // Queries per launch: at most 256 MB of scratch.
+  const long long per_query = 3LL * d.n_kv_head * max_blocks;
   const int step = (int)std::max(1LL, std::min((long long)tg::kPagedMaxQueries, (1LL << 25) / per_query));
   TG_TRY(ensure_kept(ctx, &ctx->pkeys, &ctx->pkeys_cap,
                      (size_t)std::min(step, n_seqs) * per_query));
   TG_TRY(ensure_kept(ctx, &ctx->pcount, &ctx->pcount_cap,
-                     (size_t)std::min(step, n_seqs) * d.n_kv_head, true));
+                     (size_t)2 * std::min(step, n_seqs) * d.n_kv_head, true));
   tg::PagedSelectParams p{};
   p.count = ctx->pcount;
   p.bounds = pk->bounds + (size_t)layer * pk->bounds_elems * pk->esize;

@@ -1236,127 +1236,195 @@ cudaError_t launch_paged_mma(const CUtensorMap& tk, const CUtensorMap& tv, const
 }
 
 // ------------------------------------------------------------ page selection
-
-constexpr unsigned long long kKeyForced = ~0ull;  // pages that are always taken
-
-// Unsigned integers in the order of the doubles; NaN below everything.
-__device__ __forceinline__ unsigned long long ordered_key(double v) {
-  v += 0.0;  // -0 and +0 are equal
-  const unsigned long long b = (unsigned long long)__double_as_longlong(v);
-  if (v != v) return 0ull;
-  return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
-}
-
+//
 // Score of a page for one KV head: the largest, over the head's query group,
 // of sum_d max(q_d lo_d, q_d hi_d), an upper bound of q . k for every key of
-// the page.  Sums in binary64: which of two pages is taken must not hang on
-// the order of a sum's roundings (products of a 24-bit q and a bf16 or fp32
-// bound are exact there).  q >= 0 takes hi, else lo, so that an infinite
-// bound never meets the zero half of a split q.
+// the page.  Which of two pages is taken must not hang on the order of a
+// sum's roundings, so the order of the pages is that of the scores in
+// binary64 (products of a 24-bit q and a bf16 or fp32 bound are exact
+// there).  Computing them all there is slow, so the scores come from the
+// tensor cores with a bound E on their error, and only the pages within 2 E of
+// the n_sel-th score are scored again: with T the n_sel-th largest of these
+// scores, a page above T + 2 E is taken (whatever may beat it is above T too,
+// and fewer than n_sel pages are), one below T - 2 E is not.
+
 constexpr int kSelThreads = 512;
 constexpr int kSelWarps = kSelThreads / 32;
-constexpr int kSelBits = 11, kSelBins = 1 << kSelBits;
-constexpr int kSelCached = 8192;   // keys that the picking CTA holds in shared memory
+constexpr int kSelBits = 8, kSelBins = 1 << kSelBits;
+constexpr int kSelNear = 256;       // pages near the border that are ranked by comparisons
+constexpr int kSelCached = 16384;   // binary32 keys that the picking CTA holds in shared memory
+constexpr uint32_t kKeyForced = ~0u;  // pages that are always taken
 
-// LPP lanes per page of 16 dimensions each: the bounds go to registers as
-// doubles once, then every head's q comes from shared memory (q_d, rows of 16
-// doubles padded to 18: the LPP rows of a read lie in different banks).
-template <typename T, int LPP>
-__device__ __forceinline__ unsigned long long page_key(const T* lo_p, const double* q_d, int group,
-                                                       int part) {
-  constexpr int HD = 16 * LPP, V = 16 / (int)sizeof(T);  // dimensions of a 16-byte piece
-  double lo[16], hi[16];
-#pragma unroll
-  for (int c = 0; c < 16 / V; ++c) {
-    const uint4 a = *reinterpret_cast<const uint4*>(lo_p + (c * LPP + part) * V);
-    const uint4 b = *reinterpret_cast<const uint4*>(lo_p + HD + (c * LPP + part) * V);
-    const T* ta = reinterpret_cast<const T*>(&a);
-    const T* tb = reinterpret_cast<const T*>(&b);
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      lo[c * V + e] = (double)to_f32(ta[e]);
-      hi[c * V + e] = (double)to_f32(tb[e]);
-    }
-  }
-  double best = -INFINITY;
-  bool nan = false;
-  for (int h = 0; h < group; ++h) {
-    const double* q = q_d + (h * LPP + part) * 18;
-    double s0 = 0.0, s1 = 0.0;
-#pragma unroll
-    for (int d = 0; d < 16; d += 2) {
-      const double2 x = *reinterpret_cast<const double2*>(q + d);
-      s0 = fma(x.x, x.x >= 0.0 ? hi[d] : lo[d], s0);
-      s1 = fma(x.y, x.y >= 0.0 ? hi[d + 1] : lo[d + 1], s1);
-    }
-    double sum = s0 + s1;
-#pragma unroll
-    for (int o = 1; o < LPP; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    nan |= sum != sum;
-    best = fmax(best, sum);
-  }
-  return nan ? 0ull : ordered_key(best);
+// Unsigned integers in the order of the floating-point numbers (-0 as +0).
+__device__ __forceinline__ uint32_t ordered_key(float v) {
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return (b >> 31) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ unsigned long long ordered_key(double v) {
+  const unsigned long long b = (unsigned long long)__double_as_longlong(v + 0.0);
+  return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k);
 }
 
-// Any even head_dim: one page per thread.
+// Scores of 8 pages by one warp with mma.sync: max(q, 0) times the upper
+// bounds plus min(q, 0) times the lower ones, rows 0-7 of the operand the high
+// parts of up to 8 heads, rows 8-15 the low parts (as in paged_mma_kernel).
+// The order of the dimensions in a sum is free, so a lane's part of the 8
+// page columns is whole 16-byte pieces straight from memory (piece c of lane
+// (page, qd) is piece 4 c + qd of the page's row); the q operands of every
+// product lie in shared memory as the lanes need them.  Lane (r, qd) returns
+// the scores of pages 2 qd and 2 qd + 1, the same for every r; *big is raised
+// to the largest |bound| of the lane's own pieces, or to infinity when a
+// score is not finite.  (Plain multiply-adds with q read from shared memory
+// took 14000 cycles for 444 pages x 7 heads, bound by those reads.)
+template <typename T, int HD>
+struct ScoreMma {
+  static constexpr int PIECES = HD * (int)sizeof(T) / 64;  // 16-byte pieces of a lane and bound
+  static constexpr int PER = 2;                            // products of a piece
+  static constexpr int OPERANDS = 2 * PIECES * PER;        // of a block of 8 heads
+};
+
+template <typename T, int HD>
+__device__ __forceinline__ float2 page_scores(const T* row, const uint4* q_s, int hblocks,
+                                              int last_heads, float* big) {
+  using Cfg = ScoreMma<T, HD>;
+  const int lane = threadIdx.x & 31, r = lane >> 2, qd = lane & 3;
+  uint4 b[2][Cfg::PIECES];   // upper, lower
+#pragma unroll
+  for (int c = 0; c < Cfg::PIECES; ++c) {
+    b[0][c] = reinterpret_cast<const uint4*>(row + HD)[4 * c + qd];
+    b[1][c] = reinterpret_cast<const uint4*>(row)[4 * c + qd];
+  }
+  float m = 0.f;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int c = 0; c < Cfg::PIECES; ++c) {
+      const uint32_t w[4] = {b[k][c].x, b[k][c].y, b[k][c].z, b[k][c].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(T) == 2) {
+          m = fmaxf(m, fmaxf(fabsf(__uint_as_float(w[e] << 16)),
+                             fabsf(__uint_as_float(w[e] & 0xffff0000u))));
+        } else {
+          m = fmaxf(m, fabsf(__uint_as_float(w[e])));
+        }
+      }
+    }
+  float2 best = make_float2(-INFINITY, -INFINITY);
+  bool odd = false;
+  for (int hb = 0; hb < hblocks; ++hb) {
+    float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    const uint4* q = q_s + hb * Cfg::OPERANDS * 32 + lane;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int c = 0; c < Cfg::PIECES; ++c) {
+        const uint32_t w[4] = {b[k][c].x, b[k][c].y, b[k][c].z, b[k][c].w};
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint4 x = q[((k * Cfg::PIECES + c) * 2 + u) * 32];
+          const uint32_t a[4] = {x.x, x.y, x.z, x.w};
+          if constexpr (sizeof(T) == 2) {
+            mma_bf16_16816(acc[k], a, w[2 * u], w[2 * u + 1]);
+          } else {
+            uint32_t h0, l0, h1, l1;
+            split_tf32(__uint_as_float(w[2 * u]), h0, l0);
+            split_tf32(__uint_as_float(w[2 * u + 1]), h1, l1);
+            mma_tf32_1688(acc[k], a, h0, h1);
+            mma_tf32_1688(acc[k], a, l0, l1);
+          }
+        }
+      }
+    float x0 = (acc[0][0] + acc[0][2]) + (acc[1][0] + acc[1][2]);
+    float x1 = (acc[0][1] + acc[0][3]) + (acc[1][1] + acc[1][3]);
+    if (r < (hb + 1 == hblocks ? last_heads : kPagedHeads)) {
+      odd |= !(fabsf(x0) < INFINITY) || !(fabsf(x1) < INFINITY);
+      best.x = fmaxf(best.x, x0);
+      best.y = fmaxf(best.y, x1);
+    }
+  }
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) {
+    best.x = fmaxf(best.x, __shfl_xor_sync(0xffffffffu, best.x, o));
+    best.y = fmaxf(best.y, __shfl_xor_sync(0xffffffffu, best.y, o));
+  }
+  *big = __any_sync(0xffffffffu, odd) ? INFINITY : fmaxf(*big, m);
+  return best;
+}
+
+// Score of one page by one thread, any even head_dim, in binary32.
 template <typename T>
-__device__ unsigned long long page_key_any(const T* lo_p, const double* q_d, int group, int hd) {
-  double best = -INFINITY;
-  bool nan = false;
+__device__ float page_score_any(const T* lo_p, const float* q_f, int group, int hd, float* big) {
+  float best = -INFINITY, m = 0.f;
+  bool odd = false;
   for (int h = 0; h < group; ++h) {
-    double sum = 0.0;
+    float sum = 0.f;
     for (int d = 0; d < hd; d += 2) {
       const float2 a = load_pair(lo_p + d), b = load_pair(lo_p + hd + d);
-      const double q0 = q_d[h * hd + d], q1 = q_d[h * hd + d + 1];
-      sum = fma(q0, (double)(q0 >= 0.0 ? b.x : a.x), sum);
-      sum = fma(q1, (double)(q1 >= 0.0 ? b.y : a.y), sum);
+      const float q0 = q_f[h * hd + d], q1 = q_f[h * hd + d + 1];
+      sum = fmaf(q0, q0 >= 0.f ? b.x : a.x, sum);
+      sum = fmaf(q1, q1 >= 0.f ? b.y : a.y, sum);
+      if (h == 0)
+        m = fmaxf(m, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))));
     }
-    nan |= sum != sum;
-    best = fmax(best, sum);
+    odd |= !(fabsf(sum) < INFINITY);
+    best = fmaxf(best, sum);
   }
-  return nan ? 0ull : ordered_key(best);
+  *big = odd ? INFINITY : fmaxf(*big, m);
+  return best;
 }
 
-// Inclusive sum over the block's threads; *total the sum of all.
-__device__ __forceinline__ unsigned block_scan(unsigned v, unsigned* wsum, unsigned* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
+// Binary64 score of a page for one head, by one warp.
+template <typename T>
+__device__ double exact_score(const T* lo_p, const float* q, int hd) {
+  double sum = 0.0;
+  for (int d = threadIdx.x & 31; d < hd; d += 32) {
+    const float x = q[d];
+    sum = fma((double)x, (double)to_f32(x >= 0.f ? lo_p[hd + d] : lo_p[d]), sum);
   }
-  if (lane == 31) wsum[warp] = v;
-  __syncthreads();
-  unsigned off = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kSelWarps; ++w) {
-    const unsigned x = wsum[w];
-    off += w < warp ? x : 0;
-    all += x;
-  }
-  __syncthreads();
-  *total = all;
-  return v + off;
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
 }
 
-// The n_sel largest of nb > n_sel keys, ties to the lowest index, ascending.
-// A radix search for the smallest key taken, 11 bits at a time from the
-// highest bit in which the keys differ at all (scores of one query share
-// sign and exponent bits); it ends when a digit's count is just what is
-// still needed.  Then every warp lists the taken ones of its share.
-__device__ void pick_pages(const unsigned long long* keys, int nb, int n_sel, int* out,
-                           unsigned* hist, unsigned* wsum, unsigned long long* sh) {
+// Shared memory of the picking CTA.
+struct PickShared {
+  unsigned hist[2][kSelBins];
+  unsigned count[2][kSelWarps];
+  unsigned long long wide[2][kSelWarps];
+  unsigned long long prefix;
+  unsigned left, forced, near, sure;
+  float big[kSelWarps];
+  int flag;
+  int near_at[kSelNear];
+  unsigned long long near_key[kSelNear];
+};
+
+__device__ __forceinline__ int leading_zeros(uint32_t v) { return __clz((int)v); }
+__device__ __forceinline__ int leading_zeros(unsigned long long v) { return __clzll((long long)v); }
+
+// The k-th largest of n >= k keys (k >= 1) and how many of those equal to it
+// are among the k largest.  A radix search, 8 bits at a time from the highest
+// bit in which the keys differ at all (the largest value, forced pages,
+// aside: scores of one query share sign and exponent bits); one warp finds
+// the digit, so a step has two barriers.
+template <typename K>
+__device__ K kth_key(const K* keys, int n, unsigned k, PickShared& sh, unsigned* need) {
+  constexpr int BITS = 8 * (int)sizeof(K);
+  constexpr K TOP = ~(K)0;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // Bits in which the keys that are not forced differ.
-  unsigned long long any = 0, all = ~0ull;
+  K any = 0, all = TOP;
   unsigned forced = 0;
-  for (int i = tid; i < nb; i += kSelThreads) {
-    const unsigned long long k = keys[i];
-    if (k == kKeyForced) {
+  for (int i = tid; i < n; i += kSelThreads) {
+    const K x = keys[i];
+    if (x == TOP) {
       ++forced;
     } else {
-      any |= k;
-      all &= k;
+      any |= x;
+      all &= x;
     }
   }
 #pragma unroll
@@ -1364,132 +1432,169 @@ __device__ void pick_pages(const unsigned long long* keys, int nb, int n_sel, in
     any |= __shfl_xor_sync(0xffffffffu, any, o);
     all &= __shfl_xor_sync(0xffffffffu, all, o);
   }
+  forced = __reduce_add_sync(0xffffffffu, forced);
+  __syncthreads();   // what was in sh before has been read
   if (lane == 0) {
-    sh[2 * warp] = any;
-    sh[2 * warp + 1] = all;
+    sh.wide[0][warp] = any;
+    sh.wide[1][warp] = all;
+    sh.count[0][warp] = forced;
   }
-  unsigned n_forced;
-  block_scan(forced, wsum, &n_forced);   // its barriers publish sh
+  if (tid < kSelBins) sh.hist[0][tid] = 0;
+  __syncthreads();
+  unsigned n_forced = 0;
 #pragma unroll
   for (int w = 0; w < kSelWarps; ++w) {
-    any |= sh[2 * w];
-    all &= sh[2 * w + 1];
+    any |= (K)sh.wide[0][w];
+    all &= (K)sh.wide[1][w];
+    n_forced += sh.count[0][w];
   }
-  __syncthreads();
-  // Taken: forced keys (they are the largest), then keys above `prefix` in
-  // the bits of `mask`, then the first `need` that match it.
-  unsigned long long prefix = 0, mask = 0;
-  unsigned need = (unsigned)n_sel;
-  if (n_forced >= need) {
-    prefix = mask = ~0ull;
-  } else {
-    need -= n_forced;
-    const unsigned long long diff = any & ~all;
-    int top = diff ? 64 - __clzll(diff) : 0;   // bits [0, top) differ
-    mask = top < 64 ? ~0ull << top : 0ull;
-    prefix = all & mask;                       // unforced keys agree there
-    bool whole = false;
-    while (top > 0 && !whole) {
-      const int shift = max(0, top - kSelBits);
-      const unsigned bins = 1u << (top - shift);
-      for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
-      for (int i = tid; i < nb; i += kSelThreads) {
-        const unsigned long long k = keys[i];
-        if (k != kKeyForced && (k & mask) == prefix)
-          atomicAdd(&hist[(unsigned)(k >> shift) & (bins - 1)], 1u);
-      }
-      __syncthreads();
-      // Thread t sums the bins that are t-th from the top, 4 each.
-      unsigned h[kSelBins / kSelThreads], sum = 0;
+  if (n_forced >= k) {
+    *need = k;
+    return TOP;
+  }
+  k -= n_forced;
+  const K diff = any & ~all;
+  int top = diff ? BITS - leading_zeros(diff) : 0;   // bits [0, top) differ
+  K mask = top < BITS ? (K)(TOP << top) : (K)0;
+  K prefix = all & mask;
+  for (int b = 0; top > 0; b ^= 1) {
+    const int shift = max(0, top - kSelBits);
+    const unsigned bins = 1u << (top - shift);
+    for (int i = tid; i < n; i += kSelThreads) {
+      const K x = keys[i];
+      if (x != TOP && (x & mask) == prefix)
+        atomicAdd(&sh.hist[b][(unsigned)(x >> shift) & (bins - 1)], 1u);
+    }
+    if (tid < kSelBins) sh.hist[b ^ 1][tid] = 0;
+    __syncthreads();
+    if (warp == 0) {
+      // Lane l has the 8 bins that are 8 l-th from the top.
+      constexpr int PER = kSelBins / 32;
+      unsigned h[PER], sum = 0;
 #pragma unroll
-      for (int u = 0; u < kSelBins / kSelThreads; ++u) {
-        h[u] = hist[kSelBins - 1 - (tid * (kSelBins / kSelThreads) + u)];
+      for (int u = 0; u < PER; ++u) {
+        h[u] = sh.hist[b][kSelBins - 1 - (lane * PER + u)];
         sum += h[u];
       }
-      unsigned total;
-      const unsigned incl = block_scan(sum, wsum, &total);
-      unsigned before = incl - sum;
-      if (before < need && incl >= need) {   // exactly one thread
+      unsigned incl = sum;
 #pragma unroll
-        for (int u = 0; u < kSelBins / kSelThreads; ++u) {
-          if (before < need && before + h[u] >= need) {
-            sh[0] = (unsigned long long)(kSelBins - 1 - (tid * (kSelBins / kSelThreads) + u));
-            sh[1] = need - before;
-            sh[2] = before + h[u] == need;
-            before = need;
-          } else if (before < need) {
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      unsigned before = incl - sum;
+      if (before < k && incl >= k) {   // exactly one lane
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+          if (before < k && before + h[u] >= k) {
+            sh.prefix = (unsigned long long)(prefix |
+                                             ((K)(kSelBins - 1 - (lane * PER + u)) << shift));
+            sh.left = k - before;
+            before = k;
+          } else if (before < k) {
             before += h[u];
           }
         }
       }
-      __syncthreads();
-      mask |= (unsigned long long)(bins - 1) << shift;
-      prefix |= sh[0] << shift;
-      need = (unsigned)sh[1];
-      whole = sh[2] != 0;
-      top = shift;
-      __syncthreads();
     }
+    __syncthreads();
+    mask |= (K)(bins - 1) << shift;
+    prefix = (K)sh.prefix;
+    k = sh.left;
+    top = shift;
   }
-  // Warp w lists keys [w, w + 1) * share.
-  const int share = ((nb + kSelWarps - 1) / kSelWarps + 31) & ~31;
-  const int i0 = min(nb, warp * share), i1 = min(nb, i0 + share);
-  const bool only_forced = mask == ~0ull && prefix == ~0ull;
-  unsigned ties = 0, above = 0;
+  *need = k;
+  return prefix;
+}
+
+// Lists the indices i, ascending, of the keys of at least `lo`; of those
+// equal to `tie` only the first `need`.  Every warp lists its share.
+template <typename K>
+__device__ void list_keys(const K* keys, int n, K lo, K tie, unsigned need, int* out,
+                          PickShared& sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int share = ((n + kSelWarps - 1) / kSelWarps + 31) & ~31;
+  const int i0 = min(n, warp * share), i1 = min(n, i0 + share);
+  unsigned ties = 0, rest = 0;
+#pragma unroll 4
   for (int i = i0 + lane; i < i1; i += 32) {
-    const unsigned long long k = keys[i];
-    const bool f = k == kKeyForced;
-    const bool tie = only_forced ? f : (!f && (k & mask) == prefix);
-    const bool up = only_forced ? false : (f || (k & mask) > prefix);
-    ties += tie;
-    above += up;
+    const K x = keys[i];
+    ties += x == tie;
+    rest += x >= lo && x != tie;
   }
   ties = __reduce_add_sync(0xffffffffu, ties);
-  above = __reduce_add_sync(0xffffffffu, above);
+  rest = __reduce_add_sync(0xffffffffu, rest);
+  __syncthreads();   // what was in sh before has been read
   if (lane == 0) {
-    wsum[warp] = ties;
-    hist[warp] = above;
+    sh.count[0][warp] = ties;
+    sh.count[1][warp] = rest;
   }
   __syncthreads();
-  unsigned tie_at = 0, up_at = 0;
-  for (int w = 0; w < warp; ++w) {
-    tie_at += wsum[w];
-    up_at += hist[w];
+  unsigned tie_at = 0, rest_at = 0;
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) {
+    tie_at += w < warp ? sh.count[0][w] : 0;
+    rest_at += w < warp ? sh.count[1][w] : 0;
   }
+#pragma unroll 4
   for (int b = i0; b < i1; b += 32) {
     const int i = b + lane;
-    const unsigned long long k = i < i1 ? keys[i] : 0ull;
-    const bool f = i < i1 && k == kKeyForced;
-    const bool tie = i < i1 && (only_forced ? f : (!f && (k & mask) == prefix));
-    const bool up = i < i1 && !only_forced && (f || (k & mask) > prefix);
-    const unsigned bt = __ballot_sync(0xffffffffu, tie), bu = __ballot_sync(0xffffffffu, up);
+    const K x = i < i1 ? keys[i] : (K)0;
+    const bool t = i < i1 && x == tie, r = i < i1 && x >= lo && x != tie;
+    const unsigned bt = __ballot_sync(0xffffffffu, t), br = __ballot_sync(0xffffffffu, r);
     const unsigned below = (1u << lane) - 1u;
-    const unsigned t = tie_at + __popc(bt & below);
-    const unsigned at = up_at + __popc(bu & below) + min(t, need);
-    if ((up || (tie && t < need)) && at < (unsigned)n_sel) out[at] = i;
+    const unsigned at_t = tie_at + __popc(bt & below), at_r = rest_at + __popc(br & below);
+    if (r || (t && at_t < need)) out[at_r + min(at_t, need)] = i;
     tie_at += __popc(bt);
-    up_at += __popc(bu);
+    rest_at += __popc(br);
+  }
+}
+
+// Lists the indices of the keys in [lo, hi], ascending.
+__device__ void list_range(const uint32_t* keys, int n, uint32_t lo, uint32_t hi, int* out,
+                           PickShared& sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int share = ((n + kSelWarps - 1) / kSelWarps + 31) & ~31;
+  const int i0 = min(n, warp * share), i1 = min(n, i0 + share);
+  unsigned in = 0;
+  for (int i = i0 + lane; i < i1; i += 32) in += keys[i] >= lo && keys[i] <= hi;
+  in = __reduce_add_sync(0xffffffffu, in);
+  __syncthreads();
+  if (lane == 0) sh.count[0][warp] = in;
+  __syncthreads();
+  unsigned at = 0;
+  for (int w = 0; w < warp; ++w) at += sh.count[0][w];
+  for (int b = i0; b < i1; b += 32) {
+    const int i = b + lane;
+    const bool t = i < i1 && keys[i] >= lo && keys[i] <= hi;
+    const unsigned bt = __ballot_sync(0xffffffffu, t);
+    if (t) out[at + __popc(bt & ((1u << lane) - 1u))] = i;
+    at += __popc(bt);
   }
 }
 
 // gridDim.y CTAs per (query, KV head) share its pages out; each writes its
-// keys, and the last to arrive picks (one CTA: from its own shared memory).
-// LPP 0: any head_dim.
-template <typename T, int LPP>
-__global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedSelectParams p) {
-  extern __shared__ unsigned long long sel_sm[];
-  unsigned long long* cache = sel_sm;                                   // [kSelCached]
-  unsigned long long* sh = cache + kSelCached;                          // [2 * kSelWarps]
-  unsigned* hist = reinterpret_cast<unsigned*>(sh + 2 * kSelWarps);     // [kSelBins]
-  unsigned* wsum = hist + kSelBins;                                     // [kSelWarps]
-  int* flag = reinterpret_cast<int*>(wsum + kSelWarps);
-  double* q_d = reinterpret_cast<double*>(wsum + kSelWarps + 4);        // [group][hd] (padded)
+// keys, and the last to arrive picks.  HD 0: any head_dim.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kSelThreads, sizeof(T) == 4 && HD >= 64 ? 1 : 2)
+    paged_select_kernel(const PagedSelectParams p) {
+  extern __shared__ uint4 sel_sm[];
+  PickShared& sh = *reinterpret_cast<PickShared*>(sel_sm);
+  constexpr int OFF_KEYS = (sizeof(PickShared) + 15) & ~15;
+  uint32_t* cache = reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(sel_sm) + OFF_KEYS);
+  uint4* q_s = reinterpret_cast<uint4*>(cache + kSelCached);
+  float* q_f = reinterpret_cast<float*>(q_s);
   griddep_launch_dependents();
   griddep_wait();
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x, s = row / p.n_kv, g = row - s * p.n_kv;
   const int past = p.past[s];
+  const int* table = p.table + (size_t)s * p.max_blocks;
+  // Warp w: pages 8 w .. 8 w + 7 of a pass; lane (r, qd) reads page r.  The
+  // first one's look-up does not wait for the query's length.
+  const int first = (HD ? blockIdx.y * kSelWarps * 8 + warp * 8 + (lane >> 2)
+                        : blockIdx.y * kSelThreads + tid);
+  const int first_page = first < p.max_blocks ? table[first] : 0;
   int nb = past < 0 ? 0 : (past >> p.log2p) + 1;
   if (past < -1 || nb > p.max_blocks) {
     if (blockIdx.y == 0 && tid == 0) record_error(p.err, kDevErrBadPos);
@@ -1501,88 +1606,235 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const PagedSe
       for (int i = tid; i < p.n_sel; i += kSelThreads) out[i] = i < nb ? i : -1;
     return;
   }
-  // CTAs with pages: all have the same number of passes, or one more.
-  constexpr int PAGES = LPP ? kSelThreads / LPP : kSelThreads;   // per pass
+  constexpr int PAGES = HD ? kSelWarps * 8 : kSelThreads;   // per pass
   const int ctas = min((int)gridDim.y, (nb + PAGES - 1) / PAGES);
   if ((int)blockIdx.y >= ctas) return;
-  const int hd = LPP ? 16 * LPP : p.hd;
+  const int hd = HD ? HD : p.hd;
   const float* q = p.q + ((size_t)s * p.n_head + g * p.group) * hd;
-  for (int e = tid; e < p.group * hd; e += kSelThreads) {
-    int at = e;
-    if constexpr (LPP > 0) {
-      // Piece c of V dimensions belongs to lane c % LPP.
-      constexpr int V = 16 / (int)sizeof(T);
-      const int h = e / hd, d = e - h * hd, c = d / V;
-      at = (h * LPP + c % LPP) * 18 + (c / LPP) * V + d % V;
+  const int hblocks = (p.group + kPagedHeads - 1) / kPagedHeads;
+  if constexpr (HD > 0) {
+    // Operand of lane l and product u of piece c: dimensions (4 c + qd) * V +
+    // u * V / 2 and the following, V to a 16-byte piece.
+    using Cfg = ScoreMma<T, HD>;
+    constexpr int V = 16 / (int)sizeof(T);
+    for (int e = tid; e < hblocks * Cfg::OPERANDS * 32; e += kSelThreads) {
+      const int l = e & 31, o = (e >> 5) % Cfg::OPERANDS, hb = (e >> 5) / Cfg::OPERANDS;
+      const int u = o & 1, c = (o >> 1) % Cfg::PIECES, low = (o >> 1) / Cfg::PIECES;
+      const int h = hb * kPagedHeads + (l >> 2), d = (4 * c + (l & 3)) * V + u * (V / 2);
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        x[i] = h < p.group ? q[h * HD + d + i] : 0.f;
+        // The half that this bound is for; NaN belongs to both.
+        if (low ? x[i] > 0.f : x[i] < 0.f) x[i] = 0.f;
+      }
+      uint4 w;
+      if constexpr (sizeof(T) == 2) {
+        float hi[4], lo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split_bf16(x[i], hi[i], lo[i]);
+        w = make_uint4(pack_bf16x2(hi[0], hi[1]), pack_bf16x2(lo[0], lo[1]),
+                       pack_bf16x2(hi[2], hi[3]), pack_bf16x2(lo[2], lo[3]));
+      } else {
+        split_tf32(x[0], w.x, w.y);
+        split_tf32(x[1], w.z, w.w);
+      }
+      q_s[e] = w;
     }
-    q_d[at] = (double)q[e];
+  } else {
+    for (int e = tid; e < p.group * hd; e += kSelThreads) q_f[e] = q[e];
   }
   __syncthreads();
-  const bool alone = ctas == 1 && nb <= kSelCached;
-  unsigned long long* keys = alone ? cache : p.keys + (size_t)row * p.max_blocks;
-  const int* table = p.table + (size_t)s * p.max_blocks;
+  const bool alone = ctas == 1, cached = nb <= kSelCached;
+  // Scratch of the row: binary64 keys, then three arrays of 32-bit words.
+  unsigned long long* wide = p.keys + (size_t)row * 3 * p.max_blocks;
+  uint32_t* keys_g = reinterpret_cast<uint32_t*>(wide + p.max_blocks);
+  int* near_g = reinterpret_cast<int*>(keys_g + p.max_blocks);
+  int* taken_g = near_g + p.max_blocks;
+  float* big_g = reinterpret_cast<float*>(near_g);   // of the CTAs, until one picks
+  uint32_t* keys = alone && cached ? cache : keys_g;
   const int stride = ctas * PAGES;
-  int j = blockIdx.y * PAGES + (LPP ? tid / (LPP ? LPP : 1) : tid);
-  const int part = LPP ? tid % (LPP ? LPP : 1) : 0;
-  int page = j < nb ? table[j] : 0;
-  for (int j0 = blockIdx.y * PAGES; j0 < nb; j0 += stride, j += stride) {
-    const int page_n = j + stride < nb ? table[j + stride] : 0;   // one pass ahead
-    const bool bad = page < 0 || page >= p.n_pages;
-    if (bad && part == 0) record_error(p.err, kDevErrBadPage);
-    const T* lo = static_cast<const T*>(p.bounds) + ((size_t)(bad ? 0 : page) * p.n_kv + g) * 2 * hd;
-    unsigned long long key;
-    if constexpr (LPP > 0)
-      key = page_key<T, LPP>(lo, q_d, p.group, part);
-    else
-      key = page_key_any<T>(lo, q_d, p.group, hd);
-    if (bad) key = 0ull;
-    if (j < p.keep_first || j >= nb - p.keep_last) key = kKeyForced;
-    if (j < nb && part == 0) keys[j] = key;
-    page = page_n;
-  }
-  __syncthreads();
-  if (!alone) {
-    if (ctas > 1) {
-      if (tid == 0) *flag = arrive_acq_rel(p.count + row) == (unsigned)(ctas - 1);
-      __syncthreads();
-      if (!*flag) return;
-      if (tid == 0) p.count[row] = 0;
+  float big = 0.f;
+  if constexpr (HD > 0) {
+    const int r = lane >> 2, qd = lane & 3;
+    int j0 = blockIdx.y * PAGES + warp * 8;
+    int page = j0 + r < nb ? first_page : 0;
+    for (; j0 < nb; j0 += stride) {
+      const int page_n = j0 + stride + r < nb ? table[j0 + stride + r] : 0;   // one pass ahead
+      const bool bad = page < 0 || page >= p.n_pages;
+      if (bad && qd == 0) record_error(p.err, kDevErrBadPage);
+      const T* lo =
+          static_cast<const T*>(p.bounds) + ((size_t)(bad ? 0 : page) * p.n_kv + g) * 2 * HD;
+      // (Columns behind the last page repeat page 0: their bounds raise E.)
+      const float2 x = page_scores<T, HD>(lo, q_s, hblocks,
+                                          p.group - (hblocks - 1) * kPagedHeads, &big);
+      if (r < 2) {
+        const int j = j0 + 2 * qd + r;
+        if (j < nb)
+          keys[j] = j < p.keep_first || j >= nb - p.keep_last ? kKeyForced
+                                                              : ordered_key(r ? x.y : x.x);
+      }
+      page = page_n;
     }
-    if (nb <= kSelCached) {
+  } else {
+    for (int j = first; j < nb; j += stride) {
+      int page = j == first ? first_page : table[j];
+      const bool bad = page < 0 || page >= p.n_pages;
+      if (bad) {
+        record_error(p.err, kDevErrBadPage);
+        page = 0;
+      }
+      const T* lo = static_cast<const T*>(p.bounds) + ((size_t)page * p.n_kv + g) * 2 * hd;
+      const float x = page_score_any<T>(lo, q_f, p.group, hd, &big);
+      keys[j] = j < p.keep_first || j >= nb - p.keep_last ? kKeyForced : ordered_key(x);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+  if (lane == 0) sh.big[warp] = big;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) big = fmaxf(big, sh.big[w]);
+  if (!alone) {
+    if (tid == 0) big_g[blockIdx.y] = big;
+    __syncthreads();
+    if (tid == 0) sh.flag = arrive_acq_rel(p.count + row) == (unsigned)(ctas - 1);
+    __syncthreads();
+    if (!sh.flag) return;
+    if (tid == 0) p.count[row] = 0;
+    for (int i = tid; i < ctas; i += kSelThreads) big = fmaxf(big, __ldcg(big_g + i));
+    if (cached) {
+#pragma unroll 4
       for (int i = tid; i < nb; i += kSelThreads) cache[i] = __ldcg(keys + i);
-      __syncthreads();
       keys = cache;
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+    if (lane == 0) sh.big[warp] = big;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSelWarps; ++w) big = fmaxf(big, sh.big[w]);
   }
-  pick_pages(keys, nb, p.n_sel, out, hist, wsum, sh);
+  // E, with S = big * sum |q| >= the sum of a score's absolute terms: 2 hd
+  // products and hd / 8 partial sums, each added with an error of at most
+  // 2^-23 S (the tensor cores may truncate), and 2^-17 S of split operands.
+  float sum_q = 0.f;
+  for (int h = warp; h < p.group; h += kSelWarps) {
+    float x = 0.f;
+    for (int d = lane; d < hd; d += 32) x += fabsf(q[h * hd + d]);
+    sum_q = fmaxf(sum_q, warp_sum(x));
+  }
+  __syncthreads();
+  if (lane == 0) sh.big[warp] = sum_q;
+  if (tid == 0) sh.near = sh.sure = 0;
+  unsigned need;
+  const uint32_t t_key = kth_key<uint32_t>(keys, nb, (unsigned)p.n_sel, sh, &need);
+  if (t_key == kKeyForced) {   // more forced pages than places
+    list_keys<uint32_t>(keys, nb, kKeyForced, kKeyForced, need, out, sh);
+    return;
+  }
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) sum_q = fmaxf(sum_q, sh.big[w]);
+  const float E2 = 2.02f * (2.125f * hd * 1.1920929e-7f + 7.6293945e-6f) * big * sum_q;   // 2 E, and its own roundings
+  uint32_t k_lo = 0, k_hi = kKeyForced - 1;
+  if (E2 < INFINITY) {
+    const float t = key_value(t_key);
+    k_lo = ordered_key(__fsub_rd(t, E2));
+    k_hi = ordered_key(__fadd_ru(t, E2));
+  }
+  // Pages near the border, and those surely taken.
+  unsigned near = 0, sure = 0;
+  for (int i = tid; i < nb; i += kSelThreads) {
+    const uint32_t x = keys[i];
+    sure += x > k_hi;
+    if (x >= k_lo && x <= k_hi) {
+      const unsigned at = atomicAdd(&sh.near, 1u);
+      if (at < kSelNear) sh.near_at[at] = i;
+    }
+  }
+  sure = __reduce_add_sync(0xffffffffu, sure);
+  if (lane == 0 && sure) atomicAdd(&sh.sure, sure);
+  __syncthreads();
+  near = sh.near;
+  sure = sh.sure;
+  if (sure + near == (unsigned)p.n_sel) {   // all of them
+    list_keys<uint32_t>(keys, nb, k_lo, 0u, 0u, out, sh);
+    return;
+  }
+  // Not all: in the order of their binary64 scores, ties to the lower index.
+  const unsigned left = (unsigned)p.n_sel - sure;
+  const bool few = near <= kSelNear;
+  if (!few) {
+    list_range(keys, nb, k_lo, k_hi, near_g, sh);
+    __syncthreads();
+  }
+  for (unsigned i = tid; i < near; i += kSelThreads) (few ? sh.near_key : wide)[i] = 0ull;
+  __syncthreads();
+  // A warp per (page, head); NaN is above every key while the heads meet.
+  for (unsigned e = warp; e < near * p.group; e += kSelWarps) {
+    const unsigned i = e / p.group, h = e - i * p.group;
+    const int pg = table[few ? sh.near_at[i] : near_g[i]];
+    const bool bad = pg < 0 || pg >= p.n_pages;
+    const T* lo = static_cast<const T*>(p.bounds) + ((size_t)(bad ? 0 : pg) * p.n_kv + g) * 2 * hd;
+    const double x = exact_score<T>(lo, q + h * hd, hd);
+    if (lane == 0)
+      atomicMax(&(few ? sh.near_key : wide)[i], bad || x != x ? ~0ull : ordered_key(x));
+  }
+  __syncthreads();
+  for (unsigned i = tid; i < near; i += kSelThreads) {
+    unsigned long long* x = &(few ? sh.near_key : wide)[i];
+    if (*x == ~0ull) *x = 0ull;   // NaN ranks last
+  }
+  __syncthreads();
+  if (few) {
+    if (tid < (int)near) {
+      const unsigned long long x = sh.near_key[tid];
+      const int at = sh.near_at[tid];
+      unsigned above = 0;
+      for (unsigned i = 0; i < near; ++i) {
+        const unsigned long long y = sh.near_key[i];
+        above += y > x || (y == x && sh.near_at[i] < at);
+      }
+      if (above < left) keys[at] = kKeyForced;
+    }
+  } else {
+    unsigned ties;
+    const unsigned long long t64 = kth_key<unsigned long long>(wide, (int)near, left, sh, &ties);
+    list_keys<unsigned long long>(wide, (int)near, t64, t64, ties, taken_g, sh);
+    __syncthreads();
+    for (unsigned i = tid; i < left; i += kSelThreads) keys[near_g[taken_g[i]]] = kKeyForced;
+  }
+  __syncthreads();
+  list_keys<uint32_t>(keys, nb, k_hi + 1, 0u, 0u, out, sh);
 }
 
-template <typename T, int LPP>
-static cudaError_t launch_select_cfg(const PagedSelectParams& p, int ctas, cudaStream_t st) {
+template <typename T, int HD>
+static cudaError_t launch_select_cfg(const PagedSelectParams& p, int num_sms, cudaStream_t st) {
   static bool done[64] = {};
-  cudaError_t e = allow_max_smem(paged_select_kernel<T, LPP>, done);
+  cudaError_t e = allow_max_smem(paged_select_kernel<T, HD>, done);
   if (e != cudaSuccess) return e;
-  const size_t smem = (size_t)(kSelCached + 2 * kSelWarps) * 8 + (size_t)(kSelBins + kSelWarps + 4) * 4 +
-                      (size_t)p.group * (LPP ? LPP * 18 : p.hd) * 8;
-  return launch_chained(paged_select_kernel<T, LPP>, dim3((unsigned)(p.n * p.n_kv), (unsigned)ctas),
+  const int hblocks = (p.group + kPagedHeads - 1) / kPagedHeads;
+  const size_t q_bytes = HD ? (size_t)hblocks * ScoreMma<T, HD ? HD : 64>::OPERANDS * 32 * 16
+                            : (size_t)p.group * p.hd * 4;
+  const size_t smem = ((sizeof(PickShared) + 15) & ~size_t(15)) + (size_t)kSelCached * 4 + q_bytes;
+  // Two CTAs fit an SM; more than one per row only while there are SMs
+  // without one and pages for another pass.
+  const int pages = HD ? kSelWarps * 8 : kSelThreads;
+  const int most = (p.max_blocks + pages - 1) / pages;
+  int ctas = 2 * num_sms / (p.n * p.n_kv);
+  if (ctas > most) ctas = most;
+  if (ctas < 1) ctas = 1;
+  return launch_chained(paged_select_kernel<T, HD>, dim3((unsigned)(p.n * p.n_kv), (unsigned)ctas),
                         dim3(kSelThreads), smem, st, p);
 }
 
 template <typename T>
 static cudaError_t launch_select_type(const PagedSelectParams& p, int num_sms, cudaStream_t st) {
-  // Two CTAs fit an SM (keys in shared memory); more than one per row only
-  // while there are SMs without one and pages for another pass.
-  const int lpp = p.hd == 64 ? 4 : p.hd == 128 ? 8 : p.hd == 32 ? 2 : 0;
-  const int pages = lpp ? kSelThreads / lpp : kSelThreads;
-  const int most = (p.max_blocks + pages - 1) / pages;
-  int ctas = 2 * num_sms / (p.n * p.n_kv);
-  if (ctas > most) ctas = most;
-  if (ctas < 1) ctas = 1;
-  switch (lpp) {
-    case 2: return launch_select_cfg<T, 2>(p, ctas, st);
-    case 4: return launch_select_cfg<T, 4>(p, ctas, st);
-    case 8: return launch_select_cfg<T, 8>(p, ctas, st);
-    default: return launch_select_cfg<T, 0>(p, ctas, st);
+  switch (p.hd) {
+    case 32: return launch_select_cfg<T, 32>(p, num_sms, st);
+    case 64: return launch_select_cfg<T, 64>(p, num_sms, st);
+    case 128: return launch_select_cfg<T, 128>(p, num_sms, st);
+    default: return launch_select_cfg<T, 0>(p, num_sms, st);
   }
 }
 
