@@ -1250,7 +1250,6 @@ cudaError_t launch_paged_mma(const CUtensorMap& tk, const CUtensorMap& tv, const
 
 constexpr int kSelThreads = 512;
 constexpr int kSelWarps = kSelThreads / 32;
-constexpr int kSelBits = 8, kSelBins = 1 << kSelBits;
 constexpr int kSelNear = 256;       // pages near the border that are ranked by comparisons
 constexpr int kSelCached = 16384;   // binary32 keys that the picking CTA holds in shared memory
 constexpr uint32_t kKeyForced = ~0u;  // pages that are always taken
@@ -1287,16 +1286,22 @@ struct ScoreMma {
 };
 
 template <typename T, int HD>
-__device__ __forceinline__ float2 page_scores(const T* row, const uint4* q_s, int hblocks,
-                                              int last_heads, float* big) {
-  using Cfg = ScoreMma<T, HD>;
-  const int lane = threadIdx.x & 31, r = lane >> 2, qd = lane & 3;
-  uint4 b[2][Cfg::PIECES];   // upper, lower
+__device__ __forceinline__ void load_bounds(const T* row,
+                                            uint4 (&b)[2][ScoreMma<T, HD>::PIECES]) {
+  const int qd = threadIdx.x & 3;
 #pragma unroll
-  for (int c = 0; c < Cfg::PIECES; ++c) {
-    b[0][c] = reinterpret_cast<const uint4*>(row + HD)[4 * c + qd];
-    b[1][c] = reinterpret_cast<const uint4*>(row)[4 * c + qd];
+  for (int c = 0; c < ScoreMma<T, HD>::PIECES; ++c) {
+    b[0][c] = reinterpret_cast<const uint4*>(row + HD)[4 * c + qd];   // upper
+    b[1][c] = reinterpret_cast<const uint4*>(row)[4 * c + qd];        // lower
   }
+}
+
+template <typename T, int HD>
+__device__ __forceinline__ float2 page_scores(const uint4 (&b)[2][ScoreMma<T, HD>::PIECES],
+                                              const uint4* q_s, int hblocks, int last_heads,
+                                              float* big) {
+  using Cfg = ScoreMma<T, HD>;
+  const int lane = threadIdx.x & 31, r = lane >> 2;
   float m = 0.f;
 #pragma unroll
   for (int k = 0; k < 2; ++k)
@@ -1392,60 +1397,88 @@ __device__ double exact_score(const T* lo_p, const float* q, int hd) {
 
 // Shared memory of the picking CTA.
 struct PickShared {
-  unsigned hist[2][kSelBins];
   unsigned count[2][kSelWarps];
   unsigned long long wide[2][kSelWarps];
-  unsigned long long prefix;
-  unsigned left, forced, near, sure;
+  unsigned hist[kSelThreads];
+  unsigned steps[3];
+  unsigned near, sure;
   float big[kSelWarps];
   int flag;
   int near_at[kSelNear];
   unsigned long long near_key[kSelNear];
 };
 
-__device__ __forceinline__ int leading_zeros(uint32_t v) { return __clz((int)v); }
-__device__ __forceinline__ int leading_zeros(unsigned long long v) { return __clzll((long long)v); }
+// Bit by bit from the top: does taking the bit leave k keys?  For keys so
+// many of which are equal that they cannot be told apart by bins.
+template <typename K>
+__device__ K kth_key_bits(const K* keys, int n, unsigned k, PickShared& sh, unsigned* need) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  __syncthreads();
+  if (tid < 3) sh.steps[tid] = 0;
+  __syncthreads();
+  K bound = 0;
+  int step = 0;
+  auto count = [&](K cand) -> unsigned {
+    unsigned c = 0;
+    for (int i = tid; i < n; i += kSelThreads) c += keys[i] >= cand;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane == 0 && c) atomicAdd(&sh.steps[step], c);
+    if (tid == 0) sh.steps[step == 2 ? 0 : step + 1] = 0;
+    __syncthreads();
+    c = sh.steps[step];
+    step = step == 2 ? 0 : step + 1;
+    return c;
+  };
+  for (int bit = 8 * (int)sizeof(K) - 1; bit >= 0; --bit) {
+    const K cand = bound | ((K)1 << bit);
+    if (count(cand) >= k) bound = cand;
+  }
+  *need = bound == ~(K)0 ? k : k - count(bound + 1);
+  return bound;
+}
 
 // The k-th largest of n >= k keys (k >= 1) and how many of those equal to it
-// are among the k largest.  A radix search, 8 bits at a time from the highest
-// bit in which the keys differ at all (the largest value, forced pages,
-// aside: scores of one query share sign and exponent bits); one warp finds
-// the digit, so a step has two barriers.
+// are among the k largest.  The keys' range (forced pages aside) is cut into
+// as many equal bins as there are threads; the keys of the one bin that holds
+// the k-th are ranked by comparisons.
 template <typename K>
 __device__ K kth_key(const K* keys, int n, unsigned k, PickShared& sh, unsigned* need) {
-  constexpr int BITS = 8 * (int)sizeof(K);
   constexpr K TOP = ~(K)0;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  K any = 0, all = TOP;
+  K lo = TOP, hi = 0;
   unsigned forced = 0;
+#pragma unroll 4
   for (int i = tid; i < n; i += kSelThreads) {
     const K x = keys[i];
     if (x == TOP) {
       ++forced;
     } else {
-      any |= x;
-      all &= x;
+      lo = x < lo ? x : lo;
+      hi = x > hi ? x : hi;
     }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    any |= __shfl_xor_sync(0xffffffffu, any, o);
-    all &= __shfl_xor_sync(0xffffffffu, all, o);
+    const K x = __shfl_xor_sync(0xffffffffu, lo, o), y = __shfl_xor_sync(0xffffffffu, hi, o);
+    lo = x < lo ? x : lo;
+    hi = y > hi ? y : hi;
   }
   forced = __reduce_add_sync(0xffffffffu, forced);
   __syncthreads();   // what was in sh before has been read
   if (lane == 0) {
-    sh.wide[0][warp] = any;
-    sh.wide[1][warp] = all;
+    sh.wide[0][warp] = lo;
+    sh.wide[1][warp] = hi;
     sh.count[0][warp] = forced;
   }
-  if (tid < kSelBins) sh.hist[0][tid] = 0;
+  sh.hist[tid] = 0;
+  if (tid == 0) sh.near = 0;
   __syncthreads();
   unsigned n_forced = 0;
 #pragma unroll
   for (int w = 0; w < kSelWarps; ++w) {
-    any |= (K)sh.wide[0][w];
-    all &= (K)sh.wide[1][w];
+    const K x = (K)sh.wide[0][w], y = (K)sh.wide[1][w];
+    lo = x < lo ? x : lo;
+    hi = y > hi ? y : hi;
     n_forced += sh.count[0][w];
   }
   if (n_forced >= k) {
@@ -1453,58 +1486,59 @@ __device__ K kth_key(const K* keys, int n, unsigned k, PickShared& sh, unsigned*
     return TOP;
   }
   k -= n_forced;
-  const K diff = any & ~all;
-  int top = diff ? BITS - leading_zeros(diff) : 0;   // bits [0, top) differ
-  K mask = top < BITS ? (K)(TOP << top) : (K)0;
-  K prefix = all & mask;
-  for (int b = 0; top > 0; b ^= 1) {
-    const int shift = max(0, top - kSelBits);
-    const unsigned bins = 1u << (top - shift);
-    for (int i = tid; i < n; i += kSelThreads) {
-      const K x = keys[i];
-      if (x != TOP && (x & mask) == prefix)
-        atomicAdd(&sh.hist[b][(unsigned)(x >> shift) & (bins - 1)], 1u);
-    }
-    if (tid < kSelBins) sh.hist[b ^ 1][tid] = 0;
-    __syncthreads();
-    if (warp == 0) {
-      // Lane l has the 8 bins that are 8 l-th from the top.
-      constexpr int PER = kSelBins / 32;
-      unsigned h[PER], sum = 0;
-#pragma unroll
-      for (int u = 0; u < PER; ++u) {
-        h[u] = sh.hist[b][kSelBins - 1 - (lane * PER + u)];
-        sum += h[u];
-      }
-      unsigned incl = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      unsigned before = incl - sum;
-      if (before < k && incl >= k) {   // exactly one lane
-#pragma unroll
-        for (int u = 0; u < PER; ++u) {
-          if (before < k && before + h[u] >= k) {
-            sh.prefix = (unsigned long long)(prefix |
-                                             ((K)(kSelBins - 1 - (lane * PER + u)) << shift));
-            sh.left = k - before;
-            before = k;
-          } else if (before < k) {
-            before += h[u];
-          }
-        }
-      }
-    }
-    __syncthreads();
-    mask |= (K)(bins - 1) << shift;
-    prefix = (K)sh.prefix;
-    k = sh.left;
-    top = shift;
+  int shift = 0;
+  while (((hi - lo) >> shift) >= (K)kSelThreads) ++shift;
+#pragma unroll 4
+  for (int i = tid; i < n; i += kSelThreads) {
+    const K x = keys[i];
+    if (x != TOP) atomicAdd(&sh.hist[(unsigned)((x - lo) >> shift)], 1u);
   }
-  *need = k;
-  return prefix;
+  __syncthreads();
+  // Thread t has the t-th bin from the top.
+  const unsigned mine = sh.hist[kSelThreads - 1 - tid];
+  unsigned incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) sh.count[0][warp] = incl;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) incl += w < warp ? sh.count[0][w] : 0;
+  if (incl - mine < k && incl >= k) {   // exactly one thread
+    sh.steps[0] = kSelThreads - 1 - tid;
+    sh.steps[1] = k - (incl - mine);
+    sh.steps[2] = mine;
+  }
+  __syncthreads();
+  const unsigned bin = sh.steps[0], left = sh.steps[1], m = sh.steps[2];
+  if (m > kSelNear) {
+    K t = kth_key_bits(keys, n, k + n_forced, sh, need);
+    return t;
+  }
+#pragma unroll 4
+  for (int i = tid; i < n; i += kSelThreads) {
+    const K x = keys[i];
+    if (x != TOP && (unsigned)((x - lo) >> shift) == bin)
+      sh.near_key[atomicAdd(&sh.near, 1u)] = (unsigned long long)x;
+  }
+  __syncthreads();
+  if (tid < (int)m) {
+    const unsigned long long x = sh.near_key[tid];
+    unsigned above = 0, same = 0;
+    for (unsigned i = 0; i < m; ++i) {
+      above += sh.near_key[i] > x;
+      same += sh.near_key[i] == x;
+    }
+    if (above < left && left <= above + same) {   // all threads of the same key
+      sh.wide[0][0] = x;
+      sh.steps[0] = left - above;
+    }
+  }
+  __syncthreads();
+  *need = sh.steps[0];
+  return (K)sh.wide[0][0];
 }
 
 // Lists the indices i, ascending, of the keys of at least `lo`; of those
@@ -1595,20 +1629,7 @@ __global__ void __launch_bounds__(kSelThreads, sizeof(T) == 4 && HD >= 64 ? 1 : 
   const int first = (HD ? blockIdx.y * kSelWarps * 8 + warp * 8 + (lane >> 2)
                         : blockIdx.y * kSelThreads + tid);
   const int first_page = first < p.max_blocks ? table[first] : 0;
-  int nb = past < 0 ? 0 : (past >> p.log2p) + 1;
-  if (past < -1 || nb > p.max_blocks) {
-    if (blockIdx.y == 0 && tid == 0) record_error(p.err, kDevErrBadPos);
-    nb = 0;
-  }
-  int* out = p.pages + (size_t)row * p.n_sel;
-  if (nb <= p.n_sel) {
-    if (blockIdx.y == 0)
-      for (int i = tid; i < p.n_sel; i += kSelThreads) out[i] = i < nb ? i : -1;
-    return;
-  }
-  constexpr int PAGES = HD ? kSelWarps * 8 : kSelThreads;   // per pass
-  const int ctas = min((int)gridDim.y, (nb + PAGES - 1) / PAGES);
-  if ((int)blockIdx.y >= ctas) return;
+  // Nor do the operands.
   const int hd = HD ? HD : p.hd;
   const float* q = p.q + ((size_t)s * p.n_head + g * p.group) * hd;
   const int hblocks = (p.group + kPagedHeads - 1) / kPagedHeads;
@@ -1644,6 +1665,20 @@ __global__ void __launch_bounds__(kSelThreads, sizeof(T) == 4 && HD >= 64 ? 1 : 
   } else {
     for (int e = tid; e < p.group * hd; e += kSelThreads) q_f[e] = q[e];
   }
+  int nb = past < 0 ? 0 : (past >> p.log2p) + 1;
+  if (past < -1 || nb > p.max_blocks) {
+    if (blockIdx.y == 0 && tid == 0) record_error(p.err, kDevErrBadPos);
+    nb = 0;
+  }
+  int* out = p.pages + (size_t)row * p.n_sel;
+  if (nb <= p.n_sel) {
+    if (blockIdx.y == 0)
+      for (int i = tid; i < p.n_sel; i += kSelThreads) out[i] = i < nb ? i : -1;
+    return;
+  }
+  constexpr int PAGES = HD ? kSelWarps * 8 : kSelThreads;   // per pass
+  const int ctas = min((int)gridDim.y, (nb + PAGES - 1) / PAGES);
+  if ((int)blockIdx.y >= ctas) return;
   __syncthreads();
   const bool alone = ctas == 1, cached = nb <= kSelCached;
   // Scratch of the row: binary64 keys, then three arrays of 32-bit words.
@@ -1657,16 +1692,25 @@ __global__ void __launch_bounds__(kSelThreads, sizeof(T) == 4 && HD >= 64 ? 1 : 
   float big = 0.f;
   if constexpr (HD > 0) {
     const int r = lane >> 2, qd = lane & 3;
+    constexpr int PIECES = ScoreMma<T, HD>::PIECES;
     int j0 = blockIdx.y * PAGES + warp * 8;
-    int page = j0 + r < nb ? first_page : 0;
-    for (; j0 < nb; j0 += stride) {
-      const int page_n = j0 + stride + r < nb ? table[j0 + stride + r] : 0;   // one pass ahead
+    // (Columns behind the last page repeat page 0: their bounds raise E.)
+    auto bounds_of = [&](int page) -> const T* {
       const bool bad = page < 0 || page >= p.n_pages;
       if (bad && qd == 0) record_error(p.err, kDevErrBadPage);
-      const T* lo =
-          static_cast<const T*>(p.bounds) + ((size_t)(bad ? 0 : page) * p.n_kv + g) * 2 * HD;
-      // (Columns behind the last page repeat page 0: their bounds raise E.)
-      const float2 x = page_scores<T, HD>(lo, q_s, hblocks,
+      return static_cast<const T*>(p.bounds) + ((size_t)(bad ? 0 : page) * p.n_kv + g) * 2 * HD;
+    };
+    auto entry = [&](int j) { return j + r < nb ? table[j + r] : 0; };
+    uint4 b[2][PIECES];
+    if (j0 < nb) load_bounds<T, HD>(bounds_of(j0 + r < nb ? first_page : 0), b);
+    int page = entry(j0 + stride);
+    for (; j0 < nb; j0 += stride) {
+      // The next pass's bounds and the page of the one after are on their way.
+      uint4 b_n[2][PIECES];
+      const bool more = j0 + stride < nb;
+      if (more) load_bounds<T, HD>(bounds_of(page), b_n);
+      page = entry(j0 + 2 * stride);
+      const float2 x = page_scores<T, HD>(b, q_s, hblocks,
                                           p.group - (hblocks - 1) * kPagedHeads, &big);
       if (r < 2) {
         const int j = j0 + 2 * qd + r;
@@ -1674,7 +1718,12 @@ __global__ void __launch_bounds__(kSelThreads, sizeof(T) == 4 && HD >= 64 ? 1 : 
           keys[j] = j < p.keep_first || j >= nb - p.keep_last ? kKeyForced
                                                               : ordered_key(r ? x.y : x.x);
       }
-      page = page_n;
+      if (more)
+#pragma unroll
+        for (int c = 0; c < PIECES; ++c) {
+          b[0][c] = b_n[0][c];
+          b[1][c] = b_n[1][c];
+        }
     }
   } else {
     for (int j = first; j < nb; j += stride) {
@@ -1726,7 +1775,6 @@ __global__ void __launch_bounds__(kSelThreads, sizeof(T) == 4 && HD >= 64 ? 1 : 
   }
   __syncthreads();
   if (lane == 0) sh.big[warp] = sum_q;
-  if (tid == 0) sh.near = sh.sure = 0;
   unsigned need;
   const uint32_t t_key = kth_key<uint32_t>(keys, nb, (unsigned)p.n_sel, sh, &need);
   if (t_key == kKeyForced) {   // more forced pages than places
@@ -1742,6 +1790,9 @@ __global__ void __launch_bounds__(kSelThreads, sizeof(T) == 4 && HD >= 64 ? 1 : 
     k_lo = ordered_key(__fsub_rd(t, E2));
     k_hi = ordered_key(__fadd_ru(t, E2));
   }
+  __syncthreads();
+  if (tid == 0) sh.near = sh.sure = 0;
+  __syncthreads();
   // Pages near the border, and those surely taken.
   unsigned near = 0, sure = 0;
   for (int i = tid; i < nb; i += kSelThreads) {
