@@ -239,10 +239,11 @@ def _ptr(x) -> Optional[int]:
         if not x.flags["C_CONTIGUOUS"]:
             raise ValueError("arrays must be C-contiguous")
         return x.ctypes.data
-    if hasattr(x, "data_ptr"):
+    data_ptr = getattr(x, "data_ptr", None)
+    if data_ptr is not None:
         if hasattr(x, "is_contiguous") and not x.is_contiguous():
             raise ValueError("tensors must be contiguous")
-        return x.data_ptr()
+        return data_ptr()
     raise TypeError(f"cannot take the address of {type(x).__name__}")
 
 
@@ -775,24 +776,38 @@ class PagedKVCache:
             _ints(pages, args[0] * self.n_kv_head * n_sel, "pages"), _ptr(out)))
 
     def _n_sel(self, pages, n: int) -> int:
-        shape = tuple(pages.shape)
-        if len(shape) != 3 or shape[:2] != (n, self.n_kv_head):
-            raise ValueError(f"pages is {shape}, not [{n}][{self.n_kv_head}][n_sel]")
+        shape = pages.shape
+        if len(shape) != 3 or shape[0] != n or shape[1] != self.n_kv_head:
+            raise ValueError(f"pages is {tuple(shape)}, not [{n}][{self.n_kv_head}][n_sel]")
         return shape[2]
 
 
 def _table_shape(t):
-    shape = tuple(t.shape)
+    shape = t.shape
     if len(shape) != 2:
-        raise ValueError(f"block_table is {shape}, not [n_seqs][max_blocks]")
+        raise ValueError(f"block_table is {tuple(shape)}, not [n_seqs][max_blocks]")
     return shape
+
+
+_type_names = {}  # numpy and torch types by what they are called
+
+
+def _type_name(dtype) -> str:
+    name = _type_names.get(dtype)
+    if name is None:
+        name = _type_names[dtype] = str(dtype).rsplit(".", 1)[-1]
+    return name
+
+
+def _size(x) -> int:
+    return x.size if isinstance(x, np.ndarray) else x.numel()
 
 
 def _rows(x, width: int, what: str) -> int:
     """Rows of a float32 array of `width` columns."""
-    if not str(x.dtype).endswith("float32"):
+    if _type_name(x.dtype) != "float32":
         raise ValueError(f"{what} is {x.dtype}, not float32")
-    n = x.numel() if hasattr(x, "numel") else x.size
+    n = _size(x)
     if n % width:
         raise ValueError(f"{what} has {n} values, not rows of {width}")
     return n // width
@@ -802,9 +817,9 @@ def _ints(x, n: int, what: str):
     """Address of an int32 array of n values (None for None)."""
     if x is None:
         return None
-    if not str(x.dtype).endswith("int32") or str(x.dtype).endswith("uint32"):
+    if _type_name(x.dtype) != "int32":
         raise ValueError(f"{what} is {x.dtype}, not int32")
-    if (x.numel() if hasattr(x, "numel") else x.size) != n:
+    if _size(x) != n:
         raise ValueError(f"{what} has not {n} values")
     return _ptr(x)
 

@@ -1596,6 +1596,48 @@ int ensure_kept(tg_context* ctx, T** buf, size_t* cap, size_t need, bool zero = 
   return TG_OK;
 }
 
+// Where the pointers of a paged call lie, by one driver query each (a third
+// of the time of cudaPointerGetAttributes; nothing is remembered between
+// calls).  Device memory of another GPU is refused.
+struct PagedArg {
+  const void* p;
+  const char* what;
+  bool device = false;
+};
+
+int classify_args(tg_context* ctx, PagedArg* args, int n, bool* all_device) {
+  typedef CUresult (*query_t)(unsigned, CUpointer_attribute*, void**, CUdeviceptr);
+  static const query_t query = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuPointerGetAttributes", &f, cudaEnableDefault, &q) !=
+            cudaSuccess || q != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      f = nullptr;
+    }
+    return reinterpret_cast<query_t>(f);
+  }();
+  if (!query) return fail(TG_ERR_CUDA, "cuPointerGetAttributes is not available");
+  *all_device = true;
+  for (int i = 0; i < n; ++i) {
+    if (!args[i].p) continue;
+    unsigned type = 0, managed = 0;
+    int ordinal = -1;
+    CUpointer_attribute what[3] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE,
+                                   CU_POINTER_ATTRIBUTE_IS_MANAGED,
+                                   CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL};
+    void* out[3] = {&type, &managed, &ordinal};
+    if (query(3, what, out, (CUdeviceptr)reinterpret_cast<uintptr_t>(args[i].p)) != CUDA_SUCCESS)
+      type = managed = 0;
+    args[i].device = type == CU_MEMORYTYPE_DEVICE || managed != 0;
+    if (args[i].device && !managed && ordinal != ctx->device)
+      return fail(TG_ERR_INVALID_ARG, "%s lies on device %d, the context's is %d", args[i].what,
+                  ordinal, ctx->device);
+    if (!args[i].device) *all_device = false;
+  }
+  return TG_OK;
+}
+
 int check_paged_call(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, int max_blocks) {
   if (!ctx || !pk) return fail(TG_ERR_INVALID_ARG, "null context or cache");
   if (pk->ctx != ctx) return fail(TG_ERR_INVALID_ARG, "cache belongs to another context");
@@ -1610,9 +1652,7 @@ int check_paged_call(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, in
 // Host arrays: last positions in [-1, max_blocks*page_size) and, when the
 // table is on the host too, the entries they use in [0, n_pages).
 int check_host_pages(const tg_paged_kv* pk, const int32_t* past, const int32_t* table, int n,
-                     int max_blocks) {
-  if (is_device_ptr(past)) return TG_OK;
-  const bool host_table = !is_device_ptr(table);
+                     int max_blocks, bool host_table) {
   const long long limit = (long long)max_blocks << pk->log2p;
   for (int s = 0; s < n; ++s) {
     if (past[s] < -1 || past[s] >= limit)
@@ -3097,7 +3137,11 @@ int tg_paged_append(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, int
   const tg_paged_desc& d = pk->d;
   const int row = d.n_kv_head * d.head_dim, qrow = d.n_head * d.head_dim;
   // Host arrays are checked here, device ones by the kernel.
-  const bool host_cu = cu_tokens && !is_device_ptr(cu_tokens);
+  PagedArg args[7] = {{k, "k"}, {v, "v"}, {q, "q"}, {q_out, "q_out"},
+                      {cu_tokens, "cu_tokens"}, {pos0, "pos0"}, {block_table, "block_table"}};
+  bool all_device = false;
+  TG_TRY(classify_args(ctx, args, 7, &all_device));
+  const bool host_cu = cu_tokens && !args[4].device;
   if (host_cu) {
     if (cu_tokens[0] < 0 || cu_tokens[n_seqs] > n_tokens)
       return fail(TG_ERR_INVALID_ARG, "cu_tokens outside [0, %d]", n_tokens);
@@ -3105,8 +3149,8 @@ int tg_paged_append(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, int
       if (cu_tokens[s + 1] < cu_tokens[s])
         return fail(TG_ERR_INVALID_ARG, "cu_tokens[%d] decreases", s + 1);
   }
-  if (!is_device_ptr(pos0) && (host_cu || !cu_tokens)) {
-    const bool host_table = !is_device_ptr(block_table);
+  if (!args[5].device && (host_cu || !cu_tokens)) {
+    const bool host_table = !args[6].device;
     const long long limit = std::min((long long)max_blocks << pk->log2p, (long long)d.max_pos);
     for (int s = 0; s < n_seqs; ++s) {
       const int n = cu_tokens ? cu_tokens[s + 1] - cu_tokens[s] : 1;
@@ -3123,17 +3167,19 @@ int tg_paged_append(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, int
       }
     }
   }
-  const void *dk = nullptr, *dv = nullptr, *dq = nullptr, *dcu = nullptr, *dp = nullptr, *dt = nullptr;
-  void* dqo = nullptr;
-  TG_TRY(stage_in(ctx, k, (size_t)n_tokens * row * 4, &dk));
-  TG_TRY(stage_in(ctx, v, (size_t)n_tokens * row * 4, &dv));
-  TG_TRY(stage_in(ctx, cu_tokens, cu_tokens ? (size_t)(n_seqs + 1) * 4 : 0, &dcu));
-  TG_TRY(stage_in(ctx, pos0, (size_t)n_seqs * 4, &dp));
-  TG_TRY(stage_in(ctx, block_table, (size_t)n_seqs * max_blocks * 4, &dt));
-  if (q) {
-    TG_TRY(stage_in(ctx, q, (size_t)n_tokens * qrow * 4, &dq));
-    // Host rows of padding tokens come back as they went in.
-    TG_TRY(stage_out(ctx, q_out, (size_t)n_tokens * qrow * 4, true, &dqo));
+  const void *dk = k, *dv = v, *dq = q, *dcu = cu_tokens, *dp = pos0, *dt = block_table;
+  void* dqo = q_out;
+  if (!all_device) {
+    TG_TRY(stage_in(ctx, k, (size_t)n_tokens * row * 4, &dk));
+    TG_TRY(stage_in(ctx, v, (size_t)n_tokens * row * 4, &dv));
+    TG_TRY(stage_in(ctx, cu_tokens, cu_tokens ? (size_t)(n_seqs + 1) * 4 : 0, &dcu));
+    TG_TRY(stage_in(ctx, pos0, (size_t)n_seqs * 4, &dp));
+    TG_TRY(stage_in(ctx, block_table, (size_t)n_seqs * max_blocks * 4, &dt));
+    if (q) {
+      TG_TRY(stage_in(ctx, q, (size_t)n_tokens * qrow * 4, &dq));
+      // Host rows of padding tokens come back as they went in.
+      TG_TRY(stage_out(ctx, q_out, (size_t)n_tokens * qrow * 4, true, &dqo));
+    }
   }
   TG_TRY(commit_inputs(ctx));
   const void* io[4] = {dk, dv, dq, dqo};
@@ -3182,16 +3228,23 @@ int paged_attention(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, con
   TG_TRY(check_paged_call(ctx, pk, layer, n_seqs, max_blocks));
   if (n_seqs == 0) return TG_OK;
   if (!q || !past_len || !block_table || !out) return fail(TG_ERR_INVALID_ARG, "null argument");
-  TG_TRY(check_host_pages(pk, past_len, block_table, n_seqs, max_blocks));
+  PagedArg args[5] = {{q, "q"}, {past_len, "past_len"}, {block_table, "block_table"},
+                      {pages, "pages"}, {out, "out"}};
+  bool all_device = false;
+  TG_TRY(classify_args(ctx, args, 5, &all_device));
+  if (!args[1].device)
+    TG_TRY(check_host_pages(pk, past_len, block_table, n_seqs, max_blocks, !args[2].device));
   const tg_paged_desc& d = pk->d;
   const size_t qb = (size_t)n_seqs * d.n_head * d.head_dim * 4;
-  const void *dq = nullptr, *dp = nullptr, *dt = nullptr, *dsel = nullptr;
-  void* dout = nullptr;
-  TG_TRY(stage_in(ctx, q, qb, &dq));
-  TG_TRY(stage_in(ctx, past_len, (size_t)n_seqs * 4, &dp));
-  TG_TRY(stage_in(ctx, block_table, (size_t)n_seqs * max_blocks * 4, &dt));
-  if (pages) TG_TRY(stage_in(ctx, pages, (size_t)n_seqs * d.n_kv_head * n_sel * 4, &dsel));
-  TG_TRY(stage_out(ctx, out, qb, false, &dout));
+  const void *dq = q, *dp = past_len, *dt = block_table, *dsel = pages;
+  void* dout = out;
+  if (!all_device) {
+    TG_TRY(stage_in(ctx, q, qb, &dq));
+    TG_TRY(stage_in(ctx, past_len, (size_t)n_seqs * 4, &dp));
+    TG_TRY(stage_in(ctx, block_table, (size_t)n_seqs * max_blocks * 4, &dt));
+    if (pages) TG_TRY(stage_in(ctx, pages, (size_t)n_seqs * d.n_kv_head * n_sel * 4, &dsel));
+    TG_TRY(stage_out(ctx, out, qb, false, &dout));
+  }
   TG_TRY(run_paged(ctx, pk, layer, n_seqs, static_cast<const float*>(dq),
                    static_cast<const int*>(dp), static_cast<const int*>(dt), max_blocks,
                    static_cast<const int*>(dsel), n_sel, shared_len, static_cast<float*>(dout)));
@@ -3228,16 +3281,23 @@ int tg_paged_select(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, con
                 keep_last);
   if (n_seqs == 0) return TG_OK;
   if (!q || !past_len || !block_table || !pages) return fail(TG_ERR_INVALID_ARG, "null argument");
-  TG_TRY(check_host_pages(pk, past_len, block_table, n_seqs, max_blocks));
+  PagedArg args[4] = {{q, "q"}, {past_len, "past_len"}, {block_table, "block_table"},
+                      {pages, "pages"}};
+  bool all_device = false;
+  TG_TRY(classify_args(ctx, args, 4, &all_device));
+  if (!args[1].device)
+    TG_TRY(check_host_pages(pk, past_len, block_table, n_seqs, max_blocks, !args[2].device));
   const tg_paged_desc& d = pk->d;
   const int qrow = d.n_head * d.head_dim;
-  const void *dq = nullptr, *dp = nullptr, *dt = nullptr;
-  void* dpg = nullptr;
-  TG_TRY(stage_in(ctx, q, (size_t)n_seqs * qrow * 4, &dq));
-  TG_TRY(stage_in(ctx, past_len, (size_t)n_seqs * 4, &dp));
-  TG_TRY(stage_in(ctx, block_table, (size_t)n_seqs * max_blocks * 4, &dt));
-  TG_TRY(stage_out(ctx, pages, (size_t)n_seqs * d.n_kv_head * n_sel * 4, false, &dpg));
-  TG_TRY(commit_inputs(ctx));
+  const void *dq = q, *dp = past_len, *dt = block_table;
+  void* dpg = pages;
+  if (!all_device) {
+    TG_TRY(stage_in(ctx, q, (size_t)n_seqs * qrow * 4, &dq));
+    TG_TRY(stage_in(ctx, past_len, (size_t)n_seqs * 4, &dp));
+    TG_TRY(stage_in(ctx, block_table, (size_t)n_seqs * max_blocks * 4, &dt));
+    TG_TRY(stage_out(ctx, pages, (size_t)n_seqs * d.n_kv_head * n_sel * 4, false, &dpg));
+    TG_TRY(commit_inputs(ctx));
+  }
   // Queries per launch: at most 256 MB of scratch.
   const long long per_query = 3LL * d.n_kv_head * max_blocks;
   const int step = (int)std::max(1LL, std::min((long long)tg::kPagedMaxQueries, (1LL << 25) / per_query));
