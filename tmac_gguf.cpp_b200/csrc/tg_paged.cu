@@ -281,10 +281,34 @@ __device__ __forceinline__ int query_chunks(const PagedAttnParams& p, int past, 
   return (int)((((long long)list << p.log2p) + (1 << p.lchunk) - 1) >> p.lchunk);
 }
 
-// Chunk prefix over the queries (per stream of a query) and their last
-// positions in shared memory; every thread of the CTA takes part.
-__device__ void paged_schedule(const PagedAttnParams& p, int* prefix, int* past_s, int* warp_tot) {
-  const int NT = blockDim.x, t = threadIdx.x, lane = t & 31, w = t >> 5;
+// CTAs that share the T chunks out: enough that each has a chunk for each of
+// its warps, and in any case some for every stream.
+__device__ __forceinline__ int paged_active(int grid, int T, int warps, int n_streams) {
+  return min(min(grid, T), max((T + warps - 1) / warps, 3 * n_streams));
+}
+
+// A CTA's range is an equal share of the T chunks, its ends moved to the
+// nearer end of the stream that they would cut if that stream is short
+// (kWholeRounds steps of all warps or less).  A cut costs its two CTAs a
+// record, an arrival and a merge, about 5000 cycles, as much as the chunks
+// that a moved range has too many.  A range may be empty.
+constexpr int kWholeRounds = 4;
+
+struct PagedRange {
+  int T, G;       // chunks of all streams, CTAs that share them
+  int lo, hi;     // this CTA's chunks
+  int s;          // a query at or before the one of chunk lo
+};
+
+// The schedule of a launch, in shared memory: prefix[s], the chunks of one
+// stream of each query before s, and the queries' last positions (past_s).
+// Every thread of the CTA takes part, and the thread that has a query checks
+// whether this CTA's range begins or ends in it.  warp_tot: an int per warp
+// and 4 more.
+__device__ PagedRange paged_schedule(const PagedAttnParams& p, int* prefix, int* past_s,
+                                     int* warp_tot, int streams, int warps) {
+  const int NT = blockDim.x, t = threadIdx.x, lane = t & 31, w = t >> 5, nw = NT >> 5;
+  int* found = warp_tot + nw;   // lo, hi, the query of lo
   const int per = (p.n + NT - 1) / NT;
   const int b0 = min(t * per, p.n), b1 = min(b0 + per, p.n);
   int sum = 0;
@@ -303,50 +327,52 @@ __device__ void paged_schedule(const PagedAttnParams& p, int* prefix, int* past_
     if (lane >= o) incl += v;
   }
   if (lane == 31) warp_tot[w] = incl;
+  if (t == 0) {
+    prefix[0] = 0;
+    found[0] = found[2] = 0;
+  }
   __syncthreads();
-  int off = 0;
-  for (int i = 0; i < w; ++i) off += warp_tot[i];
+  int off = 0, all = 0;
+#pragma unroll 4
+  for (int i = 0; i < nw; ++i) {
+    const int x = warp_tot[i];
+    off += i < w ? x : 0;
+    all += x;
+  }
+  PagedRange r;
+  r.T = all * streams;
+  r.G = paged_active(gridDim.x, r.T, warps, p.n * streams);
+  const int c = blockIdx.x;
+  // floor(c T / G) without 64 bits.
+  const int q = r.G > 0 ? r.T / r.G : 0, rem = r.T - q * r.G;
+  const int lo = r.G > 0 ? c * q + c * rem / r.G : 0;
+  const int hi = r.G > 0 ? (c + 1) * q + (c + 1) * rem / r.G : 0;
+  if (t == 0) found[1] = r.T;
+  __syncthreads();
   int run = off + incl - sum;
-  if (t == 0) prefix[0] = 0;
   for (int s = b0; s < b1; ++s) {
-    run += prefix[s + 1];
+    const int C = prefix[s + 1], base = run * streams;
+    run += C;
     prefix[s + 1] = run;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int at = k ? hi : lo;
+      if (at < base || at >= base + C * streams || at == 0) continue;
+      int cut = at;
+      if (C <= kWholeRounds * warps) {
+        const int in = (at - base) % C;
+        cut = 2 * in < C ? at - in : at + (C - in);
+      }
+      found[k] = cut;
+      if (k == 0) found[2] = s;
+    }
   }
   __syncthreads();
-}
-
-// Query that owns flat chunk t when every query has `streams` streams: the
-// last s with prefix[s] * streams <= t and a non-empty share.
-__device__ __forceinline__ int query_of(const int* prefix, int n, int streams, int t) {
-  int lo = 0, hi = n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (prefix[mid] * streams <= t) lo = mid; else hi = mid - 1;
-  }
-  return lo;
-}
-
-// CTAs that share the T chunks out: enough that each has a chunk for each of
-// its warps, and in any case some for every stream.
-__device__ __forceinline__ int paged_active(int grid, int T, int warps, int n_streams) {
-  return min(min(grid, T), max((T + warps - 1) / warps, 3 * n_streams));
-}
-
-// First chunk of CTA c's range: an equal share, moved to the nearer end of
-// the stream that it would cut if that stream is short (kWholeRounds steps of
-// all warps or less).  A cut costs its two CTAs a record, an arrival and a
-// merge, about 5000 cycles, as much as the chunks that a moved range has too
-// many.  A range may be empty.
-constexpr int kWholeRounds = 4;
-
-__device__ __forceinline__ int range_lo(const int* prefix, int n, int streams, int c, int G, int T,
-                                        int warps) {
-  const int t = (int)cta_tile_lo(c, G, T);
-  if (t <= 0 || t >= T) return t;
-  const int s = query_of(prefix, n, streams, t);
-  const int C = prefix[s + 1] - prefix[s], off = (t - prefix[s] * streams) % C;
-  if (C > kWholeRounds * warps) return t;
-  return 2 * off < C ? t - off : t + (C - off);
+  r.lo = found[0];
+  r.hi = found[1];
+  r.s = found[2];
+  if (c >= r.G) r.lo = r.hi = 0;
+  return r;
 }
 
 // One arrival at a split stream's count: the records written before it (by
@@ -487,7 +513,7 @@ size_t paged_core_smem(int n, int hd) {
   const size_t floats = (size_t)kPagedHeads * hd                          // q
                         + (size_t)kCoreWarps * kPagedHeads * kPagedChunk    // probabilities
                         + (size_t)kCoreWarps * kPagedHeads * (hd + 2);      // warp results
-  return floats * 4 + (size_t)(2 * n + 1 + kCoreWarps + 4) * 4;
+  return floats * 4 + (size_t)(2 * n + 1 + kCoreWarps + 4 + 4) * 4;
 }
 
 template <typename T>
@@ -513,25 +539,21 @@ __global__ void __launch_bounds__(kCoreThreads) paged_core_kernel(const PagedAtt
   int* prefix = reinterpret_cast<int*>(res + kCoreWarps * kPagedHeads * (hd + 2));
   int* past_s = prefix + p.n + 1;
   int* warp_tot = past_s + p.n;
-  int* flag = warp_tot + kCoreWarps;
+  int* flag = warp_tot + kCoreWarps + 4;
   float* my_res = res + warp * kPagedHeads * (hd + 2);
 
   griddep_launch_dependents();
   griddep_wait();
-  paged_schedule(p, prefix, past_s, warp_tot);
-  const int streams = p.n_kv * p.hblocks;
-  const int T_all = prefix[p.n] * streams;
+  const int streams = p.n_kv * p.hblocks, cta = blockIdx.x;
+  const PagedRange range = paged_schedule(p, prefix, past_s, warp_tot, streams, kCoreWarps);
   write_empty(p, prefix);
-  const int G = paged_active(gridDim.x, T_all, kCoreWarps, p.n * streams), cta = blockIdx.x;
-  if (cta >= G) return;
-  const int t_lo = range_lo(prefix, p.n, streams, cta, G, T_all, kCoreWarps);
-  const int t_hi = range_lo(prefix, p.n, streams, cta + 1, G, T_all, kCoreWarps);
+  const int T_all = range.T, G = range.G, t_lo = range.lo, t_hi = range.hi;
   if (t_lo >= t_hi) return;
   const T* kp = static_cast<const T*>(p.kp);
   const T* vp = static_cast<const T*>(p.vp);
   const int P = 1 << p.log2p;
 
-  int s = query_of(prefix, p.n, streams, t_lo);
+  int s = range.s;
   for (int t = t_lo; t < t_hi;) {
     while (prefix[s + 1] * streams <= t) ++s;
     const int C = prefix[s + 1] - prefix[s];
@@ -733,7 +755,7 @@ struct MmaPaged {
   static constexpr int OFF_META = OFF_BAR + STAGES * 8;
   static constexpr int OFF_MRG = (OFF_META + STAGES * 4 + 15) & ~15;
   static constexpr int OFF_MISC = OFF_MRG + WARPS * MRG * 4;
-  static constexpr int OFF_SCHED = OFF_MISC + 16 * 4;
+  static constexpr int OFF_SCHED = OFF_MISC + (WARPS + 5) * 4;
   static constexpr size_t smem_bytes(int n) { return 1024 + (size_t)OFF_SCHED + (size_t)(2 * n + 1) * 4; }
 };
 
@@ -853,7 +875,7 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
   uint32_t* meta = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_META);
   float* mrg = reinterpret_cast<float*>(smem + Cfg::OFF_MRG);
   int* warp_tot = reinterpret_cast<int*>(smem + Cfg::OFF_MISC);
-  int* flag = warp_tot + 14;
+  int* flag = warp_tot + WARPS + 4;
   int* prefix = reinterpret_cast<int*>(smem + Cfg::OFF_SCHED);
   int* past_s = prefix + p.n + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -866,28 +888,35 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     tma_prefetch_desc(&tmv);
   }
   griddep_wait();
-  paged_schedule(p, prefix, past_s, warp_tot);
-  const int streams = p.n_kv * p.hblocks;
-  const int T_all = prefix[p.n] * streams;
+  const int streams = p.n_kv * p.hblocks, cta = blockIdx.x;
+  const PagedRange range = paged_schedule(p, prefix, past_s, warp_tot, streams, WARPS);
   write_empty(p, prefix);
-  const int G = paged_active(gridDim.x, T_all, WARPS, p.n * streams), cta = blockIdx.x;
-  if (cta >= G) return;
-  const int t_lo = range_lo(prefix, p.n, streams, cta, G, T_all, WARPS);
-  const int t_hi = range_lo(prefix, p.n, streams, cta + 1, G, T_all, WARPS);
+  const int T_all = range.T, G = range.G, t_lo = range.lo, t_hi = range.hi;
   if (t_lo >= t_hi) return;
   const int P = 1 << p.log2p;
   const int box = min(P, CH), lbox = min(p.log2p, Cfg::LCH);   // rows of a TMA box
   const int nbx = CH >> lbox;                                  // boxes of a chunk, 1, 2 or 4
   const uint32_t cnt_full = (uint32_t)box * (nbx == 1 ? 1u : nbx == 2 ? 0x101u : 0x1010101u);
 
-  // The stream that the look-up stands in: query ls, stream lu of it, its
-  // flat chunks [l_lo, l_hi).
-  int ls = query_of(prefix, p.n, streams, t_lo);
+  // Looking a chunk's pages up takes two steps, so that neither load is waited
+  // for: `entry` walks to the chunk's stream and reads the listed entry j (if
+  // there is a list), `page` reads the table.  Lane b has box b.
+  struct Entry {
+    int s, g, j, off;    // j -1: no such box
+  };
+  struct Box {
+    int page, rows, y0;  // rows 0: nothing to load; y0: TMA row less the page's
+  };
+  // The stream that `entry` stands in: query ls, stream lu of it, flat chunks
+  // [l_lo, l_hi).
+  int ls = range.s;
+  while (prefix[ls + 1] * streams <= t_lo) ++ls;
+  int s = ls;
   int l_c = prefix[ls + 1] - prefix[ls], lu = (t_lo - prefix[ls] * streams) / l_c;
   int l_lo = prefix[ls] * streams + lu * l_c, l_hi = l_lo + l_c;
-  int s = ls;
-  // Lane b: TMA row y and attended rows cnt of box b of chunk t.
-  auto look_up = [&](int t, int& y, int& cnt) {
+  auto entry = [&](int t) -> Entry {
+    Entry e{0, 0, -1, 0};
+    if (t >= t_hi) return e;
     while (t >= l_hi) {
       if (++lu == streams) {
         lu = 0;
@@ -897,33 +926,41 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
       l_lo = l_hi;
       l_hi += l_c;
     }
-    y = cnt = 0;
-    if (lane >= nbx) return;
-    const int g = lu / p.hblocks, past = past_s[ls];
-    const int nb = (past >> p.log2p) + 1;
-    const int skip = query_skip(p, past);
+    if (lane >= nbx) return e;
+    e.s = ls;
+    e.g = p.hblocks == 1 ? lu : lu / p.hblocks;
+    const int past = past_s[ls], nb = (past >> p.log2p) + 1, skip = query_skip(p, past);
     const int list = p.sel ? min(p.n_sel, nb) : nb - skip;
-    const long long r = ((long long)(t - l_lo) * nbx + lane) << lbox;  // row of the stream
-    const int i = (int)(r >> p.log2p), off = (int)(r & (P - 1));
-    if (i >= list) return;
-    const int j = p.sel ? p.sel[((size_t)ls * p.n_kv + g) * p.n_sel + i] : skip + i;
-    if (j < 0 || j >= nb) return;
-    const int page = p.table[(size_t)ls * p.max_blocks + j];
-    if (page < 0 || page >= p.n_pages) {
-      record_error(p.err, kDevErrBadPage);
-      return;
-    }
-    cnt = max(0, min(box, past + 1 - ((j << p.log2p) + off)));
-    y = (int)(((p.page0 + page) * p.n_kv + g) << p.log2p) + off;
+    const int row = ((t - l_lo) * nbx + lane) << lbox;   // row of the stream, below 2^31
+    const int i = row >> p.log2p;
+    e.off = row & (P - 1);
+    if (i < list) e.j = p.sel ? p.sel[((size_t)ls * p.n_kv + e.g) * p.n_sel + i] : skip + i;
+    return e;
   };
-  // Fills stage st with the chunk whose boxes lanes 0..nbx-1 looked up.
-  auto load = [&](int st, int y, int cnt) {
+  auto page = [&](const Entry& e) -> Box {
+    Box b{0, 0, 0};
+    if (e.j < 0) return b;
+    const int rows = past_s[e.s] + 1 - ((e.j << p.log2p) + e.off);
+    if (e.j > past_s[e.s] >> p.log2p || rows <= 0) return b;
+    b.rows = min(box, rows);
+    b.page = p.table[(size_t)e.s * p.max_blocks + e.j];
+    b.y0 = (int)((p.page0 * p.n_kv + e.g) << p.log2p) + e.off;
+    return b;
+  };
+  // Fills stage st with the chunk whose boxes lanes 0..nbx-1 have.
+  auto load = [&](int st, const Box& x) {
+    int rows = x.rows;
+    if (rows > 0 && (x.page < 0 || x.page >= p.n_pages)) {
+      record_error(p.err, kDevErrBadPage);
+      rows = 0;
+    }
+    const int y = x.y0 + ((x.page * p.n_kv) << p.log2p);
     uint32_t m = 0;
     int loads = 0;
     for (int b = 0; b < nbx; ++b) {
-      const int x = __shfl_sync(0xffffffffu, cnt, b);
-      m |= (uint32_t)x << (8 * b);
-      loads += x > 0;
+      const int v = __shfl_sync(0xffffffffu, rows, b);
+      m |= (uint32_t)v << (8 * b);
+      loads += v > 0;
     }
     if (lane == 0) {
       meta[st] = m;
@@ -937,10 +974,10 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
       if (lane == 0 && ((m >> (8 * b)) & 255u)) {
         uint8_t* to = smem + st * Cfg::STAGE + b * box * 128;
 #pragma unroll
-        for (int x = 0; x < NX; ++x) {
-          tma_load_2d(to + x * (CH * 128), &tmk, &full[st], x * (128 / (int)sizeof(T)), yb);
-          tma_load_2d(to + Cfg::HALF + x * (CH * 128), &tmv, &full[st],
-                      x * (128 / (int)sizeof(T)), yb);
+        for (int c = 0; c < NX; ++c) {
+          tma_load_2d(to + c * (CH * 128), &tmk, &full[st], c * (128 / (int)sizeof(T)), yb);
+          tma_load_2d(to + Cfg::HALF + c * (CH * 128), &tmv, &full[st],
+                      c * (128 / (int)sizeof(T)), yb);
         }
       }
     }
@@ -952,14 +989,23 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
   const float sl2 = p.scale_log2;
   int ti = t_lo + warp;   // this warp's next chunk to compute
   int tl = ti;            // ... to load
-  int tn_y = 0, tn_cnt = 0;
-  if (tl < t_hi) look_up(tl, tn_y, tn_cnt);
-#pragma unroll 1
-  for (int i = 0; i < DEPTH; ++i) {
-    if (tl >= t_hi) break;
-    load(warp * DEPTH + i, tn_y, tn_cnt);
-    tl += WARPS;
-    if (tl < t_hi) look_up(tl, tn_y, tn_cnt);
+  Box box_n;              // pages of chunk tl, and the entries of the one after
+  Entry entry_n;
+  {
+    Entry e[DEPTH + 2];
+    Box b[DEPTH + 1];
+#pragma unroll
+    for (int i = 0; i < DEPTH + 2; ++i) e[i] = entry(ti + i * WARPS);
+#pragma unroll
+    for (int i = 0; i <= DEPTH; ++i) b[i] = page(e[i]);
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) {
+      if (tl >= t_hi) break;
+      load(warp * DEPTH + i, b[i]);
+      tl += WARPS;
+    }
+    box_n = b[DEPTH];
+    entry_n = e[DEPTH + 1];
   }
   bool failed = false;
   int slot = 0;
@@ -1085,9 +1131,11 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
           lsum += sc[nt][0] + sc[nt][1];
         }
         l_run = l_run * alpha + lsum;
+        if (__any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll
-        for (int c = 0; c < HD / 8; ++c) {
-          o[c][0] *= alpha; o[c][1] *= alpha; o[c][2] *= alpha; o[c][3] *= alpha;
+          for (int c = 0; c < HD / 8; ++c) {
+            o[c][0] *= alpha; o[c][1] *= alpha; o[c][2] *= alpha; o[c][3] *= alpha;
+          }
         }
         // O += P . V.
         if constexpr (kHalf) {
@@ -1140,9 +1188,10 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
       }
       __syncwarp();
       if (tl < t_hi && !failed) {
-        load(st, tn_y, tn_cnt);
+        load(st, box_n);
         tl += WARPS;
-        if (tl < t_hi) look_up(tl, tn_y, tn_cnt);
+        box_n = page(entry_n);
+        entry_n = entry(tl + WARPS);
       }
       if (++slot == DEPTH) {
         slot = 0;
