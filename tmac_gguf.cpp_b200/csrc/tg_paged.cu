@@ -356,10 +356,13 @@ __device__ PagedRange paged_schedule(const PagedAttnParams& p, int* prefix, int*
   const bool uniform = __syncthreads_and(same) != 0;
   r.G = paged_active(gridDim.x, r.T, warps, p.n * streams, uniform);
   const int c = blockIdx.x;
-  // floor(c T / G) without 64 bits.
-  const int q = r.G > 0 ? r.T / r.G : 0, rem = r.T - q * r.G;
-  const int lo = r.G > 0 ? c * q + c * rem / r.G : 0;
-  const int hi = r.G > 0 ? (c + 1) * q + (c + 1) * rem / r.G : 0;
+  // floor(c T / G) and floor((c + 1) T / G) without 64 bits.
+  int lo = 0, hi = 0;
+  if (c < r.G) {
+    const int q = r.T / r.G, rem = r.T - q * r.G, a = c * rem / r.G;
+    lo = c * q + a;
+    hi = lo + q + (c * rem - a * r.G + rem >= r.G);
+  }
   int run = off + incl - sum;
   for (int s = b0; s < b1; ++s) {
     const int C = prefix[s + 1], base = run * streams;
@@ -738,6 +741,29 @@ __device__ __forceinline__ void mma_tf32_1688(float* d, const uint32_t* a, uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// tma_load_2d and mbar_arrive_expect_tx by one elected lane of a converged
+// warp: with warp-uniform operands the copy is issued as it is, where a
+// branch of one lane moves each operand out of that lane's registers (a chunk
+// of two boxes took 1000 cycles to issue).
+__device__ __forceinline__ void tma_load_2d_elect(uint32_t dst, const void* tmap, uint32_t bar,
+                                                  int x, int y) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_expect_tx_elect(uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+      "r"(bytes)
+      : "memory");
+}
+
 // x = hi + lo with hi the 11 leading significant bits (a tf32 value) and lo
 // exact; as an operand lo keeps its own 11 leading bits: 2^-21 of x is lost.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
@@ -889,7 +915,9 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
   int* flag = warp_tot + WARPS + 4;
   int* prefix = reinterpret_cast<int*>(smem + Cfg::OFF_SCHED);
   int* past_s = prefix + p.n + 1;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31;
+  const int warp = (int)__reduce_max_sync(0xffffffffu, threadIdx.x >> 5);   // warp-uniform
+  const uint32_t smem_u = smem_u32(smem), full_u = smem_u32(full);
 
   griddep_launch_dependents();
   if (threadIdx.x == 0) {
@@ -965,30 +993,24 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
       record_error(p.err, kDevErrBadPage);
       rows = 0;
     }
+    // Reductions leave warp-uniform values: the rows of all boxes, and below
+    // each box's TMA row.
     const int y = x.y0 + ((x.page * p.n_kv) << p.log2p);
-    uint32_t m = 0;
+    const uint32_t m = __reduce_or_sync(0xffffffffu, lane < nbx ? (uint32_t)rows << (8 * lane) : 0u);
+    meta[st] = m;
+    const uint32_t bar = full_u + 8 * st, to = smem_u + st * Cfg::STAGE;
     int loads = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) loads += ((m >> (8 * b)) & 255u) != 0;
+    mbar_arrive_expect_tx_elect(bar, (uint32_t)(loads * box * 2 * NX * 128));
     for (int b = 0; b < nbx; ++b) {
-      const int v = __shfl_sync(0xffffffffu, rows, b);
-      m |= (uint32_t)v << (8 * b);
-      loads += v > 0;
-    }
-    if (lane == 0) {
-      meta[st] = m;
-      if (loads)
-        mbar_arrive_expect_tx(&full[st], (uint32_t)(loads * box * 2 * NX * 128));
-      else
-        mbar_arrive(&full[st]);
-    }
-    for (int b = 0; b < nbx; ++b) {
-      const int yb = __shfl_sync(0xffffffffu, y, b);
-      if (lane == 0 && ((m >> (8 * b)) & 255u)) {
-        uint8_t* to = smem + st * Cfg::STAGE + b * box * 128;
+      const int yb = (int)__reduce_max_sync(0xffffffffu, lane == b ? (uint32_t)y : 0u);
+      if ((m >> (8 * b)) & 255u) {
 #pragma unroll
         for (int c = 0; c < NX; ++c) {
-          tma_load_2d(to + c * (CH * 128), &tmk, &full[st], c * (128 / (int)sizeof(T)), yb);
-          tma_load_2d(to + Cfg::HALF + c * (CH * 128), &tmv, &full[st],
-                      c * (128 / (int)sizeof(T)), yb);
+          const uint32_t at = to + b * box * 128 + c * (CH * 128);
+          tma_load_2d_elect(at, &tmk, bar, c * (128 / (int)sizeof(T)), yb);
+          tma_load_2d_elect(at + Cfg::HALF, &tmv, bar, c * (128 / (int)sizeof(T)), yb);
         }
       }
     }
