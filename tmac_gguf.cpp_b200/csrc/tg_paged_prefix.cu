@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
   uint64_t* q_full = kv_empty + PX_STAGES;
   uint64_t* s_full = q_full + 1;   // [slot * 2 + buf]
   uint64_t* p_full = s_full + 4;   // [slot * 2 + buf]
-  uint64_t* pv_done = p_full + 4;  // [slot]
+  uint64_t* pv_done = p_full + 4;  // [slot]: the last two steps' O
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + PX_OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + PX_OFF_MISC + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
       mbar_wait(&kv_full[i % PX_STAGES], (uint32_t)((i / PX_STAGES) & 1), p.err, kDevErrWaitFull);
   } else if (warp == 1) {
     // ---------------------------------------------------------- products
-    // The whole warp walks the loop, one lane issues (see umma_f16_ts_elect).
+    // The whole warp walks the loop, one lane issues (see umma_f16_ts_x8).
     {
       constexpr uint32_t IDESC_QK = idesc_bf16(PX_ROWS, PX_KEYS, false);
       constexpr uint32_t IDESC_PV = idesc_bf16(PX_ROWS, 64, true);
@@ -218,9 +218,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         tc_fence_after();
         const uint64_t b = dk0 + (uint64_t)(st * (2 * PX_TILE >> 4));
         const uint32_t d = utmem + px_s(x, j & 1), a = utmem + px_q(x);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)   // 4 steps of 16 dimensions, hi then lo
-          umma_f16_ts_elect(d, a + 8 * kk, b + 2 * (kk & 3), IDESC_QK, kk > 0 ? 1u : 0u);
+        // 4 steps of 16 dimensions (32 bytes), the high parts and the low ones.
+        umma_f16_ts_x8<2>(d, a, b, IDESC_QK, 0u);
         umma_commit_elect(&s_full[2 * x + (j & 1)]);
         qk[x].step(by);
         last = x;
@@ -233,10 +232,11 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         tc_fence_after();
         const uint64_t b = dv0 + (uint64_t)(st * (2 * PX_TILE >> 4));
         const uint32_t d = utmem + px_o(x), a = utmem + px_s(x, j & 1);
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)   // 4 steps of 16 keys, hi then lo
-          umma_f16_ts_elect(d, a + 8 * kk, b + 128 * (kk & 3), IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
-        umma_commit_elect(&pv_done[x]);
+        // 4 steps of 16 keys (2048 bytes), the high parts and the low ones.
+        umma_f16_ts_x8<128>(d, a, b, IDESC_PV, j > 0 ? 1u : 0u);
+        // Products of one thread complete in their order: s_full of step j + 2
+        // covers this one.  The last two steps have no such product.
+        if (j + 2 >= n_x[x]) umma_commit_elect(&pv_done[x]);
         if (p.single || x == 1 || n1 == 0) umma_commit_elect(&kv_empty[st]);
         pv[x].step(by);
         last = x;
@@ -314,9 +314,12 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         m = mx;
       }
       if (__any_sync(0xffffffffu, alpha != 1.f)) {
-        // O of the steps before this one is complete, and the next product
-        // on it waits for this step's P.
-        if (!px_wait_warp(&pv_done[x], (uint32_t)((j - 1) & 1), p.err, abort_flag)) {
+        // O of the steps before this one is complete once S of the next step
+        // is (or, in the last step, the product before it), and the next
+        // product on O waits for this step's P.
+        uint64_t* bar = j + 1 < steps ? &s_full[2 * x + (b ^ 1)] : &pv_done[x];
+        const uint32_t phase = j + 1 < steps ? (uint32_t)(((j + 1) >> 1) & 1) : 0u;
+        if (!px_wait_warp(bar, phase, p.err, abort_flag)) {
           ok = false;
           break;
         }
@@ -347,9 +350,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
     }
     uint32_t ov[64];
     // The last two products in turn: a parity tells a phase only from its
-    // neighbours (s_full of the last step covers those before).
-    for (int j = max(0, steps - 2); j < steps && ok; ++j)
-      ok = px_wait_warp(&pv_done[x], (uint32_t)(j & 1), p.err, abort_flag);
+    // neighbours.
+    for (int j = 0; j < min(steps, 2) && ok; ++j)
+      ok = px_wait_warp(&pv_done[x], (uint32_t)j, p.err, abort_flag);
     if (ok && steps > 0) {
       tc_fence_after();
       TG_TMEM_LD64(base + px_o(x), ov);

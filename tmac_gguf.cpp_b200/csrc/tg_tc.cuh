@@ -135,19 +135,35 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
-// The same, and the commit, issued by one elected lane of a converged warp:
-// the operands stay warp-uniform, so an instruction costs its own issue and
-// not a move of each operand out of a lane's registers (in a branch of one
-// lane 8 of these and a commit took 600 cycles).
-__device__ __forceinline__ void umma_f16_ts_elect(uint32_t d_tmem, uint32_t a_tmem,
-                                                  uint64_t b_desc, uint32_t idesc,
-                                                  uint32_t accumulate) {
+// Eight products D (+)= A_k B_k, A_k at a_tmem + 8 k, B_k at b_desc + STEP
+// (k % 4), issued by one elected lane of a converged warp: the operands stay
+// warp-uniform, so a product costs its own issue and not a move of each
+// operand out of a lane's registers, and one election serves all eight (in a
+// branch of one lane eight products and a commit took 600 cycles; elected one
+// by one, between two softmax warps on the same scheduler, 270 to 480; their
+// execution takes 260).
+template <int STEP>
+__device__ __forceinline__ void umma_f16_ts_x8(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                               uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
+      "{\n\t.reg .pred p, q, e;\n\t.reg .b64 b1, b2, b3;\n\t"
+      ".reg .b32 a1, a2, a3, a4, a5, a6, a7;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.eq.b32 q, %5, %5;\n\t"
+      "add.u64 b1, %2, %5;\n\tadd.u64 b2, %2, %6;\n\tadd.u64 b3, %2, %7;\n\t"
+      "add.u32 a1, %1, 8;\n\tadd.u32 a2, %1, 16;\n\tadd.u32 a3, %1, 24;\n\tadd.u32 a4, %1, 32;\n\t"
+      "add.u32 a5, %1, 40;\n\tadd.u32 a6, %1, 48;\n\tadd.u32 a7, %1, 56;\n\t"
       "elect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, q;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, q;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, q;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a4], %2, %3, q;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a5], b1, %3, q;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a6], b2, %3, q;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a7], b3, %3, q;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "n"(STEP), "n"(2 * STEP),
+      "n"(3 * STEP)
       : "memory");
 }
 __device__ __forceinline__ void umma_commit_elect(uint64_t* bar) {
