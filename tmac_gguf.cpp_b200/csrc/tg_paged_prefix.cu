@@ -30,11 +30,12 @@ namespace tg {
 constexpr int PX_ROWS = 128;        // query rows of a slot (TMEM lanes)
 constexpr int PX_KEYS = 64;         // keys of a step
 constexpr int PX_STAGES = 12;       // K/V ring
-constexpr int PX_THREADS = 384;     // TMA warp, MMA warp, 2 idle, 2 x 4 softmax warps
+constexpr int PX_THREADS = 384;     // TMA warp, 2 MMA warps, an idle one, 2 x 4 softmax warps
 constexpr int PX_TILE = PX_KEYS * 128;           // bytes of a K (or V) tile
 constexpr int PX_OFF_BAR = PX_STAGES * 2 * PX_TILE;
-// kv_full[S], kv_empty[S], q_full, s_full[slot][buf], p_full[slot][buf], pv_done[slot]
-constexpr int PX_NBAR = 2 * PX_STAGES + 1 + 4 + 4 + 2;
+// kv_full[S], kv_empty[S], q_full[slot], s_full[slot][buf], p_full[slot][buf],
+// pv_done[slot], drained[slot]
+constexpr int PX_NBAR = 2 * PX_STAGES + 2 + 4 + 4 + 2 + 2;
 constexpr int PX_OFF_MISC = PX_OFF_BAR + PX_NBAR * 8;
 constexpr size_t PX_SMEM = 1024 + PX_OFF_MISC + 16;
 constexpr uint32_t PX_COLS = 512;
@@ -75,10 +76,12 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint3
 //   warp 0      TMA: K and V tiles of 64 keys (boxes of min(page, 32) rows,
 //               128-byte swizzle) into a ring; the pages of the next tile are
 //               looked up while this one is issued.
-//   warp 1      owns TMEM; one thread issues the products.  S of step j + 2
-//               goes into the buffer that P of step j has just been read
-//               from (products of one thread run in their order), so S is
-//               ready when a softmax warp comes for it.
+//   warps 1, 2  issue the products of a slot each (one warp for both spent
+//               900 of 2200 cycles of a step in waits and bookkeeping while
+//               the tensor core stood still); warp 1 owns TMEM.  S of step
+//               j + 2 goes into the buffer that P of step j has just been
+//               read from (products of one thread run in their order), so S
+//               is ready when a softmax warp comes for it.
 //   warps 4-11  softmax, a thread per query row: S to registers, running
 //               maximum (the exponent's base moves only when the maximum
 //               grew by more than 2^8; then O is rescaled in TMEM), P = 2^(S
@@ -95,20 +98,37 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
   uint64_t* kv_full = bars;
   uint64_t* kv_empty = kv_full + PX_STAGES;
   uint64_t* q_full = kv_empty + PX_STAGES;
-  uint64_t* s_full = q_full + 1;   // [slot * 2 + buf]
+  uint64_t* s_full = q_full + 2;   // [slot * 2 + buf]
   uint64_t* p_full = s_full + 4;   // [slot * 2 + buf]
   uint64_t* pv_done = p_full + 4;  // [slot]: the last two steps' O
+  uint64_t* drained = pv_done + 2; // [slot]: everything issued has completed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + PX_OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + PX_OFF_MISC + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // Item: KV head, pair of row tiles, range of key steps.
+  const int split = blockIdx.x % p.splits, gp = blockIdx.x / p.splits;
+  const int g = gp / p.pairs, pair = gp - g * p.pairs;
+  const int k0 = (int)((long long)split * p.steps / p.splits);
+  const int k1 = (int)((long long)(split + 1) * p.steps / p.splits);
+  const int rows = p.n * p.group;
+  const bool both = p.single || (2 * pair + 1) * PX_ROWS < rows;   // slot 1 has rows
+  // Steps of the slots, and the tile (from k0) of ring entry i.
+  const int n0 = p.single ? (k1 - k0 + 1) / 2 : k1 - k0;
+  const int n1 = p.single ? (k1 - k0) / 2 : (both ? k1 - k0 : 0);
+  const int entries = k1 - k0;
+  auto tile_of = [&](int i) { return p.single ? ((i & 1) ? n0 + (i >> 1) : i >> 1) : i; };
 
   griddep_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < PX_STAGES; ++i) {
       mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&kv_empty[i], !p.single && both ? 2 : 1);   // the slots that read an entry
     }
-    mbar_init(q_full, 8);
+    mbar_init(&q_full[0], 4);
+    mbar_init(&q_full[1], 4);
+    mbar_init(&drained[0], 1);
+    mbar_init(&drained[1], 1);
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
@@ -132,19 +152,6 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   griddep_wait();
-
-  // Item: KV head, pair of row tiles, range of key steps.
-  const int split = blockIdx.x % p.splits, gp = blockIdx.x / p.splits;
-  const int g = gp / p.pairs, pair = gp - g * p.pairs;
-  const int k0 = (int)((long long)split * p.steps / p.splits);
-  const int k1 = (int)((long long)(split + 1) * p.steps / p.splits);
-  const int rows = p.n * p.group;
-  const bool both = p.single || (2 * pair + 1) * PX_ROWS < rows;   // slot 1 has rows
-  // Steps of the slots, and the tile (from k0) of ring entry i.
-  const int n0 = p.single ? (k1 - k0 + 1) / 2 : k1 - k0;
-  const int n1 = p.single ? (k1 - k0) / 2 : (both ? k1 - k0 : 0);
-  const int entries = k1 - k0;
-  auto tile_of = [&](int i) { return p.single ? ((i & 1) ? n0 + (i >> 1) : i >> 1) : i; };
 
   if (warp == 0) {
     // ---------------------------------------------------------- TMA
@@ -179,89 +186,69 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
     }
     for (int i = max(0, issued - PX_STAGES); i < issued; ++i)
       mbar_wait(&kv_full[i % PX_STAGES], (uint32_t)((i / PX_STAGES) & 1), p.err, kDevErrWaitFull);
-  } else if (warp == 1) {
+  } else if (warp <= 2) {
     // ---------------------------------------------------------- products
     // The whole warp walks the loop, one lane issues (see umma_f16_ts_x8).
-    {
-      constexpr uint32_t IDESC_QK = idesc_bf16(PX_ROWS, PX_KEYS, false);
-      constexpr uint32_t IDESC_PV = idesc_bf16(PX_ROWS, 64, true);
-      const uint64_t dk0 = smem_desc_sw128(smem_u32(smem), 16, 1024);
-      const uint64_t dv0 = smem_desc_sw128(smem_u32(smem) + PX_TILE, PX_TILE, 1024);
-      const int n_x[2] = {n0, n1};
-      const uint32_t utmem = __shfl_sync(0xffffffffu, tmem, 0);
-      bool ok = px_wait_warp(q_full, 0, p.err, abort_flag);
-      int last = -1;   // slot of the last product issued
-      // A ring position: stage and phase, stepped by 1 or 2.
-      struct Ring {
-        int st = 0;
-        uint32_t ph = 0;
-        __device__ __forceinline__ void step(int by) {
-          st += by;
-          if (st >= PX_STAGES) {
-            st -= PX_STAGES;
-            ph ^= 1u;
-          }
+    constexpr uint32_t IDESC_QK = idesc_bf16(PX_ROWS, PX_KEYS, false);
+    constexpr uint32_t IDESC_PV = idesc_bf16(PX_ROWS, 64, true);
+    const uint64_t dk0 = smem_desc_sw128(smem_u32(smem), 16, 1024);
+    const uint64_t dv0 = smem_desc_sw128(smem_u32(smem) + PX_TILE, PX_TILE, 1024);
+    const int x = (int)__reduce_max_sync(0xffffffffu, threadIdx.x >> 5) - 1;   // warp-uniform
+    const uint32_t base = __reduce_max_sync(0xffffffffu, tmem) + 256u * x;
+    const int n = x ? n1 : n0;
+    // This slot's ring entries: x, x + 2, ... (single) or 0, 1, ...  qk is the
+    // one of the next S, pv the one of the next O.
+    const int by = p.single ? 2 : 1;
+    struct Ring {
+      int st;
+      uint32_t ph;
+      __device__ __forceinline__ void step(int by) {
+        st += by;
+        if (st >= PX_STAGES) {
+          st -= PX_STAGES;
+          ph ^= 1u;
         }
-      };
-      // Slot x's entries are x, x + 2, ... (single) or 0, 1, ... (both slots).
-      const int by = p.single ? 2 : 1;
-      Ring qk[2], pv[2];
-      if (p.single) {
-        qk[1].step(1);
-        pv[1].step(1);
       }
-      auto issue_qk = [&](int x, int j) -> bool {
-        const int st = qk[x].st;
-        // Both slots over the same entry: slot 0 has waited for it.
-        if ((x == 0 || p.single) && !px_wait_warp(&kv_full[st], qk[x].ph, p.err, abort_flag))
-          return false;
-        tc_fence_after();
-        const uint64_t b = dk0 + (uint64_t)(st * (2 * PX_TILE >> 4));
-        const uint32_t d = utmem + px_s(x, j & 1), a = utmem + px_q(x);
-        // 4 steps of 16 dimensions (32 bytes), the high parts and the low ones.
-        umma_f16_ts_x8<2>(d, a, b, IDESC_QK, 0u);
-        umma_commit_elect(&s_full[2 * x + (j & 1)]);
-        qk[x].step(by);
-        last = x;
-        return true;
-      };
-      auto issue_pv = [&](int x, int j) -> bool {
-        const int st = pv[x].st;
-        if (!px_wait_warp(&p_full[2 * x + (j & 1)], (uint32_t)((j >> 1) & 1), p.err, abort_flag))
-          return false;
-        tc_fence_after();
-        const uint64_t b = dv0 + (uint64_t)(st * (2 * PX_TILE >> 4));
-        const uint32_t d = utmem + px_o(x), a = utmem + px_s(x, j & 1);
-        // 4 steps of 16 keys (2048 bytes), the high parts and the low ones.
-        umma_f16_ts_x8<128>(d, a, b, IDESC_PV, j > 0 ? 1u : 0u);
-        // Products of one thread complete in their order: s_full of step j + 2
-        // covers this one.  The last two steps have no such product.
-        if (j + 2 >= n_x[x]) umma_commit_elect(&pv_done[x]);
-        if (p.single || x == 1 || n1 == 0) umma_commit_elect(&kv_empty[st]);
-        pv[x].step(by);
-        last = x;
-        return true;
-      };
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (ok && j < n_x[x]) ok = issue_qk(x, j);
-      for (int j = 0; j < n0 && ok; ++j)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (ok && j < n_x[x]) {
-            ok = issue_pv(x, j);
-            if (ok && j + 2 < n_x[x]) ok = issue_qk(x, j + 2);
-          }
-      // Everything issued has completed before TMEM is freed (q_full is
-      // done with: its second phase counts this commit and 7 arrivals).
-      if (last >= 0) {
-        if (lane < 7) mbar_arrive(q_full);
-        umma_commit_elect(q_full);
-        mbar_wait(q_full, 1, p.err, kDevErrWaitFull);
+    };
+    Ring qk{p.single ? x : 0, 0u}, pv{p.single ? x : 0, 0u};
+    auto issue_qk = [&](int j) -> bool {
+      if (!px_wait_warp(&kv_full[qk.st], qk.ph, p.err, abort_flag)) return false;
+      tc_fence_after();
+      // 4 steps of 16 dimensions (32 bytes), the high parts and the low ones.
+      umma_f16_ts_x8<2>(base + px_s(0, j & 1), base + px_q(0),
+                        dk0 + (uint64_t)(qk.st * (2 * PX_TILE >> 4)), IDESC_QK, 0u);
+      umma_commit_elect(&s_full[2 * x + (j & 1)]);
+      qk.step(by);
+      return true;
+    };
+    bool ok = n > 0 && px_wait_warp(&q_full[x], 0, p.err, abort_flag);
+    const bool any = ok;
+    for (int j = 0; j < 2 && ok; ++j)
+      if (j < n) ok = issue_qk(j);
+    for (int j = 0; j < n && ok; ++j) {
+      if (!px_wait_warp(&p_full[2 * x + (j & 1)], (uint32_t)((j >> 1) & 1), p.err, abort_flag)) {
+        ok = false;
+        break;
       }
+      tc_fence_after();
+      // 4 steps of 16 keys (2048 bytes), the high parts and the low ones.
+      umma_f16_ts_x8<128>(base + px_o(0), base + px_s(0, j & 1),
+                          dv0 + (uint64_t)(pv.st * (2 * PX_TILE >> 4)), IDESC_PV, j > 0 ? 1u : 0u);
+      umma_commit_elect(&kv_empty[pv.st]);
+      pv.step(by);
+      // Products of one thread complete in their order: s_full of step j + 2
+      // covers this one.  The last two steps have no such product.
+      if (j + 2 >= n)
+        umma_commit_elect(&pv_done[x]);
+      else
+        ok = issue_qk(j + 2);
     }
+    // Everything issued has completed before TMEM is freed.
+    if (any) {
+      umma_commit_elect(&drained[x]);
+      mbar_wait(&drained[x], 0, p.err, kDevErrWaitFull);
+    }
+    __syncwarp();
   } else if (warp >= 4) {
     // ---------------------------------------------------------- softmax
     const int x = (warp - 4) >> 2, quarter = warp & 3;
@@ -285,7 +272,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
       TG_TMEM_ST64(base + px_q(x), w);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
+      if (lane == 0) mbar_arrive(&q_full[x]);
     }
     constexpr float kLazy = 8.f;
     float m = kNegBig, l = 0.f;
