@@ -62,12 +62,40 @@ __device__ __forceinline__ bool px_wait_warp(uint64_t* bar, uint32_t parity, int
   return __all_sync(0xffffffffu, got) != 0;
 }
 
+// Pairs of floats in 64-bit registers, added by one instruction, and the
+// maximum of three: the softmax is bound by the issue of its instructions
+// beside those of the ex2 unit.
+__device__ __forceinline__ uint64_t f32x2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // Two floats as the upper halves (truncated bf16) of one register, lo first,
 // and what is left of them as a second one (rounded): off by at most 2^-16.
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
   const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
   hi = __byte_perm(ua, ub, 0x7632);
-  lo = pack_bf16x2(a - __uint_as_float(ua & 0xffff0000u), b - __uint_as_float(ub & 0xffff0000u));
+  // a - its upper half, the latter with its sign turned.
+  const uint64_t rest =
+      add_pair(f32x2(a, b), f32x2(__uint_as_float((ua & 0xffff0000u) ^ 0x80000000u),
+                                __uint_as_float((ub & 0xffff0000u) ^ 0x80000000u)));
+  float ra, rb;
+  unpair(rest, ra, rb);
+  lo = pack_bf16x2(ra, rb);
 }
 
 // One CTA: 256 query rows of a KV head (two slots of 128) x a range of the
@@ -286,13 +314,13 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
       tc_fence_after();
       uint32_t sv[64];
       TG_TMEM_LD64(base + px_s(x, b), sv);
-      float mx8[8];
+      float mx4[4];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) mx8[c] = __uint_as_float(sv[c]);
+      for (int c = 0; c < 4; ++c) mx4[c] = fmaxf(__uint_as_float(sv[c]), __uint_as_float(sv[4 + c]));
 #pragma unroll
-      for (int c = 8; c < 64; ++c) mx8[c & 7] = fmaxf(mx8[c & 7], __uint_as_float(sv[c]));
-      const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
-                             fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+      for (int c = 8; c < 64; c += 2)
+        mx4[(c >> 1) & 3] = max3(mx4[(c >> 1) & 3], __uint_as_float(sv[c]), __uint_as_float(sv[c + 1]));
+      const float mx = max3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3]));
       float alpha = 1.f;
       if (j == 0) {
         m = fmaxf(mx, kNegBig);
@@ -320,26 +348,36 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
           TG_TMEM_ST32(base + px_o(x) + c0, ov);
         }
       }
-      float ls[4] = {0.f, 0.f, 0.f, 0.f};
+      uint64_t ls[4] = {0, 0, 0, 0};   // pairs of zeros
+      const uint64_t neg = f32x2(-m, -m);
       uint32_t w[64];
 #pragma unroll
       for (int c = 0; c < 32; ++c) {
-        const float p0 = ex2(__uint_as_float(sv[2 * c]) - m);
-        const float p1 = ex2(__uint_as_float(sv[2 * c + 1]) - m);
-        ls[c & 3] += p0 + p1;
+        float p0, p1;
+        unpair(add_pair(f32x2(__uint_as_float(sv[2 * c]), __uint_as_float(sv[2 * c + 1])), neg), p0, p1);
+        p0 = ex2(p0);
+        p1 = ex2(p1);
+        ls[c & 3] = add_pair(ls[c & 3], f32x2(p0, p1));
         split_pair(p0, p1, w[c], w[32 + c]);
       }
       TG_TMEM_ST64(base + px_s(x, b), w);
-      l = l * alpha + ((ls[0] + ls[1]) + (ls[2] + ls[3]));
+      float l0, l1;
+      unpair(add_pair(add_pair(ls[0], ls[1]), add_pair(ls[2], ls[3])), l0, l1);
+      l = l * alpha + (l0 + l1);
+      // The last step first sees the product before it complete: once it has
+      // handed its P on, that phase may be two behind, which a parity cannot
+      // tell from the one to come.
+      if (j > 0 && j + 1 == steps && !px_wait_warp(&pv_done[x], 0, p.err, abort_flag)) {
+        ok = false;
+        break;
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[2 * x + b]);
     }
     uint32_t ov[64];
-    // The last two products in turn: a parity tells a phase only from its
-    // neighbours.
-    for (int j = 0; j < min(steps, 2) && ok; ++j)
-      ok = px_wait_warp(&pv_done[x], (uint32_t)j, p.err, abort_flag);
+    if (ok && steps > 0)
+      ok = px_wait_warp(&pv_done[x], steps > 1 ? 1u : 0u, p.err, abort_flag);
     if (ok && steps > 0) {
       tc_fence_after();
       TG_TMEM_LD64(base + px_o(x), ov);
