@@ -29,10 +29,11 @@ namespace tg {
 
 constexpr int PX_ROWS = 128;        // query rows of a slot (TMEM lanes)
 constexpr int PX_KEYS = 64;         // keys of a step
-constexpr int PX_STAGES = 12;       // K/V ring
+constexpr int PX_STAGES = 8;        // K/V ring
 constexpr int PX_THREADS = 384;     // TMA warp, 2 MMA warps, an idle one, 2 x 4 softmax warps
 constexpr int PX_TILE = PX_KEYS * 128;           // bytes of a K (or V) tile
-constexpr int PX_OFF_BAR = PX_STAGES * 2 * PX_TILE;
+constexpr int PX_OFF_Q = PX_STAGES * 2 * PX_TILE;   // 8 KB per softmax warp: q on its way to TMEM
+constexpr int PX_OFF_BAR = PX_OFF_Q + 8 * 32 * 64 * 4;
 // kv_full[S], kv_empty[S], q_full[slot], s_full[slot][buf], p_full[slot][buf],
 // pv_done[slot], drained[slot]
 constexpr int PX_NBAR = 2 * PX_STAGES + 2 + 4 + 4 + 2 + 2;
@@ -283,14 +284,32 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
     const int row = (p.single ? 0 : (2 * pair + x) * PX_ROWS) + quarter * 32 + lane;
     const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16);
     const int steps = x ? n1 : n0;
-    const int s = row / p.group, h = g * p.group + row - s * p.group;
     {
-      // This row of Q, scaled to log2 units, as hi and lo.
+      // This row of Q, scaled to log2 units, as hi and lo.  The warp reads its
+      // 32 rows one by one, whole, and turns them in shared memory (a lane
+      // reading a row by itself touched a line per lane and load, 8000 cycles
+      // for the 8 warps).
+      float2* turn = reinterpret_cast<float2*>(smem + PX_OFF_Q) + (warp - 4) * 32 * 32;
+      const int row0 = row - lane, live = min(32, rows - row0);
+      int hi = row0 % p.group;
+      const float2* q = reinterpret_cast<const float2*>(
+                            p.q + ((size_t)(row0 / p.group) * p.n_head + g * p.group + hi) * 64) +
+                        lane;
+      float2 v[32];   // all on their way before the first is used
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        v[i] = i < live ? *q : make_float2(0.f, 0.f);
+        const bool next = ++hi == p.group;   // the next query's heads of this KV head
+        q += next ? (p.n_head - p.group + 1) * 32 : 32;
+        hi = next ? 0 : hi;
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) turn[i * 32 + (lane ^ i)] = v[i];
+      __syncwarp();
       uint32_t w[64];
-      const float* q = p.q + ((size_t)(row < rows ? s : 0) * p.n_head + (row < rows ? h : 0)) * 64;
 #pragma unroll
       for (int c = 0; c < 32; ++c) {
-        const float2 v = row < rows ? *reinterpret_cast<const float2*>(q + 2 * c) : make_float2(0.f, 0.f);
+        const float2 v = turn[lane * 32 + (c ^ lane)];
         float h0, l0, h1, l1;
         split_bf16(v.x * p.scale_log2, h0, l0);
         split_bf16(v.y * p.scale_log2, h1, l1);
