@@ -311,18 +311,27 @@ def test_attention_shared(tg, backend, shape, dtype, page, shared):
     p.cache.destroy()
 
 
-@pytest.mark.parametrize("n,shared,page", [(1, 3000, 16), (19, 5000, 32), (37, 2049, 16),
-                                           (150, 1111, 128), (64, 20000, 64)])
-def test_attention_shared_batches(tg, backend, n, shared, page):
+@pytest.mark.parametrize("n,shared,page,shape", [
+    (1, 3000, 16, (14, 2, 64)), (19, 5000, 32, (14, 2, 64)), (37, 2049, 16, (14, 2, 64)),
+    # From here on the prefix goes to the tensor cores: one tile of rows (the
+    # keys shared out between both slots), two tiles, an odd number of them,
+    # groups of 1 to 11, pages smaller and larger than a step.
+    (10, 30011, 16, (14, 2, 64)), (19, 16000, 32, (14, 2, 64)), (37, 8001, 8, (14, 2, 64)),
+    (150, 2111, 128, (14, 2, 64)), (64, 20000, 64, (14, 2, 64)), (70, 2000, 16, (4, 4, 64)),
+    (40, 4444, 256, (12, 4, 64)), (30, 9000, 16, (22, 2, 64)), (131, 4100, 16, (3, 1, 64))])
+def test_attention_shared_batches(tg, backend, n, shared, page, shape):
+    """Suffixes of 0 to 300 rows, a query inside the shared part, an empty one."""
     rng = np.random.default_rng(n)
     sh = shared // page * page
     lens = [sh + int(x) for x in rng.integers(0, 300, n)]
-    p = Pool(tg, backend, lens, (14, 2, 64), "bf16", page, seed=n, shared=shared, scale=1.5)
+    lens[n // 2] = 0 if n > 1 else lens[0]
+    lens[n // 3] = sh - 5 if n > 3 else lens[n // 3]
+    p = Pool(tg, backend, lens, shape, "bf16", page, seed=n, shared=shared, scale=1.5)
     p.cache.attention_shared(0, p.q, p.past, p.table, shared, p.out)
     again = p.out.clone()
     p.cache.attention_shared(0, p.q, p.past, p.table, shared, again)
     backend.synchronize()
-    p.check(p.out, seqs=sorted(rng.choice(n, min(n, 12), replace=False)))
+    p.check(p.out, seqs=sorted(set(rng.choice(n, min(n, 8), replace=False)) | {n // 2, n // 3}))
     assert (p.out == again).all()
 
 

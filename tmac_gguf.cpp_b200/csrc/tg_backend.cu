@@ -1668,9 +1668,14 @@ int check_host_pages(const tg_paged_kv* pk, const int32_t* past, const int32_t* 
   return TG_OK;
 }
 
-// Whether the tensor-core kernel takes a shared prefix (see run_paged).
-bool use_prefix(int n, int group, int shared_len) {
-  return n >= 2 && shared_len >= 256;
+// Whether the tensor-core kernel takes a shared prefix (see run_paged).  It
+// costs two launches more and about 20 us in all; without it every query
+// reads the prefix for itself, mostly from L2.  Measured on a B200 (14 query /
+// 2 KV heads, us without / with): 64 x 2048 21 / 23, 64 x 4096 29 / 24,
+// 32 x 8192 29 / 25, 16 x 16384 29 / 29, 128 x 32768 275 / 54; with 8 / 4
+// heads 32 x 2048 21 / 23, 32 x 4096 29 / 24, 8 x 16384 28 / 24.
+bool use_prefix(int n, int n_kv, int shared_len) {
+  return (long long)n * n_kv * shared_len >= (1LL << 19);
 }
 
 // Attention launches on device pointers, kPagedMaxQueries queries at a time.
@@ -1685,7 +1690,7 @@ int run_paged(tg_context* ctx, const tg_paged_kv* pk, int layer, int n, const fl
   // steps: whole steps of whole pages.
   const int unit = std::max(d.page_size, tg::kPrefixKeys);
   const bool prefix = pk->tmap_ok && d.dtype == TG_DTYPE_BF16 && d.head_dim == 64 &&
-                      use_prefix(n, d.n_head / d.n_kv_head, shared_len);
+                      use_prefix(n, d.n_kv_head, shared_len);
   const int shared = prefix ? shared_len / unit * unit : 0;
   const int qdim = d.n_head * d.head_dim;
   tg::PagedAttnParams p{};
