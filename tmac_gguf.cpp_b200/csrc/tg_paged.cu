@@ -764,6 +764,27 @@ __device__ __forceinline__ void mbar_arrive_expect_tx_elect(uint32_t bar, uint32
       : "memory");
 }
 
+// A pair of floats as three pairs of bf16, each rounded from what the ones
+// before leave: all 24 bits.
+__device__ __forceinline__ void split3_pair(float x, float y, uint32_t& hi, uint32_t& lo,
+                                            uint32_t& third) {
+  float h0, r0, h1, r1, l0, l1;
+  split_bf16(x, h0, r0);
+  split_bf16(y, h1, r1);
+  hi = pack_bf16x2(h0, h1);
+  split_bf16(r0, l0, r0);
+  split_bf16(r1, l1, r1);
+  lo = pack_bf16x2(l0, l1);
+  third = pack_bf16x2(r0, r1);
+}
+
+// mma_bf16_16816 with zeros in rows 8 to 15 of A.
+__device__ __forceinline__ void mma_bf16_16816_top(float* d, const uint32_t* a, uint32_t b0,
+                                                   uint32_t b1) {
+  const uint32_t full[4] = {a[0], 0u, a[1], 0u};
+  mma_bf16_16816(d, full, b0, b1);
+}
+
 // x = hi + lo with hi the 11 leading significant bits (a tf32 value) and lo
 // exact; as an operand lo keeps its own 11 leading bits: 2^-21 of x is lost.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
@@ -894,9 +915,10 @@ __device__ void merge_parts_vec(const PagedAttnParams& p, const SegmentOut& dst,
 //
 // Products are mma.sync: a step has at most 8 query rows, far below the 64 of
 // a tcgen05 tile.  The 8 spare rows of the 16-row operand carry the low part
-// of q (and of the probabilities): x = hi + lo, two bf16 (17 bits together)
-// against the exact bf16 rows, or two tf32 against the rows split the same
-// way, so results are those of binary32 products to 2^-17 and 2^-21.
+// of q (and of the probabilities).  Against exact bf16 rows x is three bf16,
+// all its 24 bits: hi and lo in one product, the third in a second one (two
+// alone left results 3e-6 from those in 64 bits where binary32 leaves 5e-7);
+// against fp32 rows x and the rows are two tf32 each, good to 2^-21.
 template <typename T, int HD>
 __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     paged_mma_kernel(const __grid_constant__ CUtensorMap tmk,
@@ -1067,6 +1089,7 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
   int slot = 0;
   uint32_t ph = 0;
   uint32_t qa[kHalf ? HD / 16 : HD / 8][4];
+  uint32_t q3[HD / 16][2];   // bf16: the third parts
   float o[HD / 8][4];
   for (int t = t_lo; t < t_hi;) {
     while (prefix[s + 1] * streams <= t) ++s;
@@ -1083,11 +1106,7 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
       for (int half = 0; half < 2; ++half) {
         if constexpr (kHalf) {
           const float2 v = make_float2(q_raw[4 * kk + 2 * half], q_raw[4 * kk + 2 * half + 1]);
-          float h0, l0, h1, l1;
-          split_bf16(v.x, h0, l0);
-          split_bf16(v.y, h1, l1);
-          qa[kk][2 * half] = pack_bf16x2(h0, h1);
-          qa[kk][2 * half + 1] = pack_bf16x2(l0, l1);
+          split3_pair(v.x, v.y, qa[kk][2 * half], qa[kk][2 * half + 1], q3[kk][half]);
         } else {
           split_tf32(q_raw[2 * kk + half], qa[kk][2 * half], qa[kk][2 * half + 1]);
         }
@@ -1144,6 +1163,8 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
                           b1, b2, b3);
               mma_bf16_16816(acc[kq & 1], qa[2 * kq], b0, b1);
               mma_bf16_16816(acc[kq & 1], qa[2 * kq + 1], b2, b3);
+              mma_bf16_16816_top(acc[kq & 1], q3[2 * kq], b0, b1);
+              mma_bf16_16816_top(acc[kq & 1], q3[2 * kq + 1], b2, b3);
             }
           } else {
             const int row = 8 * nt + r;
@@ -1196,16 +1217,9 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
         if constexpr (kHalf) {
 #pragma unroll
           for (int kp = 0; kp < CH / 16; ++kp) {
-            uint32_t pa[4];
-            float h0, l0, h1, l1;
-            split_bf16(sc[2 * kp][0], h0, l0);
-            split_bf16(sc[2 * kp][1], h1, l1);
-            pa[0] = pack_bf16x2(h0, h1);
-            pa[1] = pack_bf16x2(l0, l1);
-            split_bf16(sc[2 * kp + 1][0], h0, l0);
-            split_bf16(sc[2 * kp + 1][1], h1, l1);
-            pa[2] = pack_bf16x2(h0, h1);
-            pa[3] = pack_bf16x2(l0, l1);
+            uint32_t pa[4], p3[2];
+            split3_pair(sc[2 * kp][0], sc[2 * kp][1], pa[0], pa[1], p3[0]);
+            split3_pair(sc[2 * kp + 1][0], sc[2 * kp + 1][1], pa[2], pa[3], p3[1]);
             const int row = 16 * kp + ((lane >> 3) & 1) * 8 + (lane & 7);
 #pragma unroll
             for (int cp = 0; cp < HD / 16; ++cp) {
@@ -1215,6 +1229,8 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
                                 b0, b1, b2, b3);
               mma_bf16_16816(o[2 * cp], pa, b0, b1);
               mma_bf16_16816(o[2 * cp + 1], pa, b2, b3);
+              mma_bf16_16816_top(o[2 * cp], p3, b0, b1);
+              mma_bf16_16816_top(o[2 * cp + 1], p3, b2, b3);
             }
           }
         } else {

@@ -85,15 +85,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// Two floats as the upper halves (truncated bf16) of one register, lo first,
-// and what is left of them as a second one (rounded): off by at most 2^-16.
+// Two floats as two pairs of bf16, the rounded values and what they leave,
+// rounded: 16 bits and a sign, off by at most 2^-18.
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
-  const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
-  hi = __byte_perm(ua, ub, 0x7632);
-  // a - its upper half, the latter with its sign turned.
-  const uint64_t rest =
-      add_pair(f32x2(a, b), f32x2(__uint_as_float((ua & 0xffff0000u) ^ 0x80000000u),
-                                __uint_as_float((ub & 0xffff0000u) ^ 0x80000000u)));
+  hi = pack_bf16x2(a, b);
+  // a - its rounded value, the latter with its sign turned.
+  const uint64_t rest = add_pair(f32x2(a, b), f32x2(__uint_as_float((hi << 16) ^ 0x80000000u),
+                                                    __uint_as_float((hi & 0xffff0000u) ^ 0x80000000u)));
   float ra, rb;
   unpair(rest, ra, rb);
   lo = pack_bf16x2(ra, rb);
