@@ -798,22 +798,24 @@ struct MmaPaged {
   static constexpr bool kHalf = sizeof(T) == 2;
   static constexpr int LCH = (kHalf && HD == 64) ? 5 : 4;   // log2 of a chunk's rows
   static constexpr int CH = 1 << LCH;
-  // 12 warps leave a thread 168 registers, which head_dim 64 keeps to without
-  // spilling, 8 warps 255.
-  static constexpr int WARPS = HD == 64 ? 11 : kHalf ? 7 : 5;
-  static constexpr int THREADS = 32 * WARPS;
+  // Warps that compute and warps that load for them.  12 in all leave a thread
+  // 168 registers, which head_dim 64 about keeps to, 8 or fewer 255.
+  static constexpr int WARPS = HD == 64 ? 8 : kHalf ? 6 : 4;
+  static constexpr int PWARPS = HD == 64 ? 4 : 2;
+  static constexpr int CTHREADS = 32 * WARPS;
+  static constexpr int THREADS = 32 * (WARPS + PWARPS);
   static constexpr int NX = HD * (int)sizeof(T) / 128;    // 128-byte column blocks of a row
   static constexpr int HALF = CH * HD * (int)sizeof(T);   // K (or V) bytes of a chunk
   static constexpr int STAGE = 2 * HALF;
-  static constexpr int DEPTH = (HD == 128 && kHalf) ? 3 : 2;  // stages of a warp
+  static constexpr int DEPTH = 3;                         // stages of a warp
   static constexpr int STAGES = DEPTH * WARPS;
   static constexpr int OSTRIDE = HD + 8;                  // floats per head in the merge area
   static constexpr int MRG = kPagedHeads * OSTRIDE + 2 * kPagedHeads;
   static constexpr int OFF_BAR = STAGES * STAGE;
-  static constexpr int OFF_META = OFF_BAR + STAGES * 8;
+  static constexpr int OFF_META = OFF_BAR + 2 * STAGES * 8;
   static constexpr int OFF_MRG = (OFF_META + STAGES * 4 + 15) & ~15;
   static constexpr int OFF_MISC = OFF_MRG + WARPS * MRG * 4;
-  static constexpr int OFF_SCHED = OFF_MISC + (WARPS + 5) * 4;
+  static constexpr int OFF_SCHED = OFF_MISC + (WARPS + PWARPS + 5) * 4;
   static constexpr size_t smem_bytes(int n) { return 1024 + (size_t)OFF_SCHED + (size_t)(2 * n + 1) * 4; }
 };
 
@@ -904,14 +906,15 @@ __device__ void merge_parts_vec(const PagedAttnParams& p, const SegmentOut& dst,
   store_segment4(dst, h, it * 4 - h * HD, a.O, a.M, a.L);
 }
 
-// bf16 or fp32 pool, head_dim 64 or 128.  Chunk k of the CTA's range is warp
-// k % WARPS's, and each warp has DEPTH stages of its own that it fills by TMA
-// itself (boxes of min(page, CH) rows, 128-byte swizzle): a stage just read
-// is refilled with the warp's chunk DEPTH further on, whose page was looked
-// up one step earlier.  The warps share nothing until a stream's segment
-// ends, and no warp's loads wait for another's (with one producer warp for
-// all, its walk of page look-ups, waits and small boxes took 740 to 950
-// cycles per 8 KB chunk where the memory delivers one in 350).
+// bf16 or fp32 pool, head_dim 64 or 128.  Chunk k of the CTA's range is
+// computing warp k % WARPS's, and each such warp has DEPTH stages of its own
+// (a stage that changed hands could be two phases ahead of a waiting warp,
+// which a parity cannot tell), so the warps share nothing until a stream's
+// segment ends.  PWARPS warps fill the stages of WARPS / PWARPS computing
+// warps each by TMA (boxes of min(page, CH) rows, 128-byte swizzle), with the
+// pages looked up two steps ahead.  One loading warp for all took 740 to 950
+// cycles per 8 KB chunk where the memory delivers one in 350; computing warps
+// that load for themselves spend 1000 cycles a chunk on it.
 //
 // Products are mma.sync: a step has at most 8 query rows, far below the 64 of
 // a tcgen05 tile.  The 8 spare rows of the 16-row operand carry the low part
@@ -925,16 +928,18 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
                      const __grid_constant__ CUtensorMap tmv, const PagedAttnParams p) {
   using Cfg = MmaPaged<T, HD>;
   constexpr int STAGES = Cfg::STAGES, NX = Cfg::NX, CH = Cfg::CH, NT = CH / 8;
-  constexpr int WARPS = Cfg::WARPS, DEPTH = Cfg::DEPTH, NCT = Cfg::THREADS;
+  constexpr int WARPS = Cfg::WARPS, PWARPS = Cfg::PWARPS, DEPTH = Cfg::DEPTH;
+  constexpr int NCT = Cfg::CTHREADS;
   constexpr bool kHalf = Cfg::kHalf;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
+  uint64_t* empty = full + STAGES;
   uint32_t* meta = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_META);
   float* mrg = reinterpret_cast<float*>(smem + Cfg::OFF_MRG);
   int* warp_tot = reinterpret_cast<int*>(smem + Cfg::OFF_MISC);
-  int* flag = warp_tot + WARPS + 4;
+  int* flag = warp_tot + WARPS + PWARPS + 4;
   int* prefix = reinterpret_cast<int*>(smem + Cfg::OFF_SCHED);
   int* past_s = prefix + p.n + 1;
   const int lane = threadIdx.x & 31;
@@ -943,7 +948,7 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
 
   griddep_launch_dependents();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < STAGES; ++i) mbar_init(&full[i], 1);
+    for (int i = 0; i < 2 * STAGES; ++i) mbar_init(&full[i], 1);   // full and empty
     fence_mbar_init();
     tma_prefetch_desc(&tmk);
     tma_prefetch_desc(&tmv);
@@ -1039,11 +1044,64 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     __syncwarp();
   };
 
+  if (warp >= WARPS) {
+    // -------------------------------------------------------------- loading
+    // Chunk n of this warp: chunk first + n % M of round n / M.
+    constexpr int M = WARPS / PWARPS, L = M * DEPTH;
+    const int first = (warp - WARPS) * M;
+    Entry e[L + 3];
+    Box b[L + 2];
+#pragma unroll
+    for (int n = 0; n < L + 3; ++n) e[n] = entry(t_lo + n / M * WARPS + first + n % M);
+#pragma unroll
+    for (int n = 0; n < L + 2; ++n) b[n] = page(e[n]);
+    int issued = 0;
+#pragma unroll
+    for (int n = 0; n < L; ++n) {
+      if (t_lo + n / M * WARPS + first + n % M >= t_hi) break;
+      load((first + n % M) * DEPTH + n / M, b[n]);
+      ++issued;
+    }
+    Box b0 = b[L], b1 = b[L + 1];
+    Entry e2 = e[L + 2];
+    int round = DEPTH, i = 0, slot = 0;   // of the next chunk
+    int round3 = (L + 3) / M, i3 = (L + 3) % M;   // of the one to look up
+    uint32_t ph = 0;
+    while (t_lo + round * WARPS + first + i < t_hi) {
+      const int st = (first + i) * DEPTH + slot;
+      const bool got = mbar_wait(&empty[st], ph, p.err, kDevErrWaitEmpty);
+      if (!__all_sync(0xffffffffu, got)) break;
+      load(st, b0);
+      ++issued;
+      b0 = b1;
+      b1 = page(e2);
+      e2 = entry(t_lo + round3 * WARPS + first + i3);
+      if (++i3 == M) {
+        i3 = 0;
+        ++round3;
+      }
+      if (++i == M) {
+        i = 0;
+        ++round;
+        if (++slot == DEPTH) {
+          slot = 0;
+          ph ^= 1u;
+        }
+      }
+    }
+    // Every load lands (bounded) before the CTA exits.
+    for (int n = max(0, issued - L); n < issued; ++n)
+      mbar_wait(&full[(first + n % M) * DEPTH + n / M % DEPTH], (uint32_t)(n / L & 1), p.err,
+                kDevErrWaitFull);
+    return;
+  }
+
+  // ---------------------------------------------------------------- computing
   const int r = lane >> 2, qd = lane & 3;
   float* my_mrg = mrg + warp * Cfg::MRG;
   const float sl2 = p.scale_log2;
-  // q of a stream, this lane's elements (row r of the operand).  Loaded ahead
-  // of the chunks: behind a full ring of tiles a load takes 5000 cycles.
+  // q of a stream, this lane's elements (row r of the operand), loaded a
+  // segment ahead: behind full rings of tiles a load takes 5000 cycles.
   float q_raw[HD / 4];
   auto load_q = [&](int qs, int qu) {
     const int g = p.hblocks == 1 ? qu : qu / p.hblocks, hb = qu - g * p.hblocks;
@@ -1066,25 +1124,6 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
   };
   load_q(ls, lu);
   int ti = t_lo + warp;   // this warp's next chunk to compute
-  int tl = ti;            // ... to load
-  Box box_n;              // pages of chunk tl, and the entries of the one after
-  Entry entry_n;
-  {
-    Entry e[DEPTH + 2];
-    Box b[DEPTH + 1];
-#pragma unroll
-    for (int i = 0; i < DEPTH + 2; ++i) e[i] = entry(ti + i * WARPS);
-#pragma unroll
-    for (int i = 0; i <= DEPTH; ++i) b[i] = page(e[i]);
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i) {
-      if (tl >= t_hi) break;
-      load(warp * DEPTH + i, b[i]);
-      tl += WARPS;
-    }
-    box_n = b[DEPTH];
-    entry_n = e[DEPTH + 1];
-  }
   bool failed = false;
   int slot = 0;
   uint32_t ph = 0;
@@ -1258,12 +1297,7 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
         }
       }
       __syncwarp();
-      if (tl < t_hi && !failed) {
-        load(st, box_n);
-        tl += WARPS;
-        box_n = page(entry_n);
-        entry_n = entry(tl + WARPS);
-      }
+      if (lane == 0) mbar_arrive(&empty[st]);
       if (++slot == DEPTH) {
         slot = 0;
         ph ^= 1u;
@@ -1318,13 +1352,6 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     }
     consumers_sync(NCT);
     t = e_hi;
-  }
-  if (failed) {
-    // Loads still in flight land (bounded) before the CTA exits.
-    for (int i = 0; i < DEPTH; ++i) {
-      mbar_wait(&full[warp * DEPTH + i], 0, p.err, kDevErrWaitFull);
-      mbar_wait(&full[warp * DEPTH + i], 1, p.err, kDevErrWaitFull);
-    }
   }
 }
 

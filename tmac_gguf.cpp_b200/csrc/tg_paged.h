@@ -18,7 +18,7 @@ namespace tg {
 
 constexpr int kPagedMinPage = 8, kPagedMaxPage = 256;
 // Queries per launch: the schedule of a launch lives in shared memory.
-constexpr int kPagedMaxQueries = 2048;
+constexpr int kPagedMaxQueries = 1024;
 constexpr int kPagedHeads = 8;    // query heads of one stream (a KV head's group in blocks of 8)
 constexpr int kPagedChunk = 32;   // cache rows per warp step of the CUDA-core kernel
 
