@@ -809,7 +809,8 @@ struct MmaPaged {
   static constexpr int STAGE = 2 * HALF;
   static constexpr int DEPTH = 3;                         // stages of a warp
   static constexpr int STAGES = DEPTH * WARPS;
-  static constexpr int OSTRIDE = HD + 8;                  // floats per head in the merge area
+  static constexpr int OT = kHalf ? HD / 16 : HD / 8;     // tiles of the output
+  static constexpr int OSTRIDE = HD + (kHalf ? 4 : 8);    // floats per head in the merge area
   static constexpr int MRG = kPagedHeads * OSTRIDE + 2 * kPagedHeads;
   static constexpr int OFF_BAR = STAGES * STAGE;
   static constexpr int OFF_META = OFF_BAR + 2 * STAGES * 8;
@@ -1129,7 +1130,7 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
   uint32_t ph = 0;
   uint32_t qa[kHalf ? HD / 16 : HD / 8][4];
   uint32_t q3[HD / 16][2];   // bf16: the third parts
-  float o[HD / 8][4];
+  float o[Cfg::OT][4];   // bf16: (16 of head_dim) x (8 heads), else (8 heads, hi and lo) x (8)
   for (int t = t_lo; t < t_hi;) {
     while (prefix[s + 1] * streams <= t) ++s;
     const int C = prefix[s + 1] - prefix[s];
@@ -1159,7 +1160,7 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
       load_q(sn, un);
     }
 #pragma unroll
-    for (int c = 0; c < HD / 8; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
+    for (int c = 0; c < Cfg::OT; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
     float m_run = kNegBig, l_run = 0.f;
 
     for (; ti < e_hi; ti += WARPS) {
@@ -1189,23 +1190,41 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
         const uint32_t kb = smem_u32(kbox), vb = smem_u32(vbox);
         // S = q . K^T in blocks of 8 rows.
         float sc[NT][2];
+        // bf16: products in turn on four accumulators or more, so that none
+        // waits for the one before it.
+        constexpr int NA = kHalf ? (NT >= 4 ? 1 : 4 / NT) : 2;
+        float acc_s[NT][NA][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int a = 0; a < NA; ++a)
+            acc_s[nt][a][0] = acc_s[nt][a][1] = acc_s[nt][a][2] = acc_s[nt][a][3] = 0.f;
+        if constexpr (kHalf) {
+#pragma unroll
+          for (int kq = 0; kq < HD / 32; ++kq) {
+            uint32_t b[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const int row = 8 * nt + (lane & 7), chunk = 4 * (kq & 1) + (lane >> 3);
+              ldmatrix_x4(kb + (kq >> 1) * (CH * 128) + row * 128 + ((chunk ^ (row & 7)) << 4),
+                          b[nt][0], b[nt][1], b[nt][2], b[nt][3]);
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma_bf16_16816(acc_s[nt][0], qa[2 * kq + x], b[nt][2 * x], b[nt][2 * x + 1]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma_bf16_16816_top(acc_s[nt][NA - 1], q3[2 * kq + x], b[nt][2 * x],
+                                   b[nt][2 * x + 1]);
+            }
+          }
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-          if constexpr (kHalf) {
-            const int row = 8 * nt + (lane & 7);
-#pragma unroll
-            for (int kq = 0; kq < HD / 32; ++kq) {
-              const int chunk = 4 * (kq & 1) + (lane >> 3);
-              uint32_t b0, b1, b2, b3;
-              ldmatrix_x4(kb + (kq >> 1) * (CH * 128) + row * 128 + ((chunk ^ (row & 7)) << 4), b0,
-                          b1, b2, b3);
-              mma_bf16_16816(acc[kq & 1], qa[2 * kq], b0, b1);
-              mma_bf16_16816(acc[kq & 1], qa[2 * kq + 1], b2, b3);
-              mma_bf16_16816_top(acc[kq & 1], q3[2 * kq], b0, b1);
-              mma_bf16_16816_top(acc[kq & 1], q3[2 * kq + 1], b2, b3);
-            }
-          } else {
+          float(&acc)[NA][4] = acc_s[nt];
+          if constexpr (!kHalf) {
             const int row = 8 * nt + r;
 #pragma unroll
             for (int kk = 0; kk < HD / 8; ++kk) {
@@ -1219,8 +1238,12 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
               mma_tf32_1688(acc[1], qa[kk], l0, l1);
             }
           }
-          sc[nt][0] = ((acc[0][0] + acc[0][2]) + (acc[1][0] + acc[1][2])) * sl2;
-          sc[nt][1] = ((acc[0][1] + acc[0][3]) + (acc[1][1] + acc[1][3])) * sl2;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = acc[0][e] + acc[0][e + 2];
+            if constexpr (NA > 1) x += acc[1][e] + acc[1][e + 2];
+            sc[nt][e] = x * sl2;
+          }
           if (!whole) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -1247,29 +1270,40 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
         }
         l_run = l_run * alpha + lsum;
         if (__any_sync(0xffffffffu, alpha != 1.f)) {
+          float a0 = alpha, a1 = alpha;
+          if constexpr (kHalf) {   // of the heads of this lane's columns
+            a0 = __shfl_sync(0xffffffffu, alpha, 8 * qd);
+            a1 = __shfl_sync(0xffffffffu, alpha, 8 * qd + 4);
+          }
 #pragma unroll
-          for (int c = 0; c < HD / 8; ++c) {
-            o[c][0] *= alpha; o[c][1] *= alpha; o[c][2] *= alpha; o[c][3] *= alpha;
+          for (int c = 0; c < Cfg::OT; ++c) {
+            o[c][0] *= a0; o[c][1] *= a1; o[c][2] *= a0; o[c][3] *= a1;
           }
         }
         // O += P . V.
         if constexpr (kHalf) {
 #pragma unroll
           for (int kp = 0; kp < CH / 16; ++kp) {
-            uint32_t pa[4], p3[2];
-            split3_pair(sc[2 * kp][0], sc[2 * kp][1], pa[0], pa[1], p3[0]);
-            split3_pair(sc[2 * kp + 1][0], sc[2 * kp + 1][1], pa[2], pa[3], p3[1]);
+            // A lane's scores (one head, two rows of K) are the B operand of
+            // O^T += V^T . P^T as they stand.
+            uint32_t ph0, ph1, pl0, pl1, p30, p31;
+            split3_pair(sc[2 * kp][0], sc[2 * kp][1], ph0, pl0, p30);
+            split3_pair(sc[2 * kp + 1][0], sc[2 * kp + 1][1], ph1, pl1, p31);
             const int row = 16 * kp + ((lane >> 3) & 1) * 8 + (lane & 7);
 #pragma unroll
-            for (int cp = 0; cp < HD / 16; ++cp) {
-              const int chunk = 2 * (cp & 3) + (lane >> 4);
-              uint32_t b0, b1, b2, b3;
-              ldmatrix_x4_trans(vb + (cp >> 2) * (CH * 128) + row * 128 + ((chunk ^ (row & 7)) << 4),
-                                b0, b1, b2, b3);
-              mma_bf16_16816(o[2 * cp], pa, b0, b1);
-              mma_bf16_16816(o[2 * cp + 1], pa, b2, b3);
-              mma_bf16_16816_top(o[2 * cp], p3, b0, b1);
-              mma_bf16_16816_top(o[2 * cp + 1], p3, b2, b3);
+            for (int x = 0; x < NX; ++x) {
+              uint32_t v[4][4];
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                ldmatrix_x4_trans(vb + x * (CH * 128) + row * 128 +
+                                      (((2 * c + (lane >> 4)) ^ (row & 7)) << 4),
+                                  v[c][0], v[c][2], v[c][1], v[c][3]);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) mma_bf16_16816(o[4 * x + c], v[c], ph0, ph1);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) mma_bf16_16816(o[4 * x + c], v[c], pl0, pl1);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) mma_bf16_16816(o[4 * x + c], v[c], p30, p31);
             }
           }
         } else {
@@ -1307,9 +1341,16 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
 #pragma unroll
-    for (int c = 0; c < HD / 8; ++c)
-      *reinterpret_cast<float2*>(my_mrg + r * Cfg::OSTRIDE + 8 * c + 2 * qd) =
-          make_float2(o[c][0] + o[c][2], o[c][1] + o[c][3]);
+    for (int c = 0; c < Cfg::OT; ++c) {
+      if constexpr (kHalf) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          my_mrg[(2 * qd + (x & 1)) * Cfg::OSTRIDE + 16 * c + 8 * (x >> 1) + r] = o[c][x];
+      } else {
+        *reinterpret_cast<float2*>(my_mrg + r * Cfg::OSTRIDE + 8 * c + 2 * qd) =
+            make_float2(o[c][0] + o[c][2], o[c][1] + o[c][3]);
+      }
+    }
     if (qd == 0) {
       my_mrg[kPagedHeads * Cfg::OSTRIDE + r] = m_run;
       my_mrg[kPagedHeads * (Cfg::OSTRIDE + 1) + r] = l_run;
