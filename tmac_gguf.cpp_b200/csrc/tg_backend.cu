@@ -3074,20 +3074,22 @@ int tg_paged_create(tg_context* ctx, const tg_paged_desc* desc, tg_paged_kv** ou
     return fail(TG_ERR_OUT_OF_MEMORY, "paged_create: %zu bytes per cache", bytes);
   }
   PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
-  if (enc && (d.head_dim == 64 || d.head_dim == 128)) {
+  if (enc && (d.head_dim == 32 || d.head_dim == 64 || d.head_dim == 128)) {
     const CUtensorMapDataType ty = d.dtype == TG_DTYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                                            : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     cuuint64_t gdim[2] = {(cuuint64_t)d.head_dim,
                           (cuuint64_t)(rows * d.n_kv_head * d.n_layers)};
     cuuint64_t gstride[1] = {(cuuint64_t)(d.head_dim * pk->esize)};
-    cuuint32_t box[2] = {(cuuint32_t)(128 / pk->esize),
+    const int width = std::min(d.head_dim * (int)pk->esize, 128);   // bytes of a box's rows
+    cuuint32_t box[2] = {(cuuint32_t)(width / (int)pk->esize),
                          (cuuint32_t)std::min(d.page_size,
                                               1 << tg::paged_mma_lchunk(d.dtype, d.head_dim))};
     cuuint32_t estr[2] = {1, 1};
     pk->tmap_ok = true;
     for (int i = 0; i < 2; ++i)
       if (enc(i ? &pk->tmv : &pk->tmk, ty, 2, i ? pk->v : pk->k, gdim, gstride, box, estr,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_INTERLEAVE_NONE,
+              width == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         pk->tmap_ok = false;

@@ -796,18 +796,19 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
 template <typename T, int HD>
 struct MmaPaged {
   static constexpr bool kHalf = sizeof(T) == 2;
-  static constexpr int LCH = (kHalf && HD == 64) ? 5 : 4;   // log2 of a chunk's rows
+  static constexpr int LCH = (kHalf && HD <= 64) ? 5 : 4;   // log2 of a chunk's rows
   static constexpr int CH = 1 << LCH;
   // Warps that compute and warps that load for them.  12 in all leave a thread
   // 168 registers, which head_dim 64 about keeps to, 8 or fewer 255.
-  static constexpr int WARPS = HD == 64 ? 8 : kHalf ? 6 : 4;
-  static constexpr int PWARPS = HD == 64 ? 4 : 2;
+  static constexpr int WARPS = HD <= 64 ? 8 : kHalf ? 6 : 4;
+  static constexpr int PWARPS = HD <= 64 ? 4 : 2;
   static constexpr int CTHREADS = 32 * WARPS;
   static constexpr int THREADS = 32 * (WARPS + PWARPS);
-  static constexpr int NX = HD * (int)sizeof(T) / 128;    // 128-byte column blocks of a row
+  static constexpr int RB = HD * (int)sizeof(T) < 128 ? HD * (int)sizeof(T) : 128;
+  static constexpr int NX = HD * (int)sizeof(T) / RB;     // column blocks of RB bytes of a row
   static constexpr int HALF = CH * HD * (int)sizeof(T);   // K (or V) bytes of a chunk
   static constexpr int STAGE = 2 * HALF;
-  static constexpr int DEPTH = 3;                         // stages of a warp
+  static constexpr int DEPTH = HD == 32 ? 4 : 3;          // stages of a warp
   static constexpr int STAGES = DEPTH * WARPS;
   static constexpr int OT = kHalf ? HD / 16 : HD / 8;     // tiles of the output
   static constexpr int OSTRIDE = HD + (kHalf ? 4 : 8);    // floats per head in the merge area
@@ -818,6 +819,11 @@ struct MmaPaged {
   static constexpr int OFF_MISC = OFF_MRG + WARPS * MRG * 4;
   static constexpr int OFF_SCHED = OFF_MISC + (WARPS + PWARPS + 5) * 4;
   static constexpr size_t smem_bytes(int n) { return 1024 + (size_t)OFF_SCHED + (size_t)(2 * n + 1) * 4; }
+  // Byte of 16-byte piece `piece` of row `row` in a column block, under the
+  // boxes' swizzle (RB bytes: 128, or 64 with half as many pieces to turn).
+  static __device__ __forceinline__ int at(int row, int piece) {
+    return row * RB + ((piece ^ (RB == 128 ? row & 7 : (row >> 1) & 3)) << 4);
+  }
 };
 
 __device__ __forceinline__ void consumers_sync(int n) {
@@ -907,12 +913,12 @@ __device__ void merge_parts_vec(const PagedAttnParams& p, const SegmentOut& dst,
   store_segment4(dst, h, it * 4 - h * HD, a.O, a.M, a.L);
 }
 
-// bf16 or fp32 pool, head_dim 64 or 128.  Chunk k of the CTA's range is
+// bf16 or fp32 pool, head_dim 32, 64 or 128.  Chunk k of the CTA's range is
 // computing warp k % WARPS's, and each such warp has DEPTH stages of its own
 // (a stage that changed hands could be two phases ahead of a waiting warp,
 // which a parity cannot tell), so the warps share nothing until a stream's
 // segment ends.  PWARPS warps fill the stages of WARPS / PWARPS computing
-// warps each by TMA (boxes of min(page, CH) rows, 128-byte swizzle), with the
+// warps each by TMA (boxes of min(page, CH) rows, swizzled), with the
 // pages looked up two steps ahead.  One loading warp for all took 740 to 950
 // cycles per 8 KB chunk where the memory delivers one in 350; computing warps
 // that load for themselves spend 1000 cycles a chunk on it.
@@ -1030,15 +1036,15 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     int loads = 0;
 #pragma unroll
     for (int b = 0; b < 4; ++b) loads += ((m >> (8 * b)) & 255u) != 0;
-    mbar_arrive_expect_tx_elect(bar, (uint32_t)(loads * box * 2 * NX * 128));
+    mbar_arrive_expect_tx_elect(bar, (uint32_t)(loads * box * 2 * NX * Cfg::RB));
     for (int b = 0; b < nbx; ++b) {
       const int yb = (int)__reduce_max_sync(0xffffffffu, lane == b ? (uint32_t)y : 0u);
       if ((m >> (8 * b)) & 255u) {
 #pragma unroll
         for (int c = 0; c < NX; ++c) {
-          const uint32_t at = to + b * box * 128 + c * (CH * 128);
-          tma_load_2d_elect(at, &tmk, bar, c * (128 / (int)sizeof(T)), yb);
-          tma_load_2d_elect(at + Cfg::HALF, &tmv, bar, c * (128 / (int)sizeof(T)), yb);
+          const uint32_t at = to + b * box * Cfg::RB + c * (CH * Cfg::RB);
+          tma_load_2d_elect(at, &tmk, bar, c * (Cfg::RB / (int)sizeof(T)), yb);
+          tma_load_2d_elect(at + Cfg::HALF, &tmv, bar, c * (Cfg::RB / (int)sizeof(T)), yb);
         }
       }
     }
@@ -1180,8 +1186,8 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
 #pragma unroll
             for (int x = 0; x < NX; ++x)
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                reinterpret_cast<uint4*>(vbox + x * (CH * 128) + row * 128)[(e + row) & 7] =
+              for (int e = 0; e < Cfg::RB / 16; ++e)
+                *reinterpret_cast<uint4*>(vbox + x * (CH * Cfg::RB) + Cfg::at(row, e)) =
                     make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
@@ -1206,8 +1212,8 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               const int row = 8 * nt + (lane & 7), chunk = 4 * (kq & 1) + (lane >> 3);
-              ldmatrix_x4(kb + (kq >> 1) * (CH * 128) + row * 128 + ((chunk ^ (row & 7)) << 4),
-                          b[nt][0], b[nt][1], b[nt][2], b[nt][3]);
+              ldmatrix_x4(kb + (kq >> 1) * (CH * Cfg::RB) + Cfg::at(row, chunk), b[nt][0],
+                          b[nt][1], b[nt][2], b[nt][3]);
             }
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
@@ -1228,12 +1234,11 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
             const int row = 8 * nt + r;
 #pragma unroll
             for (int kk = 0; kk < HD / 8; ++kk) {
-              const uint8_t* a = kbox + (kk >> 2) * (CH * 128) + row * 128 + qd * 4;
+              const uint8_t* a = kbox + (kk >> 2) * (CH * 128) + qd * 4;
               const int chunk = 2 * (kk & 3);
               uint32_t h0, l0, h1, l1;
-              split_tf32(*reinterpret_cast<const float*>(a + ((chunk ^ (row & 7)) << 4)), h0, l0);
-              split_tf32(*reinterpret_cast<const float*>(a + (((chunk + 1) ^ (row & 7)) << 4)), h1,
-                         l1);
+              split_tf32(*reinterpret_cast<const float*>(a + Cfg::at(row, chunk)), h0, l0);
+              split_tf32(*reinterpret_cast<const float*>(a + Cfg::at(row, chunk + 1)), h1, l1);
               mma_tf32_1688(acc[0], qa[kk], h0, h1);
               mma_tf32_1688(acc[1], qa[kk], l0, l1);
             }
@@ -1292,18 +1297,18 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
             const int row = 16 * kp + ((lane >> 3) & 1) * 8 + (lane & 7);
 #pragma unroll
             for (int x = 0; x < NX; ++x) {
-              uint32_t v[4][4];
+              constexpr int NC = Cfg::RB / 32;   // 16-column tiles of a block
+              uint32_t v[NC][4];
 #pragma unroll
-              for (int c = 0; c < 4; ++c)
-                ldmatrix_x4_trans(vb + x * (CH * 128) + row * 128 +
-                                      (((2 * c + (lane >> 4)) ^ (row & 7)) << 4),
+              for (int c = 0; c < NC; ++c)
+                ldmatrix_x4_trans(vb + x * (CH * Cfg::RB) + Cfg::at(row, 2 * c + (lane >> 4)),
                                   v[c][0], v[c][2], v[c][1], v[c][3]);
 #pragma unroll
-              for (int c = 0; c < 4; ++c) mma_bf16_16816(o[4 * x + c], v[c], ph0, ph1);
+              for (int c = 0; c < NC; ++c) mma_bf16_16816(o[NC * x + c], v[c], ph0, ph1);
 #pragma unroll
-              for (int c = 0; c < 4; ++c) mma_bf16_16816(o[4 * x + c], v[c], pl0, pl1);
+              for (int c = 0; c < NC; ++c) mma_bf16_16816(o[NC * x + c], v[c], pl0, pl1);
 #pragma unroll
-              for (int c = 0; c < 4; ++c) mma_bf16_16816(o[4 * x + c], v[c], p30, p31);
+              for (int c = 0; c < NC; ++c) mma_bf16_16816(o[NC * x + c], v[c], p30, p31);
             }
           }
         } else {
@@ -1318,12 +1323,11 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
             const int row = 8 * nt + 2 * qd;
 #pragma unroll
             for (int c = 0; c < HD / 8; ++c) {
-              const uint8_t* a = vbox + (c >> 2) * (CH * 128) + row * 128 + (r & 3) * 4;
+              const uint8_t* a = vbox + (c >> 2) * (CH * 128) + (r & 3) * 4;
               const int chunk = 2 * (c & 3) + (r >> 2);
               uint32_t h0, l0, h1, l1;
-              split_tf32(*reinterpret_cast<const float*>(a + ((chunk ^ (row & 7)) << 4)), h0, l0);
-              split_tf32(*reinterpret_cast<const float*>(a + 128 + ((chunk ^ ((row + 1) & 7)) << 4)),
-                         h1, l1);
+              split_tf32(*reinterpret_cast<const float*>(a + Cfg::at(row, chunk)), h0, l0);
+              split_tf32(*reinterpret_cast<const float*>(a + Cfg::at(row + 1, chunk)), h1, l1);
               mma_tf32_1688(o[c], pa, h0, h1);
               mma_tf32_1688(o[c], pa, l0, l1);
             }
@@ -1407,7 +1411,11 @@ static cudaError_t launch_mma_cfg(const CUtensorMap& tk, const CUtensorMap& tv,
 }
 
 int paged_mma_lchunk(int dtype, int hd) {
-  return dtype == 1 && hd == 64 ? MmaPaged<__nv_bfloat16, 64>::LCH : MmaPaged<float, 64>::LCH;
+  static_assert(MmaPaged<__nv_bfloat16, 32>::LCH == MmaPaged<__nv_bfloat16, 64>::LCH, "rows");
+  static_assert(MmaPaged<float, 32>::LCH == MmaPaged<float, 64>::LCH &&
+                    MmaPaged<float, 128>::LCH == MmaPaged<float, 64>::LCH &&
+                    MmaPaged<__nv_bfloat16, 128>::LCH == MmaPaged<float, 64>::LCH, "rows");
+  return dtype == 1 && hd <= 64 ? MmaPaged<__nv_bfloat16, 64>::LCH : MmaPaged<float, 64>::LCH;
 }
 
 cudaError_t launch_paged_mma(const CUtensorMap& tk, const CUtensorMap& tv, const PagedAttnParams& p,
@@ -1416,6 +1424,9 @@ cudaError_t launch_paged_mma(const CUtensorMap& tk, const CUtensorMap& tv, const
   static_assert(MmaPaged<__nv_bfloat16, 128>::smem_bytes(kPagedMaxQueries) <= 227 * 1024, "shared memory");
   static_assert(MmaPaged<float, 64>::smem_bytes(kPagedMaxQueries) <= 227 * 1024, "shared memory");
   static_assert(MmaPaged<__nv_bfloat16, 64>::smem_bytes(kPagedMaxQueries) <= 227 * 1024, "shared memory");
+  if (p.hd == 32)
+    return dtype == 1 ? launch_mma_cfg<__nv_bfloat16, 32>(tk, tv, p, grid, st)
+                      : launch_mma_cfg<float, 32>(tk, tv, p, grid, st);
   if (p.hd == 64)
     return dtype == 1 ? launch_mma_cfg<__nv_bfloat16, 64>(tk, tv, p, grid, st)
                       : launch_mma_cfg<float, 64>(tk, tv, p, grid, st);

@@ -105,8 +105,9 @@ cudaError_t launch_paged_prefix_merge(const PagedPrefixParams& p, cudaStream_t s
 cudaError_t launch_paged_append(const PagedAppendParams& p, cudaStream_t st);
 cudaError_t launch_paged_core(const PagedAttnParams& p, int dtype, int grid, cudaStream_t st);
 size_t paged_core_smem(int n, int hd);
-// head_dim 64 or 128; tk / tv are 2-D maps of the pools ({head_dim, rows}, box
-// {128 bytes, min(page, 1 << paged_mma_lchunk) rows}, 128-byte swizzle).
+// head_dim 32, 64 or 128; tk / tv are 2-D maps of the pools ({head_dim, rows},
+// box {min(row, 128 bytes), min(page, 1 << paged_mma_lchunk) rows}, swizzled
+// over the box's width).
 int paged_mma_lchunk(int dtype, int hd);
 cudaError_t launch_paged_mma(const CUtensorMap& tk, const CUtensorMap& tv, const PagedAttnParams& p,
                              int dtype, int grid, cudaStream_t st);
