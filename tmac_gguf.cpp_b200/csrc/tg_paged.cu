@@ -1581,16 +1581,28 @@ __device__ float page_score_any(const T* lo_p, const float* q_f, int group, int 
   return best;
 }
 
-// Binary64 score of a page for one head, by one warp.
-template <typename T>
-__device__ double exact_score(const T* lo_p, const float* q, int hd) {
+// Binary64 score of a page for one head, by eight lanes (a warp has four pairs
+// of page and head in hand: with one pair, 12 pages x 16 heads took 34000
+// cycles, nearly all of them latency; with eight, 9000).  Both bounds are
+// loaded, so that no load waits for q.
+template <typename T, int HD>
+__device__ __forceinline__ double exact_score(const T* lo_p, const float* q, int hd) {
   double sum = 0.0;
-  for (int d = threadIdx.x & 31; d < hd; d += 32) {
-    const float x = q[d];
-    sum = fma((double)x, (double)to_f32(x >= 0.f ? lo_p[hd + d] : lo_p[d]), sum);
+  if constexpr (HD > 0) {
+#pragma unroll
+    for (int k = 0; k < HD / 8; ++k) {
+      const int d = 8 * k + (threadIdx.x & 7);
+      const float x = q[d], up = to_f32(lo_p[HD + d]), low = to_f32(lo_p[d]);
+      sum = fma((double)x, (double)(x >= 0.f ? up : low), sum);
+    }
+  } else {
+    for (int d = threadIdx.x & 7; d < hd; d += 8) {
+      const float x = q[d], up = to_f32(lo_p[hd + d]), low = to_f32(lo_p[d]);
+      sum = fma((double)x, (double)(x >= 0.f ? up : low), sum);
+    }
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum;
 }
 
@@ -1603,7 +1615,7 @@ struct PickShared {
   unsigned near, sure;
   float big[kSelWarps];
   int flag;
-  int near_at[kSelNear];
+  int near_at[kSelNear], near_page[kSelNear];
   unsigned long long near_key[kSelNear];
 };
 
@@ -1999,7 +2011,10 @@ __global__ void __launch_bounds__(kSelThreads, sizeof(T) == 4 && HD >= 64 ? 1 : 
     sure += x > k_hi;
     if (x >= k_lo && x <= k_hi) {
       const unsigned at = atomicAdd(&sh.near, 1u);
-      if (at < kSelNear) sh.near_at[at] = i;
+      if (at < kSelNear) {
+        sh.near_at[at] = i;
+        sh.near_page[at] = table[i];
+      }
     }
   }
   sure = __reduce_add_sync(0xffffffffu, sure);
@@ -2020,14 +2035,16 @@ __global__ void __launch_bounds__(kSelThreads, sizeof(T) == 4 && HD >= 64 ? 1 : 
   }
   for (unsigned i = tid; i < near; i += kSelThreads) (few ? sh.near_key : wide)[i] = 0ull;
   __syncthreads();
-  // A warp per (page, head); NaN is above every key while the heads meet.
-  for (unsigned e = warp; e < near * p.group; e += kSelWarps) {
-    const unsigned i = e / p.group, h = e - i * p.group;
-    const int pg = table[few ? sh.near_at[i] : near_g[i]];
+  // Eight lanes per (page, head); NaN is above every key while the heads meet.
+  const unsigned pairs = near * p.group;
+  for (unsigned e0 = 4 * warp; e0 < pairs; e0 += 4 * kSelWarps) {
+    // (The lanes behind the last pair take it too.)
+    const unsigned e = min(e0 + (lane >> 3), pairs - 1), i = e / p.group, h = e - i * p.group;
+    const int pg = few ? sh.near_page[i] : table[near_g[i]];
     const bool bad = pg < 0 || pg >= p.n_pages;
     const T* lo = static_cast<const T*>(p.bounds) + ((size_t)(bad ? 0 : pg) * p.n_kv + g) * 2 * hd;
-    const double x = exact_score<T>(lo, q + h * hd, hd);
-    if (lane == 0)
+    const double x = exact_score<T, HD>(lo, q + (size_t)h * hd, hd);
+    if ((lane & 7) == 0)
       atomicMax(&(few ? sh.near_key : wide)[i], bad || x != x ? ~0ull : ordered_key(x));
   }
   __syncthreads();
