@@ -798,12 +798,16 @@ struct MmaPaged {
   static constexpr bool kHalf = sizeof(T) == 2;
   static constexpr int LCH = (kHalf && HD <= 64) ? 5 : 4;   // log2 of a chunk's rows
   static constexpr int CH = 1 << LCH;
-  // Warps that compute and warps that load for them.  12 in all leave a thread
-  // 168 registers, which head_dim 64 about keeps to, 8 or fewer 255.
+  // Warps that compute and warps that load for them.
   static constexpr int WARPS = HD <= 64 ? 8 : kHalf ? 6 : 4;
   static constexpr int PWARPS = HD <= 64 ? 4 : 2;
   static constexpr int CTHREADS = 32 * WARPS;
-  static constexpr int THREADS = 32 * (WARPS + PWARPS);
+  // head_dim 32 and 64: four warps close segments while the others go on, and 16
+  // warps share the registers of 512 threads x 128 out by role (warps of four
+  // at a time: 2 x 168 + 104 + 72).  128 needs them all where it computes.
+  static constexpr int CWARPS = HD <= 64 ? 4 : 0;
+  static constexpr int NWARPS = WARPS + PWARPS + CWARPS;
+  static constexpr int THREADS = 32 * NWARPS;
   static constexpr int RB = HD * (int)sizeof(T) < 128 ? HD * (int)sizeof(T) : 128;
   static constexpr int NX = HD * (int)sizeof(T) / RB;     // column blocks of RB bytes of a row
   static constexpr int HALF = CH * HD * (int)sizeof(T);   // K (or V) bytes of a chunk
@@ -814,10 +818,10 @@ struct MmaPaged {
   static constexpr int OSTRIDE = HD + (kHalf ? 4 : 8);    // floats per head in the merge area
   static constexpr int MRG = kPagedHeads * OSTRIDE + 2 * kPagedHeads;
   static constexpr int OFF_BAR = STAGES * STAGE;
-  static constexpr int OFF_META = OFF_BAR + 2 * STAGES * 8;
+  static constexpr int OFF_META = OFF_BAR + (2 * STAGES + 2) * 8;
   static constexpr int OFF_MRG = (OFF_META + STAGES * 4 + 15) & ~15;
   static constexpr int OFF_MISC = OFF_MRG + WARPS * MRG * 4;
-  static constexpr int OFF_SCHED = OFF_MISC + (WARPS + PWARPS + 5) * 4;
+  static constexpr int OFF_SCHED = OFF_MISC + (NWARPS + 12) * 4;
   static constexpr size_t smem_bytes(int n) { return 1024 + (size_t)OFF_SCHED + (size_t)(2 * n + 1) * 4; }
   // Byte of 16-byte piece `piece` of row `row` in a column block, under the
   // boxes' swizzle (RB bytes: 128, or 64 with half as many pieces to turn).
@@ -826,8 +830,17 @@ struct MmaPaged {
   }
 };
 
-__device__ __forceinline__ void consumers_sync(int n) {
-  asm volatile("bar.sync 1, %0;" ::"r"(n) : "memory");
+template <int N>
+__device__ __forceinline__ void setmaxnreg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void setmaxnreg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+__device__ __forceinline__ void named_sync(int bar, int n) {
+  asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(n) : "memory");
 }
 
 // Parts k0, k0 + step, ... of 16-byte item `it` (head h), merged.
@@ -876,19 +889,48 @@ __device__ __forceinline__ Merged4 merge_item(const PagedAttnParams& p, int it, 
   return a;
 }
 
+// Adds b's sums to a's.
+__device__ __forceinline__ void merge_two(Merged4& a, float M, float L, float4 O) {
+  const float mb = fmaxf(a.M, M), w0 = ex2(a.M - mb), w1 = ex2(M - mb);
+  a.O.x = fmaf(O.x, w1, a.O.x * w0);
+  a.O.y = fmaf(O.y, w1, a.O.y * w0);
+  a.O.z = fmaf(O.z, w1, a.O.z * w0);
+  a.O.w = fmaf(O.w, w1, a.O.w * w0);
+  a.L = fmaf(L, w1, a.L * w0);
+  a.M = mb;
+}
+
 // merge_parts for the tensor-core kernel: 16-byte items, the parts dealt out
-// to as many groups of threads as there are, joined in shared memory (`sh`,
-// 6 floats per thread).  All NT threads take part.
+// to `groups` sums per item that are then added in their order, whoever merges
+// (so who arrives last does not change a bit).  This one is by threads tid,
+// tid + step, ...
+template <int HD, int NT>
+__device__ __forceinline__ int merge_groups(int heads) {
+  return max(1, min(4, NT / (heads * HD / 4)));
+}
+template <int HD, int NT>
+__device__ void merge_parts_items(const PagedAttnParams& p, const SegmentOut& dst, int heads,
+                                  int c1, int n_parts, int tid, int step) {
+  const int groups = merge_groups<HD, NT>(heads);
+  for (int it = tid; it < heads * HD / 4; it += step) {
+    const int h = it * 4 / HD;
+    Merged4 a = merge_item(p, it, h, 0, groups, n_parts, c1);
+    for (int k = 1; k < groups; ++k) {
+      const Merged4 b = merge_item(p, it, h, k, groups, n_parts, c1);
+      merge_two(a, b.M, b.L, b.O);
+    }
+    store_segment4(dst, h, it * 4 - h * HD, a.O, a.M, a.L);
+  }
+}
+
+// The same by all NT computing threads, a group of them for each of an item's
+// sums, joined in shared memory (`sh`, 6 floats per thread).
 template <int HD, int NT>
 __device__ void merge_parts_vec(const PagedAttnParams& p, const SegmentOut& dst, int heads,
                                 int c1, int n_parts, int tid, float* sh) {
-  const int items = heads * HD / 4, groups = min(4, NT / items);
+  const int items = heads * HD / 4, groups = merge_groups<HD, NT>(heads);
   if (groups < 2) {
-    for (int it = tid; it < items; it += NT) {
-      const int h = it * 4 / HD;
-      const Merged4 a = merge_item(p, it, h, 0, 1, n_parts, c1);
-      store_segment4(dst, h, it * 4 - h * HD, a.O, a.M, a.L);
-    }
+    merge_parts_items<HD, NT>(p, dst, heads, c1, n_parts, tid, NT);
     return;
   }
   const int grp = tid / items, it = tid - grp * items, h = it * 4 / HD;
@@ -898,17 +940,11 @@ __device__ void merge_parts_vec(const PagedAttnParams& p, const SegmentOut& dst,
     float* x = sh + ((grp - 1) * items + it) * 6;
     x[0] = a.O.x; x[1] = a.O.y; x[2] = a.O.z; x[3] = a.O.w; x[4] = a.M; x[5] = a.L;
   }
-  consumers_sync(NT);
+  named_sync(1, NT);
   if (grp != 0) return;
   for (int k = 1; k < groups; ++k) {
     const float* x = sh + ((k - 1) * items + it) * 6;
-    const float mb = fmaxf(a.M, x[4]), w0 = ex2(a.M - mb), w1 = ex2(x[4] - mb);
-    a.O.x = a.O.x * w0 + x[0] * w1;
-    a.O.y = a.O.y * w0 + x[1] * w1;
-    a.O.z = a.O.z * w0 + x[2] * w1;
-    a.O.w = a.O.w * w0 + x[3] * w1;
-    a.L = a.L * w0 + x[5] * w1;
-    a.M = mb;
+    merge_two(a, x[4], x[5], make_float4(x[0], x[1], x[2], x[3]));
   }
   store_segment4(dst, h, it * 4 - h * HD, a.O, a.M, a.L);
 }
@@ -943,10 +979,11 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
                                              ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
   uint64_t* empty = full + STAGES;
+  uint64_t *left_bar = empty + STAGES, *closed_bar = left_bar + 1;
   uint32_t* meta = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_META);
   float* mrg = reinterpret_cast<float*>(smem + Cfg::OFF_MRG);
   int* warp_tot = reinterpret_cast<int*>(smem + Cfg::OFF_MISC);
-  int* flag = warp_tot + WARPS + PWARPS + 4;
+  int *flag = warp_tot + Cfg::NWARPS + 4, *close_flag = flag + 4;
   int* prefix = reinterpret_cast<int*>(smem + Cfg::OFF_SCHED);
   int* past_s = prefix + p.n + 1;
   const int lane = threadIdx.x & 31;
@@ -956,6 +993,8 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
   griddep_launch_dependents();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * STAGES; ++i) mbar_init(&full[i], 1);   // full and empty
+    mbar_init(left_bar, WARPS);
+    mbar_init(closed_bar, max(1, Cfg::CWARPS));
     fence_mbar_init();
     tma_prefetch_desc(&tmk);
     tma_prefetch_desc(&tmv);
@@ -1051,10 +1090,11 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     __syncwarp();
   };
 
-  if (warp >= WARPS) {
+  if (warp >= WARPS && warp < WARPS + PWARPS) {
     // -------------------------------------------------------------- loading
     // Chunk n of this warp: chunk first + n % M of round n / M.
     constexpr int M = WARPS / PWARPS, L = M * DEPTH;
+    if constexpr (Cfg::CWARPS > 0) setmaxnreg_dec<104>();
     const int first = (warp - WARPS) * M;
     Entry e[L + 3];
     Box b[L + 2];
@@ -1103,7 +1143,95 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     return;
   }
 
+  // A CTA's range falls into segments, one per stream.
+  struct Segment {
+    int u, g, hb, heads;
+    int s_lo, s_hi, e_hi;   // the stream's chunks, the segment's end
+  };
+  auto segment = [&](int t) -> Segment {   // of chunk t of query s
+    while (prefix[s + 1] * streams <= t) ++s;
+    const int C = prefix[s + 1] - prefix[s], q_base = prefix[s] * streams;
+    Segment x;
+    x.u = (t - q_base) / C;
+    x.s_lo = q_base + x.u * C;
+    x.s_hi = x.s_lo + C;
+    x.e_hi = min(t_hi, x.s_hi);
+    x.g = x.u / p.hblocks;
+    x.hb = x.u - x.g * p.hblocks;
+    x.heads = min(kPagedHeads, p.group - x.hb * kPagedHeads);
+    return x;
+  };
+  // The computing warps' sums of a segment, joined by threads first, first +
+  // step, ... and stored as the stream's result or as a part of it.
+  auto join = [&](const Segment& x, int t, int first, int step) -> bool {
+    const bool complete = t == x.s_lo && x.e_hi == x.s_hi;
+    const SegmentOut dst = complete ? segment_out(p, s, x.g, x.hb)
+                                    : part_out(p, 2 * cta + (t == x.s_lo ? 1 : 0));
+    for (int e = first; e < x.heads * HD / 4; e += step) {
+      const int h = e * 4 / HD, d = e * 4 - h * HD;
+      float M = kNegBig;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w)
+        M = fmaxf(M, mrg[w * Cfg::MRG + kPagedHeads * Cfg::OSTRIDE + h]);
+      float L = 0.f;
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float* mw = mrg + w * Cfg::MRG;
+        const float f = ex2(mw[kPagedHeads * Cfg::OSTRIDE + h] - M);
+        const float4 v = *reinterpret_cast<const float4*>(mw + h * Cfg::OSTRIDE + d);
+        L = fmaf(mw[kPagedHeads * (Cfg::OSTRIDE + 1) + h], f, L);
+        O.x = fmaf(v.x, f, O.x);
+        O.y = fmaf(v.y, f, O.y);
+        O.z = fmaf(v.z, f, O.z);
+        O.w = fmaf(v.w, f, O.w);
+      }
+      store_segment4(dst, h, d, O, M, L);
+    }
+    return complete;
+  };
+  // One arrival at a split stream: whether it is the last (its count is then
+  // back at 0), the stream's first CTA and its number of parts.
+  auto arrive_last = [&](const Segment& x, int* to) {
+    const int c1 = cta_of_tile(x.s_lo, G, T_all);
+    const int parts = cta_of_tile(x.s_hi - 1, G, T_all) - c1 + 1;
+    unsigned* count = p.count + (size_t)s * streams + x.u;
+    to[0] = arrive_acq_rel(count) == (unsigned)(parts - 1);
+    to[1] = c1;
+    to[2] = parts;
+    if (to[0]) *count = 0;
+  };
+
+  if (Cfg::CWARPS > 0 && warp >= WARPS + PWARPS) {
+    // -------------------------------------------------------------- closing
+    // All segments but the last, while the others go on with the next.
+    setmaxnreg_dec<72>();
+    constexpr int NC = 32 * Cfg::CWARPS;
+    const int ct = threadIdx.x - 32 * (WARPS + PWARPS);
+    uint32_t ph = 0;
+    for (int t = t_lo; t < t_hi; ph ^= 1u) {
+      const Segment x = segment(t);
+      if (x.e_hi >= t_hi) break;
+      mbar_wait(left_bar, ph, p.err, kDevErrWaitFull);
+      __syncwarp();
+      const bool complete = join(x, t, ct, NC);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(closed_bar);
+      if (!complete) {
+        named_sync(2, NC);
+        if (ct == 0) arrive_last(x, close_flag);
+        named_sync(2, NC);
+        if (close_flag[0])
+          merge_parts_items<HD, NCT>(p, segment_out(p, s, x.g, x.hb), x.heads, close_flag[1],
+                                     close_flag[2], ct, NC);
+      }
+      t = x.e_hi;
+    }
+    return;
+  }
+
   // ---------------------------------------------------------------- computing
+  if constexpr (Cfg::CWARPS > 0) setmaxnreg_inc<168>();
   const int r = lane >> 2, qd = lane & 3;
   float* my_mrg = mrg + warp * Cfg::MRG;
   const float sl2 = p.scale_log2;
@@ -1137,14 +1265,10 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
   uint32_t qa[kHalf ? HD / 16 : HD / 8][4];
   uint32_t q3[HD / 16][2];   // bf16: the third parts
   float o[Cfg::OT][4];   // bf16: (16 of head_dim) x (8 heads), else (8 heads, hi and lo) x (8)
+  uint32_t closed_ph = 1;   // of the segment before: none
   for (int t = t_lo; t < t_hi;) {
-    while (prefix[s + 1] * streams <= t) ++s;
-    const int C = prefix[s + 1] - prefix[s];
-    const int q_base = prefix[s] * streams;
-    const int u = (t - q_base) / C;
-    const int s_lo = q_base + u * C, s_hi = s_lo + C, e_hi = min(t_hi, s_hi);
-    const int g = u / p.hblocks, hb = u - g * p.hblocks;
-    const int heads = min(kPagedHeads, p.group - hb * kPagedHeads);
+    const Segment x = segment(t);
+    const int e_hi = x.e_hi;
     // This segment's q was loaded before; the next one's is on its way.
 #pragma unroll
     for (int kk = 0; kk < HD / (kHalf ? 16 : 8); ++kk)
@@ -1158,8 +1282,8 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
         }
       }
     if (e_hi < t_hi) {
-      int sn = s, un = u;
-      if (e_hi == s_hi && ++un == streams) {
+      int sn = s, un = x.u;
+      if (e_hi == x.s_hi && ++un == streams) {
         un = 0;
         do ++sn; while (prefix[sn + 1] == prefix[sn]);
       }
@@ -1344,12 +1468,15 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     // ---------------------------------------------------------- segment end
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
     l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
+    const bool handed = Cfg::CWARPS > 0 && e_hi < t_hi;   // to the closing warps
+    if (Cfg::CWARPS > 0 && t > t_lo) mbar_wait(closed_bar, closed_ph, p.err, kDevErrWaitEmpty);
+    closed_ph ^= 1u;
 #pragma unroll
     for (int c = 0; c < Cfg::OT; ++c) {
       if constexpr (kHalf) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          my_mrg[(2 * qd + (x & 1)) * Cfg::OSTRIDE + 16 * c + 8 * (x >> 1) + r] = o[c][x];
+        for (int e = 0; e < 4; ++e)
+          my_mrg[(2 * qd + (e & 1)) * Cfg::OSTRIDE + 16 * c + 8 * (e >> 1) + r] = o[c][e];
       } else {
         *reinterpret_cast<float2*>(my_mrg + r * Cfg::OSTRIDE + 8 * c + 2 * qd) =
             make_float2(o[c][0] + o[c][2], o[c][1] + o[c][3]);
@@ -1359,43 +1486,22 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
       my_mrg[kPagedHeads * Cfg::OSTRIDE + r] = m_run;
       my_mrg[kPagedHeads * (Cfg::OSTRIDE + 1) + r] = l_run;
     }
-    consumers_sync(NCT);
-    const bool complete = t == s_lo && e_hi == s_hi;
-    const SegmentOut fin = segment_out(p, s, g, hb);
-    const SegmentOut dst = complete ? fin : part_out(p, 2 * cta + (t == s_lo ? 1 : 0));
-    for (int e = threadIdx.x; e < heads * HD / 4; e += NCT) {
-      const int h = e * 4 / HD, d = e * 4 - h * HD;
-      float M = kNegBig;
-#pragma unroll
-      for (int w = 0; w < Cfg::WARPS; ++w)
-        M = fmaxf(M, mrg[w * Cfg::MRG + kPagedHeads * Cfg::OSTRIDE + h]);
-      float L = 0.f;
-      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < Cfg::WARPS; ++w) {
-        const float* mw = mrg + w * Cfg::MRG;
-        const float f = ex2(mw[kPagedHeads * Cfg::OSTRIDE + h] - M);
-        const float4 x = *reinterpret_cast<const float4*>(mw + h * Cfg::OSTRIDE + d);
-        L = fmaf(mw[kPagedHeads * (Cfg::OSTRIDE + 1) + h], f, L);
-        O.x = fmaf(x.x, f, O.x);
-        O.y = fmaf(x.y, f, O.y);
-        O.z = fmaf(x.z, f, O.z);
-        O.w = fmaf(x.w, f, O.w);
+    if (handed) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(left_bar);
+    } else {
+      // The last one: nothing is left to go on with, so all warps close it.
+      named_sync(1, NCT);
+      if (!join(x, t, threadIdx.x, NCT)) {
+        named_sync(1, NCT);
+        if (threadIdx.x == 0) arrive_last(x, flag);
+        named_sync(1, NCT);
+        if (flag[0])
+          merge_parts_vec<HD, NCT>(p, segment_out(p, s, x.g, x.hb), x.heads, flag[1], flag[2],
+                                   threadIdx.x, mrg);
       }
-      store_segment4(dst, h, d, O, M, L);
+      if constexpr (Cfg::CWARPS == 0) named_sync(1, NCT);
     }
-    if (!complete) {
-      const int c1 = cta_of_tile(s_lo, G, T_all), c2 = cta_of_tile(s_hi - 1, G, T_all);
-      unsigned* count = p.count + (size_t)s * streams + u;
-      consumers_sync(NCT);
-      if (threadIdx.x == 0) *flag = arrive_acq_rel(count) == (unsigned)(c2 - c1);
-      consumers_sync(NCT);
-      if (*flag) {
-        merge_parts_vec<HD, NCT>(p, fin, heads, c1, c2 - c1 + 1, threadIdx.x, mrg);
-        if (threadIdx.x == 0) *count = 0;
-      }
-    }
-    consumers_sync(NCT);
     t = e_hi;
   }
 }
