@@ -270,15 +270,16 @@ __device__ __forceinline__ int query_blocks(const PagedAttnParams& p, int past, 
   return nb;
 }
 
+// (Positions fit 31 bits, so 32 do for rows below.)
 // First table entry of a query's list: those before it are attended elsewhere
 // by the queries that attend all of them.
 __device__ __forceinline__ int query_skip(const PagedAttnParams& p, int past) {
-  return ((long long)past + 1) >= ((long long)p.skip << p.log2p) ? p.skip : 0;
+  return (unsigned)past + 1u >= (unsigned)p.skip << p.log2p ? p.skip : 0;
 }
 
 __device__ __forceinline__ int query_chunks(const PagedAttnParams& p, int past, int nb) {
   const int list = p.sel ? min(p.n_sel, nb) : nb - min(nb, query_skip(p, past));
-  return (int)((((long long)list << p.log2p) + (1 << p.lchunk) - 1) >> p.lchunk);
+  return (int)((((unsigned)list << p.log2p) + (1u << p.lchunk) - 1u) >> p.lchunk);
 }
 
 // CTAs that share the T chunks out: enough that each has a chunk for each of
@@ -311,22 +312,25 @@ struct PagedRange {
 
 // The schedule of a launch, in shared memory: prefix[s], the chunks of one
 // stream of each query before s, and the queries' last positions (past_s).
-// Every thread of the CTA takes part, and the thread that has a query checks
-// whether this CTA's range begins or ends in it.  warp_tot: an int per warp
-// and 4 more.
+// Every warp forms all of it, the same words as the others, and reads what it
+// wrote itself: with the queries dealt out to the CTA's threads, the barriers
+// that this took cost more than the work.
 __device__ PagedRange paged_schedule(const PagedAttnParams& p, int* prefix, int* past_s,
-                                     int* warp_tot, int streams, int warps) {
-  const int NT = blockDim.x, t = threadIdx.x, lane = t & 31, w = t >> 5, nw = NT >> 5;
-  int* found = warp_tot + nw;   // lo, hi, the query of lo
-  const int per = (p.n + NT - 1) / NT;
-  const int b0 = min(t * per, p.n), b1 = min(b0 + per, p.n);
+                                     int streams, int warps) {
+  const int lane = threadIdx.x & 31;
+  const bool report = blockIdx.x == 0 && threadIdx.x < 32;
+  const int per = (p.n + 31) / 32;
+  const int b0 = min(lane * per, p.n), b1 = min(b0 + per, p.n);
   int sum = 0;
+  unsigned least = 0x7fffffffu, most = 0;
+#pragma unroll 4
   for (int s = b0; s < b1; ++s) {
     const int past = p.past[s];
-    const int nb = query_blocks(p, past, blockIdx.x == 0);
+    const int nb = query_blocks(p, past, report);
     past_s[s] = nb > 0 ? past : -1;
     const int c = query_chunks(p, past, nb);
-    prefix[s + 1] = c;
+    least = min(least, (unsigned)c);
+    most = max(most, (unsigned)c);
     sum += c;
   }
   int incl = sum;
@@ -335,25 +339,9 @@ __device__ PagedRange paged_schedule(const PagedAttnParams& p, int* prefix, int*
     const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) warp_tot[w] = incl;
-  if (t == 0) {
-    prefix[0] = 0;
-    found[0] = found[2] = 0;
-    found[1] = -1;
-  }
-  __syncthreads();
-  int off = 0, all = 0;
-#pragma unroll 4
-  for (int i = 0; i < nw; ++i) {
-    const int x = warp_tot[i];
-    off += i < w ? x : 0;
-    all += x;
-  }
   PagedRange r;
-  r.T = all * streams;
-  bool same = true;
-  for (int s = b0; s < b1; ++s) same = same && prefix[s + 1] == prefix[1];
-  const bool uniform = __syncthreads_and(same) != 0;
+  r.T = __shfl_sync(0xffffffffu, incl, 31) * streams;
+  const bool uniform = __reduce_min_sync(0xffffffffu, least) == __reduce_max_sync(0xffffffffu, most);
   r.G = paged_active(gridDim.x, r.T, warps, p.n * streams, uniform);
   const int c = blockIdx.x;
   // floor(c T / G) and floor((c + 1) T / G) without 64 bits.
@@ -363,29 +351,39 @@ __device__ PagedRange paged_schedule(const PagedAttnParams& p, int* prefix, int*
     lo = c * q + a;
     hi = lo + q + (c * rem - a * r.G + rem >= r.G);
   }
-  int run = off + incl - sum;
+  int run = incl - sum;
+  if (lane == 0) prefix[0] = 0;
+#pragma unroll 4
   for (int s = b0; s < b1; ++s) {
-    const int C = prefix[s + 1], base = run * streams;
-    run += C;
+    const int past = past_s[s];
+    if (past >= 0) run += query_chunks(p, past, (past >> p.log2p) + 1);
     prefix[s + 1] = run;
+  }
+  __syncwarp();
+  // The lane in whose queries the range begins or ends looks for the place.
+  int at_lo = 0, at_hi = 0, s_lo = 0;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int at = k ? hi : lo;
-      if (at < base || at >= base + C * streams || at == 0) continue;
-      int cut = at;
-      if (C <= kWholeRounds * warps) {
-        const int in = (at - base) % C;
-        cut = 2 * in < C ? at - in : at + (C - in);
-      }
-      found[k] = cut;
-      if (k == 0) found[2] = s;
+  for (int k = 0; k < 2; ++k) {
+    const int at = k ? hi : lo;
+    if (at == 0 || at < (incl - sum) * streams || at >= incl * streams) continue;
+    int s = b0;
+    while (prefix[s + 1] * streams <= at) ++s;
+    const int C = prefix[s + 1] - prefix[s], in = (at - prefix[s] * streams) % C;
+    int cut = at;
+    if (C <= kWholeRounds * warps) cut = 2 * in < C ? at - in : at + (C - in);
+    if (k) {
+      at_hi = cut + 1;
+    } else {
+      at_lo = cut;
+      s_lo = s;
     }
   }
-  __syncthreads();
-  r.lo = found[0];
-  r.hi = found[1] < 0 ? r.T : found[1];   // the last range ends with the last chunk
-  r.s = found[2];
+  r.lo = (int)__reduce_max_sync(0xffffffffu, (unsigned)at_lo);
+  const int h = (int)__reduce_max_sync(0xffffffffu, (unsigned)at_hi);
+  r.hi = h == 0 ? r.T : h - 1;   // the last range ends with the last chunk
+  r.s = (int)__reduce_max_sync(0xffffffffu, (unsigned)s_lo);
   if (c >= r.G) r.lo = r.hi = 0;
+  __syncwarp();
   return r;
 }
 
@@ -527,7 +525,7 @@ size_t paged_core_smem(int n, int hd) {
   const size_t floats = (size_t)kPagedHeads * hd                          // q
                         + (size_t)kCoreWarps * kPagedHeads * kPagedChunk    // probabilities
                         + (size_t)kCoreWarps * kPagedHeads * (hd + 2);      // warp results
-  return floats * 4 + (size_t)(2 * n + 1 + kCoreWarps + 4 + 4) * 4;
+  return floats * 4 + (size_t)(2 * n + 1 + 4) * 4;
 }
 
 template <typename T>
@@ -552,14 +550,13 @@ __global__ void __launch_bounds__(kCoreThreads) paged_core_kernel(const PagedAtt
   float* res = sm + kPagedHeads * hd + kCoreWarps * kPagedHeads * kPagedChunk;
   int* prefix = reinterpret_cast<int*>(res + kCoreWarps * kPagedHeads * (hd + 2));
   int* past_s = prefix + p.n + 1;
-  int* warp_tot = past_s + p.n;
-  int* flag = warp_tot + kCoreWarps + 4;
+  int* flag = past_s + p.n;
   float* my_res = res + warp * kPagedHeads * (hd + 2);
 
   griddep_launch_dependents();
   griddep_wait();
   const int streams = p.n_kv * p.hblocks, cta = blockIdx.x;
-  const PagedRange range = paged_schedule(p, prefix, past_s, warp_tot, streams, kCoreWarps);
+  const PagedRange range = paged_schedule(p, prefix, past_s, streams, kCoreWarps);
   write_empty(p, prefix);
   const int T_all = range.T, G = range.G, t_lo = range.lo, t_hi = range.hi;
   if (t_lo >= t_hi) return;
@@ -821,7 +818,7 @@ struct MmaPaged {
   static constexpr int OFF_META = OFF_BAR + (2 * STAGES + 2) * 8;
   static constexpr int OFF_MRG = (OFF_META + STAGES * 4 + 15) & ~15;
   static constexpr int OFF_MISC = OFF_MRG + WARPS * MRG * 4;
-  static constexpr int OFF_SCHED = OFF_MISC + (NWARPS + 12) * 4;
+  static constexpr int OFF_SCHED = OFF_MISC + 8 * 4;
   static constexpr size_t smem_bytes(int n) { return 1024 + (size_t)OFF_SCHED + (size_t)(2 * n + 1) * 4; }
   // Byte of 16-byte piece `piece` of row `row` in a column block, under the
   // boxes' swizzle (RB bytes: 128, or 64 with half as many pieces to turn).
@@ -982,8 +979,7 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
   uint64_t *left_bar = empty + STAGES, *closed_bar = left_bar + 1;
   uint32_t* meta = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_META);
   float* mrg = reinterpret_cast<float*>(smem + Cfg::OFF_MRG);
-  int* warp_tot = reinterpret_cast<int*>(smem + Cfg::OFF_MISC);
-  int *flag = warp_tot + Cfg::NWARPS + 4, *close_flag = flag + 4;
+  int *flag = reinterpret_cast<int*>(smem + Cfg::OFF_MISC), *close_flag = flag + 4;
   int* prefix = reinterpret_cast<int*>(smem + Cfg::OFF_SCHED);
   int* past_s = prefix + p.n + 1;
   const int lane = threadIdx.x & 31;
@@ -999,9 +995,10 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     tma_prefetch_desc(&tmk);
     tma_prefetch_desc(&tmv);
   }
+  __syncthreads();
   griddep_wait();
   const int streams = p.n_kv * p.hblocks, cta = blockIdx.x;
-  const PagedRange range = paged_schedule(p, prefix, past_s, warp_tot, streams, WARPS);
+  const PagedRange range = paged_schedule(p, prefix, past_s, streams, WARPS);
   write_empty(p, prefix);
   const int T_all = range.T, G = range.G, t_lo = range.lo, t_hi = range.hi;
   if (t_lo >= t_hi) return;
