@@ -1395,63 +1395,83 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
           lsum += sc[nt][0] + sc[nt][1];
         }
         l_run = l_run * alpha + lsum;
-        if (__any_sync(0xffffffffu, alpha != 1.f)) {
-          float a0 = alpha, a1 = alpha;
-          if constexpr (kHalf) {   // of the heads of this lane's columns
-            a0 = __shfl_sync(0xffffffffu, alpha, 8 * qd);
-            a1 = __shfl_sync(0xffffffffu, alpha, 8 * qd + 4);
-          }
-#pragma unroll
-          for (int c = 0; c < Cfg::OT; ++c) {
-            o[c][0] *= a0; o[c][1] *= a1; o[c][2] *= a0; o[c][3] *= a1;
-          }
+        float a0 = alpha, a1 = alpha;
+        if constexpr (kHalf) {   // of the heads of this lane's columns
+          a0 = __shfl_sync(0xffffffffu, alpha, 8 * qd);
+          a1 = __shfl_sync(0xffffffffu, alpha, 8 * qd + 4);
         }
-        // O += P . V.
+        // O = alpha O + P . V, the chunk's product formed by itself: the
+        // tensor cores truncate what they add to an accumulator, and over a
+        // long stream that added up to 3e-6 of the result.
+        auto add_to_o = [&](float(&o)[4], const float(&d)[4]) {
+          o[0] = fmaf(o[0], a0, d[0]);
+          o[1] = fmaf(o[1], a1, d[1]);
+          o[2] = fmaf(o[2], a0, d[2]);
+          o[3] = fmaf(o[3], a1, d[3]);
+        };
         if constexpr (kHalf) {
+          // A lane's scores (one head, two rows of K) are the B operand of
+          // O^T += V^T . P^T as they stand.
+          constexpr int NK = CH / 16;
+          uint32_t p1[NK][2], p2[NK][2], p3[NK][2];
 #pragma unroll
-          for (int kp = 0; kp < CH / 16; ++kp) {
-            // A lane's scores (one head, two rows of K) are the B operand of
-            // O^T += V^T . P^T as they stand.
-            uint32_t ph0, ph1, pl0, pl1, p30, p31;
-            split3_pair(sc[2 * kp][0], sc[2 * kp][1], ph0, pl0, p30);
-            split3_pair(sc[2 * kp + 1][0], sc[2 * kp + 1][1], ph1, pl1, p31);
-            const int row = 16 * kp + ((lane >> 3) & 1) * 8 + (lane & 7);
+          for (int kp = 0; kp < NK; ++kp)
 #pragma unroll
-            for (int x = 0; x < NX; ++x) {
-              constexpr int NC = Cfg::RB / 32;   // 16-column tiles of a block
+            for (int e = 0; e < 2; ++e)
+              split3_pair(sc[2 * kp + e][0], sc[2 * kp + e][1], p1[kp][e], p2[kp][e], p3[kp][e]);
+#pragma unroll
+          for (int x = 0; x < NX; ++x) {
+            constexpr int NC = Cfg::RB / 32;   // 16-column tiles of a block
+            float d[NC][4];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) d[c][0] = d[c][1] = d[c][2] = d[c][3] = 0.f;
+#pragma unroll
+            for (int kp = 0; kp < NK; ++kp) {
+              const int row = 16 * kp + ((lane >> 3) & 1) * 8 + (lane & 7);
               uint32_t v[NC][4];
 #pragma unroll
               for (int c = 0; c < NC; ++c)
                 ldmatrix_x4_trans(vb + x * (CH * Cfg::RB) + Cfg::at(row, 2 * c + (lane >> 4)),
                                   v[c][0], v[c][2], v[c][1], v[c][3]);
 #pragma unroll
-              for (int c = 0; c < NC; ++c) mma_bf16_16816(o[NC * x + c], v[c], ph0, ph1);
+              for (int c = 0; c < NC; ++c) mma_bf16_16816(d[c], v[c], p1[kp][0], p1[kp][1]);
 #pragma unroll
-              for (int c = 0; c < NC; ++c) mma_bf16_16816(o[NC * x + c], v[c], pl0, pl1);
+              for (int c = 0; c < NC; ++c) mma_bf16_16816(d[c], v[c], p2[kp][0], p2[kp][1]);
 #pragma unroll
-              for (int c = 0; c < NC; ++c) mma_bf16_16816(o[NC * x + c], v[c], p30, p31);
+              for (int c = 0; c < NC; ++c) mma_bf16_16816(d[c], v[c], p3[kp][0], p3[kp][1]);
             }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) add_to_o(o[NC * x + c], d[c]);
           }
         } else {
           // Rows 2 qd and 2 qd + 1 of a block are the operand's k = qd and
           // k = qd + 4, so the scores are its layout already (the order of
           // the rows in a sum is free), and no two lanes share a bank.
+          uint32_t pa[NT][4];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            uint32_t pa[4];
-            split_tf32(sc[nt][0], pa[0], pa[1]);
-            split_tf32(sc[nt][1], pa[2], pa[3]);
-            const int row = 8 * nt + 2 * qd;
+            split_tf32(sc[nt][0], pa[nt][0], pa[nt][1]);
+            split_tf32(sc[nt][1], pa[nt][2], pa[nt][3]);
+          }
 #pragma unroll
-            for (int c = 0; c < HD / 8; ++c) {
-              const uint8_t* a = vbox + (c >> 2) * (CH * 128) + (r & 3) * 4;
-              const int chunk = 2 * (c & 3) + (r >> 2);
-              uint32_t h0, l0, h1, l1;
-              split_tf32(*reinterpret_cast<const float*>(a + Cfg::at(row, chunk)), h0, l0);
-              split_tf32(*reinterpret_cast<const float*>(a + Cfg::at(row + 1, chunk)), h1, l1);
-              mma_tf32_1688(o[c], pa, h0, h1);
-              mma_tf32_1688(o[c], pa, l0, l1);
-            }
+          for (int x = 0; x < NX; ++x) {
+            float d[4][4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) d[c][0] = d[c][1] = d[c][2] = d[c][3] = 0.f;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const int row = 8 * nt + 2 * qd, chunk = 2 * c + (r >> 2);
+                const uint8_t* a = vbox + x * (CH * 128) + (r & 3) * 4;
+                uint32_t h0, l0, h1, l1;
+                split_tf32(*reinterpret_cast<const float*>(a + Cfg::at(row, chunk)), h0, l0);
+                split_tf32(*reinterpret_cast<const float*>(a + Cfg::at(row + 1, chunk)), h1, l1);
+                mma_tf32_1688(d[c], pa[nt], h0, h1);
+                mma_tf32_1688(d[c], pa[nt], l0, l1);
+              }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) add_to_o(o[4 * x + c], d[c]);
           }
         }
       }

@@ -30,9 +30,11 @@ namespace tg {
 constexpr int PX_ROWS = 128;        // query rows of a slot (TMEM lanes)
 constexpr int PX_KEYS = 64;         // keys of a step
 constexpr int PX_STAGES = 8;        // K/V ring
+constexpr int PX_FLUSH = 16;        // steps that O gathers in TMEM
 constexpr int PX_THREADS = 384;     // TMA warp, 2 MMA warps, an idle one, 2 x 4 softmax warps
 constexpr int PX_TILE = PX_KEYS * 128;           // bytes of a K (or V) tile
-constexpr int PX_OFF_Q = PX_STAGES * 2 * PX_TILE;   // 8 KB per softmax warp: q on its way to TMEM
+constexpr int PX_OFF_Q = PX_STAGES * 2 * PX_TILE;   // 8 KB per softmax warp: q on its way to
+                                                    // TMEM, then what O has gathered
 constexpr int PX_OFF_BAR = PX_OFF_Q + 8 * 32 * 64 * 4;
 // kv_full[S], kv_empty[S], q_full[slot], s_full[slot][buf], p_full[slot][buf],
 // pv_done[slot], drained[slot]
@@ -260,7 +262,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
       tc_fence_after();
       // 4 steps of 16 keys (2048 bytes), the high parts and the low ones.
       umma_f16_ts_x8<128>(base + px_o(0), base + px_s(0, j & 1),
-                          dv0 + (uint64_t)(pv.st * (2 * PX_TILE >> 4)), IDESC_PV, j > 0 ? 1u : 0u);
+                          dv0 + (uint64_t)(pv.st * (2 * PX_TILE >> 4)), IDESC_PV,
+                          j % PX_FLUSH != 0 ? 1u : 0u);
       umma_commit_elect(&kv_empty[pv.st]);
       pv.step(by);
       // Products of one thread complete in their order: s_full of step j + 2
@@ -321,7 +324,14 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
     }
     constexpr float kLazy = 8.f;
     float m = kNegBig, l = 0.f;
-    bool ok = true;
+    // The tensor cores truncate what they add to an accumulator: with O in
+    // TMEM for all of 28 steps the result was off by 5.5e-6.  So every
+    // PX_FLUSH steps it goes to shared memory (piece c of a row at c * 32 +
+    // lane), in units of 2^m_acc, and begins again; a step that does so takes
+    // about 900 cycles longer.
+    float4* acc = reinterpret_cast<float4*>(smem + PX_OFF_Q) + (warp - 4) * 16 * 32 + lane;
+    float m_acc = kNegBig;
+    bool gathered = false, ok = true;
     for (int j = 0; j < steps; ++j) {
       const int b = j & 1;
       if (!px_wait_warp(&s_full[2 * x + b], (uint32_t)((j >> 1) & 1), p.err, abort_flag)) {
@@ -345,7 +355,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         alpha = ex2(m - mx);
         m = mx;
       }
-      if (__any_sync(0xffffffffu, alpha != 1.f)) {
+      const bool flush = j > 0 && j % PX_FLUSH == 0;
+      if (flush || __any_sync(0xffffffffu, alpha != 1.f)) {
         // O of the steps before this one is complete once S of the next step
         // is (or, in the last step, the product before it), and the next
         // product on O waits for this step's P.
@@ -362,7 +373,27 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
           TG_TMEM_LD32(base + px_o(x) + c0, ov);
 #pragma unroll
           for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
-          TG_TMEM_ST32(base + px_o(x) + c0, ov);
+          if (!flush) {
+            TG_TMEM_ST32(base + px_o(x) + c0, ov);
+          } else {
+            const float f = ex2(m_acc - m);
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              float4 v = make_float4(__uint_as_float(ov[c]), __uint_as_float(ov[c + 1]),
+                                     __uint_as_float(ov[c + 2]), __uint_as_float(ov[c + 3]));
+              float4* to = acc + ((c0 + c) >> 2) * 32;
+              if (gathered) {
+                const float4 a = *to;
+                v = make_float4(fmaf(a.x, f, v.x), fmaf(a.y, f, v.y), fmaf(a.z, f, v.z),
+                                fmaf(a.w, f, v.w));
+              }
+              *to = v;
+            }
+          }
+        }
+        if (flush) {
+          gathered = true;
+          m_acc = m;
         }
       }
       uint64_t ls[4] = {0, 0, 0, 0};   // pairs of zeros
@@ -399,6 +430,17 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
       tc_fence_after();
       TG_TMEM_LD64(base + px_o(x), ov);
       tc_fence_before();
+      if (gathered) {
+        const float f = ex2(m_acc - m);
+#pragma unroll
+        for (int c = 0; c < 64; c += 4) {
+          const float4 a = acc[(c >> 2) * 32];
+          ov[c] = __float_as_uint(fmaf(a.x, f, __uint_as_float(ov[c])));
+          ov[c + 1] = __float_as_uint(fmaf(a.y, f, __uint_as_float(ov[c + 1])));
+          ov[c + 2] = __float_as_uint(fmaf(a.z, f, __uint_as_float(ov[c + 2])));
+          ov[c + 3] = __float_as_uint(fmaf(a.w, f, __uint_as_float(ov[c + 3])));
+        }
+      }
     } else {
 #pragma unroll
       for (int c = 0; c < 64; ++c) ov[c] = 0u;
