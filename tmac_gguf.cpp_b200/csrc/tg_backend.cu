@@ -19,7 +19,9 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <map>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -1571,6 +1573,17 @@ int check_host_pos(const int32_t* pos, int n, int limit, const char* what) {
 
 // ------------------------------------------------ paged KV caches
 
+// Room for one more element, so that push_back cannot throw through the C ABI.
+template <typename V>
+bool make_room(V& v) {
+  try {
+    v.reserve(v.size() + 1);
+  } catch (const std::exception&) {
+    return false;
+  }
+  return true;
+}
+
 // As ensure_buf, for buffers that captured graphs may name: the old one is
 // kept until shutdown.  zero: the new one is zeroed on the stream.
 template <typename T>
@@ -1581,6 +1594,7 @@ int ensure_kept(tg_context* ctx, T** buf, size_t* cap, size_t need, bool zero = 
                 "scratch must be sized before graph capture: run the same call once first");
   size_t n = need < 1024 ? 1024 : need;
   n = n + n / 2;
+  if (!make_room(ctx->kept)) return fail(TG_ERR_OUT_OF_MEMORY, "host memory");
   T* nb = nullptr;
   TG_CUDA(cudaMalloc(&nb, n * sizeof(T)));
   if (zero) {
@@ -3035,16 +3049,18 @@ int tg_paged_create(tg_context* ctx, const tg_paged_desc* desc, tg_paged_kv** ou
   if (!d.k != !d.v) return fail(TG_ERR_INVALID_ARG, "paged_create: k and v, both or neither");
   if (d.bounds && !d.with_bounds)
     return fail(TG_ERR_INVALID_ARG, "paged_create: bounds without with_bounds");
-  for (const void* m : {d.k, d.v, d.bounds}) {
-    if (!m) continue;
-    if (!is_device_ptr(m)) return fail(TG_ERR_INVALID_ARG, "paged_create: pools are device memory");
-    if (reinterpret_cast<uintptr_t>(m) & 15)
+  PagedArg pools[3] = {{d.k, "k"}, {d.v, "v"}, {d.bounds, "bounds"}};
+  bool all_device = false;
+  TG_TRY(classify_args(ctx, pools, 3, &all_device));
+  if (!all_device) return fail(TG_ERR_INVALID_ARG, "paged_create: pools are device memory");
+  for (const PagedArg& m : pools)
+    if (reinterpret_cast<uintptr_t>(m.p) & 15)
       return fail(TG_ERR_INVALID_ARG, "paged_create: pools must be 16-byte aligned");
-  }
   if (ctx->capturing) return fail(TG_ERR_STATE, "paged_create inside a graph capture");
   RopeTable* t = nullptr;
   TG_TRY(get_table(ctx, d.rope_base, d.head_dim, d.max_pos, &t));
-  tg_paged_kv* pk = new tg_paged_kv();
+  tg_paged_kv* pk = make_room(ctx->paged) ? new (std::nothrow) tg_paged_kv() : nullptr;
+  if (!pk) return fail(TG_ERR_OUT_OF_MEMORY, "host memory");
   pk->ctx = ctx;
   pk->d = d;
   while ((1 << pk->log2p) < d.page_size) ++pk->log2p;
