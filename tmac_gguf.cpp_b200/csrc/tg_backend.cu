@@ -1685,9 +1685,11 @@ int check_host_pages(const tg_paged_kv* pk, const int32_t* past, const int32_t* 
 // Whether the tensor-core kernel takes a shared prefix (see run_paged).  It
 // costs two launches more and about 20 us in all; without it every query
 // reads the prefix for itself, mostly from L2.  Measured on a B200 (14 query /
-// 2 KV heads, us without / with): 64 x 2048 21 / 23, 64 x 4096 29 / 24,
-// 32 x 8192 29 / 25, 16 x 16384 29 / 29, 128 x 32768 275 / 54; with 8 / 4
-// heads 32 x 2048 21 / 23, 32 x 4096 29 / 24, 8 x 16384 28 / 24.
+// 2 KV heads, us without / with): 64 x 2048 20 / 25, 32 x 4096 20 / 23,
+// 16 x 8192 19 / 25; at the border 64 x 4096 30 / 25, 32 x 8192 29 / 25,
+// 16 x 16384 29 / 31, 8 x 32768 29 / 32; above it 32 x 16384 49 / 28,
+// 128 x 32768 326 / 57.  With 8 / 4 heads 32 x 2048 20 / 24, 32 x 4096 29 / 25,
+// 8 x 16384 29 / 25.
 bool use_prefix(int n, int n_kv, int shared_len) {
   return (long long)n * n_kv * shared_len >= (1LL << 19);
 }

@@ -283,25 +283,19 @@ __device__ __forceinline__ int query_chunks(const PagedAttnParams& p, int past, 
 }
 
 // CTAs that share the T chunks out: enough that each has a chunk for each of
-// its warps, and in any case some for every stream.  Streams of one length get
-// the same number of CTAs each where that leaves few out: a CTA that ends one
-// split stream and begins another is the last to finish (4 x 131072 rows, 8
-// streams: 148 CTAs 51 us, 144 CTAs 45 us).
-__device__ __forceinline__ int paged_active(int grid, int T, int warps, int n_streams,
-                                            bool uniform) {
-  int g = min(min(grid, T), max((T + warps - 1) / warps, 3 * n_streams));
-  if (uniform && n_streams <= g) {
-    const int even = g / n_streams * n_streams;
-    if (even * 20 >= g * 19) g = even;
-  }
-  return g;
+// its warps, and in any case some for every stream.
+__device__ __forceinline__ int paged_active(int grid, int T, int warps, int n_streams) {
+  return min(min(grid, T), max((T + warps - 1) / warps, 3 * n_streams));
 }
 
 // A CTA's range is an equal share of the T chunks, its ends moved to the
 // nearer end of the stream that they would cut if that stream is short
 // (kWholeRounds steps of all warps or less).  A cut costs its two CTAs a
 // record, an arrival and a merge, about 5000 cycles, as much as the chunks
-// that a moved range has too many.  A range may be empty.
+// that a moved range has too many.  A range may be empty.  Measured with 0, 2,
+// 4 and 8 rounds (us): 64 fp32 sequences of up to 256 rows 15.0, 10.7, 10.7,
+// 10.7; 64 queries over 64 listed pages of 16 rows 16.2, 16.2, 13.6, 13.6; a
+// batch of middling lengths 41.5, 41.5, 41.5, 45.1.
 constexpr int kWholeRounds = 4;
 
 struct PagedRange {
@@ -322,16 +316,12 @@ __device__ PagedRange paged_schedule(const PagedAttnParams& p, int* prefix, int*
   const int per = (p.n + 31) / 32;
   const int b0 = min(lane * per, p.n), b1 = min(b0 + per, p.n);
   int sum = 0;
-  unsigned least = 0x7fffffffu, most = 0;
 #pragma unroll 4
   for (int s = b0; s < b1; ++s) {
     const int past = p.past[s];
     const int nb = query_blocks(p, past, report);
     past_s[s] = nb > 0 ? past : -1;
-    const int c = query_chunks(p, past, nb);
-    least = min(least, (unsigned)c);
-    most = max(most, (unsigned)c);
-    sum += c;
+    sum += query_chunks(p, past, nb);
   }
   int incl = sum;
 #pragma unroll
@@ -341,8 +331,7 @@ __device__ PagedRange paged_schedule(const PagedAttnParams& p, int* prefix, int*
   }
   PagedRange r;
   r.T = __shfl_sync(0xffffffffu, incl, 31) * streams;
-  const bool uniform = __reduce_min_sync(0xffffffffu, least) == __reduce_max_sync(0xffffffffu, most);
-  r.G = paged_active(gridDim.x, r.T, warps, p.n * streams, uniform);
+  r.G = paged_active(gridDim.x, r.T, warps, p.n * streams);
   const int c = blockIdx.x;
   // floor(c T / G) and floor((c + 1) T / G) without 64 bits.
   int lo = 0, hi = 0;
@@ -946,22 +935,30 @@ __device__ void merge_parts_vec(const PagedAttnParams& p, const SegmentOut& dst,
   store_segment4(dst, h, it * 4 - h * HD, a.O, a.M, a.L);
 }
 
-// bf16 or fp32 pool, head_dim 32, 64 or 128.  Chunk k of the CTA's range is
-// computing warp k % WARPS's, and each such warp has DEPTH stages of its own
-// (a stage that changed hands could be two phases ahead of a waiting warp,
-// which a parity cannot tell), so the warps share nothing until a stream's
-// segment ends.  PWARPS warps fill the stages of WARPS / PWARPS computing
-// warps each by TMA (boxes of min(page, CH) rows, swizzled), with the
-// pages looked up two steps ahead.  One loading warp for all took 740 to 950
-// cycles per 8 KB chunk where the memory delivers one in 350; computing warps
-// that load for themselves spend 1000 cycles a chunk on it.
+// bf16 or fp32 pool, head_dim 32, 64 or 128; bound by HBM (a chunk's products
+// take 1800 cycles of a warp, eight warps; the memory delivers a chunk in 350).
+// Chunk k of the CTA's range is computing warp k % WARPS's, and each such warp
+// has DEPTH stages of its own (a stage that changed hands could be two phases
+// ahead of a waiting warp, which a parity cannot tell), so the warps share
+// nothing until a stream's segment ends.  PWARPS warps fill the stages of
+// WARPS / PWARPS computing warps each by TMA (boxes of min(page, CH) rows,
+// swizzled), with the pages looked up two steps ahead.  One loading warp for
+// all took 740 to 950 cycles per 8 KB chunk; computing warps that load for
+// themselves spend 1000 cycles a chunk on it.  CWARPS warps join a segment's
+// sums while the others are in the next one (256 x 4096 rows: 110 us without
+// them, 104 with, on one machine).
 //
 // Products are mma.sync: a step has at most 8 query rows, far below the 64 of
-// a tcgen05 tile.  The 8 spare rows of the 16-row operand carry the low part
-// of q (and of the probabilities).  Against exact bf16 rows x is three bf16,
-// all its 24 bits: hi and lo in one product, the third in a second one (two
-// alone left results 3e-6 from those in 64 bits where binary32 leaves 5e-7);
-// against fp32 rows x and the rows are two tf32 each, good to 2^-21.
+// a tcgen05 tile.  For S = q K^T the 8 spare rows of the 16-row operand carry
+// the low part of q.  Against exact bf16 rows x is three bf16, all its 24
+// bits (two alone left results 3e-6 from those in 64 bits where binary32
+// leaves 5e-7); against fp32 rows x and the rows are two tf32 each, good to
+// 2^-21.
+//
+// Measured, 14 / 2 heads of 64, bf16: 256 sequences x 4096 rows in pages of 16
+// 106 us, 5.1 TB/s; 4 x 131072 in pages of 64 53 us, 5.0 TB/s.  Of a CTA's
+// 207000 cycles in the first, 168000 are chunks at 6.2 TB/s, the rest the
+// start (7000) and the segments' ends.
 template <typename T, int HD>
 __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     paged_mma_kernel(const __grid_constant__ CUtensorMap tmk,
