@@ -498,7 +498,8 @@ TG_API int tg_attention_noalloc(void* cuda_stream, const float* q, const void* k
  * kernels, which access nothing outside the pool and report device error
  * 0x106 (the queries concerned have no result); 0x103 reports a position
  * outside the table or the rotation table, whose query counts as empty.
- * Several tokens
+ * Rows that a query does not attend may hold anything; a row with an infinity
+ * or NaN that it does attend makes its result infinite or NaN.  Several tokens
  * of one sequence in a call are several rows with the same entries.  A page
  * that tg_paged_append writes belongs to one sequence only.
  * Pointer and stream rules are those of the batched calls above; calls on

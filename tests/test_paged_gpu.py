@@ -234,6 +234,35 @@ def test_attention_split_streams(tg, backend, dtype, page):
     assert (p.out == again).all()
 
 
+@pytest.mark.parametrize("shape", [(12, 1, 32), (6, 3, 32), (9, 9, 32)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("page", [8, 32, 256])
+def test_attention_narrow_heads(tg, backend, shape, dtype, page):
+    """Rows of 64 and 128 bytes, groups of 1, 2 and 12 (two blocks of heads)."""
+    p = Pool(tg, backend, [1, 0, 700, 31, 2049, 257], shape, dtype, page, seed=page + 1)
+    p.cache.attention(0, p.q, p.past, p.table, p.out)
+    backend.synchronize()
+    p.check(p.out)
+    p.cache.destroy()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attention_many_ragged_in_place(tg, backend, dtype):
+    """Several streams of a CTA one after the other, empty ones between them,
+    and the result written over the queries."""
+    rng = np.random.default_rng(9)
+    lens = rng.integers(1, 700, 333)
+    lens[rng.integers(0, 333, 120)] = 0
+    p = Pool(tg, backend, [int(x) for x in lens], (14, 2, 64), dtype, 16, seed=10)
+    out = p.q.clone()
+    p.cache.attention(0, p.q, p.past, p.table, p.out)
+    p.cache.attention(0, out, p.past, p.table, out)
+    backend.synchronize()
+    assert (out == p.out).all()
+    p.check(p.out, seqs=range(0, 333, 4))
+    p.cache.destroy()
+
+
 def test_attention_single_long_sequence(tg, backend):
     p = Pool(tg, backend, [100003], (14, 2, 64), "bf16", 64, seed=4)
     p.cache.attention(0, p.q, p.past, p.table, p.out)
