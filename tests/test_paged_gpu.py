@@ -364,6 +364,43 @@ def test_attention_shared_batches(tg, backend, n, shared, page, shape):
     assert (p.out == again).all()
 
 
+@pytest.mark.parametrize("n,shared,page,shape,dtype", [
+    (37, 4100, 16, (8, 8, 32), "bf16"), (19, 9000, 8, (12, 4, 64), "f32"),
+    (10, 30011, 64, (4, 1, 128), "bf16"), (100, 2000, 16, (6, 3, 32), "f32"),
+    (3, 40000, 256, (3, 3, 64), "f32"), (1100, 210, 16, (8, 8, 32), "bf16")])
+def test_attention_shared_small_groups(tg, backend, n, shared, page, shape, dtype):
+    """Rows of several queries over the prefix together: whole and ragged
+    blocks of eight, one block, more queries than one launch takes."""
+    rng = np.random.default_rng(n + 1)
+    sh = shared // page * page
+    lens = [sh + int(x) for x in rng.integers(0, 90, n)]
+    lens[n // 2] = 0
+    lens[n // 3] = sh - 5 if n > 3 else lens[n // 3]
+    p = Pool(tg, backend, lens, shape, dtype, page, seed=n, shared=shared, scale=1.5)
+    p.cache.attention_shared(0, p.q, p.past, p.table, shared, p.out)
+    again = p.out.clone()
+    p.cache.attention_shared(0, p.q, p.past, p.table, shared, again)
+    backend.synchronize()
+    p.check(p.out, seqs=sorted(set(rng.choice(n, min(n, 12), replace=False)) | {n // 2, n // 3, n - 1}))
+    assert (p.out == again).all()
+
+
+@pytest.mark.parametrize("shape", [(14, 2, 64), (8, 8, 32)])
+def test_shared_position_outside_the_table(tg, backend, shape):
+    """Counts as empty, also where the prefix is attended by itself."""
+    rng = np.random.default_rng(4)
+    p = Pool(tg, backend, [6000 + int(x) for x in rng.integers(0, 40, 50)], shape, "bf16", 16,
+             seed=6, shared=6000)
+    past = p.past.clone()
+    past[7] = 10 ** 6
+    p.cache.attention_shared(0, p.q, past, p.table, 6000, p.out)
+    with pytest.raises(tg.TGError) as e:
+        backend.synchronize()
+    assert e.value.status == tg.TG_ERR_DEVICE and "0x103" in e.value.message
+    assert not p.out[7].any()
+    p.check(p.out, seqs=[0, 6, 8, 49])
+
+
 def test_shared_equals_plain(tg, backend):
     import torch
     p = Pool(tg, backend, [2100, 2048, 3000, 2047], (14, 2, 64), "bf16", 16, seed=2, shared=2048)

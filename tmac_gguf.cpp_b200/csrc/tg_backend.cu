@@ -1694,6 +1694,22 @@ bool use_prefix(int n, int n_kv, int shared_len) {
   return (long long)n * n_kv * shared_len >= (1LL << 19);
 }
 
+// Whether, where that kernel does not serve the shape, eight rows (query,
+// head) of a KV head go over the prefix together in the place of one query's
+// heads.  That takes two launches more, about 9 us, and (8 - group) / 8 of the
+// prefix's reads (from L2) away: worth it from 48 MB on.  Measured (heads, us
+// without / with): 8 / 8 of 32, bf16, 64 x 512 rows 20 / 27, 32 x 2048 28 / 26,
+// 8 x 8192 26 / 21, 64 x 32768 588 / 99; 12 / 4 of 64, fp32, 64 x 512 25 / 32,
+// 32 x 2048 35 / 34, 64 x 32768 742 / 302; 4 / 1 of 128, bf16, 64 x 2048
+// 28 / 33, 8 x 32768 44 / 44, 64 x 32768 263 / 149.
+bool use_packed(const tg_paged_kv* pk, int n, int shared_len) {
+  const int group = pk->d.n_head / pk->d.n_kv_head;
+  const long long bytes =
+      (long long)n * shared_len * pk->d.n_kv_head * pk->d.head_dim * 2 * (int)pk->esize;
+  return pk->tmap_ok && group < tg::kPagedHeads &&
+         bytes / tg::kPagedHeads * (tg::kPagedHeads - group) >= (48LL << 20);
+}
+
 // Attention launches on device pointers, kPagedMaxQueries queries at a time.
 int run_paged(tg_context* ctx, const tg_paged_kv* pk, int layer, int n, const float* q,
               const int* past, const int* table, int max_blocks, const int* sel, int n_sel,
@@ -1707,7 +1723,9 @@ int run_paged(tg_context* ctx, const tg_paged_kv* pk, int layer, int n, const fl
   const int unit = std::max(d.page_size, tg::kPrefixKeys);
   const bool prefix = pk->tmap_ok && d.dtype == TG_DTYPE_BF16 && d.head_dim == 64 &&
                       use_prefix(n, d.n_kv_head, shared_len);
-  const int shared = prefix ? shared_len / unit * unit : 0;
+  const bool packed = !prefix && use_packed(pk, n, shared_len);
+  const int shared = prefix ? shared_len / unit * unit
+                            : packed ? shared_len / d.page_size * d.page_size : 0;
   const int qdim = d.n_head * d.head_dim;
   tg::PagedAttnParams p{};
   p.kp = pk->k + (size_t)layer * pk->layer_elems * pk->esize;
@@ -1748,7 +1766,27 @@ int run_paged(tg_context* ctx, const tg_paged_kv* pk, int layer, int n, const fl
     p.count = ctx->pcount;
     cudaEvent_t ev = nullptr;
     tg::PagedPrefixParams x{};
-    if (shared > 0) {
+    tg::PagedAttnParams y{};
+    tg::PagedPackedParams z{};
+    if (packed && shared > 0) {
+      y = p;
+      y.mode = 2;
+      y.skip = 0;
+      y.n_rows = p.n * p.group;
+      y.n = (y.n_rows + tg::kPagedHeads - 1) / tg::kPagedHeads;
+      y.prefix_past = shared - 1;
+      y.table = table;
+      const size_t own = (size_t)p.n * p.n_head * (p.hd + 2);
+      TG_TRY(ensure_kept(ctx, &ctx->prec, &ctx->prec_cap,
+                         own + (size_t)y.n * p.n_kv * tg::kPagedHeads * (p.hd + 2)));
+      p.mode = 1;
+      p.records = ctx->prec;
+      p.skip = shared >> p.log2p;
+      y.records = ctx->prec + own;
+      z = {p.records, y.records, p.past, p.out, p.n, p.n_head, p.n_kv, p.group, p.hd, shared,
+           max_blocks << pk->log2p};
+      p.out = nullptr;
+    } else if (shared > 0) {
       x.q = p.q;
       x.past = p.past;
       x.table = table;
@@ -1762,6 +1800,7 @@ int run_paged(tg_context* ctx, const tg_paged_kv* pk, int layer, int n, const fl
       x.n_pages = p.n_pages;
       x.log2p = p.log2p;
       x.steps = shared / tg::kPrefixKeys;
+      x.limit = max_blocks << pk->log2p;
       x.scale_log2 = p.scale_log2;
       tg::plan_paged_prefix(&x, ctx->num_sms);
       const size_t rec = (size_t)p.n * p.n_head * (p.hd + 2);
@@ -1773,7 +1812,12 @@ int run_paged(tg_context* ctx, const tg_paged_kv* pk, int layer, int n, const fl
       p.skip = shared >> p.log2p;
     }
     TG_TRY(prof_begin(ctx, TG_PROFILE_ATTENTION, &ev));
-    if (shared > 0) {
+    if (packed && shared > 0) {
+      cudaError_t e = tg::launch_paged_mma(pk->tmk, pk->tmv, y, d.dtype, grid, ctx->stream);
+      if (e != cudaSuccess)
+        return fail(TG_ERR_CUDA, "paged prefix launch: %s", cudaGetErrorString(e));
+      ctx->launches++;
+    } else if (shared > 0) {
       cudaError_t e = tg::launch_paged_prefix(pk->tmk, pk->tmv, x, ctx->stream);
       if (e != cudaSuccess)
         return fail(TG_ERR_CUDA, "paged prefix launch: %s", cudaGetErrorString(e));
@@ -1786,7 +1830,8 @@ int run_paged(tg_context* ctx, const tg_paged_kv* pk, int layer, int n, const fl
       return fail(TG_ERR_CUDA, "paged attention launch: %s", cudaGetErrorString(e));
     ctx->launches++;
     if (shared > 0) {
-      e = tg::launch_paged_prefix_merge(x, ctx->stream);
+      e = packed ? tg::launch_paged_packed_merge(z, ctx->stream)
+                 : tg::launch_paged_prefix_merge(x, ctx->stream);
       if (e != cudaSuccess)
         return fail(TG_ERR_CUDA, "paged merge launch: %s", cudaGetErrorString(e));
       ctx->launches++;

@@ -318,7 +318,7 @@ __device__ PagedRange paged_schedule(const PagedAttnParams& p, int* prefix, int*
   int sum = 0;
 #pragma unroll 4
   for (int s = b0; s < b1; ++s) {
-    const int past = p.past[s];
+    const int past = p.mode == 2 ? p.prefix_past : p.past[s];
     const int nb = query_blocks(p, past, report);
     past_s[s] = nb > 0 ? past : -1;
     sum += query_chunks(p, past, nb);
@@ -404,7 +404,9 @@ __device__ __forceinline__ SegmentOut segment_out(const PagedAttnParams& p, int 
     r.m = r.l = nullptr;
     r.ml_stride = 0;
   } else {
-    r.o = p.records + ((size_t)s * p.n_head + h0) * (p.hd + 2);
+    const size_t at = p.mode == 1 ? (size_t)s * p.n_head + h0
+                                  : ((size_t)s * p.n_kv + g) * kPagedHeads;
+    r.o = p.records + at * (p.hd + 2);
     r.stride = r.ml_stride = p.hd + 2;
     r.m = r.o + p.hd;
     r.l = r.m + 1;
@@ -1049,7 +1051,7 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     const int rows = past_s[e.s] + 1 - ((e.j << p.log2p) + e.off);
     if (e.j > past_s[e.s] >> p.log2p || rows <= 0) return b;
     b.rows = min(box, rows);
-    b.page = p.table[(size_t)e.s * p.max_blocks + e.j];
+    b.page = p.table[(p.mode == 2 ? 0 : (size_t)e.s * p.max_blocks) + e.j];
     b.y0 = (int)((p.page0 * p.n_kv + e.g) << p.log2p) + e.off;
     return b;
   };
@@ -1152,7 +1154,8 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
     x.e_hi = min(t_hi, x.s_hi);
     x.g = x.u / p.hblocks;
     x.hb = x.u - x.g * p.hblocks;
-    x.heads = min(kPagedHeads, p.group - x.hb * kPagedHeads);
+    x.heads = min(kPagedHeads, p.mode == 2 ? p.n_rows - s * kPagedHeads
+                                           : p.group - x.hb * kPagedHeads);
     return x;
   };
   // The computing warps' sums of a segment, joined by threads first, first +
@@ -1234,9 +1237,15 @@ __global__ void __launch_bounds__(MmaPaged<T, HD>::THREADS, 1)
   float q_raw[HD / 4];
   auto load_q = [&](int qs, int qu) {
     const int g = p.hblocks == 1 ? qu : qu / p.hblocks, hb = qu - g * p.hblocks;
-    const int h = hb * kPagedHeads + r;
+    int h = hb * kPagedHeads + r;
+    bool row_ok = h < p.group;
+    if (p.mode == 2) {
+      h = qs * kPagedHeads + r;
+      row_ok = h < p.n_rows;
+      qs = h / p.group;
+      h -= qs * p.group;
+    }
     const float* q = p.q + ((size_t)qs * p.n_head + g * p.group + h) * HD;
-    const bool row_ok = h < p.group;
 #pragma unroll
     for (int kk = 0; kk < HD / (kHalf ? 16 : 8); ++kk)
 #pragma unroll
@@ -1552,6 +1561,42 @@ cudaError_t launch_paged_mma(const CUtensorMap& tk, const CUtensorMap& tv, const
                       : launch_mma_cfg<float, 64>(tk, tv, p, grid, st);
   return dtype == 1 ? launch_mma_cfg<__nv_bfloat16, 128>(tk, tv, p, grid, st)
                     : launch_mma_cfg<float, 128>(tk, tv, p, grid, st);
+}
+
+// The result of a batch behind a packed prefix: a thread per pair of
+// dimensions merges two records, 1 MB at 128 queries x 14 heads (latency).
+__global__ void __launch_bounds__(256) paged_packed_merge_kernel(const PagedPackedParams p) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const int pairs = p.hd / 2;
+  const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (e >= (long long)p.n * p.n_head * pairs) return;
+  const int d = 2 * (int)(e % pairs), row = (int)(e / pairs);
+  const int s = row / p.n_head, head = row - s * p.n_head, g = head / p.group;
+  const int x = s * p.group + head - g * p.group;   // row of the packed prefix
+  const float* a = p.own + (size_t)row * (p.hd + 2);
+  const float* b = p.packed + (((size_t)(x / kPagedHeads) * p.n_kv + g) * kPagedHeads +
+                               x % kPagedHeads) * (p.hd + 2);
+  float2 O = *reinterpret_cast<const float2*>(a + d);
+  const float2 ml = *reinterpret_cast<const float2*>(a + p.hd);
+  float L = ml.y;
+  const int past = p.past[s];
+  if (past >= p.shared - 1 && past < p.limit) {
+    const float2 o2 = *reinterpret_cast<const float2*>(b + d);
+    const float2 ml2 = *reinterpret_cast<const float2*>(b + p.hd);
+    const float M = fmaxf(ml.x, ml2.x), w = ex2(ml.x - M), w2 = ex2(ml2.x - M);
+    O.x = fmaf(o2.x, w2, O.x * w);
+    O.y = fmaf(o2.y, w2, O.y * w);
+    L = fmaf(ml2.y, w2, L * w);
+  }
+  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+  *reinterpret_cast<float2*>(p.out + (size_t)row * p.hd + d) = make_float2(O.x * inv, O.y * inv);
+}
+
+cudaError_t launch_paged_packed_merge(const PagedPackedParams& p, cudaStream_t st) {
+  const long long items = (long long)p.n * p.n_head * (p.hd / 2);
+  return launch_chained(paged_packed_merge_kernel, dim3((unsigned)((items + 255) / 256)), dim3(256),
+                        0, st, p);
 }
 
 // ------------------------------------------------------------ page selection

@@ -48,7 +48,7 @@ struct PagedAppendParams {
 struct PagedAttnParams {
   const float* q;        // [n][n_head*hd], rotated
   float* out;            // [n][n_head*hd] (mode 0)
-  float* records;        // [n][n_head][hd+2] o (un-normalised), m, l (mode 1)
+  float* records;        // [n][n_head][hd+2] o (un-normalised), m, l (mode 1); [n][n_kv][8] (2)
   const int* past;       // [n] last attended position, -1: none
   const int* table;      // [n][max_blocks]
   const int* sel;        // [n][n_kv][n_sel] listed table entries, or null: dense
@@ -63,7 +63,22 @@ struct PagedAttnParams {
   int skip;              // leading entries left out for queries that attend all of them
   int lchunk;            // log2 of the rows of a chunk
   float scale_log2;      // log2(e) / sqrt(hd)
-  int mode;              // 0 output, 1 records
+  int mode;              // 0 output, 1 records, 2 records of a packed prefix
+  // Mode 2, a prefix that n_rows / group real queries share: "query" v is rows
+  // 8 v .. 8 v + 7 of the n_rows rows query * group + head of a KV head, all
+  // of them at positions 0..prefix_past of table row 0.  hblocks is 1.
+  int n_rows, prefix_past;
+};
+
+// out = a batch's own records (mode 1) and those of its packed prefix, merged.
+struct PagedPackedParams {
+  const float* own;
+  const float* packed;
+  const int* past;
+  float* out;
+  int n, n_head, n_kv, group, hd;
+  int shared;            // positions of the prefix: queries that end in it have it in `own`
+  int limit;             // positions of the table: a query that ends behind them is empty
 };
 
 struct PagedSelectParams {
@@ -94,6 +109,7 @@ struct PagedPrefixParams {
   int n, n_head, n_kv, group, n_pages, log2p, steps;
   int single, pairs, splits, parts;   // plan_paged_prefix
   float scale_log2;
+  int limit;             // positions of the table: a query that ends behind them is empty
 };
 
 // Chooses single / pairs / splits / parts from n, group, n_kv and steps.
@@ -109,6 +125,7 @@ size_t paged_core_smem(int n, int hd);
 // box {min(row, 128 bytes), min(page, 1 << paged_mma_lchunk) rows}, swizzled
 // over the box's width).
 int paged_mma_lchunk(int dtype, int hd);
+cudaError_t launch_paged_packed_merge(const PagedPackedParams& p, cudaStream_t st);
 cudaError_t launch_paged_mma(const CUtensorMap& tk, const CUtensorMap& tv, const PagedAttnParams& p,
                              int dtype, int grid, cudaStream_t st);
 cudaError_t launch_paged_select(const PagedSelectParams& p, int num_sms, cudaStream_t st);

@@ -489,7 +489,8 @@ __global__ void __launch_bounds__(32 * kPrefixMergeWarps)
   {
     const int grp = warp % GRP, dw = (warp / GRP) * DW;
     const int row = row0 + lane;
-    const bool live = row < rows && p.past[row / p.group] + 1 >= p.steps * PX_KEYS;
+    const int past = row < rows ? p.past[row / p.group] : -1;
+    const bool live = past >= p.steps * PX_KEYS - 1 && past < p.limit;
     const float* rec = p.records + (size_t)g * 66 * rows + (live ? row : 0);
     const size_t part_stride = (size_t)p.n_kv * 66 * rows;
     float M = kNegBig, L = 0.f, O[DW];
