@@ -548,8 +548,9 @@ TG_API int tg_paged_attention(tg_context* ctx, tg_paged_kv* pk, int layer, int n
 
 /* tg_paged_attention for a batch whose sequences share their first
  * shared_len positions: the first shared_len / page_size entries (rounded
- * down) of every table row are the same pages, named by row 0, and are read
- * once for all queries.  past_len[s] may lie inside the shared part. */
+ * down) of every table row are the same pages, named by row 0; a long prefix
+ * is read for many queries at once.  past_len[s] may lie inside the shared
+ * part. */
 TG_API int tg_paged_attention_shared(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs,
                                      const float* q, const int32_t* past_len,
                                      const int32_t* block_table, int max_blocks, int shared_len,

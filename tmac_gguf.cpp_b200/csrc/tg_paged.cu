@@ -957,6 +957,9 @@ __device__ void merge_parts_vec(const PagedAttnParams& p, const SegmentOut& dst,
 // leaves 5e-7); against fp32 rows x and the rows are two tf32 each, good to
 // 2^-21.
 //
+// In mode 2 the 8 rows are (query, head) pairs of one KV head over a prefix
+// that all queries share.
+//
 // Measured, 14 / 2 heads of 64, bf16: 256 sequences x 4096 rows in pages of 16
 // 106 us, 5.1 TB/s; 4 x 131072 in pages of 64 53 us, 5.0 TB/s.  Of a CTA's
 // 207000 cycles in the first, 168000 are chunks at 6.2 TB/s, the rest the
