@@ -15,6 +15,9 @@
 // cycles of tensor core (4 x 128 x 128 x 64 multiply-adds at 4096 per cycle),
 // 1024 cycles of ex2 (16 per cycle), about 900 of instruction issue for the
 // splits: all three have to overlap.
+// Measured: 128 queries x 14 / 2 heads over 32768 rows 41 us (30 us would be all
+// three overlapped without a gap), 64 us with the queries' own rows and the
+// merge; without the kernel 326 us.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
