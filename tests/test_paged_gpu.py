@@ -367,7 +367,8 @@ def test_attention_shared_batches(tg, backend, n, shared, page, shape):
 @pytest.mark.parametrize("n,shared,page,shape,dtype", [
     (37, 4100, 16, (8, 8, 32), "bf16"), (19, 9000, 8, (12, 4, 64), "f32"),
     (10, 30011, 64, (4, 1, 128), "bf16"), (100, 2000, 16, (6, 3, 32), "f32"),
-    (3, 40000, 256, (3, 3, 64), "f32"), (1100, 210, 16, (8, 8, 32), "bf16")])
+    (3, 40000, 256, (3, 3, 64), "f32"), (1100, 210, 16, (8, 8, 32), "bf16"),
+    (1100, 1100, 16, (8, 8, 32), "bf16")])
 def test_attention_shared_small_groups(tg, backend, n, shared, page, shape, dtype):
     """Rows of several queries over the prefix together: whole and ragged
     blocks of eight, one block, more queries than one launch takes."""

@@ -1698,7 +1698,9 @@ bool use_prefix(int n, int n_kv, int shared_len) {
 // head) of a KV head go over the prefix together in the place of one query's
 // heads.  That takes two launches more, about 9 us, and leaves a reading of the
 // prefix (from L2) per block of eight in place of one per query: worth it from
-// 48 MB less on.  Measured (heads, us
+// 48 MB less on.  A short prefix is left to the queries: without it their own
+// rows share out worse (58 x (557 + 1..897), 8 / 8 of 32, fp32: 41 us without,
+// 47 with).  Measured (heads, us
 // without / with): 8 / 8 of 32, bf16, 64 x 512 rows 20 / 27, 32 x 2048 28 / 26,
 // 8 x 8192 26 / 21, 64 x 32768 588 / 99; 12 / 4 of 64, fp32, 64 x 512 25 / 32,
 // 32 x 2048 35 / 34, 64 x 32768 742 / 302; 4 / 1 of 128, bf16, 64 x 2048
@@ -1707,7 +1709,8 @@ bool use_packed(const tg_paged_kv* pk, int n, int shared_len) {
   const int group = pk->d.n_head / pk->d.n_kv_head;
   const long long blocks = ((long long)n * group + tg::kPagedHeads - 1) / tg::kPagedHeads;
   const long long row = 2LL * pk->d.n_kv_head * pk->d.head_dim * (int)pk->esize;   // K and V
-  return pk->tmap_ok && group < tg::kPagedHeads && (n - blocks) * shared_len * row >= (48LL << 20);
+  return pk->tmap_ok && group < tg::kPagedHeads && shared_len >= 1024 &&
+         (n - blocks) * shared_len * row >= (48LL << 20);
 }
 
 // Attention launches on device pointers, kPagedMaxQueries queries at a time.
