@@ -232,13 +232,19 @@ def _package():
 
 
 def _backend():
+    """The device's backend, on the current stream: what made the inputs is
+    ordered before the calls."""
     if "be" not in _kept:
         _kept["be"] = _package().CudaBackend(torch.cuda.current_device())
-        _kept["be"].set_stream(torch.cuda.current_stream().cuda_stream)
+    stream = torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    if _kept.get("stream") != stream:
+        _kept["be"].set_stream(stream)
+        _kept["stream"] = stream
     return _kept["be"]
 
 
 def _run_own(st):
+    _backend()
     c = st["cache"]
     if st["op"] == "append":
         c.append(0, st["k"], st["v"], st["pos0"], st["table"], q=st["q"], q_out=st["q_out"],
