@@ -501,7 +501,8 @@ TG_API int tg_attention_noalloc(void* cuda_stream, const float* q, const void* k
  * Rows that a query does not attend may hold anything; a row with an infinity
  * or NaN that it does attend makes its result infinite or NaN.  Several tokens
  * of one sequence in a call are several rows with the same entries.  A page
- * that tg_paged_append writes belongs to one sequence only.
+ * that tg_paged_append writes belongs to one sequence only, as the same entry
+ * of every row that names it.
  * Pointer and stream rules are those of the batched calls above; calls on
  * device pointers can be captured into graphs, once the same call ran
  * before. */
@@ -530,7 +531,10 @@ TG_API int tg_paged_layer_ptrs(tg_paged_kv* pk, int layer, void** k, void** v, v
  * must equal n_seqs).  k is rotated as by tg_rope_op (bit for bit), k and v
  * go to the page of their position (round to nearest even for bf16), and
  * with bounds every page written gets its bounds anew, over its rows up to
- * the last one written.  q ([n_tokens][n_head*head_dim], may be NULL) is
+ * the last one written.  Several table rows may hold the same sequence (the
+ * tokens of a draft, one row each): rows with the same entries write to
+ * different positions, and a page that several of them write gets one pair of
+ * bounds over the tokens of all.  q ([n_tokens][n_head*head_dim], may be NULL) is
  * rotated into q_out (which may be q).  Tokens behind cu_tokens[n_seqs] are
  * padding: nothing of them is written. */
 TG_API int tg_paged_append(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, int n_tokens,

@@ -1,0 +1,84 @@
+"""Calls of the paged cache that its header allows and that are easily left
+out: rows of one sequence in one append, keys that are NaN, tiny queries,
+tables with dropped pages, contexts in two threads."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(x):
+    import torch
+    return torch.tensor(np.asarray(x), dtype=torch.int32).cuda()
+
+
+# ------------------------------------------- rows of one sequence in one append
+
+def _rows_of_sequences(rng, lens, tokens, page, chunk, order):
+    """Table rows (sequence, first position, tokens) of a call that appends
+    tokens[s] tokens behind lens[s] rows of sequence s, `chunk` at a time."""
+    rows = []
+    for s, (n, m) in enumerate(zip(lens, tokens)):
+        at = 0
+        while at < m:
+            step = min(chunk or int(rng.integers(1, 2 * page)), m - at)
+            rows.append((s, n + at, step))
+            at += step
+    if order == "down":
+        rows.reverse()
+    elif order == "mixed":
+        rows = [rows[i] for i in rng.permutation(len(rows))]
+    return rows
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("shape,page", [((14, 2, 64), 16), ((8, 8, 32), 8), ((4, 4, 6), 256),
+                                        ((16, 1, 128), 64)])
+@pytest.mark.parametrize("chunk,order", [(1, "up"), (1, "down"), (1, "mixed"), (2, "mixed"),
+                                         (0, "up"), (0, "mixed")])
+def test_append_rows_of_one_sequence(tg, backend, O, dtype, shape, page, chunk, order):
+    """Several rows with the same entries (a draft as a row per token, a prompt
+    in chunks): one pair of bounds per page, over the tokens of all rows."""
+    import torch
+    H, G, D = shape
+    rng = np.random.default_rng(page + chunk)
+    lens = [0, 5, page - 1, page, 2 * page + 3, 7, 3 * page - 2]
+    tokens = [3, 1, 2, 5, 2 * page + 1, 0, 4]
+    cols = 6
+    order_np = rng.permutation(len(lens) * cols).astype(np.int32)
+    own = order_np.reshape(len(lens), cols)             # pages of the sequences
+    rows = _rows_of_sequences(rng, lens, tokens, page, chunk, order)
+    table = own[[s for s, _, _ in rows]]
+    pos0 = np.array([p for _, p, _ in rows], np.int32)
+    cu = np.concatenate([[0], np.cumsum([m for _, _, m in rows])]).astype(np.int32)
+    T = int(cu[-1])
+    dt = torch.bfloat16 if dtype == "bf16" else torch.float32
+    k, v = (rng.standard_normal((T, G * D)).astype(np.float32) for _ in range(2))
+    k[rng.random(T) < 0.3] *= 20.0                      # a missed key shows in the bounds
+    size = (1, order_np.size, G, page, D)
+    kp0, vp0 = torch.randn(size).to(dt), torch.randn(size).to(dt)
+    b0 = torch.full((1, order_np.size, G, 2, D), 9.0).to(dt)
+    kp, vp, bd = kp0.cuda(), vp0.cuda(), b0.cuda()
+    cache = tg.PagedKVCache(backend, 1, order_np.size, page, H, G, D,
+                            tg.DTYPE_BF16 if dtype == "bf16" else tg.DTYPE_F32, max_pos=4096,
+                            k=kp, v=vp, bounds=bd)
+    cache.append(0, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), i32(pos0), i32(table),
+                 cu_tokens=None if chunk == 1 else i32(cu))
+    backend.synchronize()
+    want_k, want_v, want_b = kp0.clone(), vp0.clone(), b0.clone()
+    for i, (s, p0, m) in enumerate(rows):
+        for x in range(m):
+            t, pos = cu[i] + x, p0 + x
+            pg, slot = own[s, pos // page], pos % page
+            want_k[0, pg, :, slot] = torch.from_numpy(O.rope_heads(k[t], G, D, pos)).view(G, D).to(dt)
+            want_v[0, pg, :, slot] = torch.from_numpy(v[t]).view(G, D).to(dt)
+    for s, (n, m) in enumerate(zip(lens, tokens)):
+        for j in range(n // page, (n + m - 1) // page + 1) if m else ():
+            x = want_k[0, own[s, j], :, :min(page, n + m - j * page)].float()
+            want_b[0, own[s, j]] = torch.stack([x.amin(1), x.amax(1)], 1).to(dt)
+    assert torch.equal(kp.cpu(), want_k)
+    assert torch.equal(vp.cpu(), want_v)
+    assert torch.equal(bd.cpu(), want_b)
+    cache.destroy()

@@ -131,20 +131,134 @@ __device__ __forceinline__ float as_stored(float v) {
 constexpr int kAppendWarps = 8;
 constexpr int kAppendBatch = 8;  // loads a lane has in flight
 
+// Whether table row i has tokens of this call on page `page`, which is entry j
+// of some other row: its tokens on it are then [a, b) of its own, the first of
+// them at row r0 of the page.
+struct PageTokens {
+  int a, b, r0;
+};
+
+__device__ __forceinline__ PageTokens tokens_on_page(const PagedAppendParams& p, int i, int j,
+                                                     int page) {
+  PageTokens x{0, 0, 0};
+  const int pos0 = p.pos0[i];
+  const int first = p.cu ? p.cu[i] : i, last = p.cu ? min(p.cu[i + 1], p.n_tokens) : i + 1;
+  const long long lo = (long long)j << p.log2p, hi = min(lo + (1ll << p.log2p), (long long)p.table_len);
+  const long long end = min((long long)pos0 + (last - first), hi);
+  if (pos0 < 0 || pos0 >= hi || end <= lo || last <= first) return x;
+  if (p.table[(size_t)i * p.max_blocks + j] != page) return x;
+  const long long from = max((long long)pos0, lo);
+  x.a = first + (int)(from - pos0);
+  x.b = first + (int)(end - pos0);
+  x.r0 = (int)(from - lo);
+  return x;
+}
+
+template <int U>
+__device__ __forceinline__ void extend(Unit<U>& lo, Unit<U>& hi, const Unit<U>& x) {
+#pragma unroll
+  for (int e = 0; e < U; ++e) {
+    lo.x[e] = fminf(lo.x[e], x.x[e]);
+    hi.x[e] = fmaxf(hi.x[e], x.x[e]);
+  }
+}
+
+// A new key as the pool holds it.
+template <typename T, int U>
+__device__ __forceinline__ Unit<U> new_row(const float* k, const float* cs) {
+  Unit<U> x = rotate_unit<U>(load_unit<U>(k), load_unit<U>(cs));
+#pragma unroll
+  for (int e = 0; e < U; ++e) x.x[e] = as_stored<T>(x.x[e]);
+  return x;
+}
+
+// The bounds of a page that row s and rows behind it write: row s's tokens
+// [t, t_end) from position pos on, the others' found by looking at all rows
+// behind it.  src: the token of each row of the page, -1 where it is in the
+// pool.  By one warp.
+template <typename T, int U>
+__device__ __forceinline__ void bounds_of_rows(const PagedAppendParams& p, int s, int t, int t_end,
+                                            int pos, int page, int* src) {
+  const int lane = threadIdx.x & 31, hd = p.hd, row = p.n_kv * hd, P = 1 << p.log2p;
+  const int slot = pos & (P - 1);
+  int end = slot + (t_end - t);
+  for (int r = lane; r < P; r += 32) src[r] = r >= slot && r < end ? t + (r - slot) : -1;
+  __syncwarp();
+  for (int i = s + 1 + lane; i < p.n_seqs; i += 32) {
+    const PageTokens x = tokens_on_page(p, i, pos >> p.log2p, page);
+    for (int a = x.a; a < x.b; ++a) atomicMax(&src[x.r0 + (a - x.a)], a);
+    if (x.b > x.a) end = max(end, x.r0 + (x.b - x.a));
+  }
+  end = __reduce_max_sync(0xffffffffu, end);
+  __syncwarp();
+  const size_t base = (size_t)page * p.n_kv;
+  T* bounds = static_cast<T*>(p.bounds);
+  for (int i = lane * U; i < row; i += 32 * U) {
+    const int g = i / hd, d = i - g * hd;
+    Unit<U> lo, hi;
+#pragma unroll
+    for (int e = 0; e < U; ++e) {
+      lo.x[e] = INFINITY;
+      hi.x[e] = -INFINITY;
+    }
+    const T* old = static_cast<const T*>(p.kp) + ((base + g) << p.log2p) * hd + d;
+    for (int r = 0; r < end; ++r)
+      extend(lo, hi, src[r] < 0 ? load_unit<U>(old + (size_t)r * hd)
+                                : new_row<T, U>(p.k + (size_t)src[r] * row + i,
+                                                p.cs + (size_t)(pos - slot + r) * hd + d));
+    store_unit<U>(bounds + (base + g) * 2 * hd + d, lo);
+    store_unit<U>(bounds + ((base + g) * 2 + 1) * hd + d, hi);
+  }
+}
+
+// The page of a table row's first or last token of this call, -1 for none.
+// Two rows that write one page both end on it: a row that writes all of a page
+// leaves no position for another.  x counts rows, or with cu their ends.
+__device__ __forceinline__ int end_page(const PagedAppendParams& p, int x) {
+  const int i = p.cu ? x >> 1 : x, pos0 = p.pos0[i];
+  const int limit = min(p.table_len, p.max_blocks << p.log2p);
+  int n = 1;
+  if (p.cu) n = min(p.cu[i + 1], p.n_tokens) - p.cu[i];
+  if (n <= 0 || pos0 < 0 || pos0 >= limit) return -1;
+  const int pos = p.cu && (x & 1) ? (int)min((long long)pos0 + n, (long long)limit) - 1 : pos0;
+  return p.table[(size_t)i * p.max_blocks + (pos >> p.log2p)];
+}
+
 // One warp per token: its q row rotated, its k row rotated and written with
 // its v row to the page of its position.  The warp of the first new token of
 // a page also writes the page's bounds: min and max over the page's rows up
 // to the last one of this call, the earlier rows from the pool and the new
 // ones rotated again from k (the few extra reads come from L2), so that no
 // warp waits for another and the bounds are the same however the rows were
-// cut into calls.
+// cut into calls.  Where several table rows write one page (tokens of one
+// sequence as rows of their own), the first of them forms the bounds over the
+// tokens of all: a warp that read the pool for a row that another warp of the
+// launch writes would race with it.
 template <typename T, int U>
-__global__ void __launch_bounds__(32 * kAppendWarps) paged_append_kernel(const PagedAppendParams p) {
+__global__ void __launch_bounds__(32 * kAppendWarps, 4) paged_append_kernel(const PagedAppendParams p) {
   __shared__ int seq_of[kAppendWarps];
+  __shared__ int open_page[kAppendWarps], open_seq[kAppendWarps];
+  __shared__ int twins_of[kAppendWarps];
+  __shared__ int source[kAppendWarps][kPagedMaxPage];
   griddep_launch_dependents();
   griddep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int t0 = blockIdx.x * kAppendWarps, t = t0 + warp;
+  // Pages that the table rows end on, for the look at shared pages below: on
+  // their way before anything waits.  Few are looked at by every warp for
+  // itself, many by the CTA together.  The look costs 0.4 us of a step of 64
+  // tokens (5.1 us in a graph without it) and of 16000 tokens of 16 prompts
+  // (28.9 us), 2 us of a step of 1024 (5.8 us); with the loads behind those of
+  // the token's own page it was 1.4, 1.5 and 6 us.
+  constexpr int kAhead = 2;
+  const int n_ends = !p.bounds ? 0 : p.cu ? 2 * p.n_seqs : p.n_seqs;
+  const bool few = n_ends <= 32 * kAhead;   // every warp looks for itself
+  int ends[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    const int x = few ? lane + 32 * u : threadIdx.x + 32 * kAppendWarps * u;
+    ends[u] = x < n_ends ? end_page(p, x) : -1;
+  }
   int s = -1;
   if (p.cu) {
     // The sequences of this CTA's tokens: every thread looks at some of the
@@ -160,20 +274,69 @@ __global__ void __launch_bounds__(32 * kAppendWarps) paged_append_kernel(const P
   } else if (t < p.n_seqs) {
     s = t;
   }
-  if (t >= p.n_tokens || s < 0) return;  // padding tokens stay as they are
-  const int first = p.cu ? p.cu[s] : t, last = p.cu ? min(p.cu[s + 1], p.n_tokens) : t + 1;
   const int P = 1 << p.log2p, hd = p.hd;
-  const long long pos_ll = (long long)p.pos0[s] + (t - first);
-  if (p.pos0[s] < 0 || pos_ll >= p.table_len || (pos_ll >> p.log2p) >= p.max_blocks) {
-    if (lane == 0) record_error(p.err, kDevErrBadPos);
-    return;
+  bool live = t < p.n_tokens && s >= 0;   // padding tokens stay as they are
+  int first = 0, last = 0, pos = 0, slot = 0, page = 0;
+  if (live) {
+    first = p.cu ? p.cu[s] : t;
+    last = p.cu ? min(p.cu[s + 1], p.n_tokens) : t + 1;
+    const long long pos_ll = (long long)p.pos0[s] + (t - first);
+    if (p.pos0[s] < 0 || pos_ll >= p.table_len || (pos_ll >> p.log2p) >= p.max_blocks) {
+      if (lane == 0) record_error(p.err, kDevErrBadPos);
+      live = false;
+    } else {
+      pos = (int)pos_ll;
+      slot = pos & (P - 1);
+      page = p.table[(size_t)s * p.max_blocks + (pos >> p.log2p)];
+      if (page < 0 || page >= p.n_pages) {
+        if (lane == 0) record_error(p.err, kDevErrBadPage);
+        live = false;
+      }
+    }
   }
-  const int pos = (int)pos_ll, slot = pos & (P - 1);
-  const int page = p.table[(size_t)s * p.max_blocks + (pos >> p.log2p)];
-  if (page < 0 || page >= p.n_pages) {
-    if (lane == 0) record_error(p.err, kDevErrBadPage);
-    return;
+  // The pages that this CTA opens, looked for among all table rows.
+  const bool opens = live && p.bounds && (t == first || slot == 0);
+  unsigned twins = 0;   // table rows that share the page: 1 before this one, 2 behind it
+  if (few) {
+    if (opens) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int x = lane + 32 * u, i = p.cu ? x >> 1 : x;
+        if (ends[u] == page && i != s) twins |= i < s ? 1 : 2;
+      }
+      twins = __reduce_or_sync(0xffffffffu, twins);
+    }
+  } else {
+    if (lane == 0) {
+      open_page[warp] = opens ? page : -2;
+      open_seq[warp] = s;
+      twins_of[warp] = 0;
+    }
+    if (__syncthreads_or(opens)) {
+      int open[kAppendWarps];
+#pragma unroll
+      for (int w = 0; w < kAppendWarps; ++w) open[w] = open_page[w];
+      auto look = [&](int x, int end) {
+        unsigned hits = 0;
+#pragma unroll
+        for (int w = 0; w < kAppendWarps; ++w) hits |= open[w] == end ? 1u << w : 0u;
+        const int i = p.cu ? x >> 1 : x;
+        for (; hits; hits &= hits - 1) {   // seldom: rows of this CTA, and twins
+          const int w = __ffs(hits) - 1;
+          if (open_seq[w] != i) atomicOr(&twins_of[w], i < open_seq[w] ? 1 : 2);
+        }
+      };
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (ends[u] >= 0) look(threadIdx.x + 32 * kAppendWarps * u, ends[u]);
+#pragma unroll 4
+      for (int x = threadIdx.x + 32 * kAppendWarps * kAhead; x < n_ends; x += 32 * kAppendWarps)
+        look(x, end_page(p, x));
+      __syncthreads();
+      twins = twins_of[warp];
+    }
   }
+  if (!live) return;
   const float* cs = p.cs + (size_t)pos * hd;
   if (p.q) {
     const int nq = p.n_head * hd;
@@ -206,7 +369,12 @@ __global__ void __launch_bounds__(32 * kAppendWarps) paged_append_kernel(const P
     store_unit<U>(kp + at, rotate_unit<U>(xk, c));
     store_unit<U>(vp + at, xv);
   }
-  if (!p.bounds || (t != first && slot != 0)) return;
+  if (!opens || (twins & 1)) return;
+  if (twins) {
+    bounds_of_rows<T, U>(p, s, t, t + min(last - t, min(P - slot, p.table_len - pos)), pos, page,
+                         source[warp]);
+    return;
+  }
   // Rows [0, slot) of the page from the pool, [slot, end) from k.
   const int end = min(min(P, slot + (last - t)), slot + (p.table_len - pos));
   T* bounds = static_cast<T*>(p.bounds);
@@ -220,25 +388,10 @@ __global__ void __launch_bounds__(32 * kAppendWarps) paged_append_kernel(const P
     }
     const T* old = kp + ((base + g) << p.log2p) * hd + d;
 #pragma unroll 8
-    for (int r = 0; r < slot; ++r) {
-      const Unit<U> x = load_unit<U>(old + (size_t)r * hd);
-#pragma unroll
-      for (int e = 0; e < U; ++e) {
-        lo.x[e] = fminf(lo.x[e], x.x[e]);
-        hi.x[e] = fmaxf(hi.x[e], x.x[e]);
-      }
-    }
+    for (int r = 0; r < slot; ++r) extend(lo, hi, load_unit<U>(old + (size_t)r * hd));
 #pragma unroll 4
-    for (int r = slot; r < end; ++r) {
-      const Unit<U> x = rotate_unit<U>(load_unit<U>(k + (size_t)(r - slot) * row + i),
-                                       load_unit<U>(cs + (size_t)(r - slot) * hd + d));
-#pragma unroll
-      for (int e = 0; e < U; ++e) {
-        const float y = as_stored<T>(x.x[e]);
-        lo.x[e] = fminf(lo.x[e], y);
-        hi.x[e] = fmaxf(hi.x[e], y);
-      }
-    }
+    for (int r = slot; r < end; ++r)
+      extend(lo, hi, new_row<T, U>(k + (size_t)(r - slot) * row + i, cs + (size_t)(r - slot) * hd + d));
     store_unit<U>(bounds + (base + g) * 2 * hd + d, lo);
     store_unit<U>(bounds + ((base + g) * 2 + 1) * hd + d, hi);
   }
