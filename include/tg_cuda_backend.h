@@ -486,8 +486,8 @@ TG_API int tg_attention_noalloc(void* cuda_stream, const float* q, const void* k
  * K and V are each laid out [n_layers][n_pages][n_kv_head][page_size]
  * [head_dim] of `dtype`; page_size is a power of two from 8 to 256.  bounds
  * (with_bounds), [n_layers][n_pages][n_kv_head][2][head_dim] of `dtype`,
- * holds the minimum and maximum of every key dimension over a page's rows,
- * which tg_paged_select needs.  k and v (both or neither) and bounds may
+ * holds the minimum and maximum of every key dimension over a page's rows
+ * (both NaN where one of them is), which tg_paged_select needs.  k and v (both or neither) and bounds may
  * name device memory of the caller, 16-byte aligned, used in place and not
  * freed; where they are NULL the library allocates and zeroes them.
  * Positions 0..max_pos-1 can be rotated.
@@ -567,7 +567,7 @@ TG_API int tg_paged_attention_shared(tg_context* ctx, tg_paged_kv* pk, int layer
  * sum_d max(q_hd * lo_d, q_hd * hi_d) with the page's bounds lo and hi --
  * no key of the page has a larger product with q.  The first keep_first and
  * the last keep_last entries rank above all others; ties go to the lower
- * index, NaN ranks last.  Needs a cache with bounds. */
+ * index, NaN (of any head) ranks last.  Needs a cache with bounds. */
 TG_API int tg_paged_select(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs,
                            const float* q, const int32_t* past_len, const int32_t* block_table,
                            int max_blocks, int keep_first, int keep_last, int n_sel,

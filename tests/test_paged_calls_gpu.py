@@ -82,3 +82,43 @@ def test_append_rows_of_one_sequence(tg, backend, O, dtype, shape, page, chunk, 
     assert torch.equal(vp.cpu(), want_v)
     assert torch.equal(bd.cpu(), want_b)
     cache.destroy()
+
+
+# ------------------------------------------------------------------- NaN keys
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows", [1, 3])
+def test_append_nan_key_reaches_the_bounds(tg, backend, dtype, rows):
+    """A page with a NaN key has NaN bounds in its dimension pair (the rotation
+    mixes two), whether the row is new or was there, and is selected last."""
+    import torch
+    dt = torch.bfloat16 if dtype == "bf16" else torch.float32
+    P, T = 16, 80
+    rng = np.random.default_rng(rows)
+    k, v = (rng.standard_normal((T, 128)).astype(np.float32) for _ in range(2))
+    k[5, 10] = k[37, 64 + 3] = np.nan                    # pages 0 and 2, KV heads 0 and 1
+    kp, vp = (torch.zeros(1, 5, 2, P, 64, dtype=dt).cuda() for _ in range(2))
+    bd = torch.zeros(1, 5, 2, 2, 64, dtype=dt).cuda()
+    c = tg.PagedKVCache(backend, 1, 5, P, dtype=tg.DTYPE_BF16 if dtype == "bf16" else tg.DTYPE_F32,
+                        max_pos=128, k=kp, v=vp, bounds=bd)
+    kd, vd = torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda()
+    table = i32(np.arange(5)[None].repeat(rows, 0))
+    cut = [0, 7, 40, T] if rows == 3 else [0, T]         # three rows of one sequence, or one
+    c.append(0, kd[:T], vd[:T], i32(cut[:-1]), table, cu_tokens=i32(cut))
+    c.append(0, kd[6:7], vd[6:7], i32([6]), table[:1].contiguous())    # page 0 again: the row was there
+    q = torch.from_numpy(rng.standard_normal((1, 896)).astype(np.float32)).cuda()
+    pages = torch.zeros(1, 2, 4, dtype=torch.int32).cuda()
+    c.select_pages(0, q, i32([T - 1]), table[:1].contiguous(), pages, 0, 0)
+    backend.synchronize()
+    nan = torch.isnan(bd.float().cpu())[0]
+    want = torch.zeros(5, 2, 2, 64, dtype=torch.bool)
+    want[0, 0, :, 10:12] = True
+    want[2, 1, :, 2:4] = True
+    assert torch.equal(nan, want)
+    rest = ~want
+    rows_k = kp.float().cpu()[0]
+    rows_k[0, :, 7:] = rows_k[0, :, :1]                  # the last append renewed 7 rows
+    ref = torch.stack([rows_k.amin(2), rows_k.amax(2)], 2)
+    assert torch.equal(bd.float().cpu()[0][rest], ref[rest])
+    assert pages[0, 0].tolist() == [1, 2, 3, 4] and pages[0, 1].tolist() == [0, 1, 3, 4]
+    c.destroy()

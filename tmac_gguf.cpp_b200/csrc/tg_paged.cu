@@ -154,12 +154,14 @@ __device__ __forceinline__ PageTokens tokens_on_page(const PagedAppendParams& p,
   return x;
 }
 
+// Bounds over one row more.  A NaN stays (fminf and fmaxf would drop it, and
+// the page would rank by its other rows).
 template <int U>
 __device__ __forceinline__ void extend(Unit<U>& lo, Unit<U>& hi, const Unit<U>& x) {
 #pragma unroll
   for (int e = 0; e < U; ++e) {
-    lo.x[e] = fminf(lo.x[e], x.x[e]);
-    hi.x[e] = fmaxf(hi.x[e], x.x[e]);
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(lo.x[e]) : "f"(x.x[e]));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi.x[e]) : "f"(x.x[e]));
   }
 }
 
