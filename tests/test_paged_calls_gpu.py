@@ -122,3 +122,41 @@ def test_append_nan_key_reaches_the_bounds(tg, backend, dtype, rows):
     assert torch.equal(bd.float().cpu()[0][rest], ref[rest])
     assert pages[0, 0].tolist() == [1, 2, 3, 4] and pages[0, 1].tolist() == [0, 1, 3, 4]
     c.destroy()
+
+
+# ------------------------------------------------- selection at the range's ends
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("shape", [(14, 2, 64), (16, 1, 128), (8, 8, 32), (4, 4, 6)])
+@pytest.mark.parametrize("q_exp,b_exp", [(0, 0), (-120, 0), (-128, 0), (-136, 0), (-144, 0),
+                                         (-70, -70), (0, -130), (60, 60)])
+def test_select_small_and_large_values(tg, backend, dtype, shape, q_exp, b_exp):
+    """The order is that of the binary64 scores where binary32 is subnormal or
+    overflows too."""
+    import torch
+    H, G, D = shape
+    rng = np.random.default_rng(D)
+    dt = torch.bfloat16 if dtype == "bf16" else torch.float32
+    nb, P, n = 300, 8, 3
+    lo = rng.standard_normal((nb, G, D)) - 1.0
+    hi = lo + np.abs(rng.standard_normal((nb, G, D)))
+    bounds = torch.from_numpy((np.stack([lo, hi], 2) * 2.0 ** b_exp)).to(dt)[None].contiguous()
+    q = torch.from_numpy((rng.standard_normal((n, H * D)) * 2.0 ** q_exp).astype(np.float32))
+    pool = [torch.zeros(1, nb, G, P, D, dtype=dt).cuda() for _ in range(2)]
+    c = tg.PagedKVCache(backend, 1, nb, P, H, G, D,
+                        tg.DTYPE_BF16 if dtype == "bf16" else tg.DTYPE_F32, max_pos=64, k=pool[0],
+                        v=pool[1], bounds=bounds.cuda())
+    table = np.stack([rng.permutation(nb) for _ in range(n)])
+    n_sel = 40
+    pages = torch.zeros(n, G, n_sel, dtype=torch.int32).cuda()
+    c.select_pages(0, q.cuda(), i32([nb * P - 1] * n), i32(table), pages, 0, 0)
+    backend.synchronize()
+    b = bounds[0].double().numpy()
+    x = q.double().numpy().reshape(n, G, H // G, D)
+    for s in range(n):
+        for g in range(G):
+            bl, bh = b[table[s], g, 0], b[table[s], g, 1]
+            score = np.maximum(x[s, g][:, None] * bl, x[s, g][:, None] * bh).sum(-1).max(0)
+            order = sorted(range(nb), key=lambda j: (-score[j], j))
+            assert pages[s, g].tolist() == sorted(order[:n_sel]), (s, g)
+    c.destroy()

@@ -2301,6 +2301,8 @@ __global__ void __launch_bounds__(kSelThreads, sizeof(T) == 4 && HD >= 64 ? 1 : 
   // E, with S = big * sum |q| >= the sum of a score's absolute terms: 2 hd
   // products and hd / 8 partial sums, each added with an error of at most
   // 2^-23 S (the tensor cores may truncate), and 2^-17 S of split operands.
+  // What is below 2^-126 may count as zero, parts of q and of bounds, products
+  // and sums: at most 2^-123 (big + sum |q| + 1) per dimension.
   float sum_q = 0.f;
   for (int h = warp; h < p.group; h += kSelWarps) {
     float x = 0.f;
@@ -2317,7 +2319,8 @@ __global__ void __launch_bounds__(kSelThreads, sizeof(T) == 4 && HD >= 64 ? 1 : 
   }
 #pragma unroll
   for (int w = 0; w < kSelWarps; ++w) sum_q = fmaxf(sum_q, sh.big[w]);
-  const float E2 = 2.02f * (2.125f * hd * 1.1920929e-7f + 7.6293945e-6f) * big * sum_q;   // 2 E, and its own roundings
+  const float E2 = 2.02f * (2.125f * hd * 1.1920929e-7f + 7.6293945e-6f) * big * sum_q   // 2 E, and its own roundings
+                   + 0x1p-122f * hd * (big + sum_q + 1.f);
   uint32_t k_lo = 0, k_hi = kKeyForced - 1;
   if (E2 < INFINITY) {
     const float t = key_value(t_key);
