@@ -160,3 +160,39 @@ def test_select_small_and_large_values(tg, backend, dtype, shape, q_exp, b_exp):
             order = sorted(range(nb), key=lambda j: (-score[j], j))
             assert pages[s, g].tolist() == sorted(order[:n_sel]), (s, g)
     c.destroy()
+
+
+@pytest.mark.parametrize("fill", [float("nan"), 1e30])
+def test_select_ignores_pages_of_nobody(tg, backend, fill):
+    """Bounds of a page that no table names change neither the result nor the
+    work (they once widened the set of pages to be scored again to all of
+    them: 36 times the time)."""
+    import torch
+    nb, n, n_sel = 8187, 4, 256                          # the last pass of a row is not full
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(1, nb + 1, 2, 64, generator=g, device="cuda")
+    bounds = torch.stack([x - 0.5, x + 0.5], 3).to(torch.bfloat16).contiguous()
+    pool = torch.zeros(1, nb + 1, 2, 8, 64, dtype=torch.bfloat16, device="cuda")
+    c = tg.PagedKVCache(backend, 1, nb + 1, 8, max_pos=64, k=pool, v=pool, bounds=bounds)
+    table = (torch.arange(nb, dtype=torch.int32, device="cuda") + 1).repeat(n, 1).contiguous()
+    q = torch.randn(n, 896, generator=g, device="cuda")
+    past = i32([nb * 8 - 1] * n)
+    backend.set_stream(torch.cuda.current_stream().cuda_stream)
+    results, times = [], []
+    for value in (0.0, fill):
+        bounds[:, 0] = value
+        pages = torch.zeros(n, 2, n_sel, dtype=torch.int32, device="cuda")
+        best = float("inf")
+        for _ in range(5):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(10):
+                c.select_pages(0, q, past, table, pages, 0, 0)
+            b.record()
+            backend.synchronize()
+            best = min(best, a.elapsed_time(b))
+        results.append(pages)
+        times.append(best)
+    assert torch.equal(results[0], results[1])
+    assert times[1] < 4 * times[0], times
+    c.destroy()

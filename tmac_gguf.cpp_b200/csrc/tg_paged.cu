@@ -2228,7 +2228,13 @@ __global__ void __launch_bounds__(kSelThreads, sizeof(T) == 4 && HD >= 64 ? 1 : 
     const int r = lane >> 2, qd = lane & 3;
     constexpr int PIECES = ScoreMma<T, HD>::PIECES;
     int j0 = blockIdx.y * PAGES + warp * 8;
-    // (Columns behind the last page repeat page 0: their bounds raise E.)
+    // Columns behind the last page repeat the warp's first one.  (They took
+    // page 0 of the pool, whatever it held, and its bounds raised E: with NaN
+    // there 4 x 8192 pages took 763 us in place of 21.)
+    auto column = [&](int j, int page) -> int {
+      const int first_column = __shfl_sync(0xffffffffu, page, 0);
+      return j + r < nb ? page : first_column;
+    };
     auto bounds_of = [&](int page) -> const T* {
       const bool bad = page < 0 || page >= p.n_pages;
       if (bad && qd == 0) record_error(p.err, kDevErrBadPage);
@@ -2236,13 +2242,13 @@ __global__ void __launch_bounds__(kSelThreads, sizeof(T) == 4 && HD >= 64 ? 1 : 
     };
     auto entry = [&](int j) { return j + r < nb ? table[j + r] : 0; };
     uint4 b[2][PIECES];
-    if (j0 < nb) load_bounds<T, HD>(bounds_of(j0 + r < nb ? first_page : 0), b);
+    if (j0 < nb) load_bounds<T, HD>(bounds_of(column(j0, first_page)), b);
     int page = entry(j0 + stride);
     for (; j0 < nb; j0 += stride) {
       // The next pass's bounds and the page of the one after are on their way.
       uint4 b_n[2][PIECES];
       const bool more = j0 + stride < nb;
-      if (more) load_bounds<T, HD>(bounds_of(page), b_n);
+      if (more) load_bounds<T, HD>(bounds_of(column(j0 + stride, page)), b_n);
       page = entry(j0 + 2 * stride);
       const float2 x = page_scores<T, HD>(b, q_s, hblocks,
                                           p.group - (hblocks - 1) * kPagedHeads, &big);
