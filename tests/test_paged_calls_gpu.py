@@ -196,3 +196,46 @@ def test_select_ignores_pages_of_nobody(tg, backend, fill):
     assert torch.equal(results[0], results[1])
     assert times[1] < 4 * times[0], times
     c.destroy()
+
+
+# ------------------------------------------------------------ dropped pages
+
+def test_sparse_reads_listed_entries_only(tg, backend):
+    """A table whose unlisted entries are no pages (dropped ones), on the host
+    and on the device; a listed one that is none is refused or reported."""
+    import torch
+    from test_paged_gpu import Pool
+    p = Pool(tg, backend, [20 * 16 - 3, 40, 9], (14, 2, 64), "bf16", 16, seed=2)
+    sel = np.full((3, 2, 4), -1, np.int32)
+    sel[0, 0], sel[0, 1] = [0, 3, 7, 19], [2, 3, 19, 10 ** 6]
+    sel[1, :, :2] = [0, 2]
+    sel[1, 1, 3] = 1                       # behind the first min(n_sel, 3) entries: not read
+    sel[2, :, 0] = 0
+    table = np.full_like(p.table_np, -1)
+    for s in range(3):
+        for j in set(sel[s, :, :min(4, -(-p.lens[s] // 16))].flatten()) & set(range(table.shape[1])):
+            table[s, j] = p.table_np[s, j]
+    ref = [[[j for j in sel[s, g, :min(4, -(-p.lens[s] // 16))] if 0 <= j < -(-p.lens[s] // 16)]
+            for g in range(2)] for s in range(3)]
+    p.cache.attention_sparse(0, p.q, p.past, i32(table), torch.from_numpy(sel).cuda(), p.out)
+    backend.synchronize()
+    p.check(p.out, ref)
+    q, past = p.q.cpu().numpy(), p.past.cpu().numpy()
+    out = np.zeros_like(q)
+    p.cache.attention_sparse(0, q, past, table, sel, out)
+    p.check(out, ref)
+    out[:] = 0
+    p.cache.attention_sparse(0, q, past, table, torch.from_numpy(sel).cuda(), out)   # a device list
+    p.check(out, ref)
+    bad = table.copy()
+    bad[0, 7] = -1
+    with pytest.raises(tg.TGError) as e:
+        p.cache.attention_sparse(0, q, past, bad, sel, out)
+    assert e.value.status == tg.TG_ERR_INVALID_ARG and "[0][7]" in e.value.message
+    with pytest.raises(tg.TGError) as e:
+        p.cache.attention_sparse(0, q, past, bad, torch.from_numpy(sel).cuda(), out)
+    assert e.value.status == tg.TG_ERR_DEVICE and "0x106" in e.value.message
+    with pytest.raises(tg.TGError) as e:                       # the dense call reads them all
+        p.cache.attention(0, q, past, table, out)
+    assert e.value.status == tg.TG_ERR_INVALID_ARG
+    p.cache.destroy()

@@ -1663,21 +1663,36 @@ int check_paged_call(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, in
   return set_device(ctx);
 }
 
+int check_host_entry(const tg_paged_kv* pk, const int32_t* table, int max_blocks, int s, int j) {
+  const int page = table[(size_t)s * max_blocks + j];
+  if (page < 0 || page >= pk->d.n_pages)
+    return fail(TG_ERR_INVALID_ARG, "block_table[%d][%d] = %d outside [0, %d)", s, j, page,
+                pk->d.n_pages);
+  return TG_OK;
+}
+
 // Host arrays: last positions in [-1, max_blocks*page_size) and, when the
-// table is on the host too, the entries they use in [0, n_pages).
+// table is on the host too (`table`, else null), the entries that the call
+// reads in [0, n_pages): all up to the last position, or with n_sel those
+// that a list on the host names (`sel`; the kernel looks at those of a list
+// on the device).
 int check_host_pages(const tg_paged_kv* pk, const int32_t* past, const int32_t* table, int n,
-                     int max_blocks, bool host_table) {
+                     int max_blocks, int n_sel = 0, const int32_t* sel = nullptr) {
   const long long limit = (long long)max_blocks << pk->log2p;
   for (int s = 0; s < n; ++s) {
     if (past[s] < -1 || past[s] >= limit)
       return fail(TG_ERR_INVALID_ARG, "past_len[%d] = %d outside [-1, %lld)", s, past[s], limit);
-    if (!host_table || past[s] < 0) continue;
-    for (int j = 0; j <= past[s] >> pk->log2p; ++j) {
-      const int page = table[(size_t)s * max_blocks + j];
-      if (page < 0 || page >= pk->d.n_pages)
-        return fail(TG_ERR_INVALID_ARG, "block_table[%d][%d] = %d outside [0, %d)", s, j, page,
-                    pk->d.n_pages);
+    if (!table || past[s] < 0) continue;
+    const int nb = (past[s] >> pk->log2p) + 1;
+    if (!n_sel) {
+      for (int j = 0; j < nb; ++j) TG_TRY(check_host_entry(pk, table, max_blocks, s, j));
+      continue;
     }
+    for (int g = 0; sel && g < pk->d.n_kv_head; ++g)
+      for (int i = 0; i < std::min(n_sel, nb); ++i) {
+        const int j = sel[((size_t)s * pk->d.n_kv_head + g) * n_sel + i];
+        if (j >= 0 && j < nb) TG_TRY(check_host_entry(pk, table, max_blocks, s, j));
+      }
   }
   return TG_OK;
 }
@@ -3233,10 +3248,7 @@ int tg_paged_append(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, int
                     pos0[s], n, limit);
       if (!host_table) continue;
       for (int j = pos0[s] >> pk->log2p; j <= (pos0[s] + n - 1) >> pk->log2p; ++j) {
-        const int page = block_table[(size_t)s * max_blocks + j];
-        if (page < 0 || page >= d.n_pages)
-          return fail(TG_ERR_INVALID_ARG, "block_table[%d][%d] = %d outside [0, %d)", s, j, page,
-                      d.n_pages);
+        TG_TRY(check_host_entry(pk, block_table, max_blocks, s, j));
       }
     }
   }
@@ -3306,7 +3318,8 @@ int paged_attention(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, con
   bool all_device = false;
   TG_TRY(classify_args(ctx, args, 5, &all_device));
   if (!args[1].device)
-    TG_TRY(check_host_pages(pk, past_len, block_table, n_seqs, max_blocks, !args[2].device));
+    TG_TRY(check_host_pages(pk, past_len, args[2].device ? nullptr : block_table, n_seqs,
+                            max_blocks, n_sel, args[3].device ? nullptr : pages));
   const tg_paged_desc& d = pk->d;
   const size_t qb = (size_t)n_seqs * d.n_head * d.head_dim * 4;
   const void *dq = q, *dp = past_len, *dt = block_table, *dsel = pages;
@@ -3359,7 +3372,8 @@ int tg_paged_select(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, con
   bool all_device = false;
   TG_TRY(classify_args(ctx, args, 4, &all_device));
   if (!args[1].device)
-    TG_TRY(check_host_pages(pk, past_len, block_table, n_seqs, max_blocks, !args[2].device));
+    TG_TRY(check_host_pages(pk, past_len, args[2].device ? nullptr : block_table, n_seqs,
+                            max_blocks));
   const tg_paged_desc& d = pk->d;
   const int qrow = d.n_head * d.head_dim;
   const void *dq = q, *dp = past_len, *dt = block_table;
