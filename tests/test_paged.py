@@ -44,3 +44,43 @@ def test_argument_checks_of_the_binding(built):
     with pytest.raises(ValueError):
         built._table_shape(i)
     assert built._table_shape(np.zeros((2, 5), np.int32)) == (2, 5)
+
+
+class DeviceTensor:
+    """What the binding looks at of a device tensor."""
+
+    def __init__(self, n, dtype):
+        import torch
+        self._n, self.dtype, self.device = n, dtype, torch.device("cuda", 0)
+
+    def numel(self):
+        return self._n
+
+    def element_size(self):
+        return self.dtype.itemsize
+
+    def data_ptr(self):
+        return 0
+
+
+@pytest.mark.parametrize("name,good", [("DTYPE_BF16", "bfloat16"), ("DTYPE_F32", "float32")])
+def test_pools_of_another_type_are_refused(built, name, good):
+    """Types of the same size among them: their bits would be read as the
+    cache's type.  The right type goes on to the library, which has no context
+    here."""
+    import torch
+
+    class Backend:
+        device, handle = 0, None
+
+    right = getattr(torch, good)
+    for wrong in (torch.float16, torch.int16, torch.int32, torch.float64, torch.bfloat16,
+                  torch.float32, torch.uint8):
+        for at in ("k", "v", "bounds"):
+            types = {"k": right, "v": right, "bounds": right, at: wrong}
+            pools = {x: DeviceTensor(4 * 2 * (16 if x != "bounds" else 2) * 64, t)
+                     for x, t in types.items()}
+            with pytest.raises(built.TGError if wrong == right else ValueError) as e:
+                built.PagedKVCache(Backend(), 1, 4, 16, dtype=getattr(built, name), **pools)
+            if wrong != right:
+                assert str(e.value).startswith(f"{at} is ")

@@ -671,8 +671,8 @@ class PagedKVCache:
             if hasattr(x, "numel"):
                 if x.numel() != size:
                     raise ValueError(f"{name} has {x.numel()} elements, not {size}")
-                if x.element_size() != (4 if dtype == DTYPE_F32 else 2):
-                    raise ValueError(f"{name} is not of the cache's type")
+                if _type_name(x.dtype) != ("float32" if dtype == DTYPE_F32 else "bfloat16"):
+                    raise ValueError(f"{name} is {x.dtype}, not of the cache's type")
                 if x.device.type != "cuda" or x.device.index != backend.device:
                     raise ValueError(f"{name} is not on device {backend.device}")
         self.backend = backend
