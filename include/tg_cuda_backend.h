@@ -490,7 +490,7 @@ TG_API int tg_attention_noalloc(void* cuda_stream, const float* q, const void* k
  * (both NaN where one of them is), which tg_paged_select needs.  k and v (both or neither) and bounds may
  * name device memory of the caller, 16-byte aligned, used in place and not
  * freed; where they are NULL the library allocates and zeroes them.
- * Positions 0..max_pos-1 can be rotated.
+ * Positions 0..max_pos-1 can be rotated, max_pos at most 2^24.
  *
  * Block tables are [n_seqs][max_blocks] int32: entry j of row s is the page
  * of positions j*page_size.. of sequence s.  Entries that a call needs must

@@ -239,3 +239,49 @@ def test_sparse_reads_listed_entries_only(tg, backend):
         p.cache.attention(0, q, past, table, out)
     assert e.value.status == tg.TG_ERR_INVALID_ARG
     p.cache.destroy()
+
+
+# ------------------------------------------------------------ rotation tables
+
+@pytest.mark.parametrize("max_pos", [0, -1, 2 ** 24 + 1, 2 ** 30, 2 ** 30 + 1, 2 ** 31 - 1])
+def test_max_pos_is_bounded(tg, backend, max_pos):
+    with pytest.raises(tg.TGError) as e:
+        tg.PagedKVCache(backend, 1, 4, 16, max_pos=max_pos)
+    assert e.value.status == tg.TG_ERR_INVALID_ARG and "max_pos" in e.value.message
+
+
+def test_rotation_table_that_does_not_fit(tg):
+    """A status and a context that goes on, not an exception or the host's
+    memory: 2^31 positions of 128 dimensions are 1 TB."""
+    import torch
+    be = tg.CudaBackend(0)
+    x = torch.ones(1, 128, device="cuda")
+    L = tg.lib()
+    assert L.tg_rope_op(be.handle, x.data_ptr(), 1, 128, 2 ** 30, 1e6) == tg.TG_ERR_OUT_OF_MEMORY
+    assert L.tg_rope_op(be.handle, x.data_ptr(), 1, 128, 2 ** 31 - 1, 1e6) == tg.TG_ERR_INVALID_ARG
+    assert L.tg_rope_op(be.handle, x.data_ptr(), 1, 128, 0, 1e6) == tg.TG_OK
+    be.synchronize()
+    assert (x == 1).all()
+    be.shutdown()
+
+
+def test_positions_across_the_pieces_of_a_table(tg, backend, O):
+    """Bit for bit the rotation of the oracle, wherever the table was cut."""
+    import torch
+    pos = [0, 1, 32767, 32768, 65535, 65536, 65537, 131071, 131072, 200_000, 262_142]
+    n, P = len(pos), 256
+    rng = np.random.default_rng(0)
+    k = rng.standard_normal((n, 128)).astype(np.float32)
+    kp, vp = (torch.zeros(1, n, 2, P, 64, device="cuda") for _ in range(2))
+    c = tg.PagedKVCache(backend, 1, n, P, dtype=tg.DTYPE_F32, max_pos=262_143, k=kp, v=vp)
+    table = np.full((n, 1024), -1)
+    for s in range(n):
+        table[s, pos[s] // P] = s
+    kd = torch.from_numpy(k).cuda()
+    c.append(0, kd, kd, i32(pos), i32(table))
+    backend.synchronize()
+    for s in range(n):
+        want = O.rope_heads(k[s], 2, 64, pos[s]).reshape(2, 64)
+        got = kp[0, s, :, pos[s] % P].cpu().numpy()
+        assert np.array_equal(got.view(np.uint32), want.view(np.uint32)), pos[s]
+    c.destroy()

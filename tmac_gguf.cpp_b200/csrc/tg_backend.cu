@@ -21,6 +21,7 @@
 #include <cstring>
 #include <exception>
 #include <map>
+#include <memory>
 #include <new>
 #include <string>
 #include <vector>
@@ -904,13 +905,25 @@ int finish_compat(tg_context* ctx) {
   return flush_regions(ctx);
 }
 
+// Room for one more element, so that push_back cannot throw through the C ABI.
+template <typename V>
+bool make_room(V& v) {
+  try {
+    v.reserve(v.size() + 1);
+  } catch (const std::exception&) {
+    return false;
+  }
+  return true;
+}
+
 // ------------------------------------------------ RoPE tables
 
 // cos/sin for positions [0, len) exactly as apply_rope computes them
 // (tmac_gguf.cpp:993-996): theta = 1/powf(base, (float)d/head_dim),
 // freq = pos*theta, cosf/sinf -- evaluated here with the host libm so the
 // device rotation reproduces the reference bit for bit.
-int get_table(tg_context* ctx, float base, int head_dim, int need_len, RopeTable** out) {
+// Built piece by piece: a table of any length takes 16 MB of the host.
+int get_table(tg_context* ctx, float base, int head_dim, long long need_len, RopeTable** out) {
   uint32_t bits;
   std::memcpy(&bits, &base, 4);
   RopeTable* t = nullptr;
@@ -921,25 +934,43 @@ int get_table(tg_context* ctx, float base, int head_dim, int need_len, RopeTable
     return TG_OK;
   }
   if (ctx->capturing)
-    return fail(TG_ERR_STATE, "RoPE table for position %d must exist before graph capture",
+    return fail(TG_ERR_STATE, "RoPE table for position %lld must exist before graph capture",
                 need_len - 1);
-  int len = 4096;
+  if (need_len > 0x7fffffffLL)
+    return fail(TG_ERR_INVALID_ARG, "position %lld is too large", need_len - 1);
+  long long len = 4096;
   while (len < need_len) len *= 2;
+  len = std::min(len, 0x7fffffffLL);
   const int half = head_dim / 2;
-  std::vector<float> theta(half);
+  const long long piece = std::max(1LL, std::min(len, (4LL << 20) / head_dim));   // positions
+  std::unique_ptr<float[]> theta(new (std::nothrow) float[half]);
+  std::unique_ptr<float[]> h(new (std::nothrow) float[(size_t)piece * head_dim]);
+  if (!theta || !h || !(t ? make_room(ctx->kept) : make_room(ctx->tables)))
+    return fail(TG_ERR_OUT_OF_MEMORY, "host memory");
   for (int j = 0; j < half; ++j) theta[j] = 1.0f / powf(base, (float)(2 * j) / head_dim);
-  std::vector<float> h((size_t)len * head_dim);
-  for (int pos = 0; pos < len; ++pos) {
-    float* row = h.data() + (size_t)pos * head_dim;
-    for (int j = 0; j < half; ++j) {
-      const float freq = pos * theta[j];
-      row[2 * j] = cosf(freq);
-      row[2 * j + 1] = sinf(freq);
+  float* d = nullptr;
+  if (cudaMalloc(&d, (size_t)len * head_dim * sizeof(float)) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(TG_ERR_OUT_OF_MEMORY, "RoPE table of %lld positions", len);
+  }
+  for (long long p0 = 0; p0 < len; p0 += piece) {
+    const long long n = std::min(piece, len - p0);
+    for (long long i = 0; i < n; ++i) {
+      const int pos = (int)(p0 + i);
+      float* row = h.get() + (size_t)i * head_dim;
+      for (int j = 0; j < half; ++j) {
+        const float freq = pos * theta[j];
+        row[2 * j] = cosf(freq);
+        row[2 * j + 1] = sinf(freq);
+      }
+    }
+    cudaError_t e = cudaMemcpy(d + (size_t)p0 * head_dim, h.get(),
+                               (size_t)n * head_dim * sizeof(float), cudaMemcpyHostToDevice);
+    if (e != cudaSuccess) {
+      cudaFree(d);
+      return fail(TG_ERR_CUDA, "RoPE table: %s", cudaGetErrorString(e));
     }
   }
-  float* d = nullptr;
-  TG_CUDA(cudaMalloc(&d, h.size() * sizeof(float)));
-  TG_CUDA(cudaMemcpy(d, h.data(), h.size() * sizeof(float), cudaMemcpyHostToDevice));
   if (!t) {
     ctx->tables.push_back(RopeTable());
     t = &ctx->tables.back();
@@ -948,7 +979,7 @@ int get_table(tg_context* ctx, float base, int head_dim, int need_len, RopeTable
   } else {
     ctx->kept.push_back(t->d);  // captured graphs may read it
   }
-  t->len = len;
+  t->len = (int)len;
   t->d = d;
   *out = t;
   return TG_OK;
@@ -1573,17 +1604,6 @@ int check_host_pos(const int32_t* pos, int n, int limit, const char* what) {
 
 // ------------------------------------------------ paged KV caches
 
-// Room for one more element, so that push_back cannot throw through the C ABI.
-template <typename V>
-bool make_room(V& v) {
-  try {
-    v.reserve(v.size() + 1);
-  } catch (const std::exception&) {
-    return false;
-  }
-  return true;
-}
-
 // As ensure_buf, for buffers that captured graphs may name: the old one is
 // kept until shutdown.  zero: the new one is zeroed on the stream.
 template <typename T>
@@ -2133,7 +2153,7 @@ int tg_rope_op(tg_context* ctx, float* data, int n_heads, int head_dim, int pos,
   TG_TRY(resolve(ctx, data, (size_t)n_heads * head_dim * 4, true, &d));
   TG_TRY(check_align8(d, "data"));
   RopeTable* t = nullptr;
-  TG_TRY(get_table(ctx, base, head_dim, pos + 1, &t));
+  TG_TRY(get_table(ctx, base, head_dim, (long long)pos + 1, &t));
   tg::RopeParams rp{};
   rp.q = reinterpret_cast<float*>(d);
   rp.pos_scalar = pos;
@@ -3097,8 +3117,11 @@ int tg_paged_create(tg_context* ctx, const tg_paged_desc* desc, tg_paged_kv** ou
   *out = nullptr;
   const tg_paged_desc& d = *desc;
   TG_TRY(check_shape(d.n_head, d.n_kv_head, d.head_dim));
-  if (d.n_layers <= 0 || d.n_pages <= 0 || d.max_pos <= 0)
+  if (d.n_layers <= 0 || d.n_pages <= 0)
     return fail(TG_ERR_INVALID_ARG, "paged_create: bad sizes");
+  if (d.max_pos <= 0 || d.max_pos > tg::kPagedMaxPos)
+    return fail(TG_ERR_INVALID_ARG, "paged_create: max_pos %d outside [1, %d]", d.max_pos,
+                tg::kPagedMaxPos);
   if (d.page_size < tg::kPagedMinPage || d.page_size > tg::kPagedMaxPage ||
       (d.page_size & (d.page_size - 1)))
     return fail(TG_ERR_INVALID_ARG, "paged_create: page_size %d (a power of two, %d to %d)",

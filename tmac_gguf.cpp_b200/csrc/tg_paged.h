@@ -17,6 +17,9 @@
 namespace tg {
 
 constexpr int kPagedMinPage = 8, kPagedMaxPage = 256;
+// Positions of the rotation table: beyond them binary32 has no angle of its own
+// for every position.
+constexpr int kPagedMaxPos = 1 << 24;
 // Queries per launch: the schedule of a launch lives in shared memory.
 constexpr int kPagedMaxQueries = 1024;
 constexpr int kPagedHeads = 8;    // query heads of one stream (a KV head's group in blocks of 8)
