@@ -285,3 +285,45 @@ def test_positions_across_the_pieces_of_a_table(tg, backend, O):
         got = kp[0, s, :, pos[s] % P].cpu().numpy()
         assert np.array_equal(got.view(np.uint32), want.view(np.uint32)), pos[s]
     c.destroy()
+
+
+# ------------------------------------------------------- contexts of threads
+
+def test_contexts_in_threads(tg):
+    """A context, cache and stream per thread, calling at once: every thread
+    has the results that it has alone."""
+    import threading
+
+    from test_paged_gpu import Pool
+    n, shared = 40, 8200
+    made = []
+    for i in range(4):
+        be = tg.CudaBackend(0)
+        p = Pool(tg, be, [shared // 16 * 16 + 7 * i + j for j in range(n)], (14, 2, 64), "bf16",
+                 16, seed=i, shared=shared)
+        made.append((be, p))
+    import torch
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(be, p):
+        try:
+            for _ in range(20):
+                p.cache.attention_shared(0, p.q, p.past, p.table, shared, p.out)
+                p.cache.attention(0, p.q, p.past, p.table, p.out)
+            p.out.zero_()
+            torch.cuda.synchronize()
+            p.cache.attention_shared(0, p.q, p.past, p.table, shared, p.out)
+            be.synchronize()
+        except Exception as e:  # noqa: BLE001 - handed to the test's own thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=x) for x in made]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for be, p in made:
+        p.check(p.out, seqs=[0, n // 2, n - 1])
+        be.shutdown()

@@ -24,6 +24,7 @@
 #include <stdint.h>
 
 #include "tg_device.cuh"
+#include "tg_launch.cuh"
 #include "tg_paged.h"
 #include "tg_shared.h"
 #include "tg_tc.cuh"
@@ -568,45 +569,19 @@ __global__ void __launch_bounds__(32 * kPrefixMergeWarps)
 
 // ------------------------------------------------------------ launches
 
-static cudaError_t launch_prefix_pdl(const void* fn, dim3 grid, dim3 block, size_t smem,
-                                     cudaStream_t st, void** args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelExC(&cfg, fn, args);
-}
-
 cudaError_t launch_paged_prefix(const CUtensorMap& tk, const CUtensorMap& tv,
                                 const PagedPrefixParams& p, cudaStream_t st) {
   static bool done[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!done[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(paged_prefix_kernel,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PX_SMEM);
-    if (e != cudaSuccess) return e;
-    done[dev] = true;
-  }
-  void* args[] = {const_cast<CUtensorMap*>(&tk), const_cast<CUtensorMap*>(&tv),
-                  const_cast<PagedPrefixParams*>(&p)};
-  return launch_prefix_pdl(reinterpret_cast<const void*>(paged_prefix_kernel),
-                           dim3((unsigned)(p.n_kv * p.pairs * p.splits)), dim3(PX_THREADS), PX_SMEM,
-                           st, args);
+  cudaError_t e = allow_max_smem(paged_prefix_kernel, done);
+  if (e != cudaSuccess) return e;
+  return launch_chained(paged_prefix_kernel, dim3((unsigned)(p.n_kv * p.pairs * p.splits)),
+                        dim3(PX_THREADS), PX_SMEM, st, tk, tv, p);
 }
 
 cudaError_t launch_paged_prefix_merge(const PagedPrefixParams& p, cudaStream_t st) {
-  void* args[] = {const_cast<PagedPrefixParams*>(&p)};
-  return launch_prefix_pdl(reinterpret_cast<const void*>(paged_prefix_merge_kernel),
-                           dim3((unsigned)(p.n_kv * ((p.n * p.group + 31) / 32)), 64 / kMergeDims),
-                           dim3(32 * kPrefixMergeWarps), 0, st, args);
+  return launch_chained(paged_prefix_merge_kernel,
+                        dim3((unsigned)(p.n_kv * ((p.n * p.group + 31) / 32)), 64 / kMergeDims),
+                        dim3(32 * kPrefixMergeWarps), 0, st, p);
 }
 
 void plan_paged_prefix(PagedPrefixParams* p, int num_sms) {
