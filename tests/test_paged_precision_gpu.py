@@ -86,8 +86,7 @@ class Rows:
         return out
 
 
-@pytest.mark.parametrize("shape,dtype,page,n,shared",
-                         [r for r in ROUTES if not r.id.startswith("prefix")])
+@pytest.mark.parametrize("shape,dtype,page,n,shared", ROUTES)
 def test_every_part_of_q_counts(tg, backend, shape, dtype, page, n, shared):
     import torch
     H, G, D = shape

@@ -8,16 +8,20 @@
 // S = Q K^T and O += P V run on tcgen05, and a key is read once for 256 rows
 // instead of once for 8.
 //
-// Results have to be those of binary32 products, as everywhere else in the
-// paged cache: q and the probabilities are each split into two bf16, hi + lo
-// (17 significant bits), against the exact bf16 keys and values, which
-// doubles the tensor work.  What a 128 x 128 block costs an SM then: 1024
-// cycles of tensor core (4 x 128 x 128 x 64 multiply-adds at 4096 per cycle),
-// 1024 cycles of ex2 (16 per cycle), about 900 of instruction issue for the
-// splits: all three have to overlap.
-// Measured: 128 queries x 14 / 2 heads over 32768 rows 41 us (30 us would be all
-// three overlapped without a gap), 64 us with the queries' own rows and the
-// merge; without the kernel 326 us.
+// Against the exact bf16 keys q is three bf16, all its 24 bits, since an error
+// of a score grows with the score: with two (17 bits) the largest error, over
+// the largest result, was 1.3e-5 at scores of 4 times the usual size and 5e-5
+// at 16, where a plain binary32 form has 3e-6 and 9e-6 (with three: 3e-6 and
+// 3e-6).  The third part costs 2.4 us of 67 at the size below.  The
+// probabilities are two bf16: what that leaves out, 2^-18 of each, has no
+// common sign over the keys.
+//
+// A step (64 keys for two slots of 128 rows) costs an SM 1280 cycles of tensor
+// core (two slots x (12 + 8) products of 128 x 64 x 16 at 4096 multiply-adds a
+// cycle) and 1024 cycles of ex2 (16 per cycle).  128 queries x 14 / 2 heads
+// over 32768 rows are 28 steps per CTA, 19 us of products; the kernel takes
+// 43: products and softmax of a slot wait for each other, and the two slots
+// overlap far less than they could.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -39,15 +43,19 @@ constexpr int PX_THREADS = 384;     // TMA warp, 2 MMA warps, an idle one, 2 x 4
 constexpr int PX_TILE = PX_KEYS * 128;           // bytes of a K (or V) tile
 constexpr int PX_OFF_Q = PX_STAGES * 2 * PX_TILE;   // 8 KB per softmax warp: q on its way to
                                                     // TMEM, then what O has gathered
-constexpr int PX_OFF_BAR = PX_OFF_Q + 8 * 32 * 64 * 4;
+constexpr int PX_OFF_Q3 = PX_OFF_Q + 8 * 32 * 64 * 4;   // third parts of q: a 128 x 64 operand
+                                                       // per slot, 128-byte swizzle
+constexpr int PX_Q3 = PX_ROWS * 128;
+constexpr int PX_OFF_BAR = PX_OFF_Q3 + 2 * PX_Q3;
 // kv_full[S], kv_empty[S], q_full[slot], s_full[slot][buf], p_full[slot][buf],
 // pv_done[slot], drained[slot]
 constexpr int PX_NBAR = 2 * PX_STAGES + 2 + 4 + 4 + 2 + 2;
 constexpr int PX_OFF_MISC = PX_OFF_BAR + PX_NBAR * 8;
 constexpr size_t PX_SMEM = 1024 + PX_OFF_MISC + 16;
+static_assert(PX_SMEM <= 227 * 1024, "shared memory");
 constexpr uint32_t PX_COLS = 512;
 // TMEM columns of slot x from 256 x: two buffers of 64 (S as binary32, then P
-// in its place: 32 columns hi, 32 lo, two bf16 each), O 64, Q 64 (hi, lo).
+// in its place: 32 columns hi, 32 lo, two bf16 each), O 64, Q 64 (lo, hi).
 __device__ __forceinline__ uint32_t px_s(int x, int buf) { return 256u * x + 64u * buf; }
 __device__ __forceinline__ uint32_t px_o(int x) { return 256u * x + 128u; }
 __device__ __forceinline__ uint32_t px_q(int x) { return 256u * x + 192u; }
@@ -227,6 +235,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
     const uint64_t dk0 = smem_desc_sw128(smem_u32(smem), 16, 1024);
     const uint64_t dv0 = smem_desc_sw128(smem_u32(smem) + PX_TILE, PX_TILE, 1024);
     const int x = (int)__reduce_max_sync(0xffffffffu, threadIdx.x >> 5) - 1;   // warp-uniform
+    const uint64_t dq3 = smem_desc_sw128(smem_u32(smem) + PX_OFF_Q3 + x * PX_Q3, 16, 1024);
     const uint32_t base = __reduce_max_sync(0xffffffffu, tmem) + 256u * x;
     const int n = x ? n1 : n0;
     // This slot's ring entries: x, x + 2, ... (single) or 0, 1, ...  qk is the
@@ -247,9 +256,11 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
     auto issue_qk = [&](int j) -> bool {
       if (!px_wait_warp(&kv_full[qk.st], qk.ph, p.err, abort_flag)) return false;
       tc_fence_after();
-      // 4 steps of 16 dimensions (32 bytes), the high parts and the low ones.
-      umma_f16_ts_x8<2>(base + px_s(0, j & 1), base + px_q(0),
-                        dk0 + (uint64_t)(qk.st * (2 * PX_TILE >> 4)), IDESC_QK, 0u);
+      // 4 steps of 16 dimensions (32 bytes), the third parts, the low and the
+      // high ones: what the tensor core truncates is small while the sum is.
+      const uint64_t dk = dk0 + (uint64_t)(qk.st * (2 * PX_TILE >> 4));
+      umma_f16_ss_x4<2, 2>(base + px_s(0, j & 1), dq3, dk, IDESC_QK, 0u);
+      umma_f16_ts_x8<2>(base + px_s(0, j & 1), base + px_q(0), dk, IDESC_QK, 1u);
       umma_commit_elect(&s_full[2 * x + (j & 1)]);
       qk.step(by);
       return true;
@@ -290,7 +301,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
     const uint32_t base = tmem + ((uint32_t)(quarter * 32) << 16);
     const int steps = x ? n1 : n0;
     {
-      // This row of Q, scaled to log2 units, as hi and lo.  The warp reads its
+      // This row of Q, scaled to log2 units, as lo and hi in TMEM and a third
+      // part, for which TMEM has no room, in shared memory.  The warp reads its
       // 32 rows one by one, whole, and turns them in shared memory (a lane
       // reading a row by itself touched a line per lane and load, 8000 cycles
       // for the 8 warps).
@@ -311,16 +323,25 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
 #pragma unroll
       for (int i = 0; i < 32; ++i) turn[i * 32 + (lane ^ i)] = v[i];
       __syncwarp();
-      uint32_t w[64];
+      uint32_t w[64], third[4];
+      const int r128 = quarter * 32 + lane;
+      uint8_t* q3 = smem + PX_OFF_Q3 + x * PX_Q3 + r128 * 128;
 #pragma unroll
       for (int c = 0; c < 32; ++c) {
         const float2 v = turn[lane * 32 + (c ^ lane)];
-        float h0, l0, h1, l1;
-        split_bf16(v.x * p.scale_log2, h0, l0);
-        split_bf16(v.y * p.scale_log2, h1, l1);
-        w[c] = pack_bf16x2(h0, h1);
-        w[32 + c] = pack_bf16x2(l0, l1);
+        float h0, l0, h1, l1, r0, r1;
+        split_bf16(v.x * p.scale_log2, h0, r0);
+        split_bf16(v.y * p.scale_log2, h1, r1);
+        split_bf16(r0, l0, r0);
+        split_bf16(r1, l1, r1);
+        w[c] = pack_bf16x2(l0, l1);
+        w[32 + c] = pack_bf16x2(h0, h1);
+        third[c & 3] = pack_bf16x2(r0, r1);
+        if ((c & 3) == 3)
+          *reinterpret_cast<uint4*>(q3 + (((c >> 2) ^ (r128 & 7)) << 4)) =
+              make_uint4(third[0], third[1], third[2], third[3]);
       }
+      fence_proxy_async_smem();   // the tensor core reads them
       TG_TMEM_ST64(base + px_q(x), w);
       tc_fence_before();
       __syncwarp();
