@@ -327,3 +327,41 @@ def test_contexts_in_threads(tg):
     for be, p in made:
         p.check(p.out, seqs=[0, n // 2, n - 1])
         be.shutdown()
+
+
+# ------------------------------------------------------- forms of a shared call
+
+@pytest.mark.parametrize("shape,dtype,n,shared,launches", [
+    ((8, 8, 64), "bf16", 1, 65536, 1), ((14, 2, 64), "bf16", 1, 131072, 1),   # nothing is shared
+    ((8, 1, 64), "bf16", 1, 131072, 1), ((4, 1, 128), "f32", 1, 131072, 1),
+    ((14, 2, 64), "bf16", 2, 65536, 1), ((14, 2, 64), "bf16", 32, 2048, 1),
+    ((8, 8, 32), "bf16", 1000, 200, 1), ((32, 8, 128), "bf16", 256, 300, 1),
+    ((8, 8, 64), "bf16", 8, 65536, 3), ((14, 2, 64), "bf16", 64, 8192, 3),    # much is
+    ((8, 8, 32), "bf16", 1000, 900, 3), ((12, 4, 64), "f32", 1000, 900, 3),
+    ((4, 4, 6), "bf16", 64, 65536, 1)])                                       # CUDA cores
+def test_shared_form_by_what_it_saves(tg, backend, shape, dtype, n, shared, launches):
+    """A prefix is attended for all queries where that is worth two launches
+    more: never for one query (which took a form of 2.3 times the time over
+    65536 rows of 8 KV heads), also for short ones of many queries."""
+    import torch
+    H, G, D = shape
+    g = torch.Generator(device="cuda").manual_seed(n)
+    P, pool = 256, 8
+    dt = torch.bfloat16 if dtype == "bf16" else torch.float32
+    k, v = (torch.randn(1, pool, G, P, D, generator=g, device="cuda").to(dt) for _ in range(2))
+    c = tg.PagedKVCache(backend, 1, pool, P, H, G, D,
+                        tg.DTYPE_BF16 if dtype == "bf16" else tg.DTYPE_F32, max_pos=64, k=k, v=v)
+    row = torch.randint(0, pool, (shared // P + 2,), generator=g, device="cuda", dtype=torch.int32)
+    table = row.repeat(n, 1).contiguous()
+    past = shared + torch.arange(n, dtype=torch.int32, device="cuda") % 200
+    q = torch.randn(n, H * D, generator=g, device="cuda")
+    outs = [torch.zeros_like(q) for _ in range(2)]
+    before = backend.launch_count()
+    c.attention_shared(0, q, past, table, shared, outs[0])
+    assert backend.launch_count() - before == launches
+    c.attention(0, q, past, table, outs[1])
+    backend.synchronize()
+    # Two ways to the same sums (|v| < 6): 2^-15 of it, and scores below 40 in
+    # binary32 products.
+    assert (outs[0] - outs[1]).abs().max() <= 6 * (2.0 ** -15 + 2 * 40 * D * 2.0 ** -24)
+    c.destroy()

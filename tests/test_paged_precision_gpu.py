@@ -23,7 +23,8 @@ ROUTES = [
     pytest.param((4, 4, 6), "f32", 16, 3, 0, id="plain-cores"),
     pytest.param((4, 4, 6), "bf16", 16, 3, 0, id="plain-cores-bf16"),
     pytest.param((14, 2, 64), "bf16", 16, 40, 9000, id="prefix"),
-    pytest.param((14, 2, 64), "bf16", 32, 9, 40000, id="prefix-one-tile"),
+    pytest.param((14, 2, 64), "bf16", 32, 9, 65000, id="prefix-one-tile"),
+    pytest.param((12, 4, 64), "bf16", 8, 10, 40003, id="prefix-30-rows"),
     pytest.param((12, 4, 64), "bf16", 256, 70, 4200, id="prefix-two-tiles"),
     pytest.param((8, 8, 32), "bf16", 16, 37, 4100, id="packed-32"),
     pytest.param((12, 4, 64), "f32", 16, 19, 9000, id="packed-f32"),
@@ -78,10 +79,13 @@ class Rows:
     def attend(self, q):
         import torch
         out = torch.full_like(q, 7.0)
+        before = self.backend.launch_count()
         if self.shared:
             self.cache.attention_shared(0, q, self.past, self.table, self.shared, out)
         else:
             self.cache.attention(0, q, self.past, self.table, out)
+        # A prefix that is attended for all takes two launches more.
+        assert self.backend.launch_count() - before == (3 if self.shared else 1)
         self.backend.synchronize()
         return out
 

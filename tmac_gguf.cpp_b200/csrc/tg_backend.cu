@@ -1717,35 +1717,66 @@ int check_host_pages(const tg_paged_kv* pk, const int32_t* past, const int32_t* 
   return TG_OK;
 }
 
-// Whether the tensor-core kernel takes a shared prefix (see run_paged).  It
-// costs two launches more and about 20 us in all; without it every query
-// reads the prefix for itself, mostly from L2.  Measured on a B200 (14 query /
-// 2 KV heads, us without / with): 64 x 2048 20 / 25, 32 x 4096 20 / 23,
-// 16 x 8192 19 / 25; at the border 64 x 4096 30 / 25, 32 x 8192 29 / 25,
-// 16 x 16384 29 / 31, 8 x 32768 29 / 32; above it 32 x 16384 49 / 28,
-// 128 x 32768 326 / 57.  With 8 / 4 heads 32 x 2048 20 / 24, 32 x 4096 29 / 25,
-// 8 x 16384 29 / 25.
-bool use_prefix(int n, int n_kv, int shared_len) {
-  return (long long)n * n_kv * shared_len >= (1LL << 19);
-}
+// Who attends the prefix that n queries share: every query for itself, the
+// tensor-core kernel, or (where that does not serve the shape) the decode
+// kernel with eight rows (query, head) of a KV head in the place of one query's
+// heads.
+enum class SharedForm { kNone, kPrefix, kPacked };
 
-// Whether, where that kernel does not serve the shape, eight rows (query,
-// head) of a KV head go over the prefix together in the place of one query's
-// heads.  That takes two launches more, about 9 us, and leaves a reading of the
-// prefix (from L2) per block of eight in place of one per query: worth it from
-// 48 MB less on.  A short prefix is left to the queries: without it their own
-// rows share out worse (58 x (557 + 1..897), 8 / 8 of 32, fp32: 41 us without,
-// 47 with).  Measured (heads, us
-// without / with): 8 / 8 of 32, bf16, 64 x 512 rows 20 / 27, 32 x 2048 28 / 26,
-// 8 x 8192 26 / 21, 64 x 32768 588 / 99; 12 / 4 of 64, fp32, 64 x 512 25 / 32,
-// 32 x 2048 35 / 34, 64 x 32768 742 / 302; 4 / 1 of 128, bf16, 64 x 2048
-// 28 / 33, 8 x 32768 44 / 44, 64 x 32768 263 / 149.
-bool use_packed(const tg_paged_kv* pk, int n, int shared_len) {
-  const int group = pk->d.n_head / pk->d.n_kv_head;
-  const long long blocks = ((long long)n * group + tg::kPagedHeads - 1) / tg::kPagedHeads;
-  const long long row = 2LL * pk->d.n_kv_head * pk->d.head_dim * (int)pk->esize;   // K and V
-  return pk->tmap_ok && group < tg::kPagedHeads && shared_len >= 1024 &&
-         (n - blocks) * shared_len * row >= (48LL << 20);
+// By what a form saves, in rows of one KV head that the decode kernel does not
+// read for a stream of up to eight heads (it reads 26000 a microsecond in bf16
+// up to 64 dimensions, most of them from L2, 7000 to 10000 in wider rows).
+// Against the rows of every query stand
+//  - the rows that the form reads itself: the tensor-core kernel for 256 rows
+//    (query, head) takes as long as the decode kernel for 10 / 3 streams, for
+//    128 in one tile as for 7 / 3; the packed form reads for eight;
+//  - about 224 rows per stream, whose own rows get a record and a merge;
+//  - two launches more, 12 us, and 50 ns for each part of the prefix's records.
+// Measured on a B200 (graph replays, us: none / prefix / packed, 1 to 128 own
+// rows each; of 1391 shapes of this kind the rule's choice is within 8 % of the
+// best of the three in all but five, and within 13 % in those):
+//  14 / 2 heads of 64, bf16: 1 x 65000 19 / 34 / 25, 4 x 65000 29 / 36 / 36,
+//   8 x 30000 27 / 33 / 33, 8 x 65000 48 / 39 / 51, 16 x 16000 28 / 31 / 34,
+//   32 x 6000 24 / 25 / 31, 32 x 10000 33 / 27 / 40, 64 x 2500 21 / 26 / 32,
+//   64 x 4000 28 / 24 / 38, 128 x 1000 23 / 26 / 33, 128 x 2500 34 / 28 / 45,
+//   256 x 600 26 / 33 / 44, 256 x 1000 34 / 33 / 51
+//  8 / 8 of 64: 1 x 65000 32 / 75 / 39, 2 x 65000 48 / 74 / 40, 4 x 10000
+//   21 / 25 / 21, 8 x 10000 33 / 26 / 23, 32 x 10000 105 / 32 / 36
+//  12 / 4 of 64: 4 x 65000 47 / 43 / 37, 16 x 4000 19 / 22 / 23, 16 x 16000
+//   47 / 27 / 33, 64 x 65000 639 / 57 / 256
+//  8 / 1 of 64: 16 x 30000 27 / 35, 16 x 65000 48 / 40
+// and none / packed: 8 / 8 of 32, bf16, 64 x 500 19 / 26, 64 x 1500 37 / 30,
+//  256 x 300 39 / 49, 256 x 500 54 / 50, 1000 x 300 157 / 163, 1000 x 1000
+//  349 / 185; the same in fp32, 1000 x 300 250 / 189; 12 / 4 of 64, fp32,
+//  64 x 1000 35 / 36, 64 x 1500 47 / 40, 256 x 300 51 / 56, 256 x 1000 112 / 83;
+//  32 / 8 of 128, bf16, 64 x 1000 76 / 78, 64 x 1500 106 / 93, 256 x 500
+//  155 / 162, 256 x 1000 277 / 223; 4 / 1 of 128, bf16, 256 x 1000 44 / 47,
+//  256 x 1500 59 / 55, 1000 x 1000 157 / 130.
+SharedForm shared_form(const tg_paged_kv* pk, int n, int shared_len, int num_sms) {
+  if (!pk->tmap_ok) return SharedForm::kNone;
+  const tg_paged_desc& d = pk->d;
+  const bool fast_rows = d.dtype == TG_DTYPE_BF16 && d.head_dim <= 64;
+  const long long group = d.n_head / d.n_kv_head, rows = n * group, len = shared_len;
+  const long long streams = (long long)n * d.n_kv_head * ((group + tg::kPagedHeads - 1) / tg::kPagedHeads);
+  constexpr long long kRecord = 224, kLaunches = 12 * 26000, kPart = 1300;
+  long long prefix = 0, packed = 0;
+  if (d.dtype == TG_DTYPE_BF16 && d.head_dim == 64) {
+    tg::PagedPrefixParams x{};
+    x.n = n;
+    x.group = (int)group;
+    x.n_kv = d.n_kv_head;
+    x.steps = shared_len / tg::kPrefixKeys;
+    tg::plan_paged_prefix(&x, num_sms);
+    prefix = streams * (len - kRecord) - x.pairs * d.n_kv_head * len * (x.single ? 7 : 10) / 3 -
+             kLaunches - x.parts * kPart;
+  }
+  if (group < tg::kPagedHeads) {
+    const long long blocks = (rows + tg::kPagedHeads - 1) / tg::kPagedHeads;
+    packed = (n - blocks) * d.n_kv_head * len - streams * kRecord -
+             (fast_rows ? kLaunches : kLaunches * 2 / 5);
+  }
+  if (prefix > 0 && prefix >= packed) return SharedForm::kPrefix;
+  return packed > 0 ? SharedForm::kPacked : SharedForm::kNone;
 }
 
 // Attention launches on device pointers, kPagedMaxQueries queries at a time.
@@ -1756,14 +1787,6 @@ int run_paged(tg_context* ctx, const tg_paged_kv* pk, int layer, int n, const fl
   TG_TRY(check_align8(q, "q"));
   TG_TRY(check_align8(out, "out"));
   const tg_paged_desc& d = pk->d;
-  // The part of a shared prefix that the tensor-core kernel takes, in its
-  // steps: whole steps of whole pages.
-  const int unit = std::max(d.page_size, tg::kPrefixKeys);
-  const bool prefix = pk->tmap_ok && d.dtype == TG_DTYPE_BF16 && d.head_dim == 64 &&
-                      use_prefix(n, d.n_kv_head, shared_len);
-  const bool packed = !prefix && use_packed(pk, n, shared_len);
-  const int shared = prefix ? shared_len / unit * unit
-                            : packed ? shared_len / d.page_size * d.page_size : 0;
   const int qdim = d.n_head * d.head_dim;
   tg::PagedAttnParams p{};
   p.kp = pk->k + (size_t)layer * pk->layer_elems * pk->esize;
@@ -1795,6 +1818,14 @@ int run_paged(tg_context* ctx, const tg_paged_kv* pk, int layer, int n, const fl
     p.past = past + s0;
     p.table = table + (size_t)s0 * max_blocks;
     p.sel = sel ? sel + (size_t)s0 * p.n_kv * n_sel : nullptr;
+    p.mode = 0;
+    p.skip = 0;
+    // The part of a shared prefix that is attended for all queries: whole
+    // pages, and whole steps of the tensor-core kernel.
+    const SharedForm form = shared_form(pk, p.n, shared_len, ctx->num_sms);
+    const bool packed = form == SharedForm::kPacked;
+    const int unit = packed ? d.page_size : std::max(d.page_size, tg::kPrefixKeys);
+    const int shared = form == SharedForm::kNone ? 0 : shared_len / unit * unit;
     int grid = ctx->num_sms;
     if (!pk->tmap_ok && 2 * (tg::paged_core_smem(p.n, p.hd) + 1024) <= 227 * 1024) grid *= 2;
     TG_TRY(ensure_kept(ctx, &ctx->ppart, &ctx->ppart_cap,
