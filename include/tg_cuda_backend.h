@@ -518,8 +518,9 @@ typedef struct tg_paged_desc {
 } tg_paged_desc;
 
 TG_API int tg_paged_create(tg_context* ctx, const tg_paged_desc* desc, tg_paged_kv** out);
-/* Destroy before tg_shutdown of its context; tg_shutdown frees caches that
- * are still alive, after which their handles must not be used. */
+/* Destroy before tg_shutdown of its context, outside a graph capture;
+ * tg_shutdown frees caches that are still alive, after which their handles
+ * must not be used. */
 TG_API int tg_paged_destroy(tg_paged_kv* pk);
 /* Device pointers of one layer; bounds NULL when the cache keeps none. */
 TG_API int tg_paged_layer_ptrs(tg_paged_kv* pk, int layer, void** k, void** v, void** bounds);

@@ -365,3 +365,34 @@ def test_shared_form_by_what_it_saves(tg, backend, shape, dtype, n, shared, laun
     # binary32 products.
     assert (outs[0] - outs[1]).abs().max() <= 6 * (2.0 ** -15 + 2 * 40 * D * 2.0 ** -24)
     c.destroy()
+
+
+# ----------------------------------------------------- caches and captures
+
+def test_destroy_inside_a_capture_is_refused(tg):
+    """The capture goes on and its graph runs; the cache is destroyed after it,
+    or by the shutdown when Python dropped it in between."""
+    import torch
+
+    from test_paged_gpu import Pool
+    be = tg.CudaBackend(0)
+    p = Pool(tg, be, [300, 7], (14, 2, 64), "bf16", 16, seed=3)
+    other, dropped = (tg.PagedKVCache(be, 1, 4, 16) for _ in range(2))
+    torch.cuda.synchronize()
+    p.cache.attention(0, p.q, p.past, p.table, p.out)
+    be.synchronize()
+    be.graph_begin()
+    p.cache.attention(0, p.q, p.past, p.table, p.out)
+    with pytest.raises(tg.TGError) as e:
+        other.destroy()
+    assert e.value.status == tg.TG_ERR_STATE
+    del dropped
+    graph = be.graph_end()
+    p.out.zero_()
+    torch.cuda.synchronize()
+    graph.launch()
+    be.synchronize()
+    p.check(p.out)
+    other.destroy()
+    graph.destroy()
+    be.shutdown()

@@ -3243,6 +3243,8 @@ int tg_paged_create(tg_context* ctx, const tg_paged_desc* desc, tg_paged_kv** ou
 
 int tg_paged_destroy(tg_paged_kv* pk) {
   if (!pk) return TG_OK;
+  // Waiting for the stream and freeing would end the capture.
+  if (pk->ctx->capturing) return fail(TG_ERR_STATE, "paged_destroy inside a graph capture");
   cudaSetDevice(pk->ctx->device);
   if (cudaStreamSynchronize(pk->ctx->stream) == cudaSuccess) stream_idle(pk->ctx);
   auto& ps = pk->ctx->paged;
