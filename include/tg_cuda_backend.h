@@ -503,6 +503,12 @@ TG_API int tg_attention_noalloc(void* cuda_stream, const float* q, const void* k
  * of one sequence in a call are several rows with the same entries.  A page
  * that tg_paged_append writes belongs to one sequence only, as the same entry
  * of every row that names it.
+ * Attention results are those of binary32 products and sums: against bf16
+ * rows q counts with all its 24 bits, against fp32 rows both count with 22
+ * (two tf32 of 11).  The weights of a shared prefix that the tensor cores
+ * attend for a whole batch (bf16, head_dim 64) count with 17 bits, all others
+ * with 22 or more.  Sums are formed in an order that depends on the lengths
+ * of the batch, the same for the same call.
  * Pointer and stream rules are those of the batched calls above; calls on
  * device pointers can be captured into graphs, once the same call ran
  * before. */
@@ -553,9 +559,9 @@ TG_API int tg_paged_attention(tg_context* ctx, tg_paged_kv* pk, int layer, int n
 
 /* tg_paged_attention for a batch whose sequences share their first
  * shared_len positions: the first shared_len / page_size entries (rounded
- * down) of every table row are the same pages, named by row 0; a long prefix
- * is read for many queries at once.  past_len[s] may lie inside the shared
- * part. */
+ * down) of every table row are the same pages, named by row 0 (also where
+ * its own past_len is -1); a prefix is read for many queries at once where
+ * that is faster.  past_len[s] may lie inside the shared part. */
 TG_API int tg_paged_attention_shared(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs,
                                      const float* q, const int32_t* past_len,
                                      const int32_t* block_table, int max_blocks, int shared_len,

@@ -3447,7 +3447,7 @@ int tg_paged_select(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, con
   TG_TRY(ensure_kept(ctx, &ctx->pkeys, &ctx->pkeys_cap,
                      (size_t)std::min(step, n_seqs) * per_query));
   TG_TRY(ensure_kept(ctx, &ctx->pcount, &ctx->pcount_cap,
-                     (size_t)2 * std::min(step, n_seqs) * d.n_kv_head, true));
+                     (size_t)std::min(step, n_seqs) * d.n_kv_head, true));
   tg::PagedSelectParams p{};
   p.count = ctx->pcount;
   p.bounds = pk->bounds + (size_t)layer * pk->bounds_elems * pk->esize;

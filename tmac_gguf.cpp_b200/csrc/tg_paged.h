@@ -90,7 +90,7 @@ struct PagedSelectParams {
   const int* table;              // [n][max_blocks]
   const void* bounds;            // layer base
   unsigned long long* keys;      // [n][n_kv][3][max_blocks] scratch
-  unsigned* count;               // [n][n_kv] arrivals and largest bound, all 0 between launches
+  unsigned* count;               // [n][n_kv] arrivals, all 0 between launches
   int* pages;                    // [n][n_kv][n_sel]
   int* err;
   int n, n_head, n_kv, group, hd, dtype;
