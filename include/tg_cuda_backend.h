@@ -543,7 +543,8 @@ TG_API int tg_paged_layer_ptrs(tg_paged_kv* pk, int layer, void** k, void** v, v
  * different positions, and a page that several of them write gets one pair of
  * bounds over the tokens of all.  q ([n_tokens][n_head*head_dim], may be NULL) is
  * rotated into q_out (which may be q).  Tokens behind cu_tokens[n_seqs] are
- * padding: nothing of them is written. */
+ * padding: nothing of them is written.  A padding row of the table is one
+ * without tokens; a row with tokens needs pos0[s] >= 0. */
 TG_API int tg_paged_append(tg_context* ctx, tg_paged_kv* pk, int layer, int n_seqs, int n_tokens,
                            const int32_t* cu_tokens, const int32_t* pos0,
                            const int32_t* block_table, int max_blocks, const float* k,

@@ -84,6 +84,38 @@ def test_append_rows_of_one_sequence(tg, backend, O, dtype, shape, page, chunk, 
     cache.destroy()
 
 
+@pytest.mark.parametrize("where", ["device", "host"])
+def test_append_to_a_padded_batch(tg, backend, O, where):
+    """Rows without tokens are padding, whatever their position and entries."""
+    import torch
+    rng = np.random.default_rng(3)
+    P, n = 16, 70
+    live = np.flatnonzero(rng.random(n) < 0.5)
+    pos0, table = np.full(n, -1, np.int32), np.full((n, 3), -1, np.int32)
+    pos0[live] = rng.integers(0, 3 * P, len(live))
+    for i, s in enumerate(live):
+        table[s, pos0[s] // P] = i
+    cu = np.concatenate([[0], np.cumsum(np.isin(np.arange(n), live))]).astype(np.int32)
+    T = n                                                # tokens of the live rows, then padding
+    k, q = (rng.standard_normal((T, w)).astype(np.float32) for w in (128, 896))
+    kp, vp = (torch.zeros(1, len(live), 2, P, 64).cuda() for _ in range(2))
+    bd = torch.full((1, len(live), 2, 2, 64), 5.0).cuda()
+    c = tg.PagedKVCache(backend, 1, len(live), P, dtype=tg.DTYPE_F32, max_pos=64, k=kp, v=vp, bounds=bd)
+    put = (lambda x: torch.from_numpy(x).cuda()) if where == "device" else (lambda x: x.copy())
+    out = put(np.full_like(q, 3.0))
+    c.append(0, put(k), put(k), put(pos0), put(table), q=put(q), q_out=out, cu_tokens=put(cu))
+    backend.synchronize()
+    out = out.cpu().numpy() if where == "device" else out
+    for i, s in enumerate(live):
+        want = O.rope_heads(k[i], 2, 64, int(pos0[s])).reshape(2, 64)
+        assert np.array_equal(kp[0, i, :, pos0[s] % P].cpu().numpy(), want)
+        assert np.array_equal(out[i], O.rope_heads(q[i], 14, 64, int(pos0[s])))
+        if pos0[s] % P == 0:
+            assert np.array_equal(bd[0, i].cpu().numpy(), np.stack([want, want], 1))
+    assert (out[len(live):] == 3.0).all()
+    c.destroy()
+
+
 # ------------------------------------------------------------------- NaN keys
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -195,6 +227,44 @@ def test_select_ignores_pages_of_nobody(tg, backend, fill):
         times.append(best)
     assert torch.equal(results[0], results[1])
     assert times[1] < 4 * times[0], times
+    c.destroy()
+
+
+@pytest.mark.parametrize("times", [50.0, 5000.0])
+@pytest.mark.parametrize("shape,dtype", [((14, 2, 64), "bf16"), ((32, 8, 128), "bf16"),
+                                         ((12, 4, 64), "f32"), ((4, 4, 6), "f32")])
+def test_select_outlier_dimension(tg, backend, shape, dtype, times):
+    """A key dimension that is far larger than the others widens the set of
+    pages that are scored again (past the 256 that one CTA ranks by itself);
+    the result is the exact one."""
+    import torch
+    H, G, D = shape
+    rng = np.random.default_rng(D)
+    dt = torch.bfloat16 if dtype == "bf16" else torch.float32
+    nb, P, n, n_sel = 3000, 8, 2, 500
+    lo = rng.standard_normal((nb, G, D)) * 0.01 - 0.5
+    hi = lo + np.abs(rng.standard_normal((nb, G, D))) * 0.01
+    lo[..., 3] *= times
+    hi[..., 3] = lo[..., 3] + np.abs(rng.standard_normal((nb, G)))
+    bounds = torch.from_numpy(np.stack([lo, hi], 2)).to(dt)[None].contiguous()
+    q = torch.from_numpy(rng.standard_normal((n, H * D)).astype(np.float32))
+    pool = torch.zeros(1, nb, G, P, D, dtype=dt).cuda()
+    c = tg.PagedKVCache(backend, 1, nb, P, H, G, D,
+                        tg.DTYPE_BF16 if dtype == "bf16" else tg.DTYPE_F32, max_pos=64, k=pool,
+                        v=pool, bounds=bounds.cuda())
+    table = np.stack([rng.permutation(nb) for _ in range(n)])
+    pages = torch.zeros(n, G, n_sel, dtype=torch.int32).cuda()
+    c.select_pages(0, q.cuda(), i32([nb * P - 1] * n), i32(table), pages)
+    backend.synchronize()
+    b = bounds[0].double().numpy()
+    x = q.double().numpy().reshape(n, G, H // G, D)
+    for s in range(n):
+        for g in range(G):
+            bl, bh = b[table[s], g, 0], b[table[s], g, 1]
+            score = np.maximum(x[s, g][:, None] * bl, x[s, g][:, None] * bh).sum(-1).max(0)
+            score[0] = score[-1] = np.inf
+            order = sorted(range(nb), key=lambda j: (-score[j], j))
+            assert pages[s, g].tolist() == sorted(order[:n_sel]), (s, g)
     c.destroy()
 
 
